@@ -286,6 +286,8 @@ const char* sam_hip_last_error(void);
 /* ABI version of this header (bumped on any signature change). */
 int sam_hip_abi_version(void);
 
+#include "sam_hip_paged.h" /* the paged memory: multi-axis rotary positions, the cache, attention over it */
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,137 @@
+// Host/device interface of the paged key/value memory: the cache's pages (kv_cache.hip) and the attention of new
+// tokens over them (paged_attn*.hip).
+//
+// A pool holds pages [pages, heads, page_size, d] of keys and another of values. Sequence b's key j lies in page
+// table[b][j / page_size], slot j % page_size. In 8 bits (e4m3) a row of d values has one scale, a power of two held
+// as its biased exponent: value = code * 2^(scale - 127).
+#pragma once
+#include "common.hpp"
+
+namespace samhip {
+
+constexpr int kE4M3 = 3;  // cache dtype code beside DType's
+struct e4m3 {
+  unsigned char bits;
+};
+
+struct PagedKv {
+  void* k;
+  void* v;
+  unsigned char* ks;  // scales [pages, heads, page_size], e4m3 only
+  unsigned char* vs;
+  const int* table;   // [batch, width]
+  const int* starts;  // [batch + 1] first token of each sequence among the new ones (null: kv_read)
+  const int* lens;    // [batch] tokens that each sequence holds, the new ones included
+  int batch, pages, heads, page, d, width;
+  unsigned magic, shift;  // j / page == (j * magic) >> shift for 0 <= j < 2^31
+};
+
+// j / d by a multiplication: with L = ceil(log2 d) and m = floor(2^(31 + L) / d) + 1, m exceeds 2^(31+L) / d by at
+// most 1 <= 2^L / d, i.e. by 2^-31 of itself at most, which is exact for every j below 2^31.
+inline void division_magic(int d, unsigned* magic, unsigned* shift) {
+  unsigned l = 0;
+  while ((1l << l) < d) ++l;
+  *shift = 31 + l;
+  *magic = (unsigned)((1ul << (31 + l)) / (unsigned)d + 1);
+}
+__host__ __device__ inline unsigned divide_magic(unsigned j, unsigned magic, unsigned shift) {
+  return (unsigned)(((unsigned long)j * magic) >> shift);
+}
+
+// Row (of the pools seen as [pages * heads * page_size, d]) of sequence b's key j for one head, or -1 where j is
+// outside the table or its entry outside the pool.
+__device__ __forceinline__ long paged_row(const PagedKv& c, int b, int head, int j, int end) {
+  if ((unsigned)j >= (unsigned)end) return -1;
+  const unsigned t = divide_magic((unsigned)j, c.magic, c.shift);
+  const int page = c.table[(long)b * c.width + t];
+  if ((unsigned)page >= (unsigned)c.pages) return -1;
+  return ((long)page * c.heads + head) * c.page + (j - (int)t * c.page);
+}
+
+// Keys that sequence b holds, inside what its table can name.
+__device__ __forceinline__ int paged_len(const PagedKv& c, int b) {
+  return max(0, min(c.lens[b], c.width * c.page));
+}
+
+__device__ __forceinline__ float pow2_of(unsigned char biased) {
+  return __uint_as_float(biased ? (unsigned)biased << 23 : 0x00400000u);  // 2^-127 is subnormal
+}
+
+// Arguments of one paged-attention launch. Strides in elements: [0] token, [1] head.
+struct PagedParams {
+  PagedKv c;
+  const void* q;
+  void* out;
+  long sq[2], so[2];
+  int tokens, heads, group;   // query heads, and how many of them share a key head
+  unsigned gmagic, gshift;    // division by group
+  float sc;                   // scale * log2(e)
+  int causal, zero_rest;
+  int rtiles, nsplit;         // row tiles per (sequence, key head) of the grid; key splits
+  float* opart;               // nsplit > 1: partial O [nsplit][tokens * heads][d], f32, not normalised
+  float* ml;                  // nsplit > 1: running (max, sum) [nsplit][tokens * heads][2], log2 units
+};
+
+// How a call runs: the kernel's rows per tile, the row tiles and key splits of its grid, its workspace.
+struct PagedPlan {
+  int kernel, rows, rtiles, nsplit;
+  long part_bytes, total;
+};
+PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
+                     int max_len, int cus);
+hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const PagedPlan& plan, hipStream_t stream);
+hipError_t paged_f32(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
+hipError_t paged_combine(int dtype, const PagedParams& p, hipStream_t stream);
+
+hipError_t kv_write(int dtype, int cache_dtype, const void* k, const void* v, const long* sk, const long* sv,
+                    const PagedKv& c, int tokens, hipStream_t stream);
+hipError_t kv_read(int dtype, int cache_dtype, void* k, void* v, const PagedKv& c, int max_len, hipStream_t stream);
+
+hipError_t rope_axes(int dtype, const void* x, const int* pos, const double* freqs, const int* axes, void* out, int b,
+                     int l, int h, int d, int pairs, int naxes, const long* sx, const long* sp, const long* so,
+                     int halves, int inverse, hipStream_t stream);
+
+// ------------------------------------------------------------------------------------------ device helpers
+
+// Workgroup i runs on XCD i % 8; give each XCD a contiguous range of the linear work index, so that the workgroups
+// that read one head's keys share an L2.
+__device__ __forceinline__ int paged_xcd_block(int i, int total) {
+  const int per = total >> 3, rem = total & 7, x = i & 7, j = i >> 3;
+  return x * per + (x < rem ? x : rem) + j;
+}
+
+// One sequence's new tokens [s0, s0 + lq), keys, and the row tile this workgroup starts with.
+struct PagedWork {
+  int tile, split, head, b;
+  int s0, lq, len;
+};
+__device__ __forceinline__ PagedWork paged_work(const PagedParams& p) {
+  const int lin = paged_xcd_block(blockIdx.x, gridDim.x);
+  PagedWork w;
+  w.tile = lin % p.rtiles;
+  w.split = lin / p.rtiles % p.nsplit;
+  const int hb = lin / (p.rtiles * p.nsplit);
+  w.head = hb % p.c.heads;
+  w.b = hb / p.c.heads;
+  w.s0 = max(0, min(p.c.starts[w.b], p.tokens));
+  w.lq = max(0, min(p.c.starts[w.b + 1], p.tokens) - w.s0);
+  w.len = paged_len(p.c, w.b);
+  return w;
+}
+
+// Sets the rows of out that belong to no sequence to zero, spread over the launch's workgroups.
+template <typename T> __device__ __forceinline__ void paged_zero_rest(const PagedParams& p) {
+  const int first = max(0, min(p.c.starts[0], p.tokens)), end = max(first, min(p.c.starts[p.c.batch], p.tokens));
+  const int rest = p.tokens - (end - first), cols = p.heads * (p.c.d / 8);
+  for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+    const long t = i < first ? i : end + (i - first);
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      const int head = c / (p.c.d / 8), col = c % (p.c.d / 8) * 8;
+      u32x4* w = reinterpret_cast<u32x4*>(reinterpret_cast<T*>(p.out) + t * p.so[0] + head * p.so[1] + col);
+      w[0] = u32x4{};
+      if (sizeof(T) == 4) w[1] = u32x4{};
+    }
+  }
+}
+
+}  // namespace samhip

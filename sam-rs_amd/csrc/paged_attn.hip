@@ -1,0 +1,35 @@
+// Which kernel runs a paged-attention call, with how many rows a tile and how many key splits.
+#include <algorithm>
+
+#include "paged.hpp"
+
+namespace samhip {
+
+PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
+                     int max_len, int cus) {
+  (void)dtype;
+  (void)cache_dtype;
+  PagedPlan plan = {};
+  const long group = heads / kv_heads, rows = (long)std::max(max_q, 1) * group;
+  plan.rows = rows <= 16 || d > 128 ? 16 : 32;
+  plan.rtiles = (int)((rows + plan.rows - 1) / plan.rows);
+  // two workgroups a CU, if every split then has a block of 32 keys for each of its four waves
+  const long base = (long)plan.rtiles * kv_heads * batch;
+  const long want = (2L * cus + base - 1) / base, most = ((long)max_len + 127) / 128;
+  plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 64L));
+  if (plan.nsplit > 1) {
+    plan.part_bytes = (long)plan.nsplit * tokens * heads * d * 4;
+    plan.total = plan.part_bytes + (long)plan.nsplit * tokens * heads * 8;
+  }
+  return plan;
+}
+
+hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const PagedPlan& plan, hipStream_t stream) {
+  p.rtiles = plan.rtiles;
+  p.nsplit = plan.nsplit;
+  hipError_t e = paged_f32(dtype, cache_dtype, p, plan.rows, stream);
+  if (e == hipSuccess && p.nsplit > 1) e = paged_combine(dtype, p, stream);
+  return e;
+}
+
+}  // namespace samhip

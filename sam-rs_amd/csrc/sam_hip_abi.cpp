@@ -11,6 +11,7 @@
 
 #include "../../include/sam_hip.h"
 #include "flash_attn.hpp"
+#include "paged.hpp"
 
 namespace samhip {
 hipError_t attn_relpos_half(int dtype, const void* q, const void* kt, const void* v, const void* table, void* out,
@@ -605,6 +606,218 @@ int sam_hip_qkv_rope(const void* y, const void* bias, const float* cos_t, const 
   return check_launch(
       samhip::qkv_rope(dtype, y, bias, cos_t, sin_t, out, tokens, n, nh, hd, reinterpret_cast<hipStream_t>(stream)),
       "qkv-rope");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------ the paged memory
+
+extern "C" {
+
+int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const int* axes, void* out, int dtype, int b,
+                      int l, int h, int d, int pairs, int naxes, const long* strides_x, const long* strides_pos,
+                      const long* strides_out, int halves, int inverse, void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("rope-axes");
+  if (!x || !out || (pairs != 0 && (!pos || !freqs || !axes)))
+    return fail(SAM_HIP_EINVAL, "rope-axes: null pointer argument");
+  if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
+  if (b < 0 || l < 0 || h <= 0 || d <= 0 || pairs < 0 || naxes <= 0)
+    return fail(SAM_HIP_EINVAL, "rope-axes: sizes b=%d l=%d h=%d d=%d pairs=%d axes=%d", b, l, h, d, pairs, naxes);
+  if (2L * pairs > d) return fail(SAM_HIP_EINVAL, "rope-axes: %d pairs do not fit in a head dim of %d", pairs, d);
+  if ((long)b * l > (1L << 31) || (long)h * d > (1L << 31) || (long)b * l * ((long)h * d) > (1L << 38))
+    return fail(SAM_HIP_EUNSUPPORTED, "rope-axes: more than 2^38 elements");
+  const int elem = dtype == 0 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(x) % elem || reinterpret_cast<uintptr_t>(out) % elem ||
+      reinterpret_cast<uintptr_t>(pos) % 4 || reinterpret_cast<uintptr_t>(freqs) % 8 ||
+      reinterpret_cast<uintptr_t>(axes) % 4)
+    return fail(SAM_HIP_EUNSUPPORTED, "rope-axes: pointers must be aligned to their elements");
+  long sx[3], so[3], sp[3];
+  contiguous_strides(sx, l, h, d);
+  contiguous_strides(so, l, h, d);
+  sp[0] = (long)l * naxes;
+  sp[1] = naxes;
+  sp[2] = 1;
+  for (int i = 0; i < 3; ++i) {
+    if (strides_x) sx[i] = strides_x[i];
+    if (strides_out) so[i] = strides_out[i];
+    if (strides_pos) sp[i] = strides_pos[i];
+    if (sx[i] < 0 || so[i] < 0 || sp[i] < 0) return fail(SAM_HIP_EUNSUPPORTED, "rope-axes: strides must not be negative");
+  }
+  if (x == out && (sx[0] != so[0] || sx[1] != so[1] || sx[2] != so[2]))
+    return fail(SAM_HIP_EINVAL, "rope-axes: in place, x and out must have the same strides");
+  return check_launch(samhip::rope_axes(dtype, x, pos, freqs, axes, out, b, l, h, d, pairs, naxes, sx, sp, so,
+                                        halves != 0, inverse != 0, reinterpret_cast<hipStream_t>(stream)),
+                      "rope-axes");
+}
+
+}  // extern "C"
+
+namespace {
+
+// The checks that every call on a paged cache shares, and its description for the kernels.
+int check_pool(const char* what, const void* k_pages, const void* v_pages, const unsigned char* k_scale,
+               const unsigned char* v_scale, const int* table, const int* lens, int dtype, int cache_dtype, int batch,
+               int pages, int kv_heads, int page_size, int d, int table_width, samhip::PagedKv* c) {
+  if (!k_pages || !v_pages || !table || !lens) return fail(SAM_HIP_EINVAL, "%s: null pointer argument", what);
+  if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
+  if (cache_dtype != dtype && cache_dtype != samhip::kE4M3)
+    return fail(SAM_HIP_EDTYPE, "%s: the cache holds dtype %d or e4m3 (%d), got %d", what, dtype, samhip::kE4M3, cache_dtype);
+  if (cache_dtype == samhip::kE4M3 && (!k_scale || !v_scale))
+    return fail(SAM_HIP_EINVAL, "%s: an e4m3 cache needs its scales", what);
+  if (batch <= 0 || pages <= 0 || kv_heads <= 0 || page_size <= 0 || d <= 0 || table_width <= 0)
+    return fail(SAM_HIP_EINVAL, "%s: sizes must be positive (batch=%d pages=%d heads=%d page=%d d=%d width=%d)", what,
+                batch, pages, kv_heads, page_size, d, table_width);
+  if (d % 8 != 0 || d > 256)
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: head dim must be a multiple of 8 and at most 256, got %d", what, d);
+  if ((long)table_width * page_size >= 1L << 30)
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: a table of %d pages of %d tokens is beyond 2^30 tokens", what, table_width,
+                page_size);
+  // rows of the pool below 2^47 / d bytes: their byte offsets stay far inside 64 bits
+  if ((long)pages * kv_heads > (1L << 40) / page_size)
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: the pool has more than 2^40 rows", what);
+  if (!aligned16(k_pages) || !aligned16(v_pages))
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: the pages must be 16-byte aligned", what);
+  *c = samhip::PagedKv{};
+  c->k = const_cast<void*>(k_pages);
+  c->v = const_cast<void*>(v_pages);
+  c->ks = const_cast<unsigned char*>(k_scale);
+  c->vs = const_cast<unsigned char*>(v_scale);
+  c->table = table;
+  c->lens = lens;
+  c->batch = batch;
+  c->pages = pages;
+  c->heads = kv_heads;
+  c->page = page_size;
+  c->d = d;
+  c->width = table_width;
+  samhip::division_magic(page_size, &c->magic, &c->shift);
+  return SAM_HIP_OK;
+}
+
+// (token, head) strides of a [tokens, heads, d] operand whose rows move in 16-byte vectors.
+int token_strides(const char* what, const char* name, const long* in, long* out, int heads, int d, int dtype) {
+  out[0] = in ? in[0] : (long)heads * d;
+  out[1] = in ? in[1] : d;
+  const int elem = dtype == 0 ? 4 : 2;
+  for (int i = 0; i < 2; ++i)
+    if (out[i] < 0 || out[i] * elem % 16 != 0)
+      return fail(SAM_HIP_EUNSUPPORTED, "%s: %s strides must be non-negative multiples of 16 bytes", what, name);
+  return SAM_HIP_OK;
+}
+
+int check_paged_sizes(const char* what, int tokens, int batch, int heads, int kv_heads, int d, int max_q, int max_len) {
+  if (tokens < 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || d <= 0 || max_q < 0 || max_len < 0)
+    return fail(SAM_HIP_EINVAL, "%s: sizes tokens=%d batch=%d heads=%d kv_heads=%d d=%d max_q=%d max_len=%d", what, tokens,
+                batch, heads, kv_heads, d, max_q, max_len);
+  if (heads % kv_heads != 0)
+    return fail(SAM_HIP_EINVAL, "%s: %d query heads do not share %d key heads evenly", what, heads, kv_heads);
+  if ((long)tokens * heads >= 1L << 31 || (long)max_q * (heads / kv_heads) >= 1L << 30 || (long)batch * kv_heads >= 1L << 24)
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: too many rows (tokens=%d heads=%d batch=%d)", what, tokens, heads, batch);
+  return SAM_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sam_hip_kv_write(const void* k, const void* v, void* k_pages, void* v_pages, unsigned char* k_scale,
+                     unsigned char* v_scale, const int* table, const int* starts, const int* lens, int dtype,
+                     int cache_dtype, int tokens, int batch, int pages, int kv_heads, int page_size, int d,
+                     int table_width, const long* strides_k, const long* strides_v, void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("kv-write");
+  if (!k || !v || !starts) return fail(SAM_HIP_EINVAL, "kv-write: null pointer argument");
+  samhip::PagedKv c;
+  if (int rc = check_pool("kv-write", k_pages, v_pages, k_scale, v_scale, table, lens, dtype, cache_dtype, batch, pages,
+                          kv_heads, page_size, d, table_width, &c);
+      rc != SAM_HIP_OK)
+    return rc;
+  c.starts = starts;
+  if (tokens < 0 || (long)tokens * kv_heads >= 1L << 31)
+    return fail(SAM_HIP_EINVAL, "kv-write: %d tokens of %d heads", tokens, kv_heads);
+  long sk[2], sv[2];
+  if (int rc = token_strides("kv-write", "k", strides_k, sk, kv_heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if (int rc = token_strides("kv-write", "v", strides_v, sv, kv_heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if (!aligned16(k) || !aligned16(v)) return fail(SAM_HIP_EUNSUPPORTED, "kv-write: k and v must be 16-byte aligned");
+  return check_launch(
+      samhip::kv_write(dtype, cache_dtype, k, v, sk, sv, c, tokens, reinterpret_cast<hipStream_t>(stream)), "kv-write");
+}
+
+int sam_hip_kv_read(void* k, void* v, const void* k_pages, const void* v_pages, const unsigned char* k_scale,
+                    const unsigned char* v_scale, const int* table, const int* lens, int dtype, int cache_dtype,
+                    int batch, int max_len, int pages, int kv_heads, int page_size, int d, int table_width,
+                    void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("kv-read");
+  if (!k || !v) return fail(SAM_HIP_EINVAL, "kv-read: null pointer argument");
+  samhip::PagedKv c;
+  if (int rc = check_pool("kv-read", k_pages, v_pages, k_scale, v_scale, table, lens, dtype, cache_dtype, batch, pages,
+                          kv_heads, page_size, d, table_width, &c);
+      rc != SAM_HIP_OK)
+    return rc;
+  if (max_len < 0) return fail(SAM_HIP_EINVAL, "kv-read: max_len %d", max_len);
+  if ((long)batch * max_len >= 1L << 31 || (long)batch * max_len * kv_heads >= 1L << 33)  // 8 rows or more a workgroup
+    return fail(SAM_HIP_EUNSUPPORTED, "kv-read: too many rows (batch=%d max_len=%d heads=%d)", batch, max_len, kv_heads);
+  if (!aligned16(k) || !aligned16(v)) return fail(SAM_HIP_EUNSUPPORTED, "kv-read: k and v must be 16-byte aligned");
+  return check_launch(samhip::kv_read(dtype, cache_dtype, k, v, c, max_len, reinterpret_cast<hipStream_t>(stream)),
+                      "kv-read");
+}
+
+long sam_hip_paged_attention_workspace_size(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads,
+                                            int d, int max_q, int max_len) {
+  if (!dtype_ok(dtype) || (cache_dtype != dtype && cache_dtype != samhip::kE4M3)) {
+    fail(SAM_HIP_EDTYPE, "paged-attention: dtype %d over a cache of dtype %d", dtype, cache_dtype);
+    return -1;
+  }
+  if (check_paged_sizes("paged-attention", tokens, batch, heads, kv_heads, d, max_q, max_len) != SAM_HIP_OK) return -1;
+  return samhip::paged_plan(dtype, cache_dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,
+                            samhip::device_cu_count())
+      .total;
+}
+
+int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pages, const unsigned char* k_scale,
+                            const unsigned char* v_scale, const int* table, const int* starts, const int* lens,
+                            void* out, int dtype, int cache_dtype, int tokens, int batch, int heads, int pages,
+                            int kv_heads, int page_size, int d, int table_width, const long* strides_q,
+                            const long* strides_o, float scale, int causal, int zero_rest, int max_q, int max_len,
+                            void* workspace, long workspace_bytes, void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("paged-attention");
+  if (!q || !starts || !out) return fail(SAM_HIP_EINVAL, "paged-attention: null pointer argument");
+  samhip::PagedParams p = {};
+  if (int rc = check_pool("paged-attention", k_pages, v_pages, k_scale, v_scale, table, lens, dtype, cache_dtype, batch,
+                          pages, kv_heads, page_size, d, table_width, &p.c);
+      rc != SAM_HIP_OK)
+    return rc;
+  if (int rc = check_paged_sizes("paged-attention", tokens, batch, heads, kv_heads, d, max_q, max_len); rc != SAM_HIP_OK)
+    return rc;
+  if (!(scale >= 0.f) || !(scale < 3.0e38f))
+    return fail(SAM_HIP_EINVAL, "paged-attention: scale must be finite and not negative, got %g", (double)scale);
+  if (int rc = token_strides("paged-attention", "q", strides_q, p.sq, heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if (int rc = token_strides("paged-attention", "out", strides_o, p.so, heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if (!aligned16(q) || !aligned16(out))
+    return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: q and out must be 16-byte aligned");
+  const samhip::PagedPlan plan = samhip::paged_plan(dtype, cache_dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,
+                                                    samhip::device_cu_count());
+  if (plan.total > 0 && (!workspace || workspace_bytes < plan.total))
+    return fail(SAM_HIP_EINVAL, "paged-attention: workspace of %ld bytes needed, got %ld", plan.total,
+                workspace ? workspace_bytes : 0L);
+  if (plan.total > 0 && !aligned16(workspace))
+    return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: the workspace must be 16-byte aligned");
+  if ((long)plan.rtiles * plan.nsplit * kv_heads * batch > 0x7fffffffL)
+    return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: too many workgroups (max_q=%d batch=%d)", max_q, batch);
+  if (tokens == 0) return ok();
+  p.c.starts = starts;
+  p.q = q;
+  p.out = out;
+  p.tokens = tokens;
+  p.heads = heads;
+  p.group = heads / kv_heads;
+  samhip::division_magic(p.group, &p.gmagic, &p.gshift);
+  p.sc = scale * 1.4426950408889634f;
+  p.causal = causal != 0;
+  p.zero_rest = zero_rest != 0;
+  p.opart = reinterpret_cast<float*>(workspace);
+  p.ml = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.part_bytes);
+  return check_launch(samhip::paged_attention(dtype, cache_dtype, p, plan, reinterpret_cast<hipStream_t>(stream)),
+                      "paged-attention");
 }
 
 }  // extern "C"

@@ -13,7 +13,14 @@ Names, argument meaning and errors follow the reference:
     sdpa(q, k, v, mask=None)                             sam3/nn.rs:26-34
     rope(x, cos, sin)                                    sam3/video.rs:106-113
     rope_attention(q, k, v, cos, sin, n_exclude)         sam3/video.rs:129-145 (after the projections)
+    rope_axes(x, pos, freqs, axes), rope_freqs(...)      rotary positions over several axes
+    kv_write(k, v, k_pages, v_pages, table, ...)         new keys and values into a paged cache (16 or 8 bits)
+    kv_read(k_pages, v_pages, table, lens, max_len)      what its sequences hold, dense
+    paged_attention(q, k_pages, v_pages, table, ...)     attention of new tokens over the pages
     set_enabled(on), enabled()                           cpu_gemm.rs:11, 25-32 (the process-wide switch)
+
+rope_axes to paged_attention are the paged form of the video memory (sam3/video.rs:133-145, 356-406); the reference
+has no entry points of that kind.
 
 There is no CPU fallback: on a machine without the built library or a GPU every call raises. While the
 switch is off every call raises SamHipDisabled without touching the device; the caller then takes its
@@ -22,6 +29,7 @@ own path, as the reference's callers do when cpu_gemm::enabled() is false.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -34,6 +42,7 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_long2 = ctypes.c_long * 2
 _long3 = ctypes.c_long * 3
 _long4 = ctypes.c_long * 4
 
@@ -95,6 +104,16 @@ def load():
         L.sam_hip_qkv_rope.restype = _i
         L.sam_hip_sdpa_mask.argtypes = [_vp] * 5 + [_i] * 6 + [_lp] * 5 + [_f, _vp, ctypes.c_long, _vp]
         L.sam_hip_sdpa_mask.restype = _i
+        L.sam_hip_rope_axes.argtypes = [_vp] * 5 + [_i] * 7 + [_lp] * 3 + [_i, _i, _vp]
+        L.sam_hip_rope_axes.restype = _i
+        L.sam_hip_kv_write.argtypes = [_vp] * 9 + [_i] * 9 + [_lp] * 2 + [_vp]
+        L.sam_hip_kv_write.restype = _i
+        L.sam_hip_kv_read.argtypes = [_vp] * 8 + [_i] * 9 + [_vp]
+        L.sam_hip_kv_read.restype = _i
+        L.sam_hip_paged_attention_workspace_size.argtypes = [_i] * 9
+        L.sam_hip_paged_attention_workspace_size.restype = ctypes.c_long
+        L.sam_hip_paged_attention.argtypes = [_vp] * 9 + [_i] * 10 + [_lp] * 2 + [_f] + [_i] * 4 + [_vp, ctypes.c_long, _vp]
+        L.sam_hip_paged_attention.restype = _i
         L.sam_hip_set_enabled.argtypes = [_i]
         L.sam_hip_set_enabled.restype = None
         L.sam_hip_enabled.argtypes = []
@@ -592,4 +611,228 @@ def rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch
     out = torch.empty((b, lq, d), dtype=q.dtype, device=q.device)
     _flash(q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2), out.unsqueeze(2), "blhd", float(d) ** -0.5, cos, sin,
            lq, rot, noalloc=noalloc)
+    return out
+
+
+# ------------------------------------------------------------------------------------------ the paged memory
+
+_E4M3 = 3  # SAM_HIP_E4M3
+
+
+def _one_device(what: str, *ts):
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise SamHipError("sam-rs HIP kernels need device tensors")
+        if t is not None and t.device != ts[0].device:
+            raise SamHipError(f"{what}: all operands must be on one device: {t.device} vs {ts[0].device}")
+
+
+def _here(t: torch.Tensor) -> bool:
+    return t.device.index == (torch.cuda.current_device() if _raw_device is None else _raw_device())
+
+
+def _on_its_device(fn):
+    """Runs fn with its first tensor's device as the current one, on that device's current stream."""
+
+    @functools.wraps(fn)
+    def run(t, *args, **kwargs):
+        if not t.is_cuda or _here(t):
+            return fn(t, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(t, *args, **kwargs)
+
+    return run
+
+
+def rope_freqs(sections, theta: float = 10000.0, scale: float = 1.0, device="cuda"):
+    """The pairs' frequencies and axes of rope_axes for one run of pairs per axis: axis a takes sections[a] pairs with
+    frequencies scale * theta^(-i / sections[a]), as rope_tables_hd gives its two axes (sam3/vision.rs:26-46).
+    Returns (freqs f64 [P], axes int32 [P]), P = sum(sections); a program keeps them."""
+    sections = [int(s) for s in sections]
+    if not sections or min(sections) < 0:
+        raise SamHipError(f"rope_freqs: sections must not be negative, got {sections}")
+    freqs = [scale * theta ** (-i / s) for s in sections for i in range(s)]
+    axes = [a for a, s in enumerate(sections) for _ in range(s)]
+    return (torch.tensor(freqs, dtype=torch.float64, device=device), torch.tensor(axes, dtype=torch.int32, device=device))
+
+
+@_on_its_device
+def rope_axes(x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, axes: torch.Tensor, pairs: str = "adjacent",
+              inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions over several axes: x [B, L, H, D] or [T, H, D], pos int32 [B, L, A] (or anything that broadcasts
+    to it; [T, A]); pair i turns by pos[..., axes[i]] * freqs[i] (freqs f64, axes int32, [P] with 2 P <= D; rope_freqs
+    makes them). pairs "adjacent" turns (x[2i], x[2i+1]), "halves" (x[i], x[i+P]); columns past 2 P are copied. inverse
+    turns back, which is also what a gradient with respect to the result takes to become one with respect to x. out may
+    be x itself."""
+    _one_device("rope_axes", x, pos, freqs, axes, out)
+    dt = _dtype(x)
+    if x.dim() not in (3, 4):
+        raise SamHipError(f"rope_axes: x must be [B, L, H, D] or [T, H, D], got {tuple(x.shape)}")
+    if pairs not in ("adjacent", "halves"):
+        raise SamHipError(f'rope_axes: pairs must be "adjacent" or "halves", got {pairs!r}')
+    if pos.dtype != torch.int32 or freqs.dtype != torch.float64 or axes.dtype != torch.int32:
+        raise SamHipError(f"rope_axes: pos and axes must be int32 and freqs f64, got {pos.dtype}, {axes.dtype}, {freqs.dtype}")
+    if freqs.dim() != 1 or axes.shape != freqs.shape or 2 * freqs.shape[0] > x.shape[-1]:
+        raise SamHipError(f"rope_axes: freqs {tuple(freqs.shape)} and axes {tuple(axes.shape)} must be [P], 2 P <= {x.shape[-1]}")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise SamHipError(f"rope_axes: out must match x (shape {tuple(x.shape)}, {x.dtype}), got {tuple(out.shape)}, {out.dtype}")
+    if x.stride(-1) != 1:
+        if out is x:
+            raise SamHipError("rope_axes: in place, the head dimension must be contiguous")
+        x = x.contiguous()
+    if out.stride(-1) != 1:
+        raise SamHipError("rope_axes: out's head dimension must be contiguous")
+    x4, o4, p3 = (x, out, pos) if x.dim() == 4 else (x.unsqueeze(0), out.unsqueeze(0), pos)
+    b, l, h, d = x4.shape
+    try:
+        p3 = p3.expand(b, l, pos.shape[-1])
+    except RuntimeError as e:
+        raise SamHipError(f"rope_axes: pos {tuple(pos.shape)} does not broadcast to {(b, l)} positions of its axes") from e
+    if x.numel() == 0:
+        return out
+    if not (freqs.is_contiguous() and axes.is_contiguous()):
+        freqs, axes = freqs.contiguous(), axes.contiguous()
+    _check(load().sam_hip_rope_axes(x4.data_ptr(), p3.data_ptr(), freqs.data_ptr(), axes.data_ptr(), o4.data_ptr(), dt, b,
+                                    l, h, d, freqs.shape[0], pos.shape[-1], _long3(*x4.stride()[:3]),
+                                    _long3(*p3.stride()), _long3(*o4.stride()[:3]), pairs == "halves", bool(inverse),
+                                    _stream()))
+    return out
+
+
+def _pool(what, k_pages, v_pages, k_scale, v_scale, table, dtype):
+    """(cache dtype code, pages, heads, page_size, d) of a pool, after its checks."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise SamHipError(f"{what}: k_pages and v_pages must be [pages, heads, page_size, d] alike, got "
+                          f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
+    if k_pages.dtype == torch.float8_e4m3fn:
+        code = _E4M3
+        for s in (k_scale, v_scale):
+            if s is None or s.dtype != torch.uint8 or s.shape != k_pages.shape[:3] or not s.is_contiguous():
+                raise SamHipError(f"{what}: an e4m3 cache needs k_scale and v_scale, uint8 {tuple(k_pages.shape[:3])} and contiguous")
+    elif k_pages.dtype == dtype:
+        code = _DTYPES[dtype]
+        if k_scale is not None or v_scale is not None:
+            raise SamHipError(f"{what}: scales belong to an e4m3 cache, not to {dtype}")
+    else:
+        raise SamHipError(f"{what}: the cache must hold {dtype} or torch.float8_e4m3fn, got {k_pages.dtype}")
+    if table.dim() != 2 or table.dtype != torch.int32:
+        raise SamHipError(f"{what}: table must be int32 [batch, width], got {table.dtype} {tuple(table.shape)}")
+    return (code, *k_pages.shape)
+
+
+def _tables(what, table, starts, lens):
+    """The tables, contiguous, after their checks."""
+    for name, t, n in (("starts", starts, table.shape[0] + 1), ("lens", lens, table.shape[0])):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,)):
+            raise SamHipError(f"{what}: {name} must be int32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    return (table.contiguous(), None if starts is None else starts.contiguous(), lens.contiguous())
+
+
+def _token_rows(what, name, t):
+    """A [T, heads, d] operand whose rows can be moved in 16-byte vectors: itself, or a copy."""
+    e = t.element_size()
+    if t.stride(2) != 1 or t.stride(0) * e % 16 or t.stride(1) * e % 16 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+@_on_its_device
+def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+             starts: torch.Tensor, lens: torch.Tensor, k_scale: torch.Tensor | None = None,
+             v_scale: torch.Tensor | None = None) -> None:
+    """Stores new tokens' keys and values k, v [T, heads, D] in their pages, in place. Sequence b's new tokens are rows
+    starts[b] .. starts[b+1] of k and v and become its last ones: token t goes to position lens[b] - (starts[b+1] - t),
+    in page table[b][position // page_size]. k_pages, v_pages [pages, heads, page_size, D] hold k's dtype, or
+    torch.float8_e4m3fn with k_scale, v_scale uint8 [pages, heads, page_size]: a row's scale is the power of two
+    2^(byte - 127) that brings its largest value nearest to 448 from below, its codes round to nearest even, and values
+    that are not finite become NaN. Tokens at a negative position, past the table, or whose table entry names no page are
+    not stored; two positions in one page slot must not be written by one call."""
+    _one_device("kv_write", k, v, k_pages, v_pages, table, starts, lens, k_scale, v_scale)
+    dt = _dtype(k, v)
+    code, pages, heads, page, d = _pool("kv_write", k_pages, v_pages, k_scale, v_scale, table, k.dtype)
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (heads, d):
+        raise SamHipError(f"kv_write: k and v must be [T, {heads}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    table, starts, lens = _tables("kv_write", table, starts, lens)
+    if k.shape[0] == 0 or table.shape[0] == 0:
+        return
+    k, v = _token_rows("kv_write", "k", k), _token_rows("kv_write", "v", v)
+    _check(load().sam_hip_kv_write(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
+                                   _ptr(v_scale), table.data_ptr(), starts.data_ptr(), lens.data_ptr(), dt, code,
+                                   k.shape[0], table.shape[0], pages, heads, page, d, table.shape[1],
+                                   _long2(k.stride(0), k.stride(1)), _long2(v.stride(0), v.stride(1)), _stream()))
+
+
+@_on_its_device
+def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int,
+            k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+            dtype: torch.dtype | None = None):
+    """What the sequences of a cache hold, dense: (k, v) [B, max_len, heads, D], zeros from lens[b] on and where a table
+    entry names no page. dtype defaults to the cache's; an e4m3 cache needs one (each value is rounded to it once)."""
+    _one_device("kv_read", k_pages, v_pages, table, lens, k_scale, v_scale)
+    dtype = k_pages.dtype if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise SamHipError(f"unsupported dtype {dtype} for a sam-rs HIP kernel")
+    code, pages, heads, page, d = _pool("kv_read", k_pages, v_pages, k_scale, v_scale, table, dtype)
+    table, _, lens = _tables("kv_read", table, None, lens)
+    max_len = int(max_len)
+    if max_len < 0:
+        raise SamHipError(f"kv_read: max_len must not be negative, got {max_len}")
+    b = table.shape[0]
+    k, v = torch.empty((2, b, max_len, heads, d), dtype=dtype, device=k_pages.device)
+    if k.numel():
+        _check(load().sam_hip_kv_read(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
+                                      _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _DTYPES[dtype], code, b, max_len,
+                                      pages, heads, page, d, table.shape[1], _stream()))
+    return k, v
+
+
+@_on_its_device
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                    starts: torch.Tensor, lens: torch.Tensor, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, scale: float | None = None, causal: bool = True,
+                    max_q: int | None = None, max_len: int | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens over a paged cache that already holds their own keys (kv_write): q [T, Hq, D] -> [T, Hq, D].
+    Rows starts[b] .. starts[b+1] of q are sequence b's last tokens; a row sees the keys 0 .. lens[b] of its sequence
+    or, causal, those up to its own position. Query head h reads key head h // (Hq // heads). scale defaults to D^-0.5.
+    max_q and max_len, the longest chunk and sequence (default: T and what the table can name), shape the launch; a
+    call whose sequences exceed them is slower, not wrong. A row that sees no key is 0. Rows of no sequence are 0, or as
+    they were in an `out` that is given."""
+    _one_device("paged_attention", q, k_pages, v_pages, table, starts, lens, k_scale, v_scale, out)
+    dt = _dtype(q)
+    code, pages, heads, page, d = _pool("paged_attention", k_pages, v_pages, k_scale, v_scale, table, q.dtype)
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or heads == 0 or q.shape[1] % heads:
+        raise SamHipError(f"paged_attention: q must be [T, a multiple of {heads}, {d}], got {tuple(q.shape)}")
+    table, starts, lens = _tables("paged_attention", table, starts, lens)
+    zero_rest = out is None
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise SamHipError(f"paged_attention: out must match q (shape {tuple(q.shape)}, {q.dtype}), got {tuple(out.shape)}, {out.dtype}")
+    elif out.stride(2) != 1:
+        raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
+    tokens, hq, _ = q.shape
+    b, width = table.shape
+    if tokens == 0:
+        return out
+    if b == 0 or width == 0:  # no sequences, or none that holds a key
+        return out.zero_() if zero_rest else out
+    q = _token_rows("paged_attention", "q", q)
+    scale = float(d) ** -0.5 if scale is None else float(scale)
+    max_q = tokens if max_q is None else int(max_q)
+    max_len = width * page if max_len is None else int(max_len)
+    L = load()
+    ws_bytes = L.sam_hip_paged_attention_workspace_size(dt, code, tokens, b, hq, heads, d, max_q, max_len)
+    if ws_bytes < 0:
+        raise SamHipError(L.sam_hip_last_error().decode())
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _check(L.sam_hip_paged_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                                     table.data_ptr(), starts.data_ptr(), lens.data_ptr(), out.data_ptr(), dt, code,
+                                     tokens, b, hq, pages, heads, page, d, width, _long2(q.stride(0), q.stride(1)),
+                                     _long2(out.stride(0), out.stride(1)), scale, bool(causal), zero_rest, max_q, max_len,
+                                     _ptr(ws), ws_bytes, _stream()))
     return out
