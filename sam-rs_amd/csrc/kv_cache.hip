@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteParams p) {
     v = load_eight(reinterpret_cast<const T*>(p.v) + t * p.sv[0] + head * p.sv[1] + col);
   }
   const int b = sequence_of<LPR>(p.c, t);
-  long row = -1;
+  long row = -1;  // 64 bits: row * d passes 32
   if (r < p.rows && b < p.c.batch && t >= p.c.starts[b] && t < p.c.starts[b + 1]) {
     const long j = (long)p.c.lens[b] - p.c.starts[b + 1] + t;  // its position: the last tokens of the sequence
     if (j >= 0 && j < (long)p.c.width * p.c.page) row = paged_row(p.c, b, head, (int)j, p.c.width * p.c.page);

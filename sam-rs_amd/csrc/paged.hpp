@@ -38,14 +38,14 @@ __host__ __device__ inline unsigned divide_magic(unsigned j, unsigned magic, uns
   return (unsigned)(((unsigned long)j * magic) >> shift);
 }
 
-// Row (of the pools seen as [pages * heads * page_size, d]) of sequence b's key j for one head, or -1 where j is
-// outside the table or its entry outside the pool.
-__device__ __forceinline__ long paged_row(const PagedKv& c, int b, int head, int j, int end) {
+// Row (of the pools seen as [pages * heads * page_size, d], fewer than 2^31 of them) of sequence b's key j for one
+// head, or -1 where j is past `end` or its table entry outside the pool.
+__device__ __forceinline__ int paged_row(const PagedKv& c, int b, int head, int j, int end) {
   if ((unsigned)j >= (unsigned)end) return -1;
   const unsigned t = divide_magic((unsigned)j, c.magic, c.shift);
   const int page = c.table[(long)b * c.width + t];
   if ((unsigned)page >= (unsigned)c.pages) return -1;
-  return ((long)page * c.heads + head) * c.page + (j - (int)t * c.page);
+  return (page * c.heads + head) * c.page + (j - (int)t * c.page);
 }
 
 // Keys that sequence b holds, inside what its table can name.
@@ -68,19 +68,21 @@ struct PagedParams {
   float sc;                   // scale * log2(e)
   int causal, zero_rest;
   int rtiles, nsplit;         // row tiles per (sequence, key head) of the grid; key splits
+  int per;                    // blocks of 32 keys per split, at least (0: even shares of what each sequence holds)
   float* opart;               // nsplit > 1: partial O [nsplit][tokens * heads][d], f32, not normalised
   float* ml;                  // nsplit > 1: running (max, sum) [nsplit][tokens * heads][2], log2 units
 };
 
 // How a call runs: the kernel's rows per tile, the row tiles and key splits of its grid, its workspace.
 struct PagedPlan {
-  int kernel, rows, rtiles, nsplit;
+  int rows, rtiles, nsplit, per;
   long part_bytes, total;
 };
 PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
                      int max_len, int cus);
 hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const PagedPlan& plan, hipStream_t stream);
-hipError_t paged_f32(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
+hipError_t paged_f32(int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
+hipError_t paged_few(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
 hipError_t paged_combine(int dtype, const PagedParams& p, hipStream_t stream);
 
 hipError_t kv_write(int dtype, int cache_dtype, const void* k, const void* v, const long* sk, const long* sv,
@@ -106,7 +108,7 @@ struct PagedWork {
   int s0, lq, len;
 };
 __device__ __forceinline__ PagedWork paged_work(const PagedParams& p) {
-  const int lin = paged_xcd_block(blockIdx.x, gridDim.x);
+  const int lin = __builtin_amdgcn_readfirstlane(paged_xcd_block(blockIdx.x, gridDim.x));
   PagedWork w;
   w.tile = lin % p.rtiles;
   w.split = lin / p.rtiles % p.nsplit;

@@ -13,10 +13,12 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
   const long group = heads / kv_heads, rows = (long)std::max(max_q, 1) * group;
   plan.rows = rows <= 16 || d > 128 ? 16 : 32;
   plan.rtiles = (int)((rows + plan.rows - 1) / plan.rows);
-  // two workgroups a CU, if every split then has a block of 32 keys for each of its four waves
+  // four workgroups a CU, if every split then has two blocks of 32 keys for each of its four waves
   const long base = (long)plan.rtiles * kv_heads * batch;
-  const long want = (2L * cus + base - 1) / base, most = ((long)max_len + 127) / 128;
-  plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 64L));
+  const long want = (4L * cus + base - 1) / base, most = ((long)max_len + 255) / 256;
+  plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
+  const long blocks = ((long)max_len + 31) / 32;
+  plan.per = (int)std::min((blocks + plan.nsplit - 1) / plan.nsplit, 1L << 26);
   if (plan.nsplit > 1) {
     plan.part_bytes = (long)plan.nsplit * tokens * heads * d * 4;
     plan.total = plan.part_bytes + (long)plan.nsplit * tokens * heads * 8;
@@ -27,7 +29,9 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
 hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const PagedPlan& plan, hipStream_t stream) {
   p.rtiles = plan.rtiles;
   p.nsplit = plan.nsplit;
-  hipError_t e = paged_f32(dtype, cache_dtype, p, plan.rows, stream);
+  p.per = plan.per;
+  hipError_t e = dtype == kF32 ? paged_f32(cache_dtype, p, plan.rows, stream)
+                               : paged_few(dtype, cache_dtype, p, plan.rows, stream);
   if (e == hipSuccess && p.nsplit > 1) e = paged_combine(dtype, p, stream);
   return e;
 }

@@ -23,20 +23,11 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
 
 // Four consecutive elements as f32.
 __device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
-template <typename T> __device__ __forceinline__ f32x4 load4(const T* p) {
-  const typename Vec<T>::x4 x = *reinterpret_cast<const typename Vec<T>::x4*>(p);
-  return f32x4{to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3])};
-}
 __device__ __forceinline__ f32x4 load4(const e4m3* p) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   const int c = *reinterpret_cast<const int*>(p);
   const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
   return f32x4{a[0], a[1], b[0], b[1]};
-}
-
-__device__ __forceinline__ long shfl_long(long v, int lane) {
-  const int lo = __shfl((int)v, lane), hi = __shfl((int)(v >> 32), lane);
-  return (long)(unsigned)lo | ((long)hi << 32);
 }
 
 template <typename T, typename C, int DP, int RB>
@@ -77,8 +68,8 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
     const int most = p.causal ? max(0, min(w.len, w.len - w.lq + tlast + 1)) : w.len;
     const int tfirst = (int)divide_magic(rt * TR, p.gmagic, p.gshift);
     const int least = p.causal ? max(0, min(w.len, w.len - w.lq + tfirst + 1)) : w.len;
-    const int blocks = (most + 31) >> 5, per = (blocks + p.nsplit - 1) / p.nsplit;
-    const int b0 = w.split * per, b1 = min(blocks, b0 + per);
+    const int blocks = (most + 31) >> 5, per = max(p.per, (blocks + p.nsplit - 1) / p.nsplit);
+    const int b0 = min(blocks, w.split * per), b1 = min(blocks, b0 + per);
 
     float m[RB], l[RB];
     f32x4 o[RB][4 * ND];
@@ -92,7 +83,7 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
     for (int blk = b0 + wave; blk < b1; blk += 4) {
       const int key0 = 32 * blk;
       const bool part = key0 + 32 > least;
-      const long row = paged_row(p.c, w.b, w.head, key0 + (lane & 31), most);  // lane l looks key l % 32 up
+      const int row = paged_row(p.c, w.b, w.head, key0 + (lane & 31), most);  // lane l looks key l % 32 up
       const unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
       float ks = 1.f, vs = 1.f;
       if (kScaled && row >= 0) {
@@ -102,7 +93,7 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
       f32x4 s[RB][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const long kr = shfl_long(row, 16 * i + n);
+        const long kr = __shfl(row, 16 * i + n);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) s[rb][i] = f32x4{};
 #pragma unroll
@@ -150,7 +141,7 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int kk = 16 * i + 4 * g + e;
-          const long vr = shfl_long(row, kk);
+          const long vr = __shfl(row, kk);
           const float f = kScaled ? __shfl(vs, kk) : 1.f;
 #pragma unroll
           for (int q = 0; q < ND; ++q) {
@@ -238,14 +229,14 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
               for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(f32_result(o[rb][4 * q + j][e] * inv));
               *reinterpret_cast<typename Vec<T>::x4*>(orow + col) = x;
             }
-        } else {
+        } else if (b0 < b1 || g == 0) {
           const long row = ((long)w.split * p.tokens + tok[rb]) * p.heads + head[rb];
 #pragma unroll
           for (int q = 0; q < ND; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int col = 64 * q + 16 * g + 4 * e;
-              if (col < d)
+              if (col < d && b0 < b1)
                 *reinterpret_cast<f32x4*>(p.opart + row * d + col) =
                     f32x4{o[rb][4 * q][e], o[rb][4 * q + 1][e], o[rb][4 * q + 2][e], o[rb][4 * q + 3][e]};
             }
@@ -272,55 +263,10 @@ template <typename T, typename C> hipError_t by_size(const PagedParams& p, int r
   return d <= 64 ? launch_f32<T, C, 64, 2>(p, stream) : launch_f32<T, C, 128, 2>(p, stream);
 }
 
-// Joins the key splits of each row: out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M). A thread takes 4 columns.
-template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
-  const int cpr = p.c.d / 4;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = i / cpr;
-  const int col = (int)(i % cpr) * 4;
-  const long rows = (long)p.tokens * p.heads;
-  if (row >= rows) return;
-  const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
-  if (tok < p.c.starts[0] || tok >= p.c.starts[p.c.batch]) return;  // rows of no sequence have no partial results
-  float top = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) top = fmaxf(top, p.ml[2 * (s * rows + row)]);
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 o = {};
-  float l = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * (s * rows + row));
-    if (ml.y == 0.f) continue;  // no keys in this split: its O was not summed
-    const float w = exp2_fast(ml.x - base);
-    l += ml.y * w;
-    o += *reinterpret_cast<const f32x4*>(p.opart + (s * rows + row) * p.c.d + col) * w;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  typename Vec<T>::x4 x;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(f32_result(o[j] * inv));
-  *reinterpret_cast<typename Vec<T>::x4*>(reinterpret_cast<T*>(p.out) + tok * p.so[0] + head * p.so[1] + col) = x;
-}
-
 }  // namespace
 
-hipError_t paged_f32(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream) {
-  if (dtype == kF32)
-    return cache_dtype == kE4M3 ? by_size<float, e4m3>(p, rows, stream) : by_size<float, float>(p, rows, stream);
-  if (dtype == kF16)
-    return cache_dtype == kE4M3 ? by_size<f16, e4m3>(p, rows, stream) : by_size<f16, f16>(p, rows, stream);
-  return cache_dtype == kE4M3 ? by_size<bf16, e4m3>(p, rows, stream) : by_size<bf16, bf16>(p, rows, stream);
-}
-
-hipError_t paged_combine(int dtype, const PagedParams& p, hipStream_t stream) {
-  const long threads = (long)p.tokens * p.heads * (p.c.d / 4);
-  const dim3 grid((unsigned)((threads + 255) / 256));
-  if (dtype == kF32)
-    hipLaunchKernelGGL(paged_combine_kernel<float>, grid, dim3(256), 0, stream, p);
-  else if (dtype == kF16)
-    hipLaunchKernelGGL(paged_combine_kernel<f16>, grid, dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL(paged_combine_kernel<bf16>, grid, dim3(256), 0, stream, p);
-  return hipGetLastError();
+hipError_t paged_f32(int cache_dtype, const PagedParams& p, int rows, hipStream_t stream) {
+  return cache_dtype == kE4M3 ? by_size<float, e4m3>(p, rows, stream) : by_size<float, float>(p, rows, stream);
 }
 
 }  // namespace samhip

@@ -1,0 +1,118 @@
+// Joins the key splits of a paged-attention call on gfx950: out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M the
+// largest m_s of the row, from the partial results that the attention kernels left. Splits are added in order, so the
+// result does not depend on their timing. A split without keys has l = 0 and no O.
+//
+// What bounds it: the partial O's bytes, 4 a column and split, and, with few rows, the latency of reading them. Up to
+// eight splits a thread reads its four columns of each; past that a workgroup takes a row, its waves a share of the
+// splits each, and they meet in LDS.
+#include "paged.hpp"
+
+namespace samhip {
+
+namespace {
+
+__device__ __forceinline__ bool row_of_a_sequence(const PagedParams& p, int tok) {
+  return tok >= p.c.starts[0] && tok < p.c.starts[p.c.batch];  // the others have no partial results
+}
+
+template <typename T> __device__ __forceinline__ void store_row4(const PagedParams& p, int tok, int head, int col,
+                                                                 f32x4 o, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is 0
+  typename Vec<T>::x4 x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(f32_result(o[j] * inv));
+  *reinterpret_cast<typename Vec<T>::x4*>(reinterpret_cast<T*>(p.out) + tok * p.so[0] + head * p.so[1] + col) = x;
+}
+
+// A thread takes 4 columns of a row.
+template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
+  const int cpr = p.c.d / 4;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long row = i / cpr;
+  const int col = (int)(i % cpr) * 4;
+  const long rows = (long)p.tokens * p.heads;
+  if (row >= rows) return;
+  const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
+  if (!row_of_a_sequence(p, tok)) return;
+  float top = -INFINITY;
+  for (int s = 0; s < p.nsplit; ++s) top = fmaxf(top, p.ml[2 * (s * rows + row)]);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 o = {};
+  float l = 0.f;
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * (s * rows + row));
+    if (ml.y == 0.f) continue;  // no keys in this split: its O was not summed
+    const float w = exp2_fast(ml.x - base);
+    l += ml.y * w;
+    o += *reinterpret_cast<const f32x4*>(p.opart + (s * rows + row) * p.c.d + col) * w;
+  }
+  store_row4<T>(p, tok, head, col, o, l);
+}
+
+constexpr int kRowWaves = 8, kMostSplits = 256;
+
+// A workgroup takes a row: weights of all splits first, then wave w the splits w, w + 8, ..., a lane 4 columns.
+template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_combine_row_kernel(PagedParams p) {
+  __shared__ float weight[kMostSplits], red[2][kRowWaves];
+  __shared__ __attribute__((aligned(16))) f32x4 part[kRowWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row = blockIdx.x, rows = (long)p.tokens * p.heads;
+  const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
+  if (!row_of_a_sequence(p, tok)) return;
+  const int s = threadIdx.x;
+  float2 ml = {-INFINITY, 0.f};
+  if (s < p.nsplit) ml = *reinterpret_cast<const float2*>(p.ml + 2 * (s * rows + row));
+  float top = ml.x;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+  if (lane == 0) red[0][wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRowWaves; ++k) top = fmaxf(top, red[0][k]);
+  const float base = top == -INFINITY ? 0.f : top;
+  const float w = ml.y == 0.f ? 0.f : exp2_fast(ml.x - base);
+  if (s < p.nsplit) weight[s] = ml.y == 0.f ? -1.f : w;  // -1: no keys, its O was not written
+  float l = ml.y == 0.f ? 0.f : ml.y * w;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) l += __shfl_xor(l, k);
+  if (lane == 0) red[1][wave] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int k = 0; k < kRowWaves; ++k) l += red[1][k];
+  const int col = 4 * lane;
+  f32x4 o = {};
+  if (col < p.c.d) {
+#pragma unroll 4
+    for (int k = wave; k < p.nsplit; k += kRowWaves) {
+      const float f = weight[k];
+      if (f >= 0.f || f != f) o += *reinterpret_cast<const f32x4*>(p.opart + (k * rows + row) * p.c.d + col) * f;
+    }
+  }
+  part[wave][lane] = o;
+  __syncthreads();
+  if (wave != 0 || col >= p.c.d) return;
+#pragma unroll
+  for (int k = 1; k < kRowWaves; ++k) o += part[k][lane];
+  store_row4<T>(p, tok, head, col, o, l);
+}
+
+template <typename T> hipError_t combine(const PagedParams& p, hipStream_t stream) {
+  const long rows = (long)p.tokens * p.heads;
+  if (p.nsplit > 8) {
+    static_assert(kMostSplits <= 64 * kRowWaves, "a thread for each split");
+    hipLaunchKernelGGL(paged_combine_row_kernel<T>, dim3((unsigned)rows), dim3(64 * kRowWaves), 0, stream, p);
+  } else {
+    const long threads = rows * (p.c.d / 4);
+    hipLaunchKernelGGL(paged_combine_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t paged_combine(int dtype, const PagedParams& p, hipStream_t stream) {
+  return dtype == kF32 ? combine<float>(p, stream) : dtype == kF16 ? combine<f16>(p, stream) : combine<bf16>(p, stream);
+}
+
+}  // namespace samhip

@@ -672,9 +672,9 @@ int check_pool(const char* what, const void* k_pages, const void* v_pages, const
   if ((long)table_width * page_size >= 1L << 30)
     return fail(SAM_HIP_EUNSUPPORTED, "%s: a table of %d pages of %d tokens is beyond 2^30 tokens", what, table_width,
                 page_size);
-  // rows of the pool below 2^47 / d bytes: their byte offsets stay far inside 64 bits
-  if ((long)pages * kv_heads > (1L << 40) / page_size)
-    return fail(SAM_HIP_EUNSUPPORTED, "%s: the pool has more than 2^40 rows", what);
+  if ((long)pages * kv_heads >= (1L << 31) / page_size)  // the kernels count rows in 32 bits, their bytes in 64
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: the pool has 2^31 rows or more (pages=%d heads=%d page=%d)", what, pages,
+                kv_heads, page_size);
   if (!aligned16(k_pages) || !aligned16(v_pages))
     return fail(SAM_HIP_EUNSUPPORTED, "%s: the pages must be 16-byte aligned", what);
   *c = samhip::PagedKv{};

@@ -125,7 +125,8 @@ def test_rows_that_see_nothing_are_zero(hip, dtype, fp8, d):
 @pytest.mark.parametrize("chunk", [3, 60, 200])
 def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(hip, dtype, fp8, d, chunk):
     """NaN and infinities in keys and values: past the end and in pages of nobody they reach no row; at a position, the
-    rows behind it alone (in f16, infinite values of a row that sees them; in 8 bits, NaN)."""
+    rows behind it alone, in the value's own column. There an infinity stays one in f32 and f16; in bf16, where P is a
+    sum of two terms of either sign (or one of them 0), it may become NaN, as inf - inf and 0 * inf are."""
     lens = [chunk + 90]
     c = Case([chunk], lens, 1, 2, d, 16, dtype, fp8)
     clean = c.run(hip, True)
@@ -161,7 +162,12 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(hip, dtype,
             if into == "v":
                 assert torch.isfinite(got[..., :5]).all() and torch.isfinite(got[..., 6:]).all()
                 seen = got[row:, :, 5]
-                assert torch.isnan(seen).all() if x != x else (seen == x).all()
+                if x != x:
+                    assert torch.isnan(seen).all()
+                elif dtype == "bf16":
+                    assert not torch.isfinite(seen).any()
+                else:
+                    assert (seen == x).all()
             elif x != x:
                 assert torch.isnan(got[row:]).all()
 
