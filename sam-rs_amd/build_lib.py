@@ -33,7 +33,7 @@ SOURCES = [
     "qkv_split.hip",
     "flash_attn.hip", "flash_attn_d256.hip", "flash_attn_f32.hip", "flash_noalloc.hip",
     "rope.hip", "qkv_rope.hip",
-    "rope_axes.hip", "kv_cache.hip", "paged_attn.hip", "paged_attn_f32.hip", "paged_attn_few.hip",
+    "rope_axes.hip", "kv_cache.hip", "paged_attn.hip", "paged_attn_f32.hip", "paged_attn_few.hip", "paged_attn_many.hip",
     "paged_combine.hip",
     "sam_hip_abi.cpp",
 ]

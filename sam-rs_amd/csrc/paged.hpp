@@ -75,7 +75,7 @@ struct PagedParams {
 
 // How a call runs: the kernel's rows per tile, the row tiles and key splits of its grid, its workspace.
 struct PagedPlan {
-  int rows, rtiles, nsplit, per;
+  int many, rows, rtiles, nsplit, per;
   long part_bytes, total;
 };
 PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
@@ -83,6 +83,7 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
 hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const PagedPlan& plan, hipStream_t stream);
 hipError_t paged_f32(int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
 hipError_t paged_few(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
+hipError_t paged_many(int dtype, int cache_dtype, const PagedParams& p, hipStream_t stream);
 hipError_t paged_combine(int dtype, const PagedParams& p, hipStream_t stream);
 
 hipError_t kv_write(int dtype, int cache_dtype, const void* k, const void* v, const long* sk, const long* sv,
@@ -95,11 +96,48 @@ hipError_t rope_axes(int dtype, const void* x, const int* pos, const double* fre
 
 // ------------------------------------------------------------------------------------------ device helpers
 
-// Workgroup i runs on XCD i % 8; give each XCD a contiguous range of the linear work index, so that the workgroups
-// that read one head's keys share an L2.
-__device__ __forceinline__ int paged_xcd_block(int i, int total) {
-  const int per = total >> 3, rem = total & 7, x = i & 7, j = i >> 3;
-  return x * per + (x < rem ? x : rem) + j;
+// Two codes (the low or the high half of w) times a power of two, as a pair of T.
+template <typename T, bool HI> __device__ __forceinline__ unsigned decode2(unsigned w, float s);
+template <> __device__ __forceinline__ unsigned decode2<f16, false>(unsigned w, float s) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, s, false));
+}
+template <> __device__ __forceinline__ unsigned decode2<f16, true>(unsigned w, float s) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, s, true));
+}
+template <> __device__ __forceinline__ unsigned decode2<bf16, false>(unsigned w, float s) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, false));
+}
+template <> __device__ __forceinline__ unsigned decode2<bf16, true>(unsigned w, float s) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, true));
+}
+
+// Bits 15 and 31 of the result say which 16-bit halves of w are infinite or NaN: their exponent bits, all ones, carry.
+template <typename T> __device__ __forceinline__ unsigned not_finite2(unsigned w) {
+  constexpr unsigned e = __is_same(T, f16) ? 0x7c00u : 0x7f80u, one = __is_same(T, f16) ? 0x0400u : 0x0080u;
+  return ((w & (e | e << 16)) + (one | one << 16)) & 0x80008000u;
+}
+// w without those halves.
+__device__ __forceinline__ unsigned without2(unsigned w, unsigned bad) {
+  return w & ~((bad >> 15) * 0xffffu);
+}
+
+// Four values of a cache row in T (each rounded to it), as f32: those that are not finite, and 0 for the others.
+template <typename T, typename C> __device__ __forceinline__ f32x4 only_not_finite4(const C* p, float s) {
+  u32x2 x;
+  if constexpr (__is_same(C, e4m3)) {
+    const unsigned w = *reinterpret_cast<const unsigned*>(p);
+    x = u32x2{decode2<T, false>(w, s), decode2<T, true>(w, s)};
+  } else {
+    x = *reinterpret_cast<const u32x2*>(p);
+  }
+  const typename Vec<T>::x4 v = __builtin_bit_cast(typename Vec<T>::x4, x);
+  f32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float f = to_f32(v[i]);
+    r[i] = fabsf(f) < INFINITY ? 0.f : f;
+  }
+  return r;
 }
 
 // One sequence's new tokens [s0, s0 + lq), keys, and the row tile this workgroup starts with.
@@ -108,13 +146,16 @@ struct PagedWork {
   int s0, lq, len;
 };
 __device__ __forceinline__ PagedWork paged_work(const PagedParams& p) {
-  const int lin = __builtin_amdgcn_readfirstlane(paged_xcd_block(blockIdx.x, gridDim.x));
+  // Workgroup i runs on XCD i % 8. The (sequence, key head) comes first, then the key split, the row tile last: a
+  // multiple of 8 of the first two leaves each head's keys to one XCD's L2, and sequences of different lengths, whose
+  // heads are neighbours, spread over all XCDs.
+  const int units = p.c.heads * p.c.batch, lin = blockIdx.x, unit = lin % units;
   PagedWork w;
-  w.tile = lin % p.rtiles;
-  w.split = lin / p.rtiles % p.nsplit;
-  const int hb = lin / (p.rtiles * p.nsplit);
-  w.head = hb % p.c.heads;
-  w.b = hb / p.c.heads;
+  w.split = lin / units % p.nsplit;
+  w.tile = lin / (units * p.nsplit);
+  if (p.causal) w.tile = p.rtiles - 1 - w.tile;  // the tiles with most keys first
+  w.head = unit % p.c.heads;
+  w.b = unit / p.c.heads;
   w.s0 = max(0, min(p.c.starts[w.b], p.tokens));
   w.lq = max(0, min(p.c.starts[w.b + 1], p.tokens) - w.s0);
   w.len = paged_len(p.c, w.b);

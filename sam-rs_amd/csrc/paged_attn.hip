@@ -7,16 +7,22 @@ namespace samhip {
 
 PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
                      int max_len, int cus) {
-  (void)dtype;
   (void)cache_dtype;
   PagedPlan plan = {};
   const long group = heads / kv_heads, rows = (long)std::max(max_q, 1) * group;
-  plan.rows = rows <= 16 || d > 128 ? 16 : 32;
+  plan.many = dtype != kF32 && rows > 32;
+  plan.rows = plan.many ? 128 : rows <= 16 || d > 128 ? 16 : 32;
   plan.rtiles = (int)((rows + plan.rows - 1) / plan.rows);
-  // four workgroups a CU, if every split then has two blocks of 32 keys for each of its four waves
   const long base = (long)plan.rtiles * kv_heads * batch;
-  const long want = (4L * cus + base - 1) / base, most = ((long)max_len + 255) / 256;
-  plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
+  if (plan.many) {
+    // as many workgroups as run at once (two a CU, one past head dim 128), with four tiles of 64 keys a split at least
+    const long slots = (d > 128 ? 1L : 2L) * cus, most = ((long)max_len + 255) / 256;
+    plan.nsplit = (int)std::max(1L, std::min(std::min(slots / base, most), 64L));
+  } else {
+    // four workgroups a CU, if every split then has two blocks of 32 keys for each of its four waves
+    const long want = (4L * cus + base - 1) / base, most = ((long)max_len + 255) / 256;
+    plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
+  }
   const long blocks = ((long)max_len + 31) / 32;
   plan.per = (int)std::min((blocks + plan.nsplit - 1) / plan.nsplit, 1L << 26);
   if (plan.nsplit > 1) {
@@ -31,6 +37,7 @@ hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const Page
   p.nsplit = plan.nsplit;
   p.per = plan.per;
   hipError_t e = dtype == kF32 ? paged_f32(cache_dtype, p, plan.rows, stream)
+                 : plan.many   ? paged_many(dtype, cache_dtype, p, stream)
                                : paged_few(dtype, cache_dtype, p, plan.rows, stream);
   if (e == hipSuccess && p.nsplit > 1) e = paged_combine(dtype, p, stream);
   return e;

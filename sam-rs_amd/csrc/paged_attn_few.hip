@@ -14,8 +14,6 @@
 // own rounding).
 //
 // The four waves of a workgroup join at its end, the key ranges of a sequence in paged_combine_kernel.
-#include <type_traits>
-
 #include "lds_dma.hpp"
 #include "paged.hpp"
 
@@ -36,24 +34,6 @@ template <> struct Raw<16> {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
-// Two codes (the low or the high half of w) times a power of two, as a pair of T.
-template <typename T, bool HI> __device__ __forceinline__ unsigned decode2(unsigned w, float s);
-template <> __device__ __forceinline__ unsigned decode2<f16, false>(unsigned w, float s) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, s, false));
-}
-template <> __device__ __forceinline__ unsigned decode2<f16, true>(unsigned w, float s) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, s, true));
-}
-template <> __device__ __forceinline__ unsigned decode2<bf16, false>(unsigned w, float s) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, false));
-}
-template <> __device__ __forceinline__ unsigned decode2<bf16, true>(unsigned w, float s) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s, true));
-}
-
-// The exponent bits that infinities and NaN have.
-template <typename T> constexpr unsigned kInfBits = __is_same(T, f16) ? 0x7c00u : 0x7f80u;
 
 template <typename T, typename C, int DP, int RB>
 __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(PagedParams p) {
@@ -164,30 +144,26 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
         }
       }
       // s[rb][i][e]: key key0 + 16 i + 4 g + e, row 16 rb + n
-      // softmax and P V: blocks that every row sees whole are nearly all of them, and need no masks
-      auto weigh = [&](auto masked) {
-      constexpr bool part = decltype(masked)::value;
+      if (blk + 4 < b1) load_k(next);  // in flight while this block's V is weighed
+      const bool part = key0 + 32 > least || there != 0xffffffffu;
       X8 b[RB], blo[RB];
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         float top = -INFINITY;
-        if constexpr (part) {
+        if (part) {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int kk = 16 * i + 4 * g + e;
-              const bool see = key0 + kk < limit[rb] && (there >> kk & 1);
-              s[rb][i][e] = see ? s[rb][i][e] : -INFINITY;
+              s[rb][i][e] = key0 + kk < limit[rb] && (there >> kk & 1) ? s[rb][i][e] : -INFINITY;
             }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = max_nc(top, s[rb][i][e]);
-        top = max_over_rows16(top);
-        const float mt = top == -INFINITY ? -INFINITY : top * p.sc;
-        const float m_new = fmaxf(m[rb], mt);
+        const float m_new = fmaxf(m[rb], max_over_rows16(top) * p.sc);
         const float base = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = exp2_fast(m[rb] - base);
         m[rb] = m_new;
@@ -197,9 +173,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
         float pv[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float x0 = s[rb][j >> 2][j & 3];
-          pv[j] = exp2_fast(fmaf(x0, p.sc, -base));
-          if constexpr (part) pv[j] = x0 == -INFINITY ? 0.f : pv[j];
+          pv[j] = exp2_fast(fmaf(s[rb][j >> 2][j & 3], p.sc, -base));
         }
         if constexpr (kSplitP) {
 #pragma unroll
@@ -212,6 +186,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
             l[rb] = __builtin_amdgcn_fdot2(f16x2{b[rb][j], b[rb][j + 1]}, f16x2{(f16)1.f, (f16)1.f}, l[rb], false);
         }
       }
+      unsigned odd = 0;
       float vs[8];
       if constexpr (kCoded) {
 #pragma unroll
@@ -237,59 +212,22 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
 #pragma unroll
             for (int h = 0; h < CW / 2; ++h) v[j][h] = vx[j][q][h];
           }
-          if constexpr (part) {  // rows that are not there hold anything
+          if (part) {  // rows that are not there hold anything; values that are not finite go apart
             const bool ok = there >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1;
 #pragma unroll
-            for (int h = 0; h < CW / 2; ++h) v[j][h] = ok ? v[j][h] : 0u;
-          }
-        }
-        auto column = [&](int c) {  // the A operand of column c
-          u32x4 a;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)  // keys 2 j and 2 j + 1
-            a[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
-          return a;
-        };
-        if constexpr (part) {
-          bool odd = false;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
             for (int h = 0; h < CW / 2; ++h) {
-              constexpr unsigned e = kInfBits<T>;
-              odd |= (v[j][h] & e) == e || (v[j][h] >> 16 & e) == e;
+              const unsigned bad = not_finite2<T>(v[j][h]);
+              v[j][h] = ok ? without2(v[j][h], bad) : 0u;
+              odd |= ok ? bad : 0u;
             }
-          if (wave_any(odd)) {
-            // A value that is not finite must not reach the rows that do not see its key (0 * inf = NaN): each number of
-            // keys that some row sees is taken by itself, over the rows that see so many
-            for (int seen = max(least - key0, 1); seen <= min(most - key0, 32); ++seen) {
-              u32x4 keep;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int kk = 16 * (j >> 1) + 4 * g + 2 * (j & 1);
-                keep[j] = (kk < seen ? 0xffffu : 0u) | (kk + 1 < seen ? 0xffff0000u : 0u);
-              }
-#pragma unroll
-              for (int c = 0; c < CW; ++c) {
-                const u32x4 a = column(c) & keep;
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                  f32x4& acc = o[rb][q * CW + c];
-                  f32x4 t = mma16(__builtin_bit_cast(X8, a), b[rb], acc);
-                  if constexpr (kSplitP) t = mma16(__builtin_bit_cast(X8, a), blo[rb], t);
-                  const bool mine = min(limit[rb] - key0, 32) == seen;
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) acc[k] = mine ? t[k] : acc[k];
-                }
-                __builtin_amdgcn_sched_barrier(0);
-              }
-            }
-            continue;
           }
         }
 #pragma unroll
         for (int c = 0; c < CW; ++c) {
-          const u32x4 a = column(c);
+          u32x4 a;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // keys 2 j and 2 j + 1 of column c
+            a[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
             f32x4& acc = o[rb][q * CW + c];
@@ -298,13 +236,29 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
           }
         }
       }
-      };
-      if (key0 + 32 > least || there != 0xffffffffu) {
-        weigh(std::true_type{});
-        if (blk + 4 < b1) load_k(next);
-      } else {
-        if (blk + 4 < b1) load_k(next);  // in flight while this block's V is weighed
-        weigh(std::false_type{});
+      if (wave_any(odd != 0)) {
+        // A value that is not finite must not reach the rows that do not see its key (0 * inf = NaN): it was taken out
+        // above, and the rows that see it add it here
+        for (int kk = 0; kk < 32; ++kk) {
+          if (!(there >> kk & 1)) continue;
+          const int kr = __shfl(row, kk);
+          const float s1 = kCoded ? pow2_of(p.c.vs[kr]) : 1.f;
+#pragma unroll
+          for (int q = 0; q < NV; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int c = 0; c < CW; c += 4) {
+                const int col = CW * (16 * q + 4 * g + e) + c;
+                if (col < d) {
+                  const f32x4 x = only_not_finite4<T>(vp + (long)kr * d + col, s1);
+#pragma unroll
+                  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[rb][q * CW + c + i][e] += key0 + kk < limit[rb] ? x[i] : 0.f;
+                }
+              }
+        }
       }
       if (blk + 4 < b1) load_v(next);
       row = next;

@@ -1,0 +1,322 @@
+// Paged attention on gfx950 for many rows a key head (a prompt's chunk, a frame's queries), f16 / bf16 queries over pages
+// of their own type or of e4m3.
+//
+// Work: a workgroup of four waves takes 128 rows (new token x query head of one key head) and one range of keys; a wave
+// owns 32 rows. Tiles of 64 keys go from their pages through registers into LDS, the next tile's loads in flight while
+// this one is worked on (e4m3 codes become 16-bit values with their row's scale on the way, once per workgroup), two
+// buffers each, one barrier a tile. A lane looks one key of the tile up; the loads take their rows from that lane.
+//   S^T = K Q^T on v_mfma_f32_32x32x16 with Q in registers: a lane holds one row's scores of 32 keys, so that softmax
+//   needs one exchange between lane halves. O^T += V^T P^T takes the scores' registers as its B operand under a fixed
+//   permutation of keys that the transposing reads of V (ds_read_b64_tr_b16) follow.
+//
+// A value that is not finite must not reach the rows that do not see its key (0 * inf = NaN). Tiles that some row does
+// not see whole are looked over as they are stored: such values go into LDS as 0, and the rows that see one add it
+// afterwards.
+//
+// Softmax statistics and sums are f32; the running maximum moves only when a tile passes it by 8 (in log2), so that O is
+// rarely rescaled. f16 P is rounded to f16 and summed as rounded; bf16 P goes as hi + lo.
+#include <type_traits>
+
+#include "lds_dma.hpp"
+#include "paged.hpp"
+
+namespace samhip {
+
+namespace {
+
+constexpr float kSlack = 8.f;
+
+template <int DP> struct ManyGeom {
+  static constexpr int KS = DP / 16, MBO = DP / 32;
+  static constexpr int KSTR = DP + 8;                     // K row stride (elements): rows 16 bytes apart mod 128
+  static constexpr int VSTR = DP + (MBO == 3 ? 0 : 32);   // 16 or 48 banks mod 64 for the transposing reads
+  static constexpr int KBUF = 64 * KSTR, VBUF = 64 * VSTR;
+  static constexpr int LDS = 2 * (KBUF + VBUF) * 2;
+  static constexpr int CPR = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // threads to a row, 8 columns each
+  static constexpr int RS = 256 / CPR, PT = 64 / RS;      // rows a round, rounds a tile
+};
+
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(PagedParams p) {
+  typedef ManyGeom<DP> G;
+  typedef typename Vec<T>::x8 X8;
+  constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
+  constexpr int KS = G::KS, MBO = G::MBO, KSTR = G::KSTR, VSTR = G::VSTR, CPR = G::CPR, RS = G::RS, PT = G::PT;
+  __shared__ int odd[2];  // the tile in each buffer that was stored without values that are not finite
+  typedef typename std::conditional<kCoded, u32x2, u32x4>::type Raw;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  T* ks_base = reinterpret_cast<T*>(smem);
+  T* vs_base = ks_base + 2 * G::KBUF;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
+  const int d = p.c.d;
+  if (p.zero_rest) paged_zero_rest<T>(p);
+  const PagedWork w = paged_work(p);
+  const int rows = w.lq * p.group;
+  const C* kp = reinterpret_cast<const C*>(p.c.k);
+  const C* vp = reinterpret_cast<const C*>(p.c.v);
+  const int srow = tid / CPR, scol = tid % CPR * 8;  // this thread's first row of a tile, and its columns
+  const bool sin = scol < d;
+
+  if (d < DP) {  // K's columns past d meet zeros of q, so they must be finite; V's only feed columns that are dropped
+    for (int c = tid; c < 2 * 64 * (DP / 8); c += 256) {
+      const int r = c / (DP / 8), c8 = c % (DP / 8) * 8;
+      if (c8 >= d) *reinterpret_cast<u32x4*>(ks_base + (r >> 6) * G::KBUF + (r & 63) * KSTR + c8) = u32x4{};
+    }
+  }
+
+  for (int rt = w.tile; (long)rt * 128 < rows; rt += p.rtiles) {
+    auto keys_of = [&](int r) {  // keys that row r sees
+      const int t = (int)divide_magic(r, p.gmagic, p.gshift);
+      return p.causal ? max(0, min(w.len, w.len - w.lq + t + 1)) : w.len;
+    };
+    const int most = keys_of(min((rt + 1) * 128, rows) - 1);
+    const int least = keys_of(rt * 128);
+    const int wfirst = rt * 128 + 32 * wave;
+    const bool rows_here = wfirst < rows;
+    const int wleast = rows_here ? keys_of(wfirst) : 0, wmost = rows_here ? keys_of(min(wfirst + 32, rows) - 1) : 0;
+    // blocks of 32 keys, as the other kernels count them; a tile is two
+    const int tiles = (most + 63) >> 6, per = max((p.per + 1) >> 1, (tiles + p.nsplit - 1) / p.nsplit);
+    const int t0 = min(tiles, w.split * per), t1 = min(tiles, t0 + per);
+
+    const int r = min(wfirst + n, rows - 1);
+    const int tk = (int)divide_magic(r, p.gmagic, p.gshift);
+    const int limit = keys_of(r);
+    const T* qr = reinterpret_cast<const T*>(p.q) + (w.s0 + tk) * p.sq[0] + (w.head * p.group + r - tk * p.group) * p.sq[1];
+
+    Raw reg[PT];  // the chunks of K or V on their way, and in 8 bits their rows' scales
+    float sreg[PT];
+    // lane l's own key of a tile; a key that is not there reads row 0 and is masked (K) or cleared (V)
+    auto look = [&](int t) { return t < t1 ? paged_row(p.c, w.b, w.head, 64 * t + lane, most) : -1; };
+    auto load = [&](const C* base, const unsigned char* scales, int own) {
+      float mine = 1.f;
+      if constexpr (kCoded) mine = pow2_of(scales[max(own, 0)]);
+#pragma unroll
+      for (int u = 0; u < PT; ++u) {
+        const long row = __shfl(own, srow + u * RS);
+        reg[u] = *reinterpret_cast<const Raw*>(base + max(row, 0l) * d + min(scol, d - 8));
+        if constexpr (kCoded) sreg[u] = __shfl(mine, srow + u * RS);
+      }
+    };
+    auto chunk = [&](int u) {
+      if constexpr (kCoded)
+        return u32x4{decode2<T, false>(reg[u][0], sreg[u]), decode2<T, true>(reg[u][0], sreg[u]),
+                     decode2<T, false>(reg[u][1], sreg[u]), decode2<T, true>(reg[u][1], sreg[u])};
+      else
+        return reg[u];
+    };
+    auto load_k = [&](int own) { load(kp, p.c.ks, own); };
+    auto load_v = [&](int own) { load(vp, p.c.vs, own); };
+    auto store_k = [&](int buf) {
+#pragma unroll
+      for (int u = 0; u < PT; ++u)
+        if (sin) *reinterpret_cast<u32x4*>(ks_base + buf * G::KBUF + (srow + u * RS) * KSTR + scol) = chunk(u);
+    };
+    auto whole = [&](int t, unsigned long there) { return 64 * t + 64 <= least && there == ~0ul; };
+    auto store_v = [&](int t, unsigned long there, int buf) {
+      const bool look_over = !whole(t, there);
+#pragma unroll
+      for (int u = 0; u < PT; ++u) {
+        const int row = srow + u * RS;
+        u32x4 x = chunk(u);
+        if (look_over) {
+          unsigned any = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const unsigned bad = not_finite2<T>(x[i]);
+            x[i] = there >> row & 1 ? without2(x[i], bad) : 0u;
+            any |= bad;
+          }
+          if (any && sin && (there >> row & 1)) odd[buf] = t;
+        }
+        if (sin) *reinterpret_cast<u32x4*>(vs_base + buf * G::VBUF + row * VSTR + scol) = x;
+      }
+    };
+
+    int own = look(t0), next = look(t0 + 1);
+    if (tid < 2) odd[tid] = -1;
+    if (t0 < t1) load_k(own);
+    X8 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int c = 16 * s + 8 * hh;
+      qf[s] = c < d ? *reinterpret_cast<const X8*>(qr + c) : X8{};
+    }
+    unsigned long there = __builtin_amdgcn_ballot_w64(own >= 0);
+    __syncthreads();
+    if (t0 < t1) {
+      store_k(0);
+      load_v(own);
+      store_v(t0, there, 0);
+    }
+    __syncthreads();
+
+    // K (A operand of S^T): row 32 mb + n, columns 16 k + 8 hh ..
+    const int koff = n * KSTR + 8 * hh;
+    // V^T (A operand of O^T): the lane's transposing reads start at key 4 (g >> 1) + gi / 4, column 16 (g & 1) + 4 (gi & 3)
+    const int voff = (4 * (g >> 1) + (gi >> 2)) * VSTR + 16 * (g & 1) + 4 * (gi & 3);
+    const float sc = p.sc;
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[MBO];
+#pragma unroll
+    for (int ob = 0; ob < MBO; ++ob) o[ob] = f32x16{};
+
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1, key0 = 64 * t;
+      const unsigned long coming = __builtin_amdgcn_ballot_w64(next >= 0);
+      const bool more = t + 1 < t1;
+      const bool here = key0 < wmost;
+      if (more) load_k(next);
+      if (here) {
+        const T* kb = ks_base + buf * G::KBUF + koff;
+        const T* vb = vs_base + buf * G::VBUF + voff;
+        f32x16 s[2];
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            s[mb] = mma32(*reinterpret_cast<const X8*>(kb + 32 * mb * KSTR + 16 * k), qf[k], k == 0 ? f32x16{} : s[mb]);
+        auto fragment = [&](int u, int ob) {  // keys 16 u + 8 (j / 4) + 4 hh + j % 4 of columns 32 ob ..
+          const T* a = vb + 16 * u * VSTR + 32 * ob;
+          return join8<T>(lds_read_tr16(a), lds_read_tr16(a + 8 * VSTR));
+        };
+        if (key0 + 64 > wleast || there != ~0ul) {
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int kk = 32 * mb + 8 * (e >> 2) + 4 * hh + (e & 3);
+              s[mb][e] = key0 + kk < limit && (there >> kk & 1) ? s[mb][e] : -INFINITY;
+            }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = max_nc(top, s[mb][e]);
+        top = max_with_partner32(top) * sc;
+        if (wave_any(top > m + kSlack)) {
+          const float mn = fmaxf(m, top), alpha = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
+          l *= alpha;
+#pragma unroll
+          for (int ob = 0; ob < MBO; ++ob) o[ob] *= alpha;
+          m = mn;
+        }
+        const float c = m == -INFINITY ? 0.f : -m;
+        X8 b[4], blo[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float pv[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pv[j] = exp2_fast(fmaf(s[u >> 1][8 * (u & 1) + j], sc, c));
+          if constexpr (kSplitP) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) l += pv[j];
+            split_hi_lo(pv, b[u], blo[u]);
+          } else {
+            b[u] = pack8(pv, (X8*)nullptr);
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+              l = __builtin_amdgcn_fdot2(h2{b[u][j], b[u][j + 1]}, h2{(f16)1.f, (f16)1.f}, l, false);
+          }
+        }
+        if (more) {  // K(t+1) makes room for V(t+1), which has the product's time to arrive
+          store_k(buf ^ 1);
+          load_v(next);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int ob = 0; ob < MBO; ++ob) {
+            const X8 a = fragment(u, ob);
+            o[ob] = mma32(a, b[u], o[ob]);
+            if constexpr (kSplitP) o[ob] = mma32(a, blo[u], o[ob]);
+          }
+        if (!whole(t, there) && odd[buf] == t) {
+          for (int kk = 0; kk < 64; ++kk) {
+            if (!(there >> kk & 1)) continue;
+            const int row = __shfl(own, kk);
+            const float vs = kCoded ? pow2_of(p.c.vs[row]) : 1.f;
+            const bool sees = key0 + kk < limit;
+#pragma unroll
+            for (int ob = 0; ob < MBO; ++ob)
+#pragma unroll
+              for (int a = 0; a < 4; ++a) {
+                const int col = 32 * ob + 8 * a + 4 * hh;
+                if (col < d) {
+                  const f32x4 x = only_not_finite4<T>(vp + (long)row * d + col, vs);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[ob][4 * a + e] += sees ? x[e] : 0.f;
+                }
+              }
+          }
+        }
+      } else if (more) {
+        store_k(buf ^ 1);
+        load_v(next);
+      }
+      if (more) store_v(t + 1, coming, buf ^ 1);
+      own = next;
+      next = look(t + 2);
+      there = coming;
+      __syncthreads();
+    }
+
+    // lane holds O^T[32 ob + 8 a + 4 hh + e][row n] in o[ob][4 a + e]
+    l = sum_with_partner32(l);
+    if (wfirst + n < rows) {
+      const long tok = w.s0 + tk;
+      const int hq = w.head * p.group + (r - tk * p.group);
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is 0
+      const long part = (w.split * (long)p.tokens + tok) * p.heads + hq;
+      auto columns = [&](auto put) {
+#pragma unroll
+        for (int ob = 0; ob < MBO; ++ob)
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+            if (32 * ob + 8 * a + 4 * hh < d)
+              put(32 * ob + 8 * a + 4 * hh, f32x4{o[ob][4 * a], o[ob][4 * a + 1], o[ob][4 * a + 2], o[ob][4 * a + 3]});
+      };
+      if (p.nsplit == 1) {
+        T* to = reinterpret_cast<T*>(p.out) + tok * p.so[0] + hq * p.so[1];
+        columns([&](int col, f32x4 x) {
+          typename Vec<T>::x4 y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(f32_result(x[e] * inv));
+          *reinterpret_cast<typename Vec<T>::x4*>(to + col) = y;
+        });
+      } else if (t0 < t1) {
+        columns([&](int col, f32x4 x) { *reinterpret_cast<f32x4*>(p.opart + part * d + col) = x; });
+      }
+      if (p.nsplit > 1 && hh == 0) *reinterpret_cast<float2*>(p.ml + 2 * part) = float2{m, l};
+    }
+    __syncthreads();  // the next rows' first tile replaces buffer 0
+  }
+}
+
+template <typename T, typename C, int DP> hipError_t launch_many(const PagedParams& p, hipStream_t stream) {
+  auto kern = paged_many_kernel<T, C, DP>;
+  static std::atomic<unsigned long long> done;  // opt-in to more than 64 KB of dynamic LDS
+  if (const hipError_t e = lds_opt_in(done, (const void*)kern, ManyGeom<DP>::LDS); e != hipSuccess) return e;
+  const long blocks = (long)p.rtiles * p.nsplit * p.c.heads * p.c.batch;
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), ManyGeom<DP>::LDS, stream, p);
+  return hipGetLastError();
+}
+template <typename T, typename C> hipError_t by_size(const PagedParams& p, hipStream_t stream) {
+  const int d = p.c.d;
+  return d <= 64 ? launch_many<T, C, 64>(p, stream)
+                 : d <= 96 ? launch_many<T, C, 96>(p, stream)
+                           : d <= 128 ? launch_many<T, C, 128>(p, stream) : launch_many<T, C, 256>(p, stream);
+}
+
+}  // namespace
+
+hipError_t paged_many(int dtype, int cache_dtype, const PagedParams& p, hipStream_t stream) {
+  if (dtype == kF16)
+    return cache_dtype == kE4M3 ? by_size<f16, e4m3>(p, stream) : by_size<f16, f16>(p, stream);
+  return cache_dtype == kE4M3 ? by_size<bf16, e4m3>(p, stream) : by_size<bf16, bf16>(p, stream);
+}
+
+}  // namespace samhip

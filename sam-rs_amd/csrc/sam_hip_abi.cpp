@@ -811,7 +811,8 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
   p.heads = heads;
   p.group = heads / kv_heads;
   samhip::division_magic(p.group, &p.gmagic, &p.gshift);
-  p.sc = scale * 1.4426950408889634f;
+  // a scale of 0 as one that leaves every finite score 0 and a masked one (-inf) masked
+  p.sc = scale * 1.4426950408889634f > 1e-37f ? scale * 1.4426950408889634f : 1e-37f;
   p.causal = causal != 0;
   p.zero_rest = zero_rest != 0;
   p.opart = reinterpret_cast<float*>(workspace);

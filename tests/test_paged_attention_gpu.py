@@ -173,6 +173,24 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(hip, dtype,
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("chunk", [4, 90])
+def test_nan_scores_stay_with_their_rows_from_the_first_key_on(hip, dtype, d, chunk):
+    """A NaN in the first key makes every row of its head NaN, also those whose later tiles are clean, and no row of the
+    other head; a NaN in a query makes that row NaN alone."""
+    c = Case([chunk], [300], 2, 1, d, 16, dtype, False)
+    clean = c.run(hip, True)
+    c.q[chunk // 2, 0, 3] = float("nan")
+    got = c.run(hip, True)
+    assert torch.isnan(got[chunk // 2, 0]).all()
+    got[chunk // 2, 0] = clean[chunk // 2, 0]
+    assert torch.equal(got, clean)
+    c.k[int(c.table[0, 0]), 1, 0, 0] = float("nan")
+    got = c.run(hip, True)
+    assert torch.isnan(got[:, 1]).all() and torch.equal(got[0, 0], clean[0, 0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("scale", [0.0, 1.0, 0.02])
 def test_scales_and_large_scores(hip, dtype, scale):
     c = Case([50], [200], 2, 2, 64, 16, dtype, False, spread=2.0)
