@@ -619,29 +619,27 @@ def rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch
 _E4M3 = 3  # SAM_HIP_E4M3
 
 
-def _one_device(what: str, *ts):
+# The calls below are made once a layer and token, where the host's time counts: an index in place of a device object
+# (0.1 against 0.2 us), no views or stride arrays for contiguous operands (1.5 and 0.3 us each), empty_like (1.2 us; empty
+# 3.5). rope_axes, kv_write, kv_read and paged_attention took the host 12, 10, 13 and 18 us with, HOSTTIMES without.
+
+
+def _device_of(what: str, *ts) -> int:
+    """The index of the one device that every tensor (None aside) lives on."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and not t.is_cuda:
-            raise SamHipError("sam-rs HIP kernels need device tensors")
-        if t is not None and t.device != ts[0].device:
-            raise SamHipError(f"{what}: all operands must be on one device: {t.device} vs {ts[0].device}")
+        if t is not None and t.get_device() != dev:
+            dev = -1
+    if dev < 0:
+        for t in ts:
+            if t is not None and not t.is_cuda:
+                raise SamHipError("sam-rs HIP kernels need device tensors")
+        raise SamHipError(f"{what}: all operands must be on one device, got {[str(t.device) for t in ts if t is not None]}")
+    return dev
 
 
-def _here(t: torch.Tensor) -> bool:
-    return t.device.index == (torch.cuda.current_device() if _raw_device is None else _raw_device())
-
-
-def _on_its_device(fn):
-    """Runs fn with its first tensor's device as the current one, on that device's current stream."""
-
-    @functools.wraps(fn)
-    def run(t, *args, **kwargs):
-        if not t.is_cuda or _here(t):
-            return fn(t, *args, **kwargs)
-        with torch.cuda.device(t.device):
-            return fn(t, *args, **kwargs)
-
-    return run
+def _is_current(dev: int) -> bool:
+    return dev == (torch.cuda.current_device() if _raw_device is None else _raw_device())
 
 
 def rope_freqs(sections, theta: float = 10000.0, scale: float = 1.0, device="cuda"):
@@ -656,91 +654,113 @@ def rope_freqs(sections, theta: float = 10000.0, scale: float = 1.0, device="cud
     return (torch.tensor(freqs, dtype=torch.float64, device=device), torch.tensor(axes, dtype=torch.int32, device=device))
 
 
-@_on_its_device
 def rope_axes(x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, axes: torch.Tensor, pairs: str = "adjacent",
               inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotary positions over several axes: x [B, L, H, D] or [T, H, D], pos int32 [B, L, A] (or anything that broadcasts
     to it; [T, A]); pair i turns by pos[..., axes[i]] * freqs[i] (freqs f64, axes int32, [P] with 2 P <= D; rope_freqs
     makes them). pairs "adjacent" turns (x[2i], x[2i+1]), "halves" (x[i], x[i+P]); columns past 2 P are copied. inverse
     turns back, which is also what a gradient with respect to the result takes to become one with respect to x. out may
-    be x itself."""
-    _one_device("rope_axes", x, pos, freqs, axes, out)
+    be x itself, and must not overlap it otherwise."""
+    dev = _device_of("rope_axes", x, pos, freqs, axes, out)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return rope_axes(x, pos, freqs, axes, pairs, inverse, out)
     dt = _dtype(x)
-    if x.dim() not in (3, 4):
-        raise SamHipError(f"rope_axes: x must be [B, L, H, D] or [T, H, D], got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) == 4:
+        b, l, h, d = shape
+    elif len(shape) == 3:
+        b, (l, h, d) = 1, shape
+    else:
+        raise SamHipError(f"rope_axes: x must be [B, L, H, D] or [T, H, D], got {tuple(shape)}")
     if pairs not in ("adjacent", "halves"):
         raise SamHipError(f'rope_axes: pairs must be "adjacent" or "halves", got {pairs!r}')
     if pos.dtype != torch.int32 or freqs.dtype != torch.float64 or axes.dtype != torch.int32:
         raise SamHipError(f"rope_axes: pos and axes must be int32 and freqs f64, got {pos.dtype}, {axes.dtype}, {freqs.dtype}")
-    if freqs.dim() != 1 or axes.shape != freqs.shape or 2 * freqs.shape[0] > x.shape[-1]:
-        raise SamHipError(f"rope_axes: freqs {tuple(freqs.shape)} and axes {tuple(axes.shape)} must be [P], 2 P <= {x.shape[-1]}")
+    n, at = freqs.shape, pos.shape
+    if len(n) != 1 or axes.shape != n or 2 * n[0] > d:
+        raise SamHipError(f"rope_axes: freqs {tuple(n)} and axes {tuple(axes.shape)} must be [P], 2 P <= {d}")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise SamHipError(f"rope_axes: out must match x (shape {tuple(x.shape)}, {x.dtype}), got {tuple(out.shape)}, {out.dtype}")
-    if x.stride(-1) != 1:
-        if out is x:
-            raise SamHipError("rope_axes: in place, the head dimension must be contiguous")
-        x = x.contiguous()
-    if out.stride(-1) != 1:
-        raise SamHipError("rope_axes: out's head dimension must be contiguous")
-    x4, o4, p3 = (x, out, pos) if x.dim() == 4 else (x.unsqueeze(0), out.unsqueeze(0), pos)
-    b, l, h, d = x4.shape
-    try:
-        p3 = p3.expand(b, l, pos.shape[-1])
-    except RuntimeError as e:
-        raise SamHipError(f"rope_axes: pos {tuple(pos.shape)} does not broadcast to {(b, l)} positions of its axes") from e
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out.shape != shape or out.dtype != x.dtype:
+        raise SamHipError(f"rope_axes: out must match x (shape {tuple(shape)}, {x.dtype}), got {tuple(out.shape)}, {out.dtype}")
+    if not (x.is_contiguous() and out.is_contiguous()):
+        if out.stride(-1) != 1 or _overlaps_itself(out):
+            raise SamHipError("rope_axes: out's head dimension must be contiguous, and its rows apart")
+        if x.stride(-1) != 1:
+            x = x.contiguous()
+        sx, so = (_long3(*t.stride()[:3]) if len(shape) == 4 else _long3(0, t.stride(0), t.stride(1)) for t in (x, out))
+    else:
+        sx = so = None
+    if at[:-1] == shape[:-2] and pos.is_contiguous():
+        sp = None
+    else:
+        try:
+            pos = pos.expand(b, l, at[-1])
+        except (RuntimeError, IndexError) as e:
+            raise SamHipError(f"rope_axes: pos {tuple(at)} does not broadcast to {(b, l)} positions of its axes") from e
+        sp = _long3(*pos.stride())
     if x.numel() == 0:
         return out
     if not (freqs.is_contiguous() and axes.is_contiguous()):
         freqs, axes = freqs.contiguous(), axes.contiguous()
-    _check(load().sam_hip_rope_axes(x4.data_ptr(), p3.data_ptr(), freqs.data_ptr(), axes.data_ptr(), o4.data_ptr(), dt, b,
-                                    l, h, d, freqs.shape[0], pos.shape[-1], _long3(*x4.stride()[:3]),
-                                    _long3(*p3.stride()), _long3(*o4.stride()[:3]), pairs == "halves", bool(inverse),
-                                    _stream()))
+    _check(load().sam_hip_rope_axes(x.data_ptr(), pos.data_ptr(), freqs.data_ptr(), axes.data_ptr(), out.data_ptr(), dt, b,
+                                    l, h, d, n[0], at[-1], sx, sp, so, pairs == "halves", bool(inverse), _stream()))
     return out
 
 
-def _pool(what, k_pages, v_pages, k_scale, v_scale, table, dtype):
-    """(cache dtype code, pages, heads, page_size, d) of a pool, after its checks."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+def _pool(what, k_pages, v_pages, k_scale, v_scale, table, starts, lens, dtype):
+    """(cache dtype code, pages, heads, page_size, d, batch, table width) of a cache, after its checks."""
+    shape, held = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or held != v_pages.dtype:
         raise SamHipError(f"{what}: k_pages and v_pages must be [pages, heads, page_size, d] alike, got "
-                          f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
+                          f"{tuple(shape)} {held} and {tuple(v_pages.shape)} {v_pages.dtype}")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
-    if k_pages.dtype == torch.float8_e4m3fn:
-        code = _E4M3
-        for s in (k_scale, v_scale):
-            if s is None or s.dtype != torch.uint8 or s.shape != k_pages.shape[:3] or not s.is_contiguous():
-                raise SamHipError(f"{what}: an e4m3 cache needs k_scale and v_scale, uint8 {tuple(k_pages.shape[:3])} and contiguous")
-    elif k_pages.dtype == dtype:
+    if held == dtype:
         code = _DTYPES[dtype]
         if k_scale is not None or v_scale is not None:
             raise SamHipError(f"{what}: scales belong to an e4m3 cache, not to {dtype}")
+    elif held == torch.float8_e4m3fn:
+        code = _E4M3
+        for s in (k_scale, v_scale):
+            if s is None or s.dtype != torch.uint8 or s.shape != shape[:3] or not s.is_contiguous():
+                raise SamHipError(f"{what}: an e4m3 cache needs k_scale and v_scale, uint8 {tuple(shape[:3])} and contiguous")
     else:
-        raise SamHipError(f"{what}: the cache must hold {dtype} or torch.float8_e4m3fn, got {k_pages.dtype}")
-    if table.dim() != 2 or table.dtype != torch.int32:
-        raise SamHipError(f"{what}: table must be int32 [batch, width], got {table.dtype} {tuple(table.shape)}")
-    return (code, *k_pages.shape)
+        raise SamHipError(f"{what}: the cache must hold {dtype} or torch.float8_e4m3fn, got {held}")
+    rows = table.shape
+    if len(rows) != 2 or table.dtype != torch.int32:
+        raise SamHipError(f"{what}: table must be int32 [batch, width], got {table.dtype} {tuple(rows)}")
+    b = rows[0]
+    if lens.dtype != torch.int32 or lens.shape != (b,):
+        raise SamHipError(f"{what}: lens must be int32 [{b}], got {lens.dtype} {tuple(lens.shape)}")
+    if starts is not None and (starts.dtype != torch.int32 or starts.shape != (b + 1,)):
+        raise SamHipError(f"{what}: starts must be int32 [{b + 1}], got {starts.dtype} {tuple(starts.shape)}")
+    return (code, *shape, *rows)
 
 
-def _tables(what, table, starts, lens):
-    """The tables, contiguous, after their checks."""
-    for name, t, n in (("starts", starts, table.shape[0] + 1), ("lens", lens, table.shape[0])):
-        if t is not None and (t.dtype != torch.int32 or t.shape != (n,)):
-            raise SamHipError(f"{what}: {name} must be int32 [{n}], got {t.dtype} {tuple(t.shape)}")
-    return (table.contiguous(), None if starts is None else starts.contiguous(), lens.contiguous())
+def _overlaps_itself(t):
+    """Whether a broadcast dimension makes rows of t share memory."""
+    return any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
 
 
-def _token_rows(what, name, t):
-    """A [T, heads, d] operand whose rows can be moved in 16-byte vectors: itself, or a copy."""
+def _plain(t):
+    """An index tensor, contiguous."""
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _token_rows(t):
+    """A [T, heads, d] operand whose rows can be moved in 16-byte vectors (itself, or a copy), and its strides (None:
+    contiguous)."""
+    if t.is_contiguous():
+        return (t, None) if t.data_ptr() % 16 == 0 else (t.clone(), None)
     e = t.element_size()
-    if t.stride(2) != 1 or t.stride(0) * e % 16 or t.stride(1) * e % 16 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s0 * e % 16 or s1 * e % 16 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format), None
+    return t, _long2(s0, s1)
 
 
-@_on_its_device
 def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
              starts: torch.Tensor, lens: torch.Tensor, k_scale: torch.Tensor | None = None,
              v_scale: torch.Tensor | None = None) -> None:
@@ -751,46 +771,60 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: t
     2^(byte - 127) that brings its largest value nearest to 448 from below, its codes round to nearest even, and values
     that are not finite become NaN. Tokens at a negative position, past the table, or whose table entry names no page are
     not stored; two positions in one page slot must not be written by one call."""
-    _one_device("kv_write", k, v, k_pages, v_pages, table, starts, lens, k_scale, v_scale)
+    dev = _device_of("kv_write", k, v, k_pages, v_pages, table, starts, lens, k_scale, v_scale)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return kv_write(k, v, k_pages, v_pages, table, starts, lens, k_scale, v_scale)
     dt = _dtype(k, v)
-    code, pages, heads, page, d = _pool("kv_write", k_pages, v_pages, k_scale, v_scale, table, k.dtype)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (heads, d):
-        raise SamHipError(f"kv_write: k and v must be [T, {heads}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    table, starts, lens = _tables("kv_write", table, starts, lens)
-    if k.shape[0] == 0 or table.shape[0] == 0:
+    code, pages, heads, page, d, b, width = _pool("kv_write", k_pages, v_pages, k_scale, v_scale, table, starts, lens, k.dtype)
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape or shape[1] != heads or shape[2] != d:
+        raise SamHipError(f"kv_write: k and v must be [T, {heads}, {d}], got {tuple(shape)} and {tuple(v.shape)}")
+    if shape[0] == 0 or b == 0 or width == 0:
         return
-    k, v = _token_rows("kv_write", "k", k), _token_rows("kv_write", "v", v)
+    table, starts, lens = _plain(table), _plain(starts), _plain(lens)
+    (k, sk), (v, sv) = _token_rows(k), _token_rows(v)
     _check(load().sam_hip_kv_write(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
                                    _ptr(v_scale), table.data_ptr(), starts.data_ptr(), lens.data_ptr(), dt, code,
-                                   k.shape[0], table.shape[0], pages, heads, page, d, table.shape[1],
-                                   _long2(k.stride(0), k.stride(1)), _long2(v.stride(0), v.stride(1)), _stream()))
+                                   shape[0], b, pages, heads, page, d, width, sk, sv, _stream()))
 
 
-@_on_its_device
 def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int,
             k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
             dtype: torch.dtype | None = None):
     """What the sequences of a cache hold, dense: (k, v) [B, max_len, heads, D], zeros from lens[b] on and where a table
     entry names no page. dtype defaults to the cache's; an e4m3 cache needs one (each value is rounded to it once)."""
-    _one_device("kv_read", k_pages, v_pages, table, lens, k_scale, v_scale)
+    dev = _device_of("kv_read", k_pages, v_pages, table, lens, k_scale, v_scale)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return kv_read(k_pages, v_pages, table, lens, max_len, k_scale, v_scale, dtype)
     dtype = k_pages.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise SamHipError(f"unsupported dtype {dtype} for a sam-rs HIP kernel")
-    code, pages, heads, page, d = _pool("kv_read", k_pages, v_pages, k_scale, v_scale, table, dtype)
-    table, _, lens = _tables("kv_read", table, None, lens)
+    code, pages, heads, page, d, b, width = _pool("kv_read", k_pages, v_pages, k_scale, v_scale, table, None, lens, dtype)
     max_len = int(max_len)
     if max_len < 0:
         raise SamHipError(f"kv_read: max_len must not be negative, got {max_len}")
-    b = table.shape[0]
-    k, v = torch.empty((2, b, max_len, heads, d), dtype=dtype, device=k_pages.device)
-    if k.numel():
+    k, v = k_pages.new_empty((2, b, max_len, heads, d), dtype=dtype).unbind()
+    if width == 0:
+        return k.zero_(), v.zero_()
+    if b and max_len and heads and d:
+        table, lens = _plain(table), _plain(lens)
         _check(load().sam_hip_kv_read(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
                                       _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _DTYPES[dtype], code, b, max_len,
-                                      pages, heads, page, d, table.shape[1], _stream()))
+                                      pages, heads, page, d, width, _stream()))
     return k, v
 
 
-@_on_its_device
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(dev: int, *sizes) -> int:
+    """Bytes that sam_hip_paged_attention needs for calls of these sizes on a device (an error's are not kept)."""
+    n = load().sam_hip_paged_attention_workspace_size(*sizes)
+    if n < 0:
+        raise SamHipError(load().sam_hip_last_error().decode())
+    return n
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                     starts: torch.Tensor, lens: torch.Tensor, k_scale: torch.Tensor | None = None,
                     v_scale: torch.Tensor | None = None, scale: float | None = None, causal: bool = True,
@@ -802,37 +836,42 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     max_q and max_len, the longest chunk and sequence (default: T and what the table can name), shape the launch; a
     call whose sequences exceed them is slower, not wrong. A row that sees no key is 0. Rows of no sequence are 0, or as
     they were in an `out` that is given."""
-    _one_device("paged_attention", q, k_pages, v_pages, table, starts, lens, k_scale, v_scale, out)
+    dev = _device_of("paged_attention", q, k_pages, v_pages, table, starts, lens, k_scale, v_scale, out)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_pages, v_pages, table, starts, lens, k_scale, v_scale, scale, causal, max_q, max_len, out)
     dt = _dtype(q)
-    code, pages, heads, page, d = _pool("paged_attention", k_pages, v_pages, k_scale, v_scale, table, q.dtype)
-    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or heads == 0 or q.shape[1] % heads:
-        raise SamHipError(f"paged_attention: q must be [T, a multiple of {heads}, {d}], got {tuple(q.shape)}")
-    table, starts, lens = _tables("paged_attention", table, starts, lens)
-    zero_rest = out is None
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise SamHipError(f"paged_attention: out must match q (shape {tuple(q.shape)}, {q.dtype}), got {tuple(out.shape)}, {out.dtype}")
-    elif out.stride(2) != 1:
-        raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
-    tokens, hq, _ = q.shape
-    b, width = table.shape
+    code, pages, heads, page, d, b, width = _pool("paged_attention", k_pages, v_pages, k_scale, v_scale, table, starts, lens,
+                                                  q.dtype)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or shape[1] == 0 or heads == 0 or shape[1] % heads:
+        raise SamHipError(f"paged_attention: q must be [T, a multiple of {heads}, {d}], got {tuple(shape)}")
+    tokens, hq = shape[0], shape[1]
+    rest = out is None  # rows of no sequence are set to 0
+    so = None
+    if rest:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != shape or out.dtype != q.dtype:
+        raise SamHipError(f"paged_attention: out must match q (shape {tuple(shape)}, {q.dtype}), got {tuple(out.shape)}, {out.dtype}")
+    elif not out.is_contiguous():
+        if out.stride(2) != 1 or _overlaps_itself(out):
+            raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
+        so = _long2(out.stride(0), out.stride(1))
     if tokens == 0:
         return out
-    if b == 0 or width == 0:  # no sequences, or none that holds a key
-        return out.zero_() if zero_rest else out
-    q = _token_rows("paged_attention", "q", q)
+    if b == 0:
+        return out.zero_() if rest else out
+    if width == 0:  # no keys: as one page that is not there
+        table, width = torch.full((b, 1), -1, dtype=torch.int32, device=q.device), 1
+    table, starts, lens = _plain(table), _plain(starts), _plain(lens)
+    q, sq = _token_rows(q)
     scale = float(d) ** -0.5 if scale is None else float(scale)
     max_q = tokens if max_q is None else int(max_q)
     max_len = width * page if max_len is None else int(max_len)
-    L = load()
-    ws_bytes = L.sam_hip_paged_attention_workspace_size(dt, code, tokens, b, hq, heads, d, max_q, max_len)
-    if ws_bytes < 0:
-        raise SamHipError(L.sam_hip_last_error().decode())
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    _check(L.sam_hip_paged_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
-                                     table.data_ptr(), starts.data_ptr(), lens.data_ptr(), out.data_ptr(), dt, code,
-                                     tokens, b, hq, pages, heads, page, d, width, _long2(q.stride(0), q.stride(1)),
-                                     _long2(out.stride(0), out.stride(1)), scale, bool(causal), zero_rest, max_q, max_len,
-                                     _ptr(ws), ws_bytes, _stream()))
+    ws_bytes = _paged_workspace(dev, dt, code, tokens, b, hq, heads, d, max_q, max_len)
+    ws = q.new_empty(ws_bytes // q.element_size()) if ws_bytes else None
+    _check(load().sam_hip_paged_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                                          table.data_ptr(), starts.data_ptr(), lens.data_ptr(), out.data_ptr(), dt, code,
+                                          tokens, b, hq, pages, heads, page, d, width, sq, so, scale, bool(causal), rest,
+                                          max_q, max_len, _ptr(ws), ws_bytes, _stream()))
     return out
