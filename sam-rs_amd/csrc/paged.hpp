@@ -38,14 +38,22 @@ __host__ __device__ inline unsigned divide_magic(unsigned j, unsigned magic, uns
   return (unsigned)(((unsigned long)j * magic) >> shift);
 }
 
-// Row (of the pools seen as [pages * heads * page_size, d], fewer than 2^31 of them) of sequence b's key j for one
-// head, or -1 where j is past `end` or its table entry outside the pool.
+// Where sequence b's key j lies for one head: first the table's entry, a load that is best on its way long before it is
+// needed, then the row (of the pools seen as [pages * heads * page_size, d], fewer than 2^31 of them), -1 where j is past
+// `end` or the entry outside the pool.
+struct PagedEntry {
+  int page, slot;
+};
+__device__ __forceinline__ PagedEntry paged_entry(const PagedKv& c, int b, int j, int end) {
+  const int at = max(0, min(j, end - 1));
+  const unsigned t = divide_magic((unsigned)at, c.magic, c.shift);
+  return {c.table[(long)b * c.width + t], at == j ? at - (int)t * c.page : -1};
+}
+__device__ __forceinline__ int paged_row(const PagedKv& c, const PagedEntry& e, int head) {
+  return (unsigned)e.page < (unsigned)c.pages && e.slot >= 0 ? (e.page * c.heads + head) * c.page + e.slot : -1;
+}
 __device__ __forceinline__ int paged_row(const PagedKv& c, int b, int head, int j, int end) {
-  if ((unsigned)j >= (unsigned)end) return -1;
-  const unsigned t = divide_magic((unsigned)j, c.magic, c.shift);
-  const int page = c.table[(long)b * c.width + t];
-  if ((unsigned)page >= (unsigned)c.pages) return -1;
-  return (page * c.heads + head) * c.page + (j - (int)t * c.page);
+  return (unsigned)j < (unsigned)end ? paged_row(c, paged_entry(c, b, j, end), head) : -1;
 }
 
 // Keys that sequence b holds, inside what its table can name.
@@ -70,7 +78,8 @@ struct PagedParams {
   int rtiles, nsplit;         // row tiles per (sequence, key head) of the grid; key splits
   int per;                    // blocks of 32 keys per split, at least (0: even shares of what each sequence holds)
   float* opart;               // nsplit > 1: partial O [nsplit][tokens * heads][d], f32, not normalised
-  float* ml;                  // nsplit > 1: running (max, sum) [nsplit][tokens * heads][2], log2 units
+  float* ml;                  // nsplit > 1: running (max, sum) [nsplit][tokens * heads][2], log2 units; a sum of -1 in
+                              // split 0: the row is finished, the other splits have written nothing
 };
 
 // How a call runs: the kernel's rows per tile, the row tiles and key splits of its grid, its workspace.

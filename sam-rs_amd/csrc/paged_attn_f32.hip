@@ -70,6 +70,8 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
     const int least = p.causal ? max(0, min(w.len, w.len - w.lq + tfirst + 1)) : w.len;
     const int blocks = (most + 31) >> 5, per = max(p.per, (blocks + p.nsplit - 1) / p.nsplit);
     const int b0 = min(blocks, w.split * per), b1 = min(blocks, b0 + per);
+    const bool direct = blocks <= per;  // one split has all keys: it writes the result itself
+    if (direct && w.split > 0) continue;
 
     float m[RB], l[RB];
     f32x4 o[RB][4 * ND];
@@ -215,7 +217,10 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         if (rt * TR + 16 * rb + n >= rows) continue;
-        if (p.nsplit == 1) {
+        const long row = ((long)w.split * p.tokens + tok[rb]) * p.heads + head[rb];
+        if (p.nsplit > 1 && g == 0)
+          *reinterpret_cast<float2*>(p.ml + 2 * row) = direct ? float2{0.f, -1.f} : float2{m[rb], l[rb]};
+        if (direct) {
           const float inv = l[rb] == 0.f ? 0.f : 1.f / l[rb];  // a row that sees no key is 0
           T* orow = reinterpret_cast<T*>(p.out) + tok[rb] * p.so[0] + head[rb] * p.so[1];
 #pragma unroll
@@ -229,18 +234,16 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
               for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(f32_result(o[rb][4 * q + j][e] * inv));
               *reinterpret_cast<typename Vec<T>::x4*>(orow + col) = x;
             }
-        } else if (b0 < b1 || g == 0) {
-          const long row = ((long)w.split * p.tokens + tok[rb]) * p.heads + head[rb];
+        } else if (b0 < b1) {
 #pragma unroll
           for (int q = 0; q < ND; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int col = 64 * q + 16 * g + 4 * e;
-              if (col < d && b0 < b1)
+              if (col < d)
                 *reinterpret_cast<f32x4*>(p.opart + row * d + col) =
                     f32x4{o[rb][4 * q][e], o[rb][4 * q + 1][e], o[rb][4 * q + 2][e], o[rb][4 * q + 3][e]};
             }
-          if (g == 0) *reinterpret_cast<float2*>(p.ml + 2 * row) = float2{m[rb], l[rb]};
         }
       }
     }

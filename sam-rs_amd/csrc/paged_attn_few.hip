@@ -63,6 +63,8 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
     // this split's blocks of 32 keys: ranges of the hint's longest sequence, longer ones where that was too short
     const int blocks = (most + 31) >> 5, per = max(p.per, (blocks + p.nsplit - 1) / p.nsplit);
     const int b0 = min(blocks, w.split * per), b1 = min(blocks, b0 + per);
+    const bool direct = blocks <= per;  // one split has all keys: it writes the result itself
+    if (direct && w.split > 0) continue;
 
     int limit[RB];
     X8 qf[RB][NK];
@@ -95,12 +97,12 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
     auto from_key = [&](int j, int v) {  // the lane whose own key is element j of group g
       return __builtin_amdgcn_ds_bpermute((int)at_g + 64 * (j >> 2) + 4 * (j & 3), v);
     };
-    auto rows_of = [&](int blk) { return blk < b1 ? paged_row(p.c, w.b, w.head, 32 * blk + (lane & 31), most) : -1; };
+    auto entry_of = [&](int blk) { return paged_entry(p.c, w.b, 32 * min(blk, b1 - 1) + (lane & 31), most); };
     KRaw kx[2][NK];
     VRaw vx[8][NV];
-    float ksx = 1.f, vsx = 1.f;  // scales of the lane's own key
+    unsigned char ksx = 127, vsx = 127;  // scales of the lane's own key
     auto load_k = [&](int row) {
-      if constexpr (kCoded) ksx = pow2_of(p.c.ks[max(row, 0)]);
+      if constexpr (kCoded) ksx = p.c.ks[max(row, 0)];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const C* kr = kp + (long)max(from_n(i, row), 0) * d;
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
       }
     };
     auto load_v = [&](int row) {
-      if constexpr (kCoded) vsx = pow2_of(p.c.vs[max(row, 0)]);
+      if constexpr (kCoded) vsx = p.c.vs[max(row, 0)];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const C* vr = vp + (long)max(from_key(j, row), 0) * d;
@@ -118,17 +120,30 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
       }
     };
 
-    int row = rows_of(b0 + wave), next = rows_of(b0 + wave + 4);
-    load_k(row);
-    load_v(row);
+    // Table entries two blocks ahead, K and V one: a wait for a load waits for those before it too, so the entries go
+    // ahead of the rows that they are not needed for.
+    int row = -1;
+    PagedEntry coming = {-1, -1};
+    if (b0 + wave < b1) {
+      const PagedEntry first = entry_of(b0 + wave);
+      coming = entry_of(b0 + wave + 4);
+      row = paged_row(p.c, first, w.head);
+      load_k(row);
+      load_v(row);
+    }
+    // Q is here: told to the compiler, whose own wait for it would stand in the loop, behind the next block's loads
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     for (int blk = b0 + wave; blk < b1; blk += 4) {
       const int key0 = 32 * blk;
+      const int next = paged_row(p.c, coming, w.head);
+      coming = entry_of(blk + 8);
       const unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
       f32x4 s[RB][2];
+      const float kso = kCoded ? pow2_of(ksx) : 1.f, vso = kCoded ? pow2_of(vsx) : 1.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float ks = 1.f;
-        if constexpr (kCoded) ks = __int_as_float(from_n(i, __float_as_int(ksx)));
+        if constexpr (kCoded) ks = __int_as_float(from_n(i, __float_as_int(kso)));
 #pragma unroll
         for (int c = 0; c < NK; ++c) {
           u32x4 a;
@@ -146,6 +161,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
       // s[rb][i][e]: key key0 + 16 i + 4 g + e, row 16 rb + n
       if (blk + 4 < b1) load_k(next);  // in flight while this block's V is weighed
       const bool part = key0 + 32 > least || there != 0xffffffffu;
+      const unsigned mine = there >> (4 * g);  // bit 16 i + e: the lane's key 16 i + 4 g + e
       X8 b[RB], blo[RB];
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
@@ -155,8 +171,8 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int kk = 16 * i + 4 * g + e;
-              s[rb][i][e] = key0 + kk < limit[rb] && (there >> kk & 1) ? s[rb][i][e] : -INFINITY;
+              const int kk = 16 * i + e;
+              s[rb][i][e] = kk < limit[rb] - key0 - 4 * g && (mine >> kk & 1) ? s[rb][i][e] : -INFINITY;
             }
         }
 #pragma unroll
@@ -190,7 +206,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
       float vs[8];
       if constexpr (kCoded) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vs[j] = __int_as_float(from_key(j, __float_as_int(vsx)));
+        for (int j = 0; j < 8; ++j) vs[j] = __int_as_float(from_key(j, __float_as_int(vso)));
       }
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
@@ -213,7 +229,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
             for (int h = 0; h < CW / 2; ++h) v[j][h] = vx[j][q][h];
           }
           if (part) {  // rows that are not there hold anything; values that are not finite go apart
-            const bool ok = there >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1;
+            const bool ok = mine >> (16 * (j >> 2) + (j & 3)) & 1;
 #pragma unroll
             for (int h = 0; h < CW / 2; ++h) {
               const unsigned bad = not_finite2<T>(v[j][h]);
@@ -262,7 +278,6 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
       }
       if (blk + 4 < b1) load_v(next);
       row = next;
-      next = rows_of(blk + 8);
     }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) l[rb] = sum_over_rows16(l[rb]);
@@ -315,7 +330,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
           for (int e = 0; e < 4; ++e) {
             const int col = CW * (16 * q + 4 * g + e);  // o[q CW + c][e]: column col + c
             if (col >= d) continue;
-            if (p.nsplit == 1) {
+            if (direct) {
               T* to = reinterpret_cast<T*>(p.out) + tok * p.so[0] + hq * p.so[1] + col;
 #pragma unroll
               for (int c = 0; c < CW; c += 4) {
@@ -332,7 +347,8 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(P
                                                           o[rb][q * CW + c + 2][e], o[rb][q * CW + c + 3][e]};
             }
           }
-        if (p.nsplit > 1 && g == 0) *reinterpret_cast<float2*>(p.ml + 2 * part) = float2{m[rb], l[rb]};
+        if (p.nsplit > 1 && g == 0)
+          *reinterpret_cast<float2*>(p.ml + 2 * part) = direct ? float2{0.f, -1.f} : float2{m[rb], l[rb]};
       }
     }
     __syncthreads();

@@ -25,6 +25,7 @@ namespace samhip {
 namespace {
 
 constexpr float kSlack = 8.f;
+constexpr int kAhead = 4;  // LDS fragments in flight ahead of their products
 
 template <int DP> struct ManyGeom {
   static constexpr int KS = DP / 16, MBO = DP / 32;
@@ -79,47 +80,55 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
     // blocks of 32 keys, as the other kernels count them; a tile is two
     const int tiles = (most + 63) >> 6, per = max((p.per + 1) >> 1, (tiles + p.nsplit - 1) / p.nsplit);
     const int t0 = min(tiles, w.split * per), t1 = min(tiles, t0 + per);
+    const bool direct = tiles <= per;  // one split has all keys: it writes the result itself
+    if (direct && w.split > 0) continue;
 
     const int r = min(wfirst + n, rows - 1);
     const int tk = (int)divide_magic(r, p.gmagic, p.gshift);
     const int limit = keys_of(r);
     const T* qr = reinterpret_cast<const T*>(p.q) + (w.s0 + tk) * p.sq[0] + (w.head * p.group + r - tk * p.group) * p.sq[1];
 
-    Raw reg[PT];  // the chunks of K or V on their way, and in 8 bits their rows' scales
-    float sreg[PT];
+    // the next tile's chunks on their way, and in 8 bits the scales of the lane's own key
+    struct Chunks {
+      Raw x[PT];
+      unsigned char scale;
+    } kreg, vreg;
     // lane l's own key of a tile; a key that is not there reads row 0 and is masked (K) or cleared (V)
-    auto look = [&](int t) { return t < t1 ? paged_row(p.c, w.b, w.head, 64 * t + lane, most) : -1; };
-    auto load = [&](const C* base, const unsigned char* scales, int own) {
-      float mine = 1.f;
-      if constexpr (kCoded) mine = pow2_of(scales[max(own, 0)]);
+    auto entry_of = [&](int t) { return paged_entry(p.c, w.b, 64 * min(t, t1 - 1) + lane, most); };
+    auto load = [&](int own) {
+      if constexpr (kCoded) {
+        kreg.scale = p.c.ks[max(own, 0)];
+        vreg.scale = p.c.vs[max(own, 0)];
+      }
+      long off[PT];
 #pragma unroll
-      for (int u = 0; u < PT; ++u) {
-        const long row = __shfl(own, srow + u * RS);
-        reg[u] = *reinterpret_cast<const Raw*>(base + max(row, 0l) * d + min(scol, d - 8));
-        if constexpr (kCoded) sreg[u] = __shfl(mine, srow + u * RS);
+      for (int u = 0; u < PT; ++u) off[u] = (long)max(__shfl(own, srow + u * RS), 0) * d + min(scol, d - 8);
+#pragma unroll
+      for (int u = 0; u < PT; ++u) kreg.x[u] = *reinterpret_cast<const Raw*>(kp + off[u]);
+#pragma unroll
+      for (int u = 0; u < PT; ++u) vreg.x[u] = *reinterpret_cast<const Raw*>(vp + off[u]);
+    };
+    auto chunk = [&](const Chunks& c, int u) {
+      if constexpr (kCoded) {
+        const float f = __shfl(pow2_of(c.scale), srow + u * RS);
+        return u32x4{decode2<T, false>(c.x[u][0], f), decode2<T, true>(c.x[u][0], f), decode2<T, false>(c.x[u][1], f),
+                     decode2<T, true>(c.x[u][1], f)};
+      } else {
+        return c.x[u];
       }
     };
-    auto chunk = [&](int u) {
-      if constexpr (kCoded)
-        return u32x4{decode2<T, false>(reg[u][0], sreg[u]), decode2<T, true>(reg[u][0], sreg[u]),
-                     decode2<T, false>(reg[u][1], sreg[u]), decode2<T, true>(reg[u][1], sreg[u])};
-      else
-        return reg[u];
-    };
-    auto load_k = [&](int own) { load(kp, p.c.ks, own); };
-    auto load_v = [&](int own) { load(vp, p.c.vs, own); };
-    auto store_k = [&](int buf) {
-#pragma unroll
-      for (int u = 0; u < PT; ++u)
-        if (sin) *reinterpret_cast<u32x4*>(ks_base + buf * G::KBUF + (srow + u * RS) * KSTR + scol) = chunk(u);
-    };
     auto whole = [&](int t, unsigned long there) { return 64 * t + 64 <= least && there == ~0ul; };
-    auto store_v = [&](int t, unsigned long there, int buf) {
+    auto store = [&](int t, unsigned long there, int buf) {
+#pragma unroll
+      for (int u = 0; u < PT; ++u) {
+        const u32x4 x = chunk(kreg, u);
+        if (sin) *reinterpret_cast<u32x4*>(ks_base + buf * G::KBUF + (srow + u * RS) * KSTR + scol) = x;
+      }
       const bool look_over = !whole(t, there);
 #pragma unroll
       for (int u = 0; u < PT; ++u) {
         const int row = srow + u * RS;
-        u32x4 x = chunk(u);
+        u32x4 x = chunk(vreg, u);
         if (look_over) {
           unsigned any = 0;
 #pragma unroll
@@ -134,9 +143,18 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
       }
     };
 
-    int own = look(t0), next = look(t0 + 1);
+    // Table entries three tiles ahead, K and V two in registers and one in LDS: a wait for a load waits for those before
+    // it too.
+    PagedEntry entry = {-1, -1};
+    int own = -1, own1 = -1;
     if (tid < 2) odd[tid] = -1;
-    if (t0 < t1) load_k(own);
+    if (t0 < t1) {
+      const PagedEntry first = entry_of(t0), second = entry_of(t0 + 1);
+      entry = entry_of(t0 + 2);
+      own = paged_row(p.c, first, w.head);
+      own1 = paged_row(p.c, second, w.head);
+      load(own);
+    }
     X8 qf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -145,11 +163,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
     }
     unsigned long there = __builtin_amdgcn_ballot_w64(own >= 0);
     __syncthreads();
-    if (t0 < t1) {
-      store_k(0);
-      load_v(own);
-      store_v(t0, there, 0);
-    }
+    if (t0 < t1) store(t0, there, 0);
+    if (t0 + 1 < t1) load(own1);
+    // Q is here: told to the compiler, whose own wait for it would stand in the loop, behind the next tile's loads
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
 
     // K (A operand of S^T): row 32 mb + n, columns 16 k + 8 hh ..
@@ -164,30 +181,54 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
 
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1, key0 = 64 * t;
-      const unsigned long coming = __builtin_amdgcn_ballot_w64(next >= 0);
-      const bool more = t + 1 < t1;
+      const int own2 = paged_row(p.c, entry, w.head);
+      const unsigned long there1 = __builtin_amdgcn_ballot_w64(own1 >= 0);
       const bool here = key0 < wmost;
-      if (more) load_k(next);
+      if (t + 1 < t1) {  // its loads have had the last tile's time to arrive
+        store(t + 1, there1, buf ^ 1);
+        entry = entry_of(t + 3);
+        if (t + 2 < t1) load(own2);
+      }
       if (here) {
         const T* kb = ks_base + buf * G::KBUF + koff;
         const T* vb = vs_base + buf * G::VBUF + voff;
+        // Product i reads its K fragment kAhead products earlier; the scheduling groups hold that order (left alone, the
+        // compiler reads each right before its product and waits for it)
         f32x16 s[2];
+        {
+          X8 kf[2 * KS];
+          auto kread = [&](int i) { kf[i] = *reinterpret_cast<const X8*>(kb + 32 * (i & 1) * KSTR + 16 * (i >> 1)); };
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb)
+          for (int i = 0; i < kAhead; ++i) kread(i);
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-            s[mb] = mma32(*reinterpret_cast<const X8*>(kb + 32 * mb * KSTR + 16 * k), qf[k], k == 0 ? f32x16{} : s[mb]);
+          for (int i = 0; i < 2 * KS; ++i) {
+            s[i & 1] = mma32(kf[i], qf[i >> 1], i < 2 ? f32x16{} : s[i & 1]);
+            if (i + kAhead < 2 * KS) kread(i + kAhead);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+          for (int i = 0; i < 2 * KS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i + kAhead < 2 * KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
         auto fragment = [&](int u, int ob) {  // keys 16 u + 8 (j / 4) + 4 hh + j % 4 of columns 32 ob ..
           const T* a = vb + 16 * u * VSTR + 32 * ob;
           return join8<T>(lds_read_tr16(a), lds_read_tr16(a + 8 * VSTR));
         };
         if (key0 + 64 > wleast || there != ~0ul) {
+          // shifted by the lane's part of the key, so that constants are left (the compiler would keep one key and one
+          // bit a score in registers)
+          const int lim = limit - key0 - 4 * hh;
+          const unsigned lo = (unsigned)(there >> (4 * hh)), hi = (unsigned)(there >> 32 >> (4 * hh));
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const int kk = 32 * mb + 8 * (e >> 2) + 4 * hh + (e & 3);
-              s[mb][e] = key0 + kk < limit && (there >> kk & 1) ? s[mb][e] : -INFINITY;
+              const int kk = 8 * (e >> 2) + (e & 3);
+              s[mb][e] = 32 * mb + kk < lim && ((mb ? hi : lo) >> kk & 1) ? s[mb][e] : -INFINITY;
             }
         }
         float top = s[0][0];
@@ -222,18 +263,26 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
               l = __builtin_amdgcn_fdot2(h2{b[u][j], b[u][j + 1]}, h2{(f16)1.f, (f16)1.f}, l, false);
           }
         }
-        if (more) {  // K(t+1) makes room for V(t+1), which has the product's time to arrive
-          store_k(buf ^ 1);
-          load_v(next);
-        }
+        // O^T += V^T P^T, each fragment read kAhead products earlier
+        {
+          X8 vf[4 * MBO];
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+          for (int i = 0; i < kAhead; ++i) vf[i] = fragment(i / MBO, i % MBO);
 #pragma unroll
-          for (int ob = 0; ob < MBO; ++ob) {
-            const X8 a = fragment(u, ob);
-            o[ob] = mma32(a, b[u], o[ob]);
-            if constexpr (kSplitP) o[ob] = mma32(a, blo[u], o[ob]);
+          for (int i = 0; i < 4 * MBO; ++i) {
+            o[i % MBO] = mma32(vf[i], b[i / MBO], o[i % MBO]);
+            if constexpr (kSplitP) o[i % MBO] = mma32(vf[i], blo[i / MBO], o[i % MBO]);
+            if (i + kAhead < 4 * MBO) vf[i + kAhead] = fragment((i + kAhead) / MBO, (i + kAhead) % MBO);
           }
+          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+#pragma unroll
+          for (int i = 0; i < 4 * MBO; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, kSplitP ? 2 : 1, 0);
+            if (i + kAhead < 4 * MBO) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
         if (!whole(t, there) && odd[buf] == t) {
           for (int kk = 0; kk < 64; ++kk) {
             if (!(there >> kk & 1)) continue;
@@ -253,15 +302,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
               }
           }
         }
-      } else if (more) {
-        store_k(buf ^ 1);
-        load_v(next);
       }
-      if (more) store_v(t + 1, coming, buf ^ 1);
-      own = next;
-      next = look(t + 2);
-      there = coming;
-      __syncthreads();
+      own = own1;
+      own1 = own2;
+      there = there1;
+      // the workgroup's LDS is in order; loads on their way into registers stay on it (__syncthreads would wait for them)
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
     // lane holds O^T[32 ob + 8 a + 4 hh + e][row n] in o[ob][4 a + e]
@@ -279,7 +325,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
             if (32 * ob + 8 * a + 4 * hh < d)
               put(32 * ob + 8 * a + 4 * hh, f32x4{o[ob][4 * a], o[ob][4 * a + 1], o[ob][4 * a + 2], o[ob][4 * a + 3]});
       };
-      if (p.nsplit == 1) {
+      if (direct) {
         T* to = reinterpret_cast<T*>(p.out) + tok * p.so[0] + hq * p.so[1];
         columns([&](int col, f32x4 x) {
           typename Vec<T>::x4 y;
@@ -290,7 +336,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
       } else if (t0 < t1) {
         columns([&](int col, f32x4 x) { *reinterpret_cast<f32x4*>(p.opart + part * d + col) = x; });
       }
-      if (p.nsplit > 1 && hh == 0) *reinterpret_cast<float2*>(p.ml + 2 * part) = float2{m, l};
+      if (p.nsplit > 1 && hh == 0) *reinterpret_cast<float2*>(p.ml + 2 * part) = direct ? float2{0.f, -1.f} : float2{m, l};
     }
     __syncthreads();  // the next rows' first tile replaces buffer 0
   }

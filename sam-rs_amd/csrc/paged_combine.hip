@@ -1,6 +1,7 @@
 // Joins the key splits of a paged-attention call on gfx950: out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M the
 // largest m_s of the row, from the partial results that the attention kernels left. Splits are added in order, so the
-// result does not depend on their timing. A split without keys has l = 0 and no O.
+// result does not depend on their timing. A split without keys has l = 0 and no O; a row whose keys are all in its
+// first split is written already, which l = -1 says.
 //
 // What bounds it: the partial O's bytes, 4 a column and split, and, with few rows, the latency of reading them. Up to
 // eight splits a thread reads its four columns of each; past that a workgroup takes a row, its waves a share of the
@@ -33,7 +34,7 @@ template <typename T> __global__ __launch_bounds__(256) void paged_combine_kerne
   const long rows = (long)p.tokens * p.heads;
   if (row >= rows) return;
   const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
-  if (!row_of_a_sequence(p, tok)) return;
+  if (!row_of_a_sequence(p, tok) || p.ml[2 * row + 1] < 0.f) return;
   float top = -INFINITY;
   for (int s = 0; s < p.nsplit; ++s) top = fmaxf(top, p.ml[2 * (s * rows + row)]);
   const float base = top == -INFINITY ? 0.f : top;
@@ -58,7 +59,7 @@ template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_co
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long row = blockIdx.x, rows = (long)p.tokens * p.heads;
   const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
-  if (!row_of_a_sequence(p, tok)) return;
+  if (!row_of_a_sequence(p, tok) || p.ml[2 * row + 1] < 0.f) return;
   const int s = threadIdx.x;
   float2 ml = {-INFINITY, 0.f};
   if (s < p.nsplit) ml = *reinterpret_cast<const float2*>(p.ml + 2 * (s * rows + row));
