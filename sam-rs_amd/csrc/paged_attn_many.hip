@@ -25,29 +25,37 @@ namespace samhip {
 namespace {
 
 constexpr float kSlack = 8.f;
-constexpr int kAhead = 4;  // LDS fragments in flight ahead of their products
 
+// LDS: rows of 128, 256 or 512 bytes without padding, as the DMA leaves them (a wave's instruction fills 1 KB). 16-byte
+// chunk c of row r lies at c ^ swizzle(r), so that the 16 rows of which a K read takes one chunk each, and the 8 rows of
+// which a V read takes 64 bytes each, fall on all 64 banks alike.
 template <int DP> struct ManyGeom {
   static constexpr int KS = DP / 16, MBO = DP / 32;
-  static constexpr int KSTR = DP + 8;                     // K row stride (elements): rows 16 bytes apart mod 128
-  static constexpr int VSTR = DP + (MBO == 3 ? 0 : 32);   // 16 or 48 banks mod 64 for the transposing reads
-  static constexpr int KBUF = 64 * KSTR, VBUF = 64 * VSTR;
-  static constexpr int LDS = 2 * (KBUF + VBUF) * 2;
-  static constexpr int CPR = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // threads to a row, 8 columns each
-  static constexpr int RS = 256 / CPR, PT = 64 / RS;      // rows a round, rounds a tile
+  static constexpr int ROW = DP <= 64 ? 128 : DP <= 128 ? 256 : 512;  // bytes
+  static constexpr int BUF = 64 * ROW, LDS = 4 * BUF + 16;            // K0, K1, V0, V1, and two flags
+  static constexpr int CPR = ROW / 16, RPI = 64 / CPR, PT = 16 / RPI; // chunks a row, rows an instruction, instructions
+  static __device__ int kswz(int r) { return ROW == 128 ? (r >> 1) & 7 : r & 15; }
+  static __device__ int vswz(int r) { return ROW == 128 ? (r >> 1 & 1) << 2 : (r & 3) << 2; }
 };
 
+// Lane l's 16 bytes at its own p land at LDS byte address lds + 16 l (lds wave-uniform; idle lanes leave theirs alone).
+__device__ __forceinline__ void dma16_from(const void* p, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_many_kernel(PagedParams p) {
   typedef ManyGeom<DP> G;
   typedef typename Vec<T>::x8 X8;
   constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
-  constexpr int KS = G::KS, MBO = G::MBO, KSTR = G::KSTR, VSTR = G::VSTR, CPR = G::CPR, RS = G::RS, PT = G::PT;
-  __shared__ int odd[2];  // the tile in each buffer that was stored without values that are not finite
+constexpr int kAhead = DP > 128 ? 4 : 2;  // LDS fragments in flight ahead of their products
+  typedef __attribute__((address_space(3))) X8 lds_x8;
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+  constexpr int KS = G::KS, MBO = G::MBO, ROW = G::ROW, BUF = G::BUF, CPR = G::CPR, RPI = G::RPI, PT = G::PT;
   typedef typename std::conditional<kCoded, u32x2, u32x4>::type Raw;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  T* ks_base = reinterpret_cast<T*>(smem);
-  T* vs_base = ks_base + 2 * G::KBUF;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const unsigned lds0 = lds_addr(smem);
+  int* odd = reinterpret_cast<int*>(smem + 4 * BUF);  // the tile in each buffer that went there without such values
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, hh = lane >> 5, g = lane >> 4, gi = lane & 15;
@@ -57,14 +65,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
   const int rows = w.lq * p.group;
   const C* kp = reinterpret_cast<const C*>(p.c.k);
   const C* vp = reinterpret_cast<const C*>(p.c.v);
-  const int srow = tid / CPR, scol = tid % CPR * 8;  // this thread's first row of a tile, and its columns
-  const bool sin = scol < d;
+  // Staging: instruction u of a wave moves rows srow(u) .. + RPI of a tile, lane l the chunk at position l % CPR of its row
+  const int spos = lane % CPR;
+  auto srow = [&](int u) { return 16 * wave + RPI * u + lane / CPR; };
+  auto kcol = [&](int u) { return 8 * (spos ^ G::kswz(RPI * u + lane / CPR)); };
+  auto vcol = [&](int u) { return 8 * (spos ^ G::vswz(RPI * u + lane / CPR)); };
 
-  if (d < DP) {  // K's columns past d meet zeros of q, so they must be finite; V's only feed columns that are dropped
-    for (int c = tid; c < 2 * 64 * (DP / 8); c += 256) {
-      const int r = c / (DP / 8), c8 = c % (DP / 8) * 8;
-      if (c8 >= d) *reinterpret_cast<u32x4*>(ks_base + (r >> 6) * G::KBUF + (r & 63) * KSTR + c8) = u32x4{};
-    }
+  if (d < ROW / 2) {  // columns past d are never written: K's meet zeros of q, and V's only feed columns that are dropped
+    for (int c = tid; c < 4 * BUF / 16; c += 256) *(lds_u32x4*)(size_t)(lds0 + 16 * c) = u32x4{};
   }
 
   for (int rt = w.tile; (long)rt * 128 < rows; rt += p.rtiles) {
@@ -88,72 +96,100 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
     const int limit = keys_of(r);
     const T* qr = reinterpret_cast<const T*>(p.q) + (w.s0 + tk) * p.sq[0] + (w.head * p.group + r - tk * p.group) * p.sq[1];
 
-    // the next tile's chunks on their way, and in 8 bits the scales of the lane's own key
-    struct Chunks {
-      Raw x[PT];
-      unsigned char scale;
-    } kreg, vreg;
     // lane l's own key of a tile; a key that is not there reads row 0 and is masked (K) or cleared (V)
     auto entry_of = [&](int t) { return paged_entry(p.c, w.b, 64 * min(t, t1 - 1) + lane, most); };
-    auto load = [&](int own) {
-      if constexpr (kCoded) {
-        kreg.scale = p.c.ks[max(own, 0)];
-        vreg.scale = p.c.vs[max(own, 0)];
-      }
-      long off[PT];
-#pragma unroll
-      for (int u = 0; u < PT; ++u) off[u] = (long)max(__shfl(own, srow + u * RS), 0) * d + min(scol, d - 8);
-#pragma unroll
-      for (int u = 0; u < PT; ++u) kreg.x[u] = *reinterpret_cast<const Raw*>(kp + off[u]);
-#pragma unroll
-      for (int u = 0; u < PT; ++u) vreg.x[u] = *reinterpret_cast<const Raw*>(vp + off[u]);
-    };
-    auto chunk = [&](const Chunks& c, int u) {
-      if constexpr (kCoded) {
-        const float f = __shfl(pow2_of(c.scale), srow + u * RS);
-        return u32x4{decode2<T, false>(c.x[u][0], f), decode2<T, true>(c.x[u][0], f), decode2<T, false>(c.x[u][1], f),
-                     decode2<T, true>(c.x[u][1], f)};
-      } else {
-        return c.x[u];
-      }
-    };
+    auto held = [&](int row) { return __builtin_amdgcn_ballot_w64(row >= 0); };
     auto whole = [&](int t, unsigned long there) { return 64 * t + 64 <= least && there == ~0ul; };
-    auto store = [&](int t, unsigned long there, int buf) {
+    // A tile that every row sees whole goes from its pages straight to LDS; one to be looked over, and e4m3, through
+    // registers
+    auto direct_to_lds = [&](int t, unsigned long there) { return !kCoded && whole(t, there); };
+    auto dma = [&](int own, int buf) {
+      long row[PT];
+#pragma unroll
+      for (int u = 0; u < PT; ++u) row[u] = __shfl(own, srow(u));
+      auto rows_to = [&](const C* base, unsigned to, auto col) {
+        if (d == ROW / 2) {
+#pragma unroll
+          for (int u = 0; u < PT; ++u) dma16_from(base + row[u] * d + col(u), to + 1024 * u);
+        } else {
+#pragma unroll
+          for (int u = 0; u < PT; ++u)
+            if (col(u) < d) dma16_from(base + row[u] * d + col(u), to + 1024 * u);
+        }
+      };
+      rows_to(kp, lds0 + buf * BUF + 16 * wave * ROW, kcol);
+      rows_to(vp, lds0 + (2 + buf) * BUF + 16 * wave * ROW, vcol);
+    };
+    // e4m3: the next tile's chunks on their way beside this one's products. Else a tile that is looked over comes after
+    // them, V once K is stored, in registers that the products have had.
+    Raw kreg[PT], vbuf[kCoded ? PT : 1];
+    Raw* vreg = kCoded ? vbuf : kreg;
+    unsigned char kscale = 127, vscale = 127;  // of the lane's own key
+    auto load = [&](const C* base, const unsigned char* scales, int own, auto col, Raw* reg, unsigned char& scale) {
+      if constexpr (kCoded) scale = scales[max(own, 0)];
 #pragma unroll
       for (int u = 0; u < PT; ++u) {
-        const u32x4 x = chunk(kreg, u);
-        if (sin) *reinterpret_cast<u32x4*>(ks_base + buf * G::KBUF + (srow + u * RS) * KSTR + scol) = x;
+        const long row = max(__shfl(own, srow(u)), 0);
+        reg[u] = *reinterpret_cast<const Raw*>(base + row * d + min(col(u), d - 8));
       }
-      const bool look_over = !whole(t, there);
+    };
+    auto load_k = [&](int own) { load(kp, p.c.ks, own, kcol, kreg, kscale); };
+    auto load_v = [&](int own) { load(vp, p.c.vs, own, vcol, vreg, vscale); };
+    auto values = [&](const Raw* reg, unsigned char scale, u32x4* x) {
+      if constexpr (kCoded) {
+        float f[PT];
+        const float mine = pow2_of(scale);
 #pragma unroll
-      for (int u = 0; u < PT; ++u) {
-        const int row = srow + u * RS;
-        u32x4 x = chunk(vreg, u);
-        if (look_over) {
-          unsigned any = 0;
+        for (int u = 0; u < PT; ++u) f[u] = __shfl(mine, srow(u));  // all before their use: each takes LDS's latency
+#pragma unroll
+        for (int u = 0; u < PT; ++u)
+          x[u] = u32x4{decode2<T, false>(reg[u][0], f[u]), decode2<T, true>(reg[u][0], f[u]),
+                       decode2<T, false>(reg[u][1], f[u]), decode2<T, true>(reg[u][1], f[u])};
+      } else {
+#pragma unroll
+        for (int u = 0; u < PT; ++u) x[u] = reg[u];
+      }
+    };
+    const unsigned to = lds0 + 16 * wave * ROW + 16 * lane;
+    auto store_k = [&](int buf) {
+      u32x4 x[PT];
+      values(kreg, kscale, x);
+#pragma unroll
+      for (int u = 0; u < PT; ++u)
+        if (kcol(u) < d) *(lds_u32x4*)(size_t)(to + buf * BUF + 1024 * u) = x[u];
+    };
+    auto store_v = [&](int t, unsigned long there, int buf) {
+      u32x4 x[PT];
+      values(vreg, vscale, x);
+      if (!whole(t, there)) {
+        unsigned any = 0;
+#pragma unroll
+        for (int u = 0; u < PT; ++u) {
+          const bool ok = (there >> srow(u) & 1) && vcol(u) < d;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const unsigned bad = not_finite2<T>(x[i]);
-            x[i] = there >> row & 1 ? without2(x[i], bad) : 0u;
-            any |= bad;
+            const unsigned bad = not_finite2<T>(x[u][i]);
+            x[u][i] = ok ? without2(x[u][i], bad) : 0u;
+            any |= ok ? bad : 0u;
           }
-          if (any && sin && (there >> row & 1)) odd[buf] = t;
         }
-        if (sin) *reinterpret_cast<u32x4*>(vs_base + buf * G::VBUF + row * VSTR + scol) = x;
+        if (any) odd[buf] = t;
       }
+#pragma unroll
+      for (int u = 0; u < PT; ++u)
+        if (vcol(u) < d) *(lds_u32x4*)(size_t)(to + (2 + buf) * BUF + 1024 * u) = x[u];
     };
 
-    // Table entries three tiles ahead, K and V two in registers and one in LDS: a wait for a load waits for those before
-    // it too.
+    // Table entries two tiles ahead, K and V one
     PagedEntry entry = {-1, -1};
-    int own = -1, own1 = -1;
+    int own = -1;
     if (tid < 2) odd[tid] = -1;
     if (t0 < t1) {
-      const PagedEntry first = entry_of(t0), second = entry_of(t0 + 1);
-      entry = entry_of(t0 + 2);
+      const PagedEntry first = entry_of(t0);
+      entry = entry_of(t0 + 1);
       own = paged_row(p.c, first, w.head);
-      own1 = paged_row(p.c, second, w.head);
-      load(own);
+      load_k(own);
+      if (kCoded) load_v(own);
     }
     X8 qf[KS];
 #pragma unroll
@@ -161,18 +197,22 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
       const int c = 16 * s + 8 * hh;
       qf[s] = c < d ? *reinterpret_cast<const X8*>(qr + c) : X8{};
     }
-    unsigned long there = __builtin_amdgcn_ballot_w64(own >= 0);
+    unsigned long there = held(own);
     __syncthreads();
-    if (t0 < t1) store(t0, there, 0);
-    if (t0 + 1 < t1) load(own1);
+    if (t0 < t1) {
+      store_k(0);
+      if (!kCoded) load_v(own);
+      store_v(t0, there, 0);
+    }
     // Q is here: told to the compiler, whose own wait for it would stand in the loop, behind the next tile's loads
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
 
-    // K (A operand of S^T): row 32 mb + n, columns 16 k + 8 hh ..
-    const int koff = n * KSTR + 8 * hh;
-    // V^T (A operand of O^T): the lane's transposing reads start at key 4 (g >> 1) + gi / 4, column 16 (g & 1) + 4 (gi & 3)
-    const int voff = (4 * (g >> 1) + (gi >> 2)) * VSTR + 16 * (g & 1) + 4 * (gi & 3);
+    // K (A operand of S^T): row 32 h + n, chunk 2 k + hh; the swizzle of the even part is an exclusive or with 32 k
+    const unsigned kad = lds0 + n * ROW + 16 * (hh ^ G::kswz(n));
+    // V^T (A operand of O^T): the transposing reads start at key 4 (g >> 1) + gi / 4, column 16 (g & 1) + 4 (gi & 3)
+    const int vkey = 4 * (g >> 1) + (gi >> 2);
+    const unsigned vad = lds0 + 2 * BUF + vkey * ROW + 16 * G::vswz(vkey) + 32 * (g & 1) + 8 * (gi & 3);
     const float sc = p.sc;
     float m = -INFINITY, l = 0.f;
     f32x16 o[MBO];
@@ -181,108 +221,137 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
 
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1, key0 = 64 * t;
-      const int own2 = paged_row(p.c, entry, w.head);
-      const unsigned long there1 = __builtin_amdgcn_ballot_w64(own1 >= 0);
-      const bool here = key0 < wmost;
-      if (t + 1 < t1) {  // its loads have had the last tile's time to arrive
-        store(t + 1, there1, buf ^ 1);
-        entry = entry_of(t + 3);
-        if (t + 2 < t1) load(own2);
-      }
-      if (here) {
-        const T* kb = ks_base + buf * G::KBUF + koff;
-        const T* vb = vs_base + buf * G::VBUF + voff;
-        // Product i reads its K fragment kAhead products earlier; the scheduling groups hold that order (left alone, the
-        // compiler reads each right before its product and waits for it)
-        f32x16 s[2];
-        {
-          X8 kf[2 * KS];
-          auto kread = [&](int i) { kf[i] = *reinterpret_cast<const X8*>(kb + 32 * (i & 1) * KSTR + 16 * (i >> 1)); };
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int i = 0; i < kAhead; ++i) kread(i);
-#pragma unroll
-          for (int i = 0; i < 2 * KS; ++i) {
-            s[i & 1] = mma32(kf[i], qf[i >> 1], i < 2 ? f32x16{} : s[i & 1]);
-            if (i + kAhead < 2 * KS) kread(i + kAhead);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-          for (int i = 0; i < 2 * KS; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (i + kAhead < 2 * KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+      const int next = paged_row(p.c, entry, w.head);
+      const unsigned long coming = held(next);
+      const bool more = t + 1 < t1, straight = direct_to_lds(t + 1, coming);
+      entry = entry_of(t + 2);
+      if (more) {
+        if (straight) {
+          dma(next, buf ^ 1);
+        } else if (kCoded) {
+          load_k(next);
+          load_v(next);
         }
-        auto fragment = [&](int u, int ob) {  // keys 16 u + 8 (j / 4) + 4 hh + j % 4 of columns 32 ob ..
-          const T* a = vb + 16 * u * VSTR + 32 * ob;
-          return join8<T>(lds_read_tr16(a), lds_read_tr16(a + 8 * VSTR));
+      }
+      if (key0 < wmost) {
+        const unsigned kb = kad + buf * BUF, vb = vad + buf * BUF;
+        const bool masks = key0 + 64 > wleast || there != ~0ul;
+        // The tile's two halves of 32 keys, one's softmax on the vector unit beside the other's products on the matrix
+        // unit: S0 | S1 with softmax 0 | P0 V0 with softmax 1 | P1 V1. LDS fragments are read kAhead products before
+        // their use. The scheduling groups hold these orders, which the compiler does not find.
+        f32x16 s[2];
+        X8 kf[2 * KS], vf[4 * MBO], b[4], blo[4];
+        float alpha = 1.f;
+        auto kread = [&](int i) { kf[i] = *(const lds_x8*)(size_t)((kb ^ 32 * (i % KS & 7)) + 256 * (i % KS >> 3) + 32 * ROW * (i / KS)); };
+        auto vread = [&](int i) {  // keys 16 u + 8 (j / 4) + 4 hh + j % 4 of columns 32 ob ..; i = u MBO + ob
+          const unsigned a = (vb ^ 64 * (i % MBO & 3)) + 256 * (i % MBO >> 2) + 16 * ROW * (i / MBO);
+          vf[i] = join8<T>(lds_read_tr16_at(a), lds_read_tr16_at(a + 8 * ROW));
         };
-        if (key0 + 64 > wleast || there != ~0ul) {
+        auto qk = [&](int i) {
+          s[i / KS] = mma32(kf[i], qf[i % KS], i % KS == 0 ? f32x16{} : s[i / KS]);
+          if (i + kAhead < 2 * KS) kread(i + kAhead);
+        };
+        auto pv = [&](int i) {
+          o[i % MBO] = mma32(vf[i], b[i / MBO], o[i % MBO]);
+          if constexpr (kSplitP) o[i % MBO] = mma32(vf[i], blo[i / MBO], o[i % MBO]);
+          if (i + kAhead < 4 * MBO) vread(i + kAhead);
+        };
+        auto mask = [&](int h) {
           // shifted by the lane's part of the key, so that constants are left (the compiler would keep one key and one
           // bit a score in registers)
-          const int lim = limit - key0 - 4 * hh;
-          const unsigned lo = (unsigned)(there >> (4 * hh)), hi = (unsigned)(there >> 32 >> (4 * hh));
+          const int lim = limit - key0 - 32 * h - 4 * hh;
+          const unsigned bits = (unsigned)(there >> (32 * h)) >> (4 * hh);
 #pragma unroll
-          for (int mb = 0; mb < 2; ++mb)
+          for (int e = 0; e < 16; ++e) {
+            const int kk = 8 * (e >> 2) + (e & 3);
+            s[h][e] = kk < lim && (bits >> kk & 1) ? s[h][e] : -INFINITY;
+          }
+        };
+        auto softmax = [&](int h) {  // of half h: b[2 h], b[2 h + 1], and alpha, by which O is to be scaled first
+          float top = s[h][0];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int kk = 8 * (e >> 2) + (e & 3);
-              s[mb][e] = 32 * mb + kk < lim && ((mb ? hi : lo) >> kk & 1) ? s[mb][e] : -INFINITY;
-            }
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) top = max_nc(top, s[mb][e]);
-        top = max_with_partner32(top) * sc;
-        if (wave_any(top > m + kSlack)) {
-          const float mn = fmaxf(m, top), alpha = exp2_fast(m - (mn == -INFINITY ? 0.f : mn));
+          for (int e = 1; e < 16; ++e) top = max_nc(top, s[h][e]);
+          top = max_with_partner32(top) * sc;
+          const float mn = top > m + kSlack ? top : m, base = mn == -INFINITY ? 0.f : mn;
+          alpha = exp2_fast(m - base);  // m == mn: 1, or 0 while both are -inf and O is 0
+          m = mn;
           l *= alpha;
 #pragma unroll
-          for (int ob = 0; ob < MBO; ++ob) o[ob] *= alpha;
-          m = mn;
-        }
-        const float c = m == -INFINITY ? 0.f : -m;
-        X8 b[4], blo[4];
+          for (int u = 2 * h; u < 2 * h + 2; ++u) {
+            float pr[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float pv[8];
+            for (int j = 0; j < 8; ++j) pr[j] = exp2_fast(fmaf(s[h][8 * (u & 1) + j], sc, -base));
+            if constexpr (kSplitP) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) pv[j] = exp2_fast(fmaf(s[u >> 1][8 * (u & 1) + j], sc, c));
-          if constexpr (kSplitP) {
+              for (int j = 0; j < 8; ++j) l += pr[j];
+              split_hi_lo(pr, b[u], blo[u]);
+            } else {
+              b[u] = pack8(pr, (X8*)nullptr);
+              typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) l += pv[j];
-            split_hi_lo(pv, b[u], blo[u]);
-          } else {
-            b[u] = pack8(pv, (X8*)nullptr);
-            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-            for (int j = 0; j < 8; j += 2)
-              l = __builtin_amdgcn_fdot2(h2{b[u][j], b[u][j + 1]}, h2{(f16)1.f, (f16)1.f}, l, false);
+              for (int j = 0; j < 8; j += 2)
+                l = __builtin_amdgcn_fdot2(h2{b[u][j], b[u][j + 1]}, h2{(f16)1.f, (f16)1.f}, l, false);
+            }
           }
-        }
-        // O^T += V^T P^T, each fragment read kAhead products earlier
-        {
-          X8 vf[4 * MBO];
-          __builtin_amdgcn_sched_barrier(0);
+        };
+        auto rescale = [&]() {
+          if (wave_any(alpha != 1.f)) {
 #pragma unroll
-          for (int i = 0; i < kAhead; ++i) vf[i] = fragment(i / MBO, i % MBO);
-#pragma unroll
-          for (int i = 0; i < 4 * MBO; ++i) {
-            o[i % MBO] = mma32(vf[i], b[i / MBO], o[i % MBO]);
-            if constexpr (kSplitP) o[i % MBO] = mma32(vf[i], blo[i / MBO], o[i % MBO]);
-            if (i + kAhead < 4 * MBO) vf[i + kAhead] = fragment((i + kAhead) / MBO, (i + kAhead) % MBO);
+            for (int ob = 0; ob < MBO; ++ob) o[ob] *= alpha;
           }
-          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+        };
+        constexpr int kVec = (kSplitP ? 96 : 48), kTrans = 17;  // a half's softmax, in vector and exponential instructions
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < 4 * MBO; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, kSplitP ? 2 : 1, 0);
-            if (i + kAhead < 4 * MBO) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < kAhead; ++i) kread(i);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) qk(i);
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (masks) mask(0);
+        __builtin_amdgcn_sched_barrier(0);
+        softmax(0);
+#pragma unroll
+        for (int i = KS; i < 2 * KS; ++i) qk(i);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) vread(i);
+#pragma unroll
+        for (int i = KS; i < 2 * KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, (kVec + KS - 1) / KS, 0);
+          __builtin_amdgcn_sched_group_barrier(0x400, (kTrans + KS - 1) / KS, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        rescale();
+        if (masks) mask(1);
+        __builtin_amdgcn_sched_barrier(0);
+        softmax(1);
+#pragma unroll
+        for (int i = 0; i < 2 * MBO; ++i) pv(i);
+#pragma unroll
+        for (int i = 0; i < 2 * MBO; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, kSplitP ? 2 : 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, (kVec + 2 * MBO - 1) / (2 * MBO), 0);
+          __builtin_amdgcn_sched_group_barrier(0x400, (kTrans + 2 * MBO - 1) / (2 * MBO), 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        rescale();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 2 * MBO; i < 4 * MBO; ++i) pv(i);
+#pragma unroll
+        for (int i = 2 * MBO; i < 4 * MBO; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, kSplitP ? 2 : 1, 0);
+          if (i + kAhead < 4 * MBO) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         if (!whole(t, there) && odd[buf] == t) {
           for (int kk = 0; kk < 64; ++kk) {
             if (!(there >> kk & 1)) continue;
@@ -303,11 +372,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_many_kernel(Paged
           }
         }
       }
-      own = own1;
-      own1 = own2;
-      there = there1;
-      // the workgroup's LDS is in order; loads on their way into registers stay on it (__syncthreads would wait for them)
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (more && !straight) {
+        if (!kCoded) load_k(next);
+        store_k(buf ^ 1);
+        if (!kCoded) load_v(next);
+        store_v(t + 1, coming, buf ^ 1);
+      }
+      own = next;
+      there = coming;
+      wait_vm<0>();  // the tile on its way to LDS
+      __syncthreads();
     }
 
     // lane holds O^T[32 ob + 8 a + 4 hh + e][row n] in o[ob][4 a + e]
