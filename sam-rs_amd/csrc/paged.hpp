@@ -171,6 +171,12 @@ __device__ __forceinline__ PagedWork paged_work(const PagedParams& p) {
   return w;
 }
 
+// Key blocks of a split where n are shared out in pieces of `most` at best, `splits` pieces at most: even ones.
+__device__ __forceinline__ int paged_share(int n, int most, int splits) {
+  const int per = max(max(most, 1), (n + splits - 1) / splits), pieces = max(1, (n + per - 1) / per);
+  return (n + pieces - 1) / pieces;
+}
+
 // Sets the rows of out that belong to no sequence to zero, spread over the launch's workgroups.
 template <typename T> __device__ __forceinline__ void paged_zero_rest(const PagedParams& p) {
   const int first = max(0, min(p.c.starts[0], p.tokens)), end = max(first, min(p.c.starts[p.c.batch], p.tokens));

@@ -15,12 +15,13 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
   plan.rtiles = (int)((rows + plan.rows - 1) / plan.rows);
   const long base = (long)plan.rtiles * kv_heads * batch;
   if (plan.many) {
-    // as many workgroups as run at once (two a CU, one past head dim 128), with four tiles of 64 keys a split at least
-    const long slots = (d > 128 ? 1L : 2L) * cus, most = ((long)max_len + 255) / 256;
+    // as many workgroups as run at once (three a CU up to head dim 64, two to 128, one past it), with four tiles of 64
+    // keys a split at least
+    const long slots = (d > 128 ? 1L : d > 64 ? 2L : 3L) * cus, most = ((long)max_len + 255) / 256;
     plan.nsplit = (int)std::max(1L, std::min(std::min(slots / base, most), 64L));
   } else {
-    // four workgroups a CU, if every split then has two blocks of 32 keys for each of its four waves
-    const long want = (4L * cus + base - 1) / base, most = ((long)max_len + 255) / 256;
+    // eight workgroups a CU, if every split then has eight blocks of 32 keys for each of its four waves
+    const long want = (8L * cus + base - 1) / base, most = ((long)max_len + 1023) / 1024;
     plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
   }
   const long blocks = ((long)max_len + 31) / 32;

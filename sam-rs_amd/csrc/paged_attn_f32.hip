@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
     const int most = p.causal ? max(0, min(w.len, w.len - w.lq + tlast + 1)) : w.len;
     const int tfirst = (int)divide_magic(rt * TR, p.gmagic, p.gshift);
     const int least = p.causal ? max(0, min(w.len, w.len - w.lq + tfirst + 1)) : w.len;
-    const int blocks = (most + 31) >> 5, per = max(p.per, (blocks + p.nsplit - 1) / p.nsplit);
+    const int blocks = (most + 31) >> 5, per = paged_share(blocks, p.per, p.nsplit);
     const int b0 = min(blocks, w.split * per), b1 = min(blocks, b0 + per);
     const bool direct = blocks <= per;  // one split has all keys: it writes the result itself
     if (direct && w.split > 0) continue;

@@ -86,7 +86,7 @@ constexpr int kAhead = DP > 128 ? 4 : 2;  // LDS fragments in flight ahead of th
     const bool rows_here = wfirst < rows;
     const int wleast = rows_here ? keys_of(wfirst) : 0, wmost = rows_here ? keys_of(min(wfirst + 32, rows) - 1) : 0;
     // blocks of 32 keys, as the other kernels count them; a tile is two
-    const int tiles = (most + 63) >> 6, per = max((p.per + 1) >> 1, (tiles + p.nsplit - 1) / p.nsplit);
+    const int tiles = (most + 63) >> 6, per = paged_share(tiles, (p.per + 1) >> 1, p.nsplit);
     const int t0 = min(tiles, w.split * per), t1 = min(tiles, t0 + per);
     const bool direct = tiles <= per;  // one split has all keys: it writes the result itself
     if (direct && w.split > 0) continue;

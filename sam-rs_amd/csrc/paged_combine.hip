@@ -4,8 +4,9 @@
 // first split is written already, which l = -1 says.
 //
 // What bounds it: the partial O's bytes, 4 a column and split, and, with few rows, the latency of reading them. Up to
-// eight splits a thread reads its four columns of each; past that a workgroup takes a row, its waves a share of the
-// splits each, and they meet in LDS.
+// eight splits a thread reads its four columns of each; past that a workgroup takes 32 columns of a row, its lanes a
+// share of the splits each, and they meet in LDS (16 rows of 128 columns and 256 splits: 15.4 us with a lane for each 4
+// columns and a wave for each 32 splits, COMBINEROW so).
 #include "paged.hpp"
 
 namespace samhip {
@@ -50,16 +51,26 @@ template <typename T> __global__ __launch_bounds__(256) void paged_combine_kerne
   store_row4<T>(p, tok, head, col, o, l);
 }
 
-constexpr int kRowWaves = 8, kMostSplits = 256;
+constexpr int kRowWaves = 8, kMostSplits = 256, kCols = 32;
 
-// A workgroup takes a row: weights of all splits first, then wave w the splits w, w + 8, ..., a lane 4 columns.
+// A workgroup takes 32 columns of a row: 8 lanes' 16 bytes of 64 splits at a time. Every partial result is on its way
+// before the weights are known, so that the two dependent reads overlap.
 template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_combine_row_kernel(PagedParams p) {
+  constexpr int kDeep = kMostSplits / (8 * kRowWaves);
   __shared__ float weight[kMostSplits], red[2][kRowWaves];
-  __shared__ __attribute__((aligned(16))) f32x4 part[kRowWaves][64];
+  __shared__ __attribute__((aligned(16))) f32x4 part[kRowWaves][8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long row = blockIdx.x, rows = (long)p.tokens * p.heads;
+  const int groups = (p.c.d + kCols - 1) / kCols;
+  const long row = blockIdx.x / groups, rows = (long)p.tokens * p.heads;
   const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
   if (!row_of_a_sequence(p, tok) || p.ml[2 * row + 1] < 0.f) return;
+  const int col = (int)(blockIdx.x % groups) * kCols + 4 * (lane & 7), s0 = 8 * wave + (lane >> 3);
+  f32x4 x[kDeep];
+#pragma unroll
+  for (int k = 0; k < kDeep; ++k) {
+    const long s = min(s0 + 64 * k, p.nsplit - 1);
+    if (64 * k < p.nsplit) x[k] = *reinterpret_cast<const f32x4*>(p.opart + (s * rows + row) * p.c.d + min(col, p.c.d - 4));
+  }
   const int s = threadIdx.x;
   float2 ml = {-INFINITY, 0.f};
   if (s < p.nsplit) ml = *reinterpret_cast<const float2*>(p.ml + 2 * (s * rows + row));
@@ -72,7 +83,7 @@ template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_co
   for (int k = 0; k < kRowWaves; ++k) top = fmaxf(top, red[0][k]);
   const float base = top == -INFINITY ? 0.f : top;
   const float w = ml.y == 0.f ? 0.f : exp2_fast(ml.x - base);
-  if (s < p.nsplit) weight[s] = ml.y == 0.f ? -1.f : w;  // -1: no keys, its O was not written
+  if (s < kMostSplits) weight[s] = ml.y == 0.f ? -1.f : w;  // -1: no keys, its O was not written
   float l = ml.y == 0.f ? 0.f : ml.y * w;
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) l += __shfl_xor(l, k);
@@ -81,18 +92,21 @@ template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_co
   l = 0.f;
 #pragma unroll
   for (int k = 0; k < kRowWaves; ++k) l += red[1][k];
-  const int col = 4 * lane;
   f32x4 o = {};
-  if (col < p.c.d) {
-#pragma unroll 4
-    for (int k = wave; k < p.nsplit; k += kRowWaves) {
-      const float f = weight[k];
-      if (f >= 0.f || f != f) o += *reinterpret_cast<const f32x4*>(p.opart + (k * rows + row) * p.c.d + col) * f;
+#pragma unroll
+  for (int k = 0; k < kDeep; ++k) {
+    if (64 * k < p.nsplit) {
+      const float f = weight[s0 + 64 * k];
+      if (f != -1.f) o += x[k] * f;
     }
   }
-  part[wave][lane] = o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int k = 8; k < 64; k *= 2) o[j] += __shfl_xor(o[j], k);
+  if (lane < 8) part[wave][lane] = o;
   __syncthreads();
-  if (wave != 0 || col >= p.c.d) return;
+  if (threadIdx.x >= 8 || col >= p.c.d) return;
 #pragma unroll
   for (int k = 1; k < kRowWaves; ++k) o += part[k][lane];
   store_row4<T>(p, tok, head, col, o, l);
@@ -102,7 +116,8 @@ template <typename T> hipError_t combine(const PagedParams& p, hipStream_t strea
   const long rows = (long)p.tokens * p.heads;
   if (p.nsplit > 8) {
     static_assert(kMostSplits <= 64 * kRowWaves, "a thread for each split");
-    hipLaunchKernelGGL(paged_combine_row_kernel<T>, dim3((unsigned)rows), dim3(64 * kRowWaves), 0, stream, p);
+    const long blocks = rows * ((p.c.d + kCols - 1) / kCols);
+    hipLaunchKernelGGL(paged_combine_row_kernel<T>, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, stream, p);
   } else {
     const long threads = rows * (p.c.d / 4);
     hipLaunchKernelGGL(paged_combine_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p);
