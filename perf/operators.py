@@ -23,12 +23,10 @@ E4M3_MAX = 448.0
 
 
 def _hip():
-    path = os.path.abspath("sam-rs_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
-    import sam_hip
-
-    return sam_hip
+    if "sam_hip" not in sys.modules:  # a program imports it once
+        sys.path.insert(0, os.path.abspath("sam-rs_amd"))
+        import sam_hip  # noqa: F401
+    return sys.modules["sam_hip"]
 
 
 def listed():
