@@ -36,7 +36,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 template <typename T, typename C, int DP, int RB>
-__global__ __launch_bounds__(256, DP * RB > 128 ? 1 : 2) void paged_few_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C, e4m3) ? 2 : 3) void paged_few_kernel(PagedParams p) {
   typedef typename Vec<T>::x8 X8;
   constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
   constexpr int TR = 16 * RB, NK = DP / 32;
