@@ -11,6 +11,7 @@
 //
 // What bounds it: the f32 matrix rate (64 flops a cycle and SIMD) where many rows share the keys, else the bytes of
 // K and V. 16 rows use each value loaded for 8 flops a byte, twice what L1 would need to keep up.
+#include "lds_dma.hpp"
 #include "paged.hpp"
 
 namespace samhip {
@@ -21,32 +22,38 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Four consecutive elements as f32.
-__device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
-__device__ __forceinline__ f32x4 load4(const e4m3* p) {
+// Four elements of a cache row as they lie there, and as f32 (times their row's scale).
+template <typename C> struct Raw4 {
+  typedef f32x4 t;
+};
+template <> struct Raw4<e4m3> {
+  typedef int t;
+};
+__device__ __forceinline__ f32x4 widen(f32x4 x, float) { return x; }
+__device__ __forceinline__ f32x4 widen(int c, float s) {
   typedef float f2 __attribute__((ext_vector_type(2)));
-  const int c = *reinterpret_cast<const int*>(p);
   const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-  return f32x4{a[0], a[1], b[0], b[1]};
+  return f32x4{a[0] * s, a[1] * s, b[0] * s, b[1] * s};
 }
 
-template <typename T, typename C, int DP, int RB>
-__global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(PagedParams p) {
+template <typename C, int DP, int RB>
+__global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(PagedParams p) {
   constexpr int NC = DP / 16, ND = DP / 64, TR = 16 * RB;
   constexpr bool kScaled = __is_same(C, e4m3);
+  typedef typename Raw4<C>::t Raw;
   __shared__ float sm_m[2][TR], sm_l[2][TR];
   extern __shared__ __attribute__((aligned(16))) float sm_o[];  // [2][RB][DP / 4 * 64]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int d = p.c.d;
-  if (p.zero_rest) paged_zero_rest<T>(p);
+  if (p.zero_rest) paged_zero_rest<float>(p);
   const PagedWork w = paged_work(p);
   const int rows = w.lq * p.group;
   const C* kp = reinterpret_cast<const C*>(p.c.k);
   const C* vp = reinterpret_cast<const C*>(p.c.v);
 
   for (int rt = w.tile; (long)rt * TR < rows; rt += p.rtiles) {
-    long qoff[RB];
+    // hidden from the optimiser, which would keep every address derived from the lane in a register across tiles
+    const int lane = (int)opaque(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
     int limit[RB], tok[RB], head[RB];
     f32x4 qf[RB][NC];
 #pragma unroll
@@ -56,18 +63,18 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
       tok[rb] = w.s0 + t;
       head[rb] = w.head * p.group + (r - t * p.group);
       limit[rb] = p.causal ? max(0, min(w.len, w.len - w.lq + t + 1)) : w.len;
-      qoff[rb] = tok[rb] * p.sq[0] + head[rb] * p.sq[1];
+      const float* qr = reinterpret_cast<const float*>(p.q) + tok[rb] * p.sq[0] + head[rb] * p.sq[1];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int col = 16 * c + 4 * g;
-        qf[rb][c] = col < d ? load4(reinterpret_cast<const T*>(p.q) + qoff[rb] + col) : f32x4{};
+        qf[rb][c] = col < d ? *reinterpret_cast<const f32x4*>(qr + col) : f32x4{};
       }
     }
-    // the keys that the tile's last row sees; this split's blocks of 32 of them
-    const int tlast = (int)divide_magic(min((rt + 1) * TR, rows) - 1, p.gmagic, p.gshift);
-    const int most = p.causal ? max(0, min(w.len, w.len - w.lq + tlast + 1)) : w.len;
+    // the keys that the tile's first and last row see; this split's blocks of 32 of them
     const int tfirst = (int)divide_magic(rt * TR, p.gmagic, p.gshift);
+    const int tlast = (int)divide_magic(min((rt + 1) * TR, rows) - 1, p.gmagic, p.gshift);
     const int least = p.causal ? max(0, min(w.len, w.len - w.lq + tfirst + 1)) : w.len;
+    const int most = p.causal ? max(0, min(w.len, w.len - w.lq + tlast + 1)) : w.len;
     const int blocks = (most + 31) >> 5, per = paged_share(blocks, p.per, p.nsplit);
     const int b0 = min(blocks, w.split * per), b1 = min(blocks, b0 + per);
     const bool direct = blocks <= per;  // one split has all keys: it writes the result itself
@@ -82,48 +89,89 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
 #pragma unroll
       for (int i = 0; i < 4 * ND; ++i) o[rb][i] = f32x4{};
     }
-    for (int blk = b0 + wave; blk < b1; blk += 4) {
-      const int key0 = 32 * blk;
-      const bool part = key0 + 32 > least;
-      const int row = paged_row(p.c, w.b, w.head, key0 + (lane & 31), most);  // lane l looks key l % 32 up
-      const unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
-      float ks = 1.f, vs = 1.f;
-      if (kScaled && row >= 0) {
-        ks = pow2_of(p.c.ks[row]);
-        vs = pow2_of(p.c.vs[row]);
-      }
-      f32x4 s[RB][2];
+    // lane l looks key l % 32 of a block up; rows that are not there read row 0 and are masked (K) or cleared (V)
+    auto entry_of = [&](int blk) { return paged_entry(p.c, w.b, 32 * min(blk, b1 - 1) + (lane & 31), most); };
+    const unsigned at_n = opaque(4 * n), at_g = opaque(16 * g);  // lanes n and 4 g, as bpermute addresses
+    auto from_n = [&](int i, int v) { return __builtin_amdgcn_ds_bpermute((int)at_n + 64 * i, v); };
+    auto from_key = [&](int j, int v) {  // the lane whose own key is 16 (j / 4) + 4 g + j % 4
+      return __builtin_amdgcn_ds_bpermute((int)at_g + 64 * (j >> 2) + 4 * (j & 3), v);
+    };
+    Raw kx[2][NC], vx[8][ND];
+    unsigned char ksx = 127, vsx = 127;
+    auto load_k = [&](int row) {
+      if constexpr (kScaled) ksx = p.c.ks[max(row, 0)];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const long kr = __shfl(row, 16 * i + n);
+        const C* kr = kp + (long)max(from_n(i, row), 0) * d;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) s[rb][i] = f32x4{};
+        for (int c = 0; c < NC; ++c) kx[i][c] = *reinterpret_cast<const Raw*>(kr + min(16 * c + 4 * g, d - 4));
+      }
+    };
+    auto load_v = [&](int row) {
+      if constexpr (kScaled) vsx = p.c.vs[max(row, 0)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const C* vr = vp + (long)max(from_key(j, row), 0) * d;
+#pragma unroll
+        for (int q = 0; q < ND; ++q) vx[j][q] = *reinterpret_cast<const Raw*>(vr + min(64 * q + 4 * n, d - 4));
+      }
+    };
+    // Table entries two blocks ahead, K one, V while its block's scores are made
+    int row = -1;
+    PagedEntry coming = {-1, -1};
+    if (b0 + wave < b1) {
+      const PagedEntry first = entry_of(b0 + wave);
+      coming = entry_of(b0 + wave + 4);
+      row = paged_row(p.c, first, w.head);
+      load_k(row);
+    }
+    // Q is here: told to the compiler, whose own wait for it would stand in the loop, behind the next block's loads
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    for (int blk = b0 + wave; blk < b1; blk += 4) {
+      const int key0 = 32 * blk;
+      const int next = paged_row(p.c, coming, w.head);
+      coming = entry_of(blk + 8);
+      load_v(row);
+      const unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
+      const bool part = key0 + 32 > least || there != 0xffffffffu;
+      const unsigned mine = there >> (4 * g);  // bit 16 i + e: the lane's key 16 i + 4 g + e
+      f32x4 s[RB][2];
+      const float kso = kScaled ? pow2_of(ksx) : 1.f;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) s[rb][0] = s[rb][1] = f32x4{};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float f = 1.f;
+        if constexpr (kScaled) f = __int_as_float(from_n(i, __float_as_int(kso)));
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const int col = 16 * c + 4 * g;
-          const f32x4 a = kr >= 0 && col < d ? load4(kp + kr * d + col) : f32x4{};
+          f32x4 a = widen(kx[i][c], f);
+          if (16 * c + 16 > d && 16 * c + 4 * g >= d) a = f32x4{};
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[rb][i] = mma4(a[j], qf[rb][c][j], s[rb][i]);
+            for (int rb = 0; rb < RB; ++rb) s[rb][i] = mma4(a[j], qf[rb][c][j], s[rb][i]);
         }
       }
+      if (blk + 4 < b1) load_k(next);
       // s[rb][i][e]: key key0 + 16 i + 4 g + e, row 16 rb + n
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
+        if (part) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int kk = 16 * i + e;
+              s[rb][i][e] = kk < limit[rb] - key0 - 4 * g && (mine >> kk & 1) ? s[rb][i][e] : -INFINITY;
+            }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int kk = 16 * i + 4 * g + e;
-            const bool sees = key0 + kk < limit[rb] && (there >> kk & 1);
-            const float f = kScaled ? __shfl(ks, kk) : 1.f;
-            s[rb][i][e] = sees ? s[rb][i][e] * (p.sc * f) : -INFINITY;
-            top = max_nc(top, s[rb][i][e]);
-          }
-        top = max_over_rows16(top);
-        const float mn = fmaxf(m[rb], top);
+          for (int e = 0; e < 4; ++e) top = max_nc(top, s[rb][i][e]);
+        const float mn = fmaxf(m[rb], max_over_rows16(top) * p.sc);
         const float base = mn == -INFINITY ? 0.f : mn;
         const float alpha = exp2_fast(m[rb] - base);
         m[rb] = mn;
@@ -134,50 +182,60 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[rb][i][e] = exp2_fast(s[rb][i][e] - base);
+            s[rb][i][e] = exp2_fast(s[rb][i][e] * p.sc - base);
             l[rb] += s[rb][i][e];
           }
       }
+      bool odd = false;
+      const float vso = kScaled ? pow2_of(vsx) : 1.f;
+      float vs[8];
+      if constexpr (kScaled) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 8; ++j) vs[j] = __int_as_float(from_key(j, __float_as_int(vso)));
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int kk = 16 * i + 4 * g + e;
-          const long vr = __shfl(row, kk);
-          const float f = kScaled ? __shfl(vs, kk) : 1.f;
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int q = 0; q < ND; ++q) {
-            const int col = 64 * q + 4 * n;
-            f32x4 a = vr >= 0 && col < d ? load4(vp + vr * d + col) : f32x4{};
-            // a value that is not finite must not reach the rows that do not see its key (0 * inf = NaN): where the
-            // block's keys are not seen by every row, such values are taken out, and the rows that see one get
-            // inf for +inf, -inf for -inf and both for NaN, counted on the matrix unit
-            bool odd = false;
-            if (part) {
+        for (int q = 0; q < ND; ++q) {
+          f32x4 a = widen(vx[j][q], kScaled ? vs[j] : 1.f);
+          if (part) {  // rows that are not there hold anything; values that are not finite go apart
+            const bool ok = mine >> (16 * (j >> 2) + (j & 3)) & 1;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) odd |= !(fabsf(a[j]) < INFINITY);
+            for (int i = 0; i < 4; ++i) {
+              const bool fin = fabsf(a[i]) < INFINITY;
+              odd |= ok && !fin;
+              a[i] = ok && fin ? a[i] : 0.f;
             }
-            if (part && wave_any(odd)) {
+          }
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float up = !(a[j] < INFINITY) ? 1.f : 0.f, down = !(a[j] > -INFINITY) ? 1.f : 0.f;
-                a[j] = up + down > 0.f ? 0.f : a[j];
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                  const float sees = key0 + kk < limit[rb] ? 1.f : 0.f;
-                  const f32x4 hi = mma4(up, sees, f32x4{}), lo = mma4(down, sees, f32x4{});
+            for (int rb = 0; rb < RB; ++rb) o[rb][4 * q + i] = mma4(a[i], s[rb][j >> 2][j & 3], o[rb][4 * q + i]);
+        }
+      if (wave_any(odd)) {
+        // A value that is not finite must not reach the rows that do not see its key (0 * inf = NaN): it was taken out
+        // above, and the rows that see it add it here
+        for (int kk = 0; kk < 32; ++kk) {
+          if (!(there >> kk & 1)) continue;
+          const int kr = __shfl(row, kk);
+          const float f = kScaled ? pow2_of(p.c.vs[kr]) : 1.f;
 #pragma unroll
-                  for (int k = 0; k < 4; ++k)
-                    o[rb][4 * q + j][k] += (hi[k] > 0.f ? INFINITY : 0.f) + (lo[k] > 0.f ? -INFINITY : 0.f);
-                }
+          for (int q = 0; q < ND; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int col = 64 * q + 16 * g + 4 * e;
+              if (col < d) {
+                const f32x4 x = widen(*reinterpret_cast<const Raw*>(vp + (long)kr * d + col), f);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    o[rb][4 * q + j][e] += key0 + kk < limit[rb] && !(fabsf(x[j]) < INFINITY) ? x[j] : 0.f;
               }
             }
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) o[rb][4 * q + j] = mma4(a[j], s[rb][i][e] * f, o[rb][4 * q + j]);
-          }
         }
+      }
+      row = next;
     }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) l[rb] = sum_over_rows16(l[rb]);
@@ -222,17 +280,17 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
           *reinterpret_cast<float2*>(p.ml + 2 * row) = direct ? float2{0.f, -1.f} : float2{m[rb], l[rb]};
         if (direct) {
           const float inv = l[rb] == 0.f ? 0.f : 1.f / l[rb];  // a row that sees no key is 0
-          T* orow = reinterpret_cast<T*>(p.out) + tok[rb] * p.so[0] + head[rb] * p.so[1];
+          float* orow = reinterpret_cast<float*>(p.out) + tok[rb] * p.so[0] + head[rb] * p.so[1];
 #pragma unroll
           for (int q = 0; q < ND; ++q)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int col = 64 * q + 16 * g + 4 * e;
               if (col >= d) continue;
-              typename Vec<T>::x4 x;
+              f32x4 x;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(f32_result(o[rb][4 * q + j][e] * inv));
-              *reinterpret_cast<typename Vec<T>::x4*>(orow + col) = x;
+              for (int j = 0; j < 4; ++j) x[j] = o[rb][4 * q + j][e] * inv;
+              *reinterpret_cast<f32x4*>(orow + col) = x;
             }
         } else if (b0 < b1) {
 #pragma unroll
@@ -251,25 +309,25 @@ __global__ __launch_bounds__(256, DP * RB <= 128 ? 2 : 1) void paged_f32_kernel(
   }
 }
 
-template <typename T, typename C, int DP, int RB> hipError_t launch_f32(const PagedParams& p, hipStream_t stream) {
+template <typename C, int DP, int RB> hipError_t launch_f32(const PagedParams& p, hipStream_t stream) {
   constexpr int lds = 2 * RB * (DP / 4) * 64 * 4;
   static_assert(lds <= 64 << 10, "the joining buffer");
   const long blocks = (long)p.rtiles * p.nsplit * p.c.heads * p.c.batch;
-  hipLaunchKernelGGL((paged_f32_kernel<T, C, DP, RB>), dim3((unsigned)blocks), dim3(256), lds, stream, p);
+  hipLaunchKernelGGL((paged_f32_kernel<C, DP, RB>), dim3((unsigned)blocks), dim3(256), lds, stream, p);
   return hipGetLastError();
 }
-template <typename T, typename C> hipError_t by_size(const PagedParams& p, int rows, hipStream_t stream) {
+template <typename C> hipError_t by_size(const PagedParams& p, int rows, hipStream_t stream) {
   const int d = p.c.d;
   if (rows == 16)
-    return d <= 64 ? launch_f32<T, C, 64, 1>(p, stream)
-                   : d <= 128 ? launch_f32<T, C, 128, 1>(p, stream) : launch_f32<T, C, 256, 1>(p, stream);
-  return d <= 64 ? launch_f32<T, C, 64, 2>(p, stream) : launch_f32<T, C, 128, 2>(p, stream);
+    return d <= 64 ? launch_f32<C, 64, 1>(p, stream)
+                   : d <= 128 ? launch_f32<C, 128, 1>(p, stream) : launch_f32<C, 256, 1>(p, stream);
+  return d <= 64 ? launch_f32<C, 64, 2>(p, stream) : launch_f32<C, 128, 2>(p, stream);
 }
 
 }  // namespace
 
 hipError_t paged_f32(int cache_dtype, const PagedParams& p, int rows, hipStream_t stream) {
-  return cache_dtype == kE4M3 ? by_size<float, e4m3>(p, rows, stream) : by_size<float, float>(p, rows, stream);
+  return cache_dtype == kE4M3 ? by_size<e4m3>(p, rows, stream) : by_size<float>(p, rows, stream);
 }
 
 }  // namespace samhip
