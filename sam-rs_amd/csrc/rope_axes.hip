@@ -28,12 +28,17 @@ struct RopeAxesParams {
   int l, h, d, pairs, naxes;
   int halves, copy;  // copy: columns past 2 * pairs are to be written too
   int units, hgroups;  // vectors (or elements) of a head to handle, groups of heads
-  long total;        // b * l * units * hgroups threads
+  unsigned umagic, ushift, hmagic, hshift, lmagic, lshift;  // divisions by units, hgroups and l
+  long tok0;  // this launch's first token
+  int ntok;   // its tokens
+  int groups;  // of a thread's tokens
+  int total;  // threads: groups * hgroups * units, in this order of their digits
   float sign;
 };
 
+// Cosine and sine (times sign) of pos * freq turns.
 __device__ __forceinline__ void turn_of(double freq, int pos, float sign, float& c, float& s) {
-  const double t = (double)pos * (freq * 0.15915494309189533577);
+  const double t = (double)pos * freq;
   const float f = (float)(t - rint(t));       // turns, -1/2 .. 1/2
   const float k = rintf(4.f * f);
   const float y = 6.2831853071795864769f * (f - 0.25f * k), y2 = y * y;  // f - k / 4 is exact
@@ -67,75 +72,96 @@ template <typename T> __device__ __forceinline__ void turn(T& a, T& b, float c, 
   b = from_f32<T>(f32_result(fmaf(x1, c, x0 * s)));
 }
 
-// Vectors of 8 elements; a thread's HP heads are hgroups apart, so that they are in flight together.
-template <typename T, int HP>
+// Vectors of 8 elements: a thread takes one unit of NT tokens and HP heads of each, the tokens `groups` apart and the
+// heads hgroups, so that all their loads are in flight together. The positions of up to four axes are loaded before it is
+// known which of them the pairs want (AX; with more, after that).
+template <typename T, int HP, int NT, bool AX>
 __global__ __launch_bounds__(256) void rope_axes_vec(RopeAxesParams p) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= p.total) return;
-  const int u = (int)(i % p.units);
-  const long r = i / p.units;
-  const int hg = (int)(r % p.hgroups);
-  const long tok = r / p.hgroups;
-  const long bi = tok / p.l, li = tok % p.l;
-  const T* xr = reinterpret_cast<const T*>(p.x) + bi * p.sx[0] + li * p.sx[1];
-  T* yr = reinterpret_cast<T*>(p.out) + bi * p.so[0] + li * p.so[1];
+  const int r = (int)divide_magic((unsigned)i, p.umagic, p.ushift), u = i - r * p.units;
+  const int tg = (int)divide_magic((unsigned)r, p.hmagic, p.hshift), hg = r - tg * p.hgroups;
   const int turning = p.halves ? p.pairs / 8 : p.pairs / 4;
   const bool still = u >= turning;
   const int c0 = still ? 2 * p.pairs + 8 * (u - turning) : 8 * u;
   const int c1 = c0 + (p.halves && !still ? p.pairs : 0);  // the partners' columns
-  Vec8<T> a[HP], b[HP];
+  const int first = p.halves ? 8 * u : 4 * u;              // the unit's first pair
+  constexpr int NP = 8;
+  Vec8<T> a[NT][HP], b[NT][HP];
+  long from[NT], to[NT];
+  const int* pr[NT];
+  int at[NT][4];
 #pragma unroll
-  for (int k = 0; k < HP; ++k) {
-    const int h = hg + k * p.hgroups;
-    if (h < p.h) {
-      a[k] = load8(xr + h * p.sx[2] + c0);
-      if (c1 != c0) b[k] = load8(xr + h * p.sx[2] + c1);
+  for (int k = 0; k < NT; ++k) {
+    const long tok = p.tok0 + min(tg + (long)k * p.groups, p.ntok - 1);
+    const long bi = divide_magic((unsigned)tok, p.lmagic, p.lshift), li = tok - bi * p.l;
+    from[k] = bi * p.sx[0] + li * p.sx[1];
+    to[k] = bi * p.so[0] + li * p.so[1];
+    pr[k] = p.pos + bi * p.sp[0] + li * p.sp[1];
+    if (AX) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) at[k][x] = pr[k][min(x, p.naxes - 1) * p.sp[2]];
     }
   }
+#pragma unroll
+  for (int k = 0; k < NT; ++k)
+#pragma unroll
+    for (int j = 0; j < HP; ++j) {
+      const long h = min(hg + j * p.hgroups, p.h - 1);
+      a[k][j] = load8(reinterpret_cast<const T*>(p.x) + from[k] + h * p.sx[2] + c0);
+      if (c1 != c0) b[k][j] = load8(reinterpret_cast<const T*>(p.x) + from[k] + h * p.sx[2] + c1);
+    }
   if (!still) {
-    const int* pr = p.pos + bi * p.sp[0] + li * p.sp[1];
-    if (p.halves) {
-      float c[8], s[8];
+    double f[NP];
+    int ax[NP];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int ax = p.axes[8 * u + j];
-        turn_of(p.freqs[8 * u + j], (unsigned)ax < (unsigned)p.naxes ? pr[ax * p.sp[2]] : 0, p.sign, c[j], s[j]);
+    for (int j = 0; j < NP; ++j)
+      if (j < 4 || p.halves) {
+        f[j] = p.freqs[first + j] * 0.15915494309189533577;  // turns per unit of position
+        ax[j] = p.axes[first + j];
       }
 #pragma unroll
-      for (int k = 0; k < HP; ++k)
+    for (int k = 0; k < NT; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) turn(a[k].v[j], b[k].v[j], c[j], s[j]);
-    } else {
-      float c[4], s[4];
+      for (int j = 0; j < NP; ++j)
+        if (j < 4 || p.halves) {
+          int x = 0;
+          if ((unsigned)ax[j] < (unsigned)p.naxes) {
+            if (AX)
+              x = ax[j] & 2 ? (ax[j] & 1 ? at[k][3] : at[k][2]) : (ax[j] & 1 ? at[k][1] : at[k][0]);
+            else
+              x = pr[k][ax[j] * p.sp[2]];
+          }
+          float c, s;
+          turn_of(f[j], x, p.sign, c, s);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int ax = p.axes[4 * u + j];
-        turn_of(p.freqs[4 * u + j], (unsigned)ax < (unsigned)p.naxes ? pr[ax * p.sp[2]] : 0, p.sign, c[j], s[j]);
+          for (int m = 0; m < HP; ++m) {
+            if (p.halves)
+              turn(a[k][m].v[j], b[k][m].v[j], c, s);
+            else
+              turn(a[k][m].v[2 * j & 7], a[k][m].v[(2 * j & 7) + 1], c, s);
+          }
+        }
+  }
+#pragma unroll
+  for (int k = 0; k < NT; ++k)
+#pragma unroll
+    for (int j = 0; j < HP; ++j) {
+      const int h = hg + j * p.hgroups;
+      if (h < p.h && tg + (long)k * p.groups < p.ntok) {
+        store8(reinterpret_cast<T*>(p.out) + to[k] + h * p.so[2] + c0, a[k][j]);
+        if (c1 != c0) store8(reinterpret_cast<T*>(p.out) + to[k] + h * p.so[2] + c1, b[k][j]);
       }
-#pragma unroll
-      for (int k = 0; k < HP; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) turn(a[k].v[2 * j], a[k].v[2 * j + 1], c[j], s[j]);
     }
-  }
-#pragma unroll
-  for (int k = 0; k < HP; ++k) {
-    const int h = hg + k * p.hgroups;
-    if (h < p.h) {
-      store8(yr + h * p.so[2] + c0, a[k]);
-      if (c1 != c0) store8(yr + h * p.so[2] + c1, b[k]);
-    }
-  }
 }
 
 // Any sizes and strides: a thread takes one pair, or one column past the pairs, of every head of its token.
 template <typename T>
 __global__ __launch_bounds__(256) void rope_axes_any(RopeAxesParams p) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= p.total) return;
-  const int u = (int)(i % p.units);
-  const long tok = i / p.units;
-  const long bi = tok / p.l, li = tok % p.l;
+  const int t = (int)divide_magic((unsigned)i, p.umagic, p.ushift), u = i - t * p.units;
+  const long tok = p.tok0 + t, bi = divide_magic((unsigned)tok, p.lmagic, p.lshift), li = tok - bi * p.l;
   const T* xr = reinterpret_cast<const T*>(p.x) + bi * p.sx[0] + li * p.sx[1];
   T* yr = reinterpret_cast<T*>(p.out) + bi * p.so[0] + li * p.so[1];
   if (u >= p.pairs) {
@@ -145,8 +171,8 @@ __global__ __launch_bounds__(256) void rope_axes_any(RopeAxesParams p) {
   }
   const int c0 = p.halves ? u : 2 * u, c1 = p.halves ? u + p.pairs : 2 * u + 1, ax = p.axes[u];
   float c, s;
-  turn_of(p.freqs[u], (unsigned)ax < (unsigned)p.naxes ? p.pos[bi * p.sp[0] + li * p.sp[1] + ax * p.sp[2]] : 0, p.sign,
-          c, s);
+  turn_of(p.freqs[u] * 0.15915494309189533577,
+          (unsigned)ax < (unsigned)p.naxes ? p.pos[bi * p.sp[0] + li * p.sp[1] + ax * p.sp[2]] : 0, p.sign, c, s);
   for (int h = 0; h < p.h; ++h) {
     T a = xr[h * p.sx[2] + c0], b = xr[h * p.sx[2] + c1];
     turn(a, b, c, s);
@@ -162,22 +188,37 @@ template <typename T> hipError_t launch(RopeAxesParams p, long tokens, hipStream
   };
   const int rest = p.copy ? p.d - 2 * p.pairs : 0;
   const bool vec = vec_ok(p.x, p.sx) && vec_ok(p.out, p.so) && p.pairs % (p.halves ? 8 : 4) == 0 && rest % 8 == 0;
-  if (!vec) {
-    p.units = p.pairs + rest;
-    p.hgroups = 1;
-    p.total = tokens * p.units;
-    hipLaunchKernelGGL(rope_axes_any<T>, dim3((unsigned)((p.total + 255) / 256)), dim3(256), 0, stream, p);
-    return hipGetLastError();
+  // Heads and tokens of a thread, once there are threads enough for the card. 41472 tokens of 16 heads of 64, f16: 4 and 2
+  // 37.6 us, 4 and 1 43.8, 2 and 2 37.5, 2 and 4 41.7 (a copy of the bytes 34.2); f32, 65536 of 8 heads of 80: 2 and 2 62.6,
+  // 4 and 2 69.0 (copy 63.4); one head of 256, 65536 tokens, bf16: 2 tokens 18.6, 4 20.7, 8 21.9, 1 25.7 (the angles; copy
+  // 10.5).
+  constexpr int kHeads = sizeof(T) == 4 ? 2 : 4;
+  const long work = tokens * (p.d / 8) * p.h;  // vectors of 8 elements
+  const int hp = vec && p.h >= 4 && work >= 1 << 17 ? kHeads : 1, nt = vec && work >= 1 << 19 ? 2 : 1;
+  p.units = vec ? p.pairs / (p.halves ? 8 : 4) + rest / 8 : p.pairs + rest;
+  p.hgroups = vec ? (p.h + hp - 1) / hp : 1;
+  division_magic(p.units, &p.umagic, &p.ushift);
+  division_magic(p.hgroups, &p.hmagic, &p.hshift);
+  division_magic(p.l, &p.lmagic, &p.lshift);
+  const long most = ((1l << 31) - 256) / ((long)p.units * p.hgroups);  // tokens of a launch: threads count in 32 bits
+  for (p.tok0 = 0; p.tok0 < tokens; p.tok0 += most) {
+    p.ntok = (int)(tokens - p.tok0 < most ? tokens - p.tok0 : most);
+    p.groups = (p.ntok + nt - 1) / nt;
+    p.total = p.groups * p.hgroups * p.units;
+    const dim3 grid((unsigned)((p.total + 255l) / 256));
+    auto run = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p); };
+    const bool ax = p.naxes <= 4;
+    if (!vec)
+      run(rope_axes_any<T>);
+    else if (hp > 1 && nt > 1)
+      ax ? run(rope_axes_vec<T, kHeads, 2, true>) : run(rope_axes_vec<T, kHeads, 2, false>);
+    else if (hp > 1)
+      ax ? run(rope_axes_vec<T, kHeads, 1, true>) : run(rope_axes_vec<T, kHeads, 1, false>);
+    else if (nt > 1)
+      ax ? run(rope_axes_vec<T, 1, 2, true>) : run(rope_axes_vec<T, 1, 2, false>);
+    else
+      ax ? run(rope_axes_vec<T, 1, 1, true>) : run(rope_axes_vec<T, 1, 1, false>);
   }
-  p.units = p.pairs / (p.halves ? 8 : 4) + rest / 8;
-  const bool four = p.h >= 4 && tokens * p.units * p.h >= 1 << 17;
-  p.hgroups = four ? (p.h + 3) / 4 : p.h;
-  p.total = tokens * p.units * p.hgroups;
-  const dim3 grid((unsigned)((p.total + 255) / 256));
-  if (four)
-    hipLaunchKernelGGL((rope_axes_vec<T, 4>), grid, dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL((rope_axes_vec<T, 1>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
