@@ -18,6 +18,8 @@ namespace samhip {
 
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 struct RopeAxesParams {
   const void* x;
   const int* pos;
@@ -48,6 +50,11 @@ __device__ __forceinline__ void turn_of(double freq, int pos, float sign, float&
   const float a = q & 1 ? -sn : cs, b = q & 1 ? cs : sn;
   c = q & 2 ? -a : a;
   s = sign * (q & 2 ? -b : b);
+}
+
+__device__ __forceinline__ int axis_of(i32x4 v, int i) {
+  const int lo = i & 1 ? v.y : v.x, hi = i & 1 ? v.w : v.z;
+  return i & 2 ? hi : lo;
 }
 
 template <typename T> struct Vec8 {
@@ -90,7 +97,7 @@ __global__ __launch_bounds__(256) void rope_axes_vec(RopeAxesParams p) {
   Vec8<T> a[NT][HP], b[NT][HP];
   long from[NT], to[NT];
   const int* pr[NT];
-  int at[NT][4];
+  i32x4 at[NT];  // a vector: an array here, picked from by the axis, went to LDS and cost 12 us in each launch
 #pragma unroll
   for (int k = 0; k < NT; ++k) {
     const long tok = p.tok0 + min(tg + (long)k * p.groups, p.ntok - 1);
@@ -128,7 +135,7 @@ __global__ __launch_bounds__(256) void rope_axes_vec(RopeAxesParams p) {
           int x = 0;
           if ((unsigned)ax[j] < (unsigned)p.naxes) {
             if (AX)
-              x = ax[j] & 2 ? (ax[j] & 1 ? at[k][3] : at[k][2]) : (ax[j] & 1 ? at[k][1] : at[k][0]);
+              x = axis_of(at[k], ax[j]);
             else
               x = pr[k][ax[j] * p.sp[2]];
           }
