@@ -9,11 +9,13 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
                      int max_len, int cus) {
   (void)cache_dtype;
   PagedPlan plan = {};
-  const long group = heads / kv_heads, rows = (long)std::max(max_q, 1) * group;
+  const long group = heads / kv_heads, rows = (long)std::max(std::min(max_q, tokens), 1) * group;
   plan.many = dtype != kF32 && rows > 32;
   plan.rows = plan.many ? 128 : rows <= 16 || d > 128 ? 16 : 32;
-  plan.rtiles = (int)((rows + plan.rows - 1) / plan.rows);
-  const long base = (long)plan.rtiles * kv_heads * batch;
+  // a workgroup goes on to further tiles: where max_q is far above most chunks, a million of them do
+  const long units = (long)kv_heads * batch, cap = std::max(1L, (1L << 20) / units);
+  plan.rtiles = (int)std::min((rows + plan.rows - 1) / plan.rows, cap);
+  const long base = plan.rtiles * units;
   if (plan.many) {
     // as many workgroups as run at once (three a CU up to head dim 64, two to 128, one past it), with four tiles of 64
     // keys a split at least
@@ -24,6 +26,7 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
     const long want = (8L * cus + base - 1) / base, most = ((long)max_len + 1023) / 1024;
     plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
   }
+  if ((long)tokens * heads * (d / 4) >= 1L << 32) plan.nsplit = 1;  // more than the joining launch has threads for
   const long blocks = ((long)max_len + 31) / 32;
   plan.per = (int)std::min((blocks + plan.nsplit - 1) / plan.nsplit, 1L << 26);
   if (plan.nsplit > 1) {

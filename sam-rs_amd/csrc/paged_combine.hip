@@ -114,9 +114,9 @@ template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_co
 
 template <typename T> hipError_t combine(const PagedParams& p, hipStream_t stream) {
   const long rows = (long)p.tokens * p.heads;
-  if (p.nsplit > 8) {
+  const long blocks = rows * ((p.c.d + kCols - 1) / kCols);
+  if (p.nsplit > 8 && blocks * 64 * kRowWaves < 1l << 32) {  // the threads of a launch count in 32 bits
     static_assert(kMostSplits <= 64 * kRowWaves, "a thread for each split");
-    const long blocks = rows * ((p.c.d + kCols - 1) / kCols);
     hipLaunchKernelGGL(paged_combine_row_kernel<T>, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, stream, p);
   } else {
     const long threads = rows * (p.c.d / 4);

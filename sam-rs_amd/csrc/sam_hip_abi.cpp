@@ -732,8 +732,9 @@ int sam_hip_kv_write(const void* k, const void* v, void* k_pages, void* v_pages,
       rc != SAM_HIP_OK)
     return rc;
   c.starts = starts;
-  if (tokens < 0 || (long)tokens * kv_heads >= 1L << 31)
-    return fail(SAM_HIP_EINVAL, "kv-write: %d tokens of %d heads", tokens, kv_heads);
+  if (tokens < 0) return fail(SAM_HIP_EINVAL, "kv-write: %d tokens", tokens);
+  if ((long)tokens * kv_heads >= 1L << 27)  // up to 32 threads a row, which a launch counts in 32 bits
+    return fail(SAM_HIP_EUNSUPPORTED, "kv-write: too many rows (tokens=%d heads=%d)", tokens, kv_heads);
   long sk[2], sv[2];
   if (int rc = token_strides("kv-write", "k", strides_k, sk, kv_heads, d, dtype); rc != SAM_HIP_OK) return rc;
   if (int rc = token_strides("kv-write", "v", strides_v, sv, kv_heads, d, dtype); rc != SAM_HIP_OK) return rc;
@@ -754,7 +755,7 @@ int sam_hip_kv_read(void* k, void* v, const void* k_pages, const void* v_pages, 
       rc != SAM_HIP_OK)
     return rc;
   if (max_len < 0) return fail(SAM_HIP_EINVAL, "kv-read: max_len %d", max_len);
-  if ((long)batch * max_len >= 1L << 31 || (long)batch * max_len * kv_heads >= 1L << 33)  // 8 rows or more a workgroup
+  if ((long)batch * max_len >= 1L << 27 || (long)batch * max_len * kv_heads >= 1L << 27)  // up to 32 threads a row
     return fail(SAM_HIP_EUNSUPPORTED, "kv-read: too many rows (batch=%d max_len=%d heads=%d)", batch, max_len, kv_heads);
   if (!aligned16(k) || !aligned16(v)) return fail(SAM_HIP_EUNSUPPORTED, "kv-read: k and v must be 16-byte aligned");
   return check_launch(samhip::kv_read(dtype, cache_dtype, k, v, c, max_len, reinterpret_cast<hipStream_t>(stream)),
@@ -801,7 +802,7 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
                 workspace ? workspace_bytes : 0L);
   if (plan.total > 0 && !aligned16(workspace))
     return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: the workspace must be 16-byte aligned");
-  if ((long)plan.rtiles * plan.nsplit * kv_heads * batch > 0x7fffffffL)
+  if ((long)plan.rtiles * plan.nsplit * kv_heads * batch >= 1L << 24)
     return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: too many workgroups (max_q=%d batch=%d)", max_q, batch);
   if (tokens == 0) return ok();
   p.c.starts = starts;

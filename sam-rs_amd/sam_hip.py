@@ -621,7 +621,7 @@ _E4M3 = 3  # SAM_HIP_E4M3
 
 # The calls below are made once a layer and token, where the host's time counts: an index in place of a device object
 # (0.1 against 0.2 us), no views or stride arrays for contiguous operands (1.5 and 0.3 us each), empty_like (1.2 us; empty
-# 3.5). rope_axes, kv_write, kv_read and paged_attention took the host 12, 10, 13 and 18 us with, HOSTTIMES without.
+# 3.5). rope_axes, kv_write, kv_read and paged_attention took the host 12, 10, 13 and 18 us with, 8, 8, 10 and 10 without.
 
 
 def _device_of(what: str, *ts) -> int:
@@ -636,6 +636,13 @@ def _device_of(what: str, *ts) -> int:
                 raise SamHipError("sam-rs HIP kernels need device tensors")
         raise SamHipError(f"{what}: all operands must be on one device, got {[str(t.device) for t in ts if t is not None]}")
     return dev
+
+
+def _sizes(what: str, *sizes) -> None:
+    """The C calls take sizes as 32-bit numbers."""
+    for n in sizes:
+        if n >> 31:
+            raise SamHipError(f"{what}: sizes must be below 2^31, got {sizes}")
 
 
 def _is_current(dev: int) -> bool:
@@ -680,6 +687,8 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, axes: tor
     n, at = freqs.shape, pos.shape
     if len(n) != 1 or axes.shape != n or 2 * n[0] > d:
         raise SamHipError(f"rope_axes: freqs {tuple(n)} and axes {tuple(axes.shape)} must be [P], 2 P <= {d}")
+    if (b | l | h | d) >> 31:
+        _sizes("rope_axes", b, l, h, d)
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != x.dtype:
@@ -736,7 +745,11 @@ def _pool(what, k_pages, v_pages, k_scale, v_scale, table, starts, lens, dtype):
         raise SamHipError(f"{what}: lens must be int32 [{b}], got {lens.dtype} {tuple(lens.shape)}")
     if starts is not None and (starts.dtype != torch.int32 or starts.shape != (b + 1,)):
         raise SamHipError(f"{what}: starts must be int32 [{b + 1}], got {starts.dtype} {tuple(starts.shape)}")
-    return (code, *shape, *rows)
+    pages, heads, page, d = shape
+    width = rows[1]
+    if (pages | heads | page | d | b | width) >> 31:
+        _sizes(what, pages, heads, page, d, b, width)
+    return code, pages, heads, page, d, b, width
 
 
 def _overlaps_itself(t):
@@ -780,13 +793,16 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: t
     shape = k.shape
     if len(shape) != 3 or shape != v.shape or shape[1] != heads or shape[2] != d:
         raise SamHipError(f"kv_write: k and v must be [T, {heads}, {d}], got {tuple(shape)} and {tuple(v.shape)}")
-    if shape[0] == 0 or b == 0 or width == 0:
+    tokens = shape[0]
+    if tokens == 0 or b == 0 or width == 0:
         return
+    if tokens >> 31:
+        _sizes("kv_write", tokens)
     table, starts, lens = _plain(table), _plain(starts), _plain(lens)
     (k, sk), (v, sv) = _token_rows(k), _token_rows(v)
     _check(load().sam_hip_kv_write(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
                                    _ptr(v_scale), table.data_ptr(), starts.data_ptr(), lens.data_ptr(), dt, code,
-                                   shape[0], b, pages, heads, page, d, width, sk, sv, _stream()))
+                                   tokens, b, pages, heads, page, d, width, sk, sv, _stream()))
 
 
 def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int,
@@ -805,6 +821,8 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, l
     max_len = int(max_len)
     if max_len < 0:
         raise SamHipError(f"kv_read: max_len must not be negative, got {max_len}")
+    if max_len >> 31:
+        _sizes("kv_read", max_len)
     k, v = k_pages.new_empty((2, b, max_len, heads, d), dtype=dtype).unbind()
     if width == 0:
         return k.zero_(), v.zero_()
@@ -835,7 +853,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     or, causal, those up to its own position. Query head h reads key head h // (Hq // heads). scale defaults to D^-0.5.
     max_q and max_len, the longest chunk and sequence (default: T and what the table can name), shape the launch; a
     call whose sequences exceed them is slower, not wrong. A row that sees no key is 0. Rows of no sequence are 0, or as
-    they were in an `out` that is given."""
+    they were in an `out` that is given, which must not overlap the other tensors."""
     dev = _device_of("paged_attention", q, k_pages, v_pages, table, starts, lens, k_scale, v_scale, out)
     if not _is_current(dev):
         with torch.cuda.device(dev):
@@ -866,8 +884,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table, starts, lens = _plain(table), _plain(starts), _plain(lens)
     q, sq = _token_rows(q)
     scale = float(d) ** -0.5 if scale is None else float(scale)
-    max_q = tokens if max_q is None else int(max_q)
-    max_len = width * page if max_len is None else int(max_len)
+    if tokens >> 31:
+        _sizes("paged_attention", tokens)
+    max_q = tokens if max_q is None else min(int(max_q), tokens)
+    max_len = width * page if max_len is None else min(int(max_len), width * page)
+    if (max_q | max_len) >> 31:
+        _sizes("paged_attention", max_q, max_len)
     ws_bytes = _paged_workspace(dev, dt, code, tokens, b, hq, heads, d, max_q, max_len)
     ws = q.new_empty(ws_bytes // q.element_size()) if ws_bytes else None
     _check(load().sam_hip_paged_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),

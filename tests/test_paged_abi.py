@@ -106,6 +106,13 @@ def test_paged_attention_refuses(lib, change, code):
     assert lib.sam_hip_last_error()
 
 
+def test_launches_past_32_bits_of_threads_are_refused(lib):
+    assert write(lib, tokens=1 << 26) == 3 and read(lib, max_len=1 << 25, batch=4) == 3
+    size = lib.sam_hip_paged_attention_workspace_size
+    # partial results that the joining launch has no threads for: no splits
+    assert size(1, 1, 1 << 26, 1, 2, 2, 128, 1, 1 << 20) == 0 < size(1, 1, 1 << 20, 1, 2, 2, 128, 1, 1 << 20)
+
+
 def test_a_missing_or_short_workspace_is_refused(lib):
     size = lib.sam_hip_paged_attention_workspace_size
     need = size(1, 1, 1, 1, 8, 1, 128, 1, 1 << 16)

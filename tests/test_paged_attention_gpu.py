@@ -233,3 +233,30 @@ def test_refusals(hip):
         with pytest.raises(hip.SamHipError):
             call()
     assert c.run(hip, True, q=c.q[:0]).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_many_short_sequences_without_hints(hip, dtype):
+    """A launch shaped by T and the table's width alone, whose workgroups mostly have nothing to do or several tiles."""
+    chunks = [i * 7 % 9 for i in range(3000)]
+    c = Case(chunks, [n + i * 5 % 8 for i, n in enumerate(chunks)], 4, 1, 64, 8, dtype, False)
+    c.check(c.run(hip, True), True)
+
+
+def test_sizes_past_32_bits_are_refused(hip):
+    t = lambda *s, dt=torch.float16: torch.zeros(s, dtype=dt, device="cuda")
+    i = lambda *s: t(*s, dt=torch.int32)
+    big = 1 << 32
+    kp = t(1, 1, 8, 8)
+    with pytest.raises(hip.SamHipError, match="below 2\\^31"):
+        hip.paged_attention(t(1, 1, 8), kp, kp, i(1, 1).expand(1, big), i(2), i(1))
+    with pytest.raises(hip.SamHipError, match="below 2\\^31"):
+        hip.paged_attention(t(1, 1, 8), kp, kp, i(1, 1), i(2), i(1), max_q=-1)
+    with pytest.raises(hip.SamHipError, match="below 2\\^31"):
+        hip.kv_read(kp, kp, i(1, 1), i(1), big)
+    with pytest.raises(hip.SamHipError, match="below 2\\^31"):
+        hip.kv_write(t(1, 1, 8).expand(big, 1, 8), t(1, 1, 8).expand(big, 1, 8), kp, kp.clone(), i(1, 1), i(2), i(1))
+    with pytest.raises(hip.SamHipError, match="below 2\\^31"):
+        hip.rope_axes(t(1, 1, 8).expand(big, 1, 8), i(1, 1), t(4, dt=torch.float64), i(4))
+    assert hip.paged_attention(t(1, 1, 8), kp, kp, i(1, 1), torch.tensor([0, 1], dtype=torch.int32, device="cuda"),
+                               torch.ones(1, dtype=torch.int32, device="cuda"), max_q=big, max_len=big).shape == (1, 1, 8)
