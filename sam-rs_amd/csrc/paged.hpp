@@ -76,6 +76,7 @@ struct PagedParams {
   float sc;                   // scale * log2(e)
   int causal, zero_rest;
   int rtiles, nsplit;         // row tiles per (sequence, key head) of the grid; key splits
+  int round;                  // row tiles of one workgroup a CU (0: less than one)
   int per;                    // blocks of 32 keys per split, at least (0: even shares of what each sequence holds)
   float* opart;               // nsplit > 1: partial O [nsplit][tokens * heads][d], f32, not normalised
   float* ml;                  // nsplit > 1: running (max, sum) [nsplit][tokens * heads][2], log2 units; a sum of -1 in
@@ -84,11 +85,10 @@ struct PagedParams {
 
 // How a call runs: the kernel's rows per tile, the row tiles and key splits of its grid, its workspace.
 struct PagedPlan {
-  int many, rows, rtiles, nsplit, per;
+  int many, rows, rtiles, nsplit, per, round;
   long part_bytes, total;
 };
-PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
-                     int max_len, int cus);
+PagedPlan paged_plan(int dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q, int max_len, int cus);
 hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const PagedPlan& plan, hipStream_t stream);
 hipError_t paged_f32(int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
 hipError_t paged_few(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
@@ -162,7 +162,16 @@ __device__ __forceinline__ PagedWork paged_work(const PagedParams& p) {
   PagedWork w;
   w.split = lin / units % p.nsplit;
   w.tile = lin / (units * p.nsplit);
-  if (p.causal) w.tile = p.rtiles - 1 - w.tile;  // the tiles with most keys first
+  if (p.causal) {
+    // The tiles with most keys first, and every second round of one workgroup a CU in the other order, so that a CU's
+    // first two have as many keys together as any other's (workgroups i and i + 256 share a CU; 8192 tokens over their own
+    // keys, 8 heads of 128 in f16: 252 -> 227 us; 4 sequences of 2048 in bf16: 88 -> 81).
+    if (p.round > 0) {
+      const int from = w.tile / p.round * p.round, many = min(p.round, p.rtiles - from);
+      if (w.tile / p.round & 1) w.tile = 2 * from + many - 1 - w.tile;
+    }
+    w.tile = p.rtiles - 1 - w.tile;
+  }
   w.head = unit % p.c.heads;
   w.b = unit / p.c.heads;
   w.s0 = max(0, min(p.c.starts[w.b], p.tokens));

@@ -5,28 +5,37 @@
 
 namespace samhip {
 
-PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
-                     int max_len, int cus) {
-  (void)cache_dtype;
+PagedPlan paged_plan(int dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q, int max_len, int cus) {
   PagedPlan plan = {};
   const long group = heads / kv_heads, rows = (long)std::max(std::min(max_q, tokens), 1) * group;
+  // The many-row kernel past 32 rows a key head, which the other takes in two passes over the keys: 8 sequences of 8192, 8
+  // heads of 128 in f16, 33 rows each 56 against 110 us, 32 rows 55 against 62; at 64 42 against 52 and 41 against 35; 4 of 4
+  // heads of 256, 54 against 69 and 53 against 42; one of 65536 with 2 heads of 128 35 against 29 and 33 against 28.
   plan.many = dtype != kF32 && rows > 32;
+  // 32 rows a tile above 16 where registers allow it: the first of these calls at 17 rows 61 us against 90 with two tiles of
+  // 16, the third (which they do not) 42
   plan.rows = plan.many ? 128 : rows <= 16 || d > 128 ? 16 : 32;
   // a workgroup goes on to further tiles: where max_q is far above most chunks, a million of them do
   const long units = (long)kv_heads * batch, cap = std::max(1L, (1L << 20) / units);
   plan.rtiles = (int)std::min((rows + plan.rows - 1) / plan.rows, cap);
   const long base = plan.rtiles * units;
   if (plan.many) {
-    // as many workgroups as run at once (three a CU up to head dim 64, two to 128, one past it), with four tiles of 64
-    // keys a split at least
+    // As many workgroups as run at once (three a CU up to head dim 64, two to 128, one past it), with four tiles of 64
+    // keys a split at least. More only add partial results: six sequences of up to 7000 keys, 8 heads of 64, 1024 rows each,
+    // 155, 113, 115 and 120 us with 1, 2, 3 and 4 splits; 4096 rows over 28736 keys, 256, 229 and 315 with 8 and 16.
     const long slots = (d > 128 ? 1L : d > 64 ? 2L : 3L) * cus, most = ((long)max_len + 255) / 256;
     plan.nsplit = (int)std::max(1L, std::min(std::min(slots / base, most), 64L));
   } else {
-    // eight workgroups a CU, if every split then has eight blocks of 32 keys for each of its four waves
-    const long want = (8L * cus + base - 1) / base, most = ((long)max_len + 1023) / 1024;
+    // Eight workgroups a CU, so that sequences of different lengths share the card evenly, if every split then has eight
+    // blocks of 32 keys for each of its four waves: 32 sequences of up to 8192 keys, 8 key heads of 128 in e4m3, take 85, 87,
+    // 83, 93 and 97 us with 4, 6, 8, 12 and 16 splits; one of 131072, 2 heads of 128 in f16, 34, 29, 30 and 31 with 64, 96, 128
+    // and 256; one of 577 keys 9.8 with one and 13.2 with two. Where f32 products bound the call, two: 2048 rows over 4096
+    // keys, 8 heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
+    const long want = ((plan.rtiles > 1 && dtype == kF32 ? 2L : 8L) * cus + base - 1) / base, most = ((long)max_len + 1023) / 1024;
     plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
   }
   if ((long)tokens * heads * (d / 4) >= 1L << 32) plan.nsplit = 1;  // more than the joining launch has threads for
+  plan.round = (int)(cus / (units * plan.nsplit));
   const long blocks = ((long)max_len + 31) / 32;
   plan.per = (int)std::min((blocks + plan.nsplit - 1) / plan.nsplit, 1L << 26);
   if (plan.nsplit > 1) {
@@ -40,6 +49,7 @@ hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const Page
   p.rtiles = plan.rtiles;
   p.nsplit = plan.nsplit;
   p.per = plan.per;
+  p.round = plan.round;
   hipError_t e = dtype == kF32 ? paged_f32(cache_dtype, p, plan.rows, stream)
                  : plan.many   ? paged_many(dtype, cache_dtype, p, stream)
                                : paged_few(dtype, cache_dtype, p, plan.rows, stream);

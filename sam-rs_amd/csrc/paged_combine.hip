@@ -6,7 +6,7 @@
 // What bounds it: the partial O's bytes, 4 a column and split, and, with few rows, the latency of reading them. Up to
 // eight splits a thread reads its four columns of each; past that a workgroup takes 32 columns of a row, its lanes a
 // share of the splits each, and they meet in LDS (16 rows of 128 columns and 256 splits: 15.4 us with a lane for each 4
-// columns and a wave for each 32 splits, COMBINEROW so).
+// columns and a wave for each 32 splits, 4.1 so).
 #include "paged.hpp"
 
 namespace samhip {
