@@ -121,7 +121,8 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
     };
 
     // Table entries two blocks ahead, K and V one: a wait for a load waits for those before it too, so the entries go
-    // ahead of the rows that they are not needed for.
+    // ahead of the rows that they are not needed for. After its last block a wave loads the range's last again: loads under
+    // a condition would have the next scores wait for V too, as the compiler counts what is in flight on the shorter path.
     int row = -1;
     PagedEntry coming = {-1, -1};
     if (b0 + wave < b1) {
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
         }
       }
       // s[rb][i][e]: key key0 + 16 i + 4 g + e, row 16 rb + n
-      if (blk + 4 < b1) load_k(next);  // in flight while this block's V is weighed
+      load_k(next);  // in flight while this block's V is weighed
       const bool part = key0 + 32 > least || there != 0xffffffffu;
       const unsigned mine = there >> (4 * g);  // bit 16 i + e: the lane's key 16 i + 4 g + e
       X8 b[RB], blo[RB];
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
               }
         }
       }
-      if (blk + 4 < b1) load_v(next);
+      load_v(next);
       row = next;
     }
 #pragma unroll
