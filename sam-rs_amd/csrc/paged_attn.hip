@@ -26,15 +26,18 @@ PagedPlan paged_plan(int dtype, int tokens, int batch, int heads, int kv_heads, 
     const long slots = (d > 128 ? 1L : d > 64 ? 2L : 3L) * cus, most = ((long)max_len + 255) / 256;
     plan.nsplit = (int)std::max(1L, std::min(std::min(slots / base, most), 64L));
   } else {
-    // Eight workgroups a CU, so that sequences of different lengths share the card evenly, if every split then has eight
-    // blocks of 32 keys for each of its four waves: 32 sequences of up to 8192 keys, 8 key heads of 128 in e4m3, take 85, 87,
-    // 83, 93 and 97 us with 4, 6, 8, 12 and 16 splits; one of 131072, 2 heads of 128 in f16, 34, 29, 30 and 31 with 64, 96, 128
-    // and 256; one of 577 keys 9.8 with one and 13.2 with two. Where f32 products bound the call, two: 2048 rows over 4096
-    // keys, 8 heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
-    const long want = ((plan.rtiles > 1 && dtype == kF32 ? 2L : 8L) * cus + base - 1) / base, most = ((long)max_len + 1023) / 1024;
+    // Four workgroups a CU (two past head dim 128, where one runs at a time), so that sequences of different lengths share
+    // the card, if every split then has eight blocks of 32 keys for each of its four waves. 32 sequences, 8 key heads of 128
+    // in e4m3: 820 to 8192 keys 92, 94, 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125,
+    // 134 and 148; 4 heads of 256 in e4m3, 8192 each, 103, 112 and 132 with 2, 4 and 8. One of 131072, 2 heads of 128 in f16,
+    // 31, 29, 29 and 30 with 64, 96, 128 and 256; one of 577 keys 9.8 with one and 13.2 with two. Where f32 products bound
+    // the call, two a CU: 2048 rows over 4096 keys, 8 heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
+    const long want = ((d > 128 || (plan.rtiles > 1 && dtype == kF32) ? 2L : 4L) * cus + base - 1) / base, most = ((long)max_len + 1023) / 1024;
     plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
   }
-  if ((long)tokens * heads * (d / 4) >= 1L << 32) plan.nsplit = 1;  // more than the joining launch has threads for
+  // no more threads for the launch that joins the splits than 32 bits count: d / 4 a row to 8 splits, 512 for 32 columns past
+  if ((long)tokens * heads * ((d + 31) / 32) >= 1L << 23) plan.nsplit = std::min(plan.nsplit, 8);
+  if ((long)tokens * heads * (d / 4) >= 1L << 32) plan.nsplit = 1;
   plan.round = (int)(cus / (units * plan.nsplit));
   const long blocks = ((long)max_len + 31) / 32;
   plan.per = (int)std::min((blocks + plan.nsplit - 1) / plan.nsplit, 1L << 26);

@@ -26,27 +26,37 @@ template <typename T> __device__ __forceinline__ void store_row4(const PagedPara
   *reinterpret_cast<typename Vec<T>::x4*>(reinterpret_cast<T*>(p.out) + tok * p.so[0] + head * p.so[1] + col) = x;
 }
 
-// A thread takes 4 columns of a row.
-template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
-  const int cpr = p.c.d / 4;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = i / cpr;
-  const int col = (int)(i % cpr) * 4;
+// A thread takes 4 columns of a row and up to N splits: all their maxima and sums are on their way together, then all
+// their partial results (4096 rows of 256 and 8 splits: 11.0 us one after the other, 7.9 so).
+template <typename T, int N> __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
+  const unsigned cpr = p.c.d / 4, i = blockIdx.x * 256u + threadIdx.x;  // fewer than 2^32 threads
+  const unsigned row = i / cpr;
+  const int col = (int)(i - row * cpr) * 4;
   const long rows = (long)p.tokens * p.heads;
   if (row >= rows) return;
-  const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
-  if (!row_of_a_sequence(p, tok) || p.ml[2 * row + 1] < 0.f) return;
-  float top = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) top = fmaxf(top, p.ml[2 * (s * rows + row)]);
+  const int tok = (int)(row / (unsigned)p.heads), head = (int)(row - tok * (unsigned)p.heads);
+  float2 ml[N];
+#pragma unroll
+  for (int s = 0; s < N; ++s) ml[s] = *reinterpret_cast<const float2*>(p.ml + 2 * (min(s, p.nsplit - 1) * rows + row));
+  if (!row_of_a_sequence(p, tok) || ml[0].y < 0.f) return;
+  f32x4 x[N];
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    x[s] = *reinterpret_cast<const f32x4*>(p.opart + (min(s, p.nsplit - 1) * rows + row) * p.c.d + col);
+    if (s >= p.nsplit) ml[s] = float2{-INFINITY, 0.f};
+  }
+  float top = ml[0].x;
+#pragma unroll
+  for (int s = 1; s < N; ++s) top = fmaxf(top, ml[s].x);
   const float base = top == -INFINITY ? 0.f : top;
   f32x4 o = {};
   float l = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * (s * rows + row));
-    if (ml.y == 0.f) continue;  // no keys in this split: its O was not summed
-    const float w = exp2_fast(ml.x - base);
-    l += ml.y * w;
-    o += *reinterpret_cast<const f32x4*>(p.opart + (s * rows + row) * p.c.d + col) * w;
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    const float w = exp2_fast(ml[s].x - base);
+    l += ml[s].y == 0.f ? 0.f : ml[s].y * w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += ml[s].y == 0.f ? 0.f : x[s][j] * w;  // no keys in this split: its O was not written
   }
   store_row4<T>(p, tok, head, col, o, l);
 }
@@ -61,9 +71,10 @@ template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_co
   __shared__ __attribute__((aligned(16))) f32x4 part[kRowWaves][8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int groups = (p.c.d + kCols - 1) / kCols;
-  const long row = blockIdx.x / groups, rows = (long)p.tokens * p.heads;
-  const int tok = (int)(row / p.heads), head = (int)(row % p.heads);
-  if (!row_of_a_sequence(p, tok) || p.ml[2 * row + 1] < 0.f) return;
+  const unsigned row = blockIdx.x / (unsigned)groups;
+  const long rows = (long)p.tokens * p.heads;
+  const int tok = (int)(row / (unsigned)p.heads), head = (int)(row - tok * (unsigned)p.heads);
+  if (!row_of_a_sequence(p, tok) || p.ml[2l * row + 1] < 0.f) return;
   const int col = (int)(blockIdx.x % groups) * kCols + 4 * (lane & 7), s0 = 8 * wave + (lane >> 3);
   f32x4 x[kDeep];
 #pragma unroll
@@ -115,12 +126,13 @@ template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_co
 template <typename T> hipError_t combine(const PagedParams& p, hipStream_t stream) {
   const long rows = (long)p.tokens * p.heads;
   const long blocks = rows * ((p.c.d + kCols - 1) / kCols);
-  if (p.nsplit > 8 && blocks * 64 * kRowWaves < 1l << 32) {  // the threads of a launch count in 32 bits
+  if (p.nsplit > 8) {
     static_assert(kMostSplits <= 64 * kRowWaves, "a thread for each split");
     hipLaunchKernelGGL(paged_combine_row_kernel<T>, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, stream, p);
   } else {
     const long threads = rows * (p.c.d / 4);
-    hipLaunchKernelGGL(paged_combine_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p);
+    auto kern = p.nsplit <= 2 ? paged_combine_kernel<T, 2> : p.nsplit <= 4 ? paged_combine_kernel<T, 4> : paged_combine_kernel<T, 8>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p);
   }
   return hipGetLastError();
 }
