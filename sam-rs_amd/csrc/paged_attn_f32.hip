@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
             for (int rb = 0; rb < RB; ++rb) s[rb][i] = mma4(a[j], qf[rb][c][j], s[rb][i]);
         }
       }
-      if (blk + 4 < b1) load_k(next);
+      load_k(next);  // after the last block the range's last again: under a condition, V would wait for it too
       // s[rb][i][e]: key key0 + 16 i + 4 g + e, row 16 rb + n
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
