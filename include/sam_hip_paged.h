@@ -47,7 +47,8 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
  * What the tables say is checked on the device: lens are held to 0 .. table_width * page_size, starts to 0 .. tokens;
  * tokens outside every sequence or at a negative position are not written; a table entry outside 0 .. pages - 1 stands
  * for a page that is not there (not written, read as zeros, its keys not attended). Two positions that share a page slot
- * must not be written in one call. Limits: d % 8 == 0, d <= 256, table_width * page_size < 2^30.
+ * must not be written in one call. Limits: d % 8 == 0, d <= 256, table_width * page_size < 2^30, fewer than 2^31 rows in
+ * a pool and 2^27 in a write or a read.
  */
 #define SAM_HIP_E4M3 3
 int sam_hip_kv_write(const void* k, const void* v, void* k_pages, void* v_pages, unsigned char* k_scale,
@@ -64,7 +65,8 @@ int sam_hip_kv_read(void* k, void* v, const void* k_pages, const void* v_pages, 
  *   out[t, hq, :] = softmax_j(scale * q[t, hq, :] . k_j) . v_j over the keys j < lens[b] of key head hq / (heads / kv_heads)
  * and, with causal, j <= t's own position lens[b] - (starts[b+1] - t). q and out [tokens, heads, d] (strides (token,
  * head), multiples of 16 bytes; NULL = contiguous). A row that sees no key is 0; a key, or a value that is not finite,
- * reaches the rows that see it alone. Rows of no sequence stay as they are, or become 0 with zero_rest.
+ * reaches the rows that see it alone. Rows of no sequence stay as they are, or become 0 with zero_rest. out
+ * must not overlap the other tensors.
  * max_q and max_len are the longest chunk and the longest sequence as the caller expects them: they size the grid and
  * the key splits, and a call whose sequences exceed them is computed all the same, more slowly.
  * Workspace: sam_hip_paged_attention_workspace_size() bytes of device memory for the key splits' partial results (it
