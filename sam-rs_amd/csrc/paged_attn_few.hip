@@ -14,6 +14,10 @@
 // own rounding).
 //
 // The four waves of a workgroup join at its end, the key ranges of a sequence in paged_combine_kernel.
+//
+// Measured, 32 sequences of 8192 keys, 8 key heads of 128, one token of 4 query heads a key head: f16 pages 187 us (5.7
+// TB/s), e4m3 pages 107 with f16 queries and 123 with bf16 (5.0 and 4.4; not for their instructions: a fifth fewer took as
+// long). 64-key blocks of e4m3 were no faster.
 #include "lds_dma.hpp"
 #include "paged.hpp"
 
@@ -35,6 +39,8 @@ template <> struct Raw<16> {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
+// Workgroups a CU: as many as registers allow with a block of K and one of V in flight. Three for e4m3 at head dim 128
+// (131 us for the bf16 call above with eight splits, 137 with two).
 template <typename T, typename C, int DP, int RB>
 __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C, e4m3) ? 2 : 3) void paged_few_kernel(PagedParams p) {
   typedef typename Vec<T>::x8 X8;
