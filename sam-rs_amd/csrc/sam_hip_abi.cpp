@@ -643,6 +643,8 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
     if (strides_pos) sp[i] = strides_pos[i];
     if (sx[i] < 0 || so[i] < 0 || sp[i] < 0) return fail(SAM_HIP_EUNSUPPORTED, "rope-axes: strides must not be negative");
   }
+  if ((b > 1 && so[0] == 0) || (l > 1 && so[1] == 0) || (h > 1 && so[2] == 0))
+    return fail(SAM_HIP_EINVAL, "rope-axes: out's rows must lie apart (a stride of 0)");
   if (x == out && (sx[0] != so[0] || sx[1] != so[1] || sx[2] != so[2]))
     return fail(SAM_HIP_EINVAL, "rope-axes: in place, x and out must have the same strides");
   return check_launch(samhip::rope_axes(dtype, x, pos, freqs, axes, out, b, l, h, d, pairs, naxes, sx, sp, so,
@@ -793,6 +795,8 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
     return fail(SAM_HIP_EINVAL, "paged-attention: scale must be finite and not negative, got %g", (double)scale);
   if (int rc = token_strides("paged-attention", "q", strides_q, p.sq, heads, d, dtype); rc != SAM_HIP_OK) return rc;
   if (int rc = token_strides("paged-attention", "out", strides_o, p.so, heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if ((tokens > 1 && p.so[0] == 0) || (heads > 1 && p.so[1] == 0))
+    return fail(SAM_HIP_EINVAL, "paged-attention: out's rows must lie apart (a stride of 0)");
   if (!aligned16(q) || !aligned16(out))
     return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: q and out must be 16-byte aligned");
   const samhip::PagedPlan plan = samhip::paged_plan(dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,

@@ -113,6 +113,12 @@ def test_launches_past_32_bits_of_threads_are_refused(lib):
     assert size(1, 1, 1 << 26, 1, 2, 2, 128, 1, 1 << 20) == 0 < size(1, 1, 1 << 20, 1, 2, 2, 128, 1, 1 << 20)
 
 
+def test_outputs_whose_rows_share_memory_are_refused(lib):
+    assert attend(lib, so=strides(0, 64)) == 1 and attend(lib, so=strides(256, 0)) == 1
+    assert rope(lib, so=strides(512, 0, 64)) == 1 and rope(lib, so=strides(512, 128, 0)) == 1
+    assert rope(lib, b=2, so=strides(0, 128, 64)) == 1
+
+
 def test_a_missing_or_short_workspace_is_refused(lib):
     size = lib.sam_hip_paged_attention_workspace_size
     need = size(1, 1, 1, 1, 8, 1, 128, 1, 1 << 16)
