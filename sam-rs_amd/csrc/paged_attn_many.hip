@@ -59,7 +59,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
   typedef __attribute__((address_space(3))) X8 lds_x8;
   typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
   constexpr int KS = G::KS, MBO = G::MBO, ROW = G::ROW, BUF = G::BUF, CPR = G::CPR, RPI = G::RPI, PT = G::PT;
-  typedef typename std::conditional<kCoded, u32x2, u32x4>::type Raw;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const unsigned lds0 = lds_addr(smem);
   int* odd = reinterpret_cast<int*>(smem + 4 * BUF);  // the tile in each buffer that went there without such values
@@ -77,6 +76,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
   auto srow = [&](int u) { return 16 * wave + RPI * u + lane / CPR; };
   auto kcol = [&](int u) { return 8 * (spos ^ G::kswz(RPI * u + lane / CPR)); };
   auto vcol = [&](int u) { return 8 * (spos ^ G::vswz(RPI * u + lane / CPR)); };
+  // e4m3: a load brings two chunks of a row, 16 codes, to the lane of LPR that stores them
+  constexpr int CH = kCoded ? 2 : 1, PR = PT / CH, LPR = CPR / CH;
+  const int rlane = lane / LPR, rcol = 8 * CH * (lane % LPR);
+  auto rrow = [&](int u) { return 16 * wave + CH * RPI * u + rlane; };
 
   if (d < ROW / 2) {  // columns past d are never written: K's meet zeros of q, and V's only feed columns that are dropped
     for (int c = tid; c < 4 * BUF / 16; c += 256) *(lds_u32x4*)(size_t)(lds0 + 16 * c) = u32x4{};
@@ -129,41 +132,64 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
     };
     // e4m3: the next tile's chunks on their way beside this one's products. Else a tile that is looked over comes after
     // them, V once K is stored, in registers that the products have had.
-    Raw kreg[PT], vbuf[kCoded ? PT : 1];
-    Raw* vreg = kCoded ? vbuf : kreg;
+    u32x4 kreg[PR], vbuf[kCoded ? PR : 1];
+    u32x4* vreg = kCoded ? vbuf : kreg;
     unsigned char kscale = 127, vscale = 127;  // of the lane's own key
-    auto load = [&](const C* base, const unsigned char* scales, int own, auto col, Raw* reg, unsigned char& scale) {
-      if constexpr (kCoded) scale = scales[max(own, 0)];
+    auto load = [&](const C* base, const unsigned char* scales, int own, auto col, u32x4* reg, unsigned char& scale) {
+      auto at = [&](int u) { return base + (long)max(__shfl(own, rrow(u)), 0) * d; };
+      if constexpr (kCoded) {
+        scale = scales[max(own, 0)];
+        if (d % 16 == 0) {
 #pragma unroll
-      for (int u = 0; u < PT; ++u) {
-        const long row = max(__shfl(own, srow(u)), 0);
-        reg[u] = *reinterpret_cast<const Raw*>(base + row * d + min(col(u), d - 8));
+          for (int u = 0; u < PR; ++u) reg[u] = *reinterpret_cast<const u32x4*>(at(u) + min(rcol, d - 16));
+        } else {  // a row's last chunk alone: 16 bytes would leave the row
+#pragma unroll
+          for (int u = 0; u < PR; ++u) {
+            const C* r = at(u);
+            const u32x2 lo = *reinterpret_cast<const u32x2*>(r + min(rcol, d - 8)),
+                        hi = *reinterpret_cast<const u32x2*>(r + min(rcol + 8, d - 8));
+            reg[u] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < PR; ++u) reg[u] = *reinterpret_cast<const u32x4*>(at(u) + min(col(u), d - 8));
       }
     };
     auto load_k = [&](int own) { load(kp, p.c.ks, own, kcol, kreg, kscale); };
     auto load_v = [&](int own) { load(vp, p.c.vs, own, vcol, vreg, vscale); };
-    auto values = [&](const Raw* reg, unsigned char scale, u32x4* x) {
+    auto values = [&](const u32x4* reg, unsigned char scale, u32x4* x) {  // x[CH u + c]: chunk c of load u
       if constexpr (kCoded) {
-        float f[PT];
+        float f[PR];
         const float mine = pow2_of(scale);
 #pragma unroll
-        for (int u = 0; u < PT; ++u) f[u] = __shfl(mine, srow(u));  // all before their use: each takes LDS's latency
+        for (int u = 0; u < PR; ++u) f[u] = __shfl(mine, rrow(u));  // all before their use: each takes LDS's latency
 #pragma unroll
-        for (int u = 0; u < PT; ++u)
-          x[u] = u32x4{decode2<T, false>(reg[u][0], f[u]), decode2<T, true>(reg[u][0], f[u]),
-                       decode2<T, false>(reg[u][1], f[u]), decode2<T, true>(reg[u][1], f[u])};
+        for (int u = 0; u < PR; ++u)
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            x[CH * u + c] = u32x4{decode2<T, false>(reg[u][2 * c], f[u]), decode2<T, true>(reg[u][2 * c], f[u]),
+                                  decode2<T, false>(reg[u][2 * c + 1], f[u]), decode2<T, true>(reg[u][2 * c + 1], f[u])};
       } else {
 #pragma unroll
-        for (int u = 0; u < PT; ++u) x[u] = reg[u];
+        for (int u = 0; u < PR; ++u) x[u] = reg[u];
       }
     };
-    const unsigned to = lds0 + 16 * wave * ROW + 16 * lane;
+    // Chunk c of load u is for column col(u, c) and goes to its swizzled place: where the lane's own is, or, of e4m3, the
+    // even chunk's place of the lane's first row with c and the row's part of the swizzle exclusive-ored in.
+    auto chunk_col = [&](int u, int c, auto col) { return kCoded ? rcol + 8 * c : col(u); };
+    auto store = [&](unsigned to, int u, int c, auto col, int lane_swz, int u_swz, u32x4 x) {
+      const unsigned at = kCoded ? ((to + (16 * wave + rlane) * ROW + 16 * ((rcol / 8) ^ lane_swz)) ^ 16 * (c ^ u_swz)) + CH * RPI * ROW * u
+                                 : to + 16 * wave * ROW + 16 * lane + 1024 * u;
+      if (chunk_col(u, c, col) < d) *(lds_u32x4*)(size_t)at = x;
+    };
     auto store_k = [&](int buf) {
       u32x4 x[PT];
       values(kreg, kscale, x);
 #pragma unroll
-      for (int u = 0; u < PT; ++u)
-        if (kcol(u) < d) *(lds_u32x4*)(size_t)(to + buf * BUF + 1024 * u) = x[u];
+      for (int u = 0; u < PR; ++u)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) store(lds0 + buf * BUF, u, c, kcol, G::kswz(rlane), G::kswz(CH * RPI * u), x[CH * u + c]);
     };
     auto store_v = [&](int t, unsigned long there, int buf) {
       u32x4 x[PT];
@@ -171,20 +197,23 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
       if (!whole(t, there)) {
         unsigned any = 0;
 #pragma unroll
-        for (int u = 0; u < PT; ++u) {
-          const bool ok = (there >> srow(u) & 1) && vcol(u) < d;
+        for (int u = 0; u < PR; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const unsigned bad = not_finite2<T>(x[u][i]);
-            x[u][i] = ok ? without2(x[u][i], bad) : 0u;
-            any |= ok ? bad : 0u;
+          for (int c = 0; c < CH; ++c) {
+            const bool ok = (there >> rrow(u) & 1) && chunk_col(u, c, vcol) < d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const unsigned bad = not_finite2<T>(x[CH * u + c][i]);
+              x[CH * u + c][i] = ok ? without2(x[CH * u + c][i], bad) : 0u;
+              any |= ok ? bad : 0u;
+            }
           }
-        }
         if (any) odd[buf] = t;
       }
 #pragma unroll
-      for (int u = 0; u < PT; ++u)
-        if (vcol(u) < d) *(lds_u32x4*)(size_t)(to + (2 + buf) * BUF + 1024 * u) = x[u];
+      for (int u = 0; u < PR; ++u)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) store(lds0 + (2 + buf) * BUF, u, c, vcol, G::vswz(rlane), G::vswz(CH * RPI * u), x[CH * u + c]);
     };
 
     // Table entries two tiles ahead, K and V one

@@ -243,6 +243,15 @@ def test_many_short_sequences_without_hints(hip, dtype):
     c.check(c.run(hip, True), True)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [8, 16, 24, 40, 56, 88, 104, 120, 136, 248])
+def test_many_rows_at_every_width_of_a_last_chunk(hip, dtype, d):
+    """e4m3 rows in pieces of 16 codes, the last of them a half one, in the last row of the pool too."""
+    c = Case([70, 40], [150, 64], 2, 1, d, 16, dtype, True, spare=0)
+    for causal in (True, False):
+        c.check(c.run(hip, causal), causal)
+
+
 def test_sizes_past_32_bits_are_refused(hip):
     t = lambda *s, dt=torch.float16: torch.zeros(s, dtype=dt, device="cuda")
     i = lambda *s: t(*s, dt=torch.int32)
