@@ -114,17 +114,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
     // registers
     auto direct_to_lds = [&](int t, unsigned long there) { return !kCoded && whole(t, there); };
     auto dma = [&](int own, int buf) {
-      long row[PT];
+      unsigned row[PT];  // all there: the products below are one instruction each
 #pragma unroll
-      for (int u = 0; u < PT; ++u) row[u] = __shfl(own, srow(u));
+      for (int u = 0; u < PT; ++u) row[u] = (unsigned)__shfl(own, srow(u));
       auto rows_to = [&](const C* base, unsigned to, auto col) {
         if (d == ROW / 2) {
 #pragma unroll
-          for (int u = 0; u < PT; ++u) dma16_from(base + row[u] * d + col(u), to + 1024 * u);
+          for (int u = 0; u < PT; ++u) dma16_from(base + (unsigned long)row[u] * (ROW / 2) + col(u), to + 1024 * u);
         } else {
 #pragma unroll
           for (int u = 0; u < PT; ++u)
-            if (col(u) < d) dma16_from(base + row[u] * d + col(u), to + 1024 * u);
+            if (col(u) < d) dma16_from(base + (unsigned long)row[u] * (unsigned)d + col(u), to + 1024 * u);
         }
       };
       rows_to(kp, lds0 + buf * BUF + 16 * wave * ROW, kcol);
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
     u32x4* vreg = kCoded ? vbuf : kreg;
     unsigned char kscale = 127, vscale = 127;  // of the lane's own key
     auto load = [&](const C* base, const unsigned char* scales, int own, auto col, u32x4* reg, unsigned char& scale) {
-      auto at = [&](int u) { return base + (long)max(__shfl(own, rrow(u)), 0) * d; };
+      auto at = [&](int u) { return base + (unsigned long)(unsigned)max(__shfl(own, rrow(u)), 0) * (unsigned)d; };
       if constexpr (kCoded) {
         scale = scales[max(own, 0)];
         if (d % 16 == 0) {
