@@ -17,9 +17,12 @@
 // rarely rescaled. f16 P is rounded to f16 and summed as rounded; bf16 P goes as hi + lo.
 //
 // What bounds it: products, softmax and LDS reads beside each other on too few waves (a loop of the products alone, fed
-// from LDS, reaches 1.11 PFLOP/s at head dim 128). 8192 rows over 8192 keys, f16: head dim 64 433 us (16 heads, 0.63
-// PFLOP/s), 96 271 to 278 (8 heads, 0.75), 128 317 (8 heads, 0.87), 256 342 (4 heads, 0.80); bf16 at 128 387 (0.71, with 1.5
-// times the products); e4m3 at 128 378 (0.73), at 256 417 (0.66). kAhead 2 took 319, 279 and 370 us at 128, 96 and 256.
+// from LDS, reaches 1.11 PFLOP/s at head dim 128). The vector units' and the matrix units' busy cycles add up to the whole
+// time, also where more of them run beside each other: fewer instructions count, not a closer order. 8192 rows over 8192
+// keys, f16: head dim 64 367 us (16 heads, 0.75 PFLOP/s), 96 255 (8 heads, 0.81), 128 301 (8 heads, 0.91), 256 329 (4 heads,
+// 0.83); bf16 at 64 535 (0.51), at 128 377 (0.73), with 1.5 times the products; e4m3 at 128 321 (0.86), at 256 372 (0.74), where
+// 8 codes a load instead of 16 took 377 and 417. On a card a tenth slower kAhead 2 took 319, 279 and 370 us at 128, 96 and
+// 256, and 4 317, 271 and 345.
 #include <type_traits>
 
 #include "lds_dma.hpp"
