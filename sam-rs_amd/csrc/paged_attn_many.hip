@@ -2,9 +2,10 @@
 // of their own type or of e4m3.
 //
 // Work: a workgroup of four waves takes 128 rows (new token x query head of one key head) and one range of keys; a wave
-// owns 32 rows. Tiles of 64 keys go from their pages through registers into LDS, the next tile's loads in flight while
-// this one is worked on (e4m3 codes become 16-bit values with their row's scale on the way, once per workgroup), two
-// buffers each, one barrier a tile. A lane looks one key of the tile up; the loads take their rows from that lane.
+// owns 32 rows. Tiles of 64 keys go from their pages into LDS, the next one on its way while this one is worked on, two
+// buffers each, one barrier a tile: 16-bit tiles that every row sees whole straight, others and e4m3 through registers
+// (codes become 16-bit values with their row's scale on the way, once per workgroup). A lane looks one key of the tile up;
+// the loads take their rows from that lane.
 //   S^T = K Q^T on v_mfma_f32_32x32x16 with Q in registers: a lane holds one row's scores of 32 keys, so that softmax
 //   needs one exchange between lane halves. O^T += V^T P^T takes the scores' registers as its B operand under a fixed
 //   permutation of keys that the transposing reads of V (ds_read_b64_tr_b16) follow.
