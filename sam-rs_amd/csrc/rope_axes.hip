@@ -198,10 +198,11 @@ template <typename T> hipError_t launch(RopeAxesParams p, long tokens, hipStream
   // Heads and tokens of a thread, once there are threads enough for the card. 41472 tokens of 16 heads of 64, f16: 4 and 2
   // 37.6 us, 4 and 1 43.8, 2 and 2 37.5, 2 and 4 41.7 (a copy of the bytes 34.2); f32, 65536 of 8 heads of 80: 2 and 2 62.6,
   // 4 and 2 69.0 (copy 63.4); one head of 256, 65536 tokens, bf16: 2 tokens 18.6, 4 20.7, 8 21.9, 1 25.7 (the angles; copy
-  // 10.5).
+  // 10.5). Halves have two vectors a head: 16384 tokens of 8 heads of 128 in f16 4 and 1 17.0, 4 and 2 18.4 (copy 14.0), one
+  // head of 256 28.5 and 24.5 with 1 and 2.
   constexpr int kHeads = sizeof(T) == 4 ? 2 : 4;
   const long work = tokens * (p.d / 8) * p.h;  // vectors of 8 elements
-  const int hp = vec && p.h >= 4 && work >= 1 << 17 ? kHeads : 1, nt = vec && work >= 1 << 19 ? 2 : 1;
+  const int hp = vec && p.h >= 4 && work >= 1 << 17 ? kHeads : 1, nt = vec && work >= 1 << 19 && !(p.halves && hp > 1) ? 2 : 1;
   p.units = vec ? p.pairs / (p.halves ? 8 : 4) + rest / 8 : p.pairs + rest;
   p.hgroups = vec ? (p.h + hp - 1) / hp : 1;
   division_magic(p.units, &p.umagic, &p.ushift);
