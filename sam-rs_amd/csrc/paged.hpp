@@ -88,7 +88,8 @@ struct PagedPlan {
   int many, rows, rtiles, nsplit, per, round;
   long part_bytes, total;
 };
-PagedPlan paged_plan(int dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q, int max_len, int cus);
+PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
+                     int max_len, int cus);
 hipError_t paged_attention(int dtype, int cache_dtype, PagedParams p, const PagedPlan& plan, hipStream_t stream);
 hipError_t paged_f32(int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);
 hipError_t paged_few(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream);

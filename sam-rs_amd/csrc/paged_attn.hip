@@ -5,7 +5,8 @@
 
 namespace samhip {
 
-PagedPlan paged_plan(int dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q, int max_len, int cus) {
+PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
+                     int max_len, int cus) {
   PagedPlan plan = {};
   const long group = heads / kv_heads, rows = (long)std::max(std::min(max_q, tokens), 1) * group;
   // The many-row kernel past 32 rows a key head, which the other takes in two passes over the keys: 8 sequences of 8192, 8
@@ -27,13 +28,18 @@ PagedPlan paged_plan(int dtype, int tokens, int batch, int heads, int kv_heads, 
     plan.nsplit = (int)std::max(1L, std::min(std::min(slots / base, most), 64L));
   } else {
     // Four workgroups a CU (two past head dim 128, where one runs at a time), so that sequences of different lengths share
-    // the card, if every split then has eight blocks of 32 keys for each of its four waves. 32 sequences, 8 key heads of 128
-    // in e4m3: 820 to 8192 keys 92, 94, 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125,
-    // 134 and 148; 4 heads of 256 in e4m3, 8192 each, 103, 112 and 132 with 2, 4 and 8. One of 131072, 2 heads of 128 in f16,
-    // 31, 29, 29 and 30 with 64, 96, 128 and 256; one of 577 keys 9.8 with one and 13.2 with two. Where f32 products bound
-    // the call, two a CU: 2048 rows over 4096 keys, 8 heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
-    const long want = ((d > 128 || (plan.rtiles > 1 && dtype == kF32) ? 2L : 4L) * cus + base - 1) / base, most = ((long)max_len + 1023) / 1024;
-    plan.nsplit = (int)std::max(1L, std::min(std::min(want, most), 256L));
+    // the card, of 512 KB of keys and values each at least. 32 sequences, 8 key heads of 128 in e4m3: 820 to 8192 keys 92, 94,
+    // 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125, 134 and 148; 4 heads of 256 in e4m3,
+    // 8192 each, 103, 112 and 132 with 2, 4 and 8. Where f32 products bound the call, two a CU: 2048 rows over 4096 keys, 8
+    // heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
+    const long bytes = 2L * d * (cache_dtype == kE4M3 ? 1 : dtype == kF32 ? 4 : 2) * max_len;  // a sequence's, of one head
+    const long many = std::min(((d > 128 || (plan.rtiles > 1 && dtype == kF32) ? 2L : 4L) * cus + base - 1) / base, bytes >> 19);
+    // One a CU, of 128 KB each at least: a CU alone reads 60 GB/s. In f16, 2048 keys of 4 heads of 128 take 22.6, 16.4, 12.2 and
+    // 10.3 us with 1, 2, 4 and 8 splits, 4096 of 4 heads of 64 25.4, 17.2, 11.9 and 9.6, 1024 of 8 heads of 128 14.0, 11.7 and
+    // 9.7 with 1, 2 and 4. Below 448 KB the second launch costs what it gains (577 keys of 8 heads of 64 8.0 and 8.1 with 1
+    // and 4, without the host's 3 us).
+    const long few = bytes > 448 << 10 ? std::min(cus / base, (bytes + (1 << 17) - 1) >> 17) : 1;
+    plan.nsplit = (int)std::min(std::max(std::max(many, few), 1L), 256L);
   }
   // no more threads for the launch that joins the splits than 32 bits count: d / 4 a row to 8 splits, 512 for 32 columns past
   if ((long)tokens * heads * ((d + 31) / 32) >= 1L << 23) plan.nsplit = std::min(plan.nsplit, 8);

@@ -771,7 +771,7 @@ long sam_hip_paged_attention_workspace_size(int dtype, int cache_dtype, int toke
     return -1;
   }
   if (check_paged_sizes("paged-attention", tokens, batch, heads, kv_heads, d, max_q, max_len) != SAM_HIP_OK) return -1;
-  return samhip::paged_plan(dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,
+  return samhip::paged_plan(dtype, cache_dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,
                             samhip::device_cu_count())
       .total;
 }
@@ -799,7 +799,7 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
     return fail(SAM_HIP_EINVAL, "paged-attention: out's rows must lie apart (a stride of 0)");
   if (!aligned16(q) || !aligned16(out))
     return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: q and out must be 16-byte aligned");
-  const samhip::PagedPlan plan = samhip::paged_plan(dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,
+  const samhip::PagedPlan plan = samhip::paged_plan(dtype, cache_dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,
                                                     samhip::device_cu_count());
   if (plan.total > 0 && (!workspace || workspace_bytes < plan.total))
     return fail(SAM_HIP_EINVAL, "paged-attention: workspace of %ld bytes needed, got %ld", plan.total,
