@@ -24,8 +24,13 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
     // As many workgroups as run at once (three a CU up to head dim 64, two to 128, one past it), with four tiles of 64
     // keys a split at least. More only add partial results: six sequences of up to 7000 keys, 8 heads of 64, 1024 rows each,
     // 155, 113, 115 and 120 us with 1, 2, 3 and 4 splits; 4096 rows over 28736 keys, 256, 229 and 315 with 8 and 16.
-    const long slots = (d > 128 ? 1L : d > 64 ? 2L : 3L) * cus, most = ((long)max_len + 255) / 256;
-    plan.nsplit = (int)std::max(1L, std::min(std::min(slots / base, most), 64L));
+    const long slots = (d > 128 ? 1L : d > 64 ? 2L : 3L) * cus, full = std::min(slots / base, max_len / 256L);
+    // Up to eight of a tile each while they are one a CU: 100 rows over 1000 keys, 8 heads of 64, 22, 13 and 12 us with 1, 4
+    // and 8, 64 over 500, 8 heads of 128, 18, 13 and 11; 1000 over 1000, 8 heads of 64, 23, 16 and 18.
+    const long small = max_len >= 384 ? std::min(std::min(cus / base, max_len / 64L), 8L) : 1;
+    plan.nsplit = (int)std::max(1L, std::min(std::max(full, small), 64L));
+    // more than eight are joined in a loop: 1000 rows over 3000 keys, 2 key heads of 128, 27 us with 8, 31 with 12, 30 with 16
+    if (plan.nsplit > 8 && plan.nsplit < 16) plan.nsplit = 8;
   } else {
     // Four workgroups a CU (two past head dim 128, where one runs at a time), so that sequences of different lengths share
     // the card, of 512 KB of keys and values each at least. 32 sequences, 8 key heads of 128 in e4m3: 820 to 8192 keys 92, 94,

@@ -3,10 +3,10 @@
 // result does not depend on their timing. A split without keys has l = 0 and no O; a row whose keys are all in its
 // first split is written already, which l = -1 says.
 //
-// What bounds it: the partial O's bytes, 4 a column and split, and, with few rows, the latency of reading them. Up to
-// eight splits a thread reads its four columns of each; past that a workgroup takes 32 columns of a row, its lanes a
-// share of the splits each, and they meet in LDS (16 rows of 128 columns and 256 splits: 15.4 us with a lane for each 4
-// columns and a wave for each 32 splits, 4.1 so).
+// What bounds it: the partial O's bytes, 4 a column and split, and, with few rows, the latency of reading them. A thread
+// reads its four columns of each split, eight of them at a time; past eight splits and while there are few rows a
+// workgroup takes 32 columns of a row, its lanes a share of the splits each, and they meet in LDS (16 rows of 128 columns
+// and 256 splits: 15.4 us with a lane for each 4 columns and a wave for each 32 splits, 4.1 so).
 #include "paged.hpp"
 
 namespace samhip {
@@ -57,6 +57,48 @@ template <typename T, int N> __global__ __launch_bounds__(256) void paged_combin
     l += ml[s].y == 0.f ? 0.f : ml[s].y * w;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] += ml[s].y == 0.f ? 0.f : x[s][j] * w;  // no keys in this split: its O was not written
+  }
+  store_row4<T>(p, tok, head, col, o, l);
+}
+
+// The same for more splits, eight of them at a time.
+template <typename T> __global__ __launch_bounds__(256) void paged_combine_long_kernel(PagedParams p) {
+  const unsigned cpr = p.c.d / 4, i = blockIdx.x * 256u + threadIdx.x;  // fewer than 2^32 threads
+  const unsigned row = i / cpr;
+  const int col = (int)(i - row * cpr) * 4;
+  const long rows = (long)p.tokens * p.heads;
+  if (row >= rows) return;
+  const int tok = (int)(row / (unsigned)p.heads), head = (int)(row - tok * (unsigned)p.heads);
+  float2 ml[8];
+  auto load_ml = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ml[k] = *reinterpret_cast<const float2*>(p.ml + 2 * (min(s0 + k, p.nsplit - 1) * rows + row));
+  };
+  load_ml(0);
+  if (!row_of_a_sequence(p, tok) || ml[0].y < 0.f) return;
+  float top = -INFINITY;
+  for (int s0 = 0; s0 < p.nsplit; s0 += 8) {
+    load_ml(s0);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 o = {};
+  float l = 0.f;
+  for (int s0 = 0; s0 < p.nsplit; s0 += 8) {
+    load_ml(s0);
+    f32x4 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[k] = *reinterpret_cast<const f32x4*>(p.opart + (min(s0 + k, p.nsplit - 1) * rows + row) * p.c.d + col);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool none = s0 + k >= p.nsplit || ml[k].y == 0.f;  // no keys in this split: its O was not written
+      const float w = exp2_fast(ml[k].x - base);
+      l += none ? 0.f : ml[k].y * w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += none ? 0.f : x[k][j] * w;
+    }
   }
   store_row4<T>(p, tok, head, col, o, l);
 }
@@ -123,14 +165,20 @@ template <typename T> __global__ __launch_bounds__(64 * kRowWaves) void paged_co
   store_row4<T>(p, tok, head, col, o, l);
 }
 
+// A workgroup for 32 columns of a row while there are few rows: with 12 splits, attention of 4000 rows of 128 and joining
+// take 73 us so and 31 with threads, of 800 rows of 64 17.5 and 14.1, of 400 of 128 (32 splits) 29.9 and 29.7.
+constexpr long kMostBlocks = 1024;
+
 template <typename T> hipError_t combine(const PagedParams& p, hipStream_t stream) {
   const long rows = (long)p.tokens * p.heads;
   const long blocks = rows * ((p.c.d + kCols - 1) / kCols);
-  if (p.nsplit > 8) {
+  const long threads = rows * (p.c.d / 4);
+  if (p.nsplit > 8 && blocks > kMostBlocks) {
+    hipLaunchKernelGGL(paged_combine_long_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p);
+  } else if (p.nsplit > 8) {
     static_assert(kMostSplits <= 64 * kRowWaves, "a thread for each split");
     hipLaunchKernelGGL(paged_combine_row_kernel<T>, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, stream, p);
   } else {
-    const long threads = rows * (p.c.d / 4);
     auto kern = p.nsplit <= 2 ? paged_combine_kernel<T, 2> : p.nsplit <= 4 ? paged_combine_kernel<T, 4> : paged_combine_kernel<T, 8>;
     hipLaunchKernelGGL(kern, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, p);
   }

@@ -252,6 +252,19 @@ def test_many_rows_at_every_width_of_a_last_chunk(hip, dtype, d):
         c.check(c.run(hip, causal), causal)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("chunks, lens, hkv, g, d", [
+    ([300, 260, 7], [5000, 2600, 300], 1, 1, 64), ([600], [6000], 1, 2, 136), ([40], [2100], 1, 1, 256), ([3, 1], [9000, 600], 1, 2, 64)])
+def test_more_than_eight_splits(hip, dtype, chunks, lens, hkv, g, d):
+    """Key splits joined in a loop and by workgroups, with sequences that need fewer of them or one."""
+    c = Case(chunks, lens, hkv, g, d, 16, dtype, False)
+    hint = dict(max_q=max(chunks), max_len=max(lens))
+    assert hip._paged_workspace(0, 1 if dtype == "f16" else 2, 1 if dtype == "f16" else 2, sum(chunks), len(chunks), hkv * g, hkv, d,
+                                max(chunks), max(lens)) > 8 * sum(chunks) * hkv * g * d * 4
+    for causal in (True, False):
+        c.check(c.run(hip, causal, **hint), causal)
+
+
 def test_sizes_past_32_bits_are_refused(hip):
     t = lambda *s, dt=torch.float16: torch.zeros(s, dtype=dt, device="cuda")
     i = lambda *s: t(*s, dt=torch.int32)
