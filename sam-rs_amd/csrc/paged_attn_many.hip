@@ -278,7 +278,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
         const bool masks = key0 + 64 > wleast || there != ~0ul;
         // The tile's two halves of 32 keys, one's softmax on the vector unit beside the other's products on the matrix
         // unit: S0 | S1 with softmax 0 | P0 V0 with softmax 1 | P1 V1. LDS fragments are read kAhead products before
-        // their use. The scheduling groups hold these orders, which the compiler does not find.
+        // their use. The scheduling groups hold these orders, which the compiler does not find. It moves a half's exponentials
+        // behind the branch that may rescale O, to other waves' products: held before it they cost 3 to 6%.
         f32x16 s[2];
         X8 kf[2 * KS], vf[4 * MBO], b[4], blo[4];
         float alpha = 1.f;
