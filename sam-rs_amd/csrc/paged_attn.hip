@@ -35,10 +35,11 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
     // Four workgroups a CU (two past head dim 128, where one runs at a time), so that sequences of different lengths share
     // the card, of 512 KB of keys and values each at least. 32 sequences, 8 key heads of 128 in e4m3: 820 to 8192 keys 92, 94,
     // 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125, 134 and 148; 4 heads of 256 in e4m3,
-    // 8192 each, 103, 112 and 132 with 2, 4 and 8. Where f32 products bound the call, two a CU: 2048 rows over 4096 keys, 8
-    // heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
+    // 8192 each, 103, 112 and 132 with 2, 4 and 8. Where f32 products bound the call, two a CU at most: 2048 rows over 4096
+    // keys, 8 heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
     const long bytes = 2L * d * (cache_dtype == kE4M3 ? 1 : dtype == kF32 ? 4 : 2) * max_len;  // a sequence's, of one head
-    const long many = std::min(((d > 128 || (plan.rtiles > 1 && dtype == kF32) ? 2L : 4L) * cus + base - 1) / base, bytes >> 19);
+    const long want = plan.rtiles > 1 && dtype == kF32 ? 2L * cus / base : ((d > 128 ? 2L : 4L) * cus + base - 1) / base;
+    const long many = std::min(want, bytes >> 19);
     // One a CU, of 128 KB each at least: a CU alone reads 60 GB/s. In f16, 2048 keys of 4 heads of 128 take 22.6, 16.4, 12.2 and
     // 10.3 us with 1, 2, 4 and 8 splits, 4096 of 4 heads of 64 25.4, 17.2, 11.9 and 9.6, 1024 of 8 heads of 128 14.0, 11.7 and
     // 9.7 with 1, 2 and 4. Below 448 KB the second launch costs what it gains (577 keys of 8 heads of 64 8.0 and 8.1 with 1

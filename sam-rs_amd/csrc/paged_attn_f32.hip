@@ -40,11 +40,11 @@ __device__ __forceinline__ f32x4 widen(int c, float s) {
 
 template <typename C, int DP, int RB>
 __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(PagedParams p) {
-  constexpr int NC = DP / 16, ND = DP / 64, TR = 16 * RB;
+  constexpr int NC = DP / 16, ND = (DP + 63) / 64, TR = 16 * RB;
   constexpr bool kScaled = __is_same(C, e4m3);
   typedef typename Raw4<C>::t Raw;
   __shared__ float sm_m[2][TR], sm_l[2][TR];
-  extern __shared__ __attribute__((aligned(16))) float sm_o[];  // [2][RB][DP / 4 * 64]
+  extern __shared__ __attribute__((aligned(16))) float sm_o[];  // [2][RB][4 ND][256]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int d = p.c.d;
   if (p.zero_rest) paged_zero_rest<float>(p);
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
 }
 
 template <typename C, int DP, int RB> hipError_t launch_f32(const PagedParams& p, hipStream_t stream) {
-  constexpr int lds = 2 * RB * (DP / 4) * 64 * 4;
+  constexpr int lds = 2 * RB * 4 * ((DP + 63) / 64) * 256 * 4;
   static_assert(lds <= 64 << 10, "the joining buffer");
   const long blocks = (long)p.rtiles * p.nsplit * p.c.heads * p.c.batch;
   hipLaunchKernelGGL((paged_f32_kernel<C, DP, RB>), dim3((unsigned)blocks), dim3(256), lds, stream, p);
@@ -323,7 +323,8 @@ template <typename C> hipError_t by_size(const PagedParams& p, int rows, hipStre
   if (rows == 16)
     return d <= 64 ? launch_f32<C, 64, 1>(p, stream)
                    : d <= 128 ? launch_f32<C, 128, 1>(p, stream) : launch_f32<C, 256, 1>(p, stream);
-  return d <= 64 ? launch_f32<C, 64, 2>(p, stream) : launch_f32<C, 128, 2>(p, stream);
+  return d <= 64 ? launch_f32<C, 64, 2>(p, stream)
+                 : d <= 96 ? launch_f32<C, 96, 2>(p, stream) : launch_f32<C, 128, 2>(p, stream);
 }
 
 }  // namespace
