@@ -5,6 +5,18 @@
 
 namespace samhip {
 
+// Key splits of a call bound by f32 products, `base` workgroups of which `slots` run at once: the fewest rounds, where a
+// split costs 5% more. 2048 rows over 4096 keys, 8 heads of 128 (two whole rounds), 401, 425, 468 and 550 us with 1, 2, 4 and
+// 8 splits; 41 chunks of 125 rows over 4320 keys, one head, at 256 (1.3 rounds) 605, 491, 473 and 547 with 1 to 4, at 96 (0.6)
+// 169, 183, 138 and 157; 9 with 8 heads of 128 (1.1) 374, 304, 301 and 301.
+static long f32_splits(long base, long slots) {
+  long best = 1;
+  auto cost = [&](long n) { return (double)((base * n + slots - 1) / slots) / n * (1 + 0.05 * (n - 1)); };
+  for (long n = 2; n <= 64; ++n)
+    if (cost(n) < cost(best)) best = n;
+  return best;
+}
+
 PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads, int d, int max_q,
                      int max_len, int cus) {
   PagedPlan plan = {};
@@ -35,10 +47,10 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
     // Four workgroups a CU (two past head dim 128, where one runs at a time), so that sequences of different lengths share
     // the card, of 512 KB of keys and values each at least. 32 sequences, 8 key heads of 128 in e4m3: 820 to 8192 keys 92, 94,
     // 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125, 134 and 148; 4 heads of 256 in e4m3,
-    // 8192 each, 103, 112 and 132 with 2, 4 and 8. Where f32 products bound the call, two a CU at most: 2048 rows over 4096
-    // keys, 8 heads of 128, 401, 425, 468 and 550 us with 1, 2, 4 and 8 splits.
+    // 8192 each, 103, 112 and 132 with 2, 4 and 8. Calls that f32 products bound count rounds.
     const long bytes = 2L * d * (cache_dtype == kE4M3 ? 1 : dtype == kF32 ? 4 : 2) * max_len;  // a sequence's, of one head
-    const long want = plan.rtiles > 1 && dtype == kF32 ? 2L * cus / base : ((d > 128 ? 2L : 4L) * cus + base - 1) / base;
+    const long want = plan.rtiles > 1 && dtype == kF32 ? f32_splits(base, (d > 64 ? 1L : 2L) * cus)
+                                                       : ((d > 128 ? 2L : 4L) * cus + base - 1) / base;
     const long many = std::min(want, bytes >> 19);
     // One a CU, of 128 KB each at least: a CU alone reads 60 GB/s. In f16, 2048 keys of 4 heads of 128 take 22.6, 16.4, 12.2 and
     // 10.3 us with 1, 2, 4 and 8 splits, 4096 of 4 heads of 64 25.4, 17.2, 11.9 and 9.6, 1024 of 8 heads of 128 14.0, 11.7 and
