@@ -21,7 +21,7 @@ extern "C" {
  * for (x0, x1) = (x[2i], x[2i+1]) or, with halves, (x[i], x[i + pairs]); columns past 2 * pairs are copied. inverse
  * turns by the negative angle (the gradient's way back). pos [b, l, naxes] int32 with strides (batch, token, axis), 0 to
  * share positions; freqs [pairs] f64, radians per unit of position; axes [pairs] int32 in [0, naxes) (another value
- * takes position 0). The angle is formed in f64, sine, cosine and the turn in f32. Strides of x and out: (batch, token,
+ * takes position 0); with pairs == 0 all three may be NULL. The angle is formed in f64, sine, cosine and the turn in f32. Strides of x and out: (batch, token,
  * head) elements, NULL = contiguous; the head dimension is contiguous. out may be x with the same strides; it must not
  * overlap x otherwise. Pointers are aligned to their elements; 16-byte aligned rows with pairs % 4 == 0 (halves:
  * pairs % 8 == 0) run on the vector kernel.

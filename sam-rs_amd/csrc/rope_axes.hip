@@ -215,7 +215,7 @@ template <typename T> hipError_t launch(RopeAxesParams p, long tokens, hipStream
     p.total = p.groups * p.hgroups * p.units;
     const dim3 grid((unsigned)((p.total + 255l) / 256));
     auto run = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p); };
-    const bool ax = p.naxes <= 4;
+    const bool ax = p.naxes <= 4 && p.pairs > 0;  // without pairs pos may be null
     if (!vec)
       run(rope_axes_any<T>);
     else if (hp > 1 && nt > 1)

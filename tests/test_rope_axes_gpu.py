@@ -119,3 +119,19 @@ def test_empty_calls_and_refusals(hip):
                  lambda: hip.rope_axes(x[0, 0], pos, freqs, axes), lambda: hip.rope_axes(x, pos.cpu(), freqs, axes)):
         with pytest.raises(hip.SamHipError):
             call()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("naxes", [1, 4, 5])
+@pytest.mark.parametrize("shape, off", [((2, 5, 3, 64), 0), ((1, 9000, 8, 128), 0), ((2, 5, 3, 30), 0), ((2, 5, 3, 64), 1)])
+def test_no_pairs_need_no_positions(hip, dtype, naxes, shape, off):
+    """The C entry takes NULL for pos, freqs and axes where pairs is 0: out becomes a copy of x, with vectors and without."""
+    b, l, h, d = shape
+    x = torch.randn(b * l * h * d + off, device="cuda").to(DT[dtype])[off:].view(shape)
+    out = torch.zeros_like(x)
+    code = {"f32": 0, "f16": 1, "bf16": 2}[dtype]
+    for halves in (0, 1):
+        out.zero_()
+        rc = hip.load().sam_hip_rope_axes(x.data_ptr(), None, None, None, out.data_ptr(), code, b, l, h, d, 0, naxes, None, None,
+                                          None, halves, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(out, x)
