@@ -10,8 +10,9 @@
 //   the reduction index is permuted alike: element j of lane group g is key 16 (j / 4) + 4 g + j % 4.
 // e4m3 codes become 16-bit values with their row's scale in one conversion, exactly (in f16, values below 2^-14 to
 // f16's subnormal step). Softmax statistics and sums are f32. f16 P is rounded to f16 and its sum taken over the rounded
-// values; bf16 P goes as hi + lo, which leaves 2^-16 of it (one bf16 term would leave 2^-8, as much as the output's
-// own rounding).
+// values, all of it times 2^15, which O / l cancels: weights keep f16's 11 bits down to 2^-29 of the largest, so that
+// thousands of keys far below one that dominates are not lost (each is off by 2^-40 of it at most). bf16 P goes as
+// hi + lo, which leaves 2^-16 of it (one bf16 term would leave 2^-8, as much as the output's own rounding).
 //
 // The four waves of a workgroup join at its end, the key ranges of a sequence in paged_combine_kernel.
 //
@@ -45,6 +46,7 @@ template <typename T, typename C, int DP, int RB>
 __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C, e4m3) ? 2 : 3) void paged_few_kernel(PagedParams p) {
   typedef typename Vec<T>::x8 X8;
   constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
+  constexpr float kLift = kSplitP ? 0.f : 15.f;  // P is lifted by 2^kLift
   constexpr int TR = 16 * RB, NK = DP / 32;
   constexpr int CW = DP >= 128 ? 8 : DP / 16, NV = DP / (16 * CW);  // columns of a value row that a lane takes at once
   typedef typename Raw<8 * (int)sizeof(C)>::t KRaw;
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = max_nc(top, s[rb][i][e]);
-        const float m_new = fmaxf(m[rb], max_over_rows16(top) * p.sc);
+        const float m_new = fmaxf(m[rb], max_over_rows16(top) * p.sc - kLift);
         const float base = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = exp2_fast(m[rb] - base);
         m[rb] = m_new;

@@ -14,8 +14,13 @@
 // not see whole are looked over as they are stored: such values go into LDS as 0, and the rows that see one add it
 // afterwards.
 //
-// Softmax statistics and sums are f32; the running maximum moves only when a tile passes it by 8 (in log2), so that O is
-// rarely rescaled. f16 P is rounded to f16 and summed as rounded; bf16 P goes as hi + lo.
+// Softmax statistics and sums are f32; the running maximum moves only when a tile passes it by 4 (in log2), so that O is
+// rarely rescaled. f16 P is rounded to f16 and summed as rounded, all of it times 2^11, which O / l cancels: P then ends
+// below 2^15, and weights keep f16's 11 bits down to 2^-25 of the largest, so that thousands of keys far below one that
+// dominates are not lost (each is off by 2^-36 of it at most). A maximum that moves later would leave less of f16's range:
+// 8192 rows and keys, 4 heads of 256 in f16 on a card a tenth slower: 358 us with 8, 348 with 4, 368, 386 and 441 with 3, 2
+// and 0; at 128 319, 323, 321, 323 and 333.
+// bf16 P goes as hi + lo, whose range is f32's.
 //
 // What bounds it: products, softmax and LDS reads beside each other on too few waves (a loop of the products alone, fed
 // from LDS, reaches 1.11 PFLOP/s at head dim 128). The vector units' and the matrix units' busy cycles add up to the whole
@@ -33,7 +38,7 @@ namespace samhip {
 
 namespace {
 
-constexpr float kSlack = 8.f;
+constexpr float kSlack = 4.f;  // how far a tile may pass the running maximum, in log2
 
 // LDS: rows of 128, 256 or 512 bytes without padding, as the DMA leaves them (a wave's instruction fills 1 KB). 16-byte
 // chunk c of row r lies at c ^ swizzle(r), so that the 16 rows of which a K read takes one chunk each, and the 8 rows of
@@ -57,6 +62,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
   typedef ManyGeom<DP> G;
   typedef typename Vec<T>::x8 X8;
   constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
+  constexpr float kLift = kSplitP ? 0.f : 15.f - kSlack;  // P is lifted by 2^kLift
   // LDS fragments in flight ahead of their products: bf16 at head dim 64 has registers for two (8192 rows
   // and keys, 16 heads: 561 us against 568 with four, from e4m3 577 against 608)
   constexpr int kAhead = DP <= 64 && kSplitP ? 2 : 4;
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
           float top = s[h][0];
 #pragma unroll
           for (int e = 1; e < 16; ++e) top = max_nc(top, s[h][e]);
-          top = max_with_partner32(top) * sc;
+          top = max_with_partner32(top) * sc - kLift;
           const float mn = top > m + kSlack ? top : m, base = mn == -INFINITY ? 0.f : mn;
           alpha = exp2_fast(m - base);  // m == mn: 1, or 0 while both are -inf and O is 0
           m = mn;

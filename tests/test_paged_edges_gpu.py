@@ -1,0 +1,56 @@
+"""The paged memory at the edges of what its header defines: weights far below a row's largest."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+# P beside v: f32 as it is, f16 to half a step of f16, bf16 as two bf16 terms (2^-16)
+P_UNIT = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -16}
+
+
+@pytest.fixture(scope="module")
+def hip():
+    import sam_hip
+
+    sam_hip.load()
+    assert torch.cuda.is_available(), "no GPU visible"
+    return sam_hip
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 20, 50])
+@pytest.mark.parametrize("gap, length", [(16.0, 8192), (17.5, 8192), (17.5, 28736)])
+def test_thousands_of_keys_far_below_a_dominant_one(hip, dtype, d, rows, gap, length):
+    """A key of value 0 that holds nearly all of a row's weight, at either end, and thousands of equal ones `gap` nats
+    lower, whose values are all that is left of the result. Scores are exact (0 and 8 * gap / 8), so that the bound is
+    P's rounding in numerator and denominator, the sums' at one f32 rounding a key, an exponent's (4 roundings of
+    gap log2 e), and the output's. (f16 weights of the many-row kernel leave the normal range at 2^-25 of the largest; at
+    17.5 nats, 2^-25.25, half a subnormal step is 2^-10.75 of one, while the denominator, the dominant key, is exact.)"""
+    dt, page = DT[dtype], 64
+    w = math.exp(-gap)
+    for first in (True, False):
+        gen = torch.Generator(device="cuda").manual_seed(d + rows)
+        k = torch.zeros(length, 1, d, device="cuda", dtype=dt)
+        v = (0.5 + torch.rand(length, 1, d, generator=gen, device="cuda")).to(dt)
+        at = 0 if first else length - 1
+        k[at, 0, 0], v[at] = gap / 8, 0
+        q = torch.zeros(rows, 1, d, device="cuda", dtype=dt)
+        q[:, 0, 0] = 8
+        pages = -(-length // page)
+        kp, vp = (torch.zeros(pages, 1, page, d, device="cuda", dtype=dt) for _ in range(2))
+        table = torch.arange(pages, device="cuda", dtype=torch.int32).view(1, -1)
+        hip.kv_write(k, v, kp, vp, table, ints([0, length]), ints([length]))
+        got = hip.paged_attention(q, kp, vp, table, ints([0, rows]), ints([length]), scale=1.0, causal=False)
+        want = (v.double().sum(0) * w / (1 + (length - 1) * w)).expand(rows, 1, d).cpu()
+        rel = 2 * P_UNIT[dtype] + (length + 16) * ref.F32_U + 2 * 4 * gap * ref.F32_U
+        bound = ref.with_rounding(rel * want, want, dt)
+        assert ((got.cpu().double() - want).abs() <= bound).all()
