@@ -44,10 +44,11 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
  * ones. sam_hip_kv_read writes rows 0 .. max_len of every sequence to k, v [batch, max_len, kv_heads, d] of `dtype`, zeros
  * from lens[b] on (from an e4m3 cache in any dtype, each value rounded to it once).
  *
- * What the tables say is checked on the device: lens are held to 0 .. table_width * page_size, starts to 0 .. tokens;
- * tokens outside every sequence or at a negative position are not written; a table entry outside 0 .. pages - 1 stands
- * for a page that is not there (not written, read as zeros, its keys not attended). Two positions that share a page slot
- * must not be written in one call. Limits: d % 8 == 0, d <= 256, table_width * page_size < 2^30, fewer than 2^31 rows in
+ * What the tables say is checked on the device. A sequence holds its keys below both lens[b] and table_width * page_size;
+ * its new tokens are those of 0 .. tokens - 1 that starts names, at the positions that lens[b] and starts[b+1] as they are
+ * give them, in kv-write and in attention alike. Tokens outside every sequence, at a negative position or past the table
+ * are not written; a table entry outside 0 .. pages - 1 stands for a page that is not there (not written, read as zeros,
+ * its keys not attended). Two positions that share a page slot must not be written in one call. Limits: d % 8 == 0, d <= 256, table_width * page_size < 2^30, fewer than 2^31 rows in
  * a pool and 2^27 in a write or a read.
  */
 #define SAM_HIP_E4M3 3

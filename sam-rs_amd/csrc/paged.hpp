@@ -150,11 +150,16 @@ template <typename T, typename C> __device__ __forceinline__ f32x4 only_not_fini
   return r;
 }
 
-// One sequence's new tokens [s0, s0 + lq), keys, and the row tile this workgroup starts with.
+// One sequence's new tokens [s0, s0 + lq), keys, and the row tile this workgroup starts with. Its token t sits at position
+// before + t, where kv_write puts it: behind the table's end too, if lens passes that.
 struct PagedWork {
   int tile, split, head, b;
-  int s0, lq, len;
+  int s0, lq, len, before;
 };
+// Keys that token t of a sequence sees, of those it holds.
+__device__ __forceinline__ int paged_keys(const PagedWork& w, int causal, int t) {
+  return causal ? max(0, min(w.len, w.before + t + 1)) : w.len;
+}
 __device__ __forceinline__ PagedWork paged_work(const PagedParams& p) {
   // Workgroup i runs on XCD i % 8. The (sequence, key head) comes first, then the key split, the row tile last: a
   // multiple of 8 of the first two leaves each head's keys to one XCD's L2, and sequences of different lengths, whose
@@ -175,9 +180,12 @@ __device__ __forceinline__ PagedWork paged_work(const PagedParams& p) {
   }
   w.head = unit % p.c.heads;
   w.b = unit / p.c.heads;
+  const int end = p.c.starts[w.b + 1], held = p.c.lens[w.b];
   w.s0 = max(0, min(p.c.starts[w.b], p.tokens));
-  w.lq = max(0, min(p.c.starts[w.b + 1], p.tokens) - w.s0);
+  w.lq = max(0, min(end, p.tokens) - w.s0);
   w.len = paged_len(p.c, w.b);
+  // 64 bits, for any lens and starts: before + lq <= lens, and what is below -2^31 sees no key either way
+  w.before = (int)max((long)held - end + w.s0, -(1l << 31));
   return w;
 }
 

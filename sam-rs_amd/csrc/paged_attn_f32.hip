@@ -11,7 +11,7 @@
 //
 // What bounds it: the f32 matrix rate (64 flops a cycle and SIMD) where many rows share the keys, else the bytes of
 // K and V. 16 rows use each value loaded for 8 flops a byte, twice what L1 would need to keep up. 2048 rows over 4096 keys,
-// 8 heads: head dim 64 191 us (90 TFLOP/s), 128 387 (89; a large library product 153), 256 with 4 heads 504 (68); a step of 32
+// 8 heads: head dim 64 191 us (90 TFLOP/s), 128 387 (89; a large library product 153), 256 with 4 heads 515 (67); a step of 32
 // sequences of 4096 keys, 8 key heads of 128, 210 (5.1 TB/s).
 #include "lds_dma.hpp"
 #include "paged.hpp"
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
       const int t = (int)divide_magic(r, p.gmagic, p.gshift);
       tok[rb] = w.s0 + t;
       head[rb] = w.head * p.group + (r - t * p.group);
-      limit[rb] = p.causal ? max(0, min(w.len, w.len - w.lq + t + 1)) : w.len;
+      limit[rb] = paged_keys(w, p.causal, t);
       const float* qr = reinterpret_cast<const float*>(p.q) + tok[rb] * p.sq[0] + head[rb] * p.sq[1];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -75,8 +75,8 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
     // the keys that the tile's first and last row see; this split's blocks of 32 of them
     const int tfirst = (int)divide_magic(rt * TR, p.gmagic, p.gshift);
     const int tlast = (int)divide_magic(min((rt + 1) * TR, rows) - 1, p.gmagic, p.gshift);
-    const int least = p.causal ? max(0, min(w.len, w.len - w.lq + tfirst + 1)) : w.len;
-    const int most = p.causal ? max(0, min(w.len, w.len - w.lq + tlast + 1)) : w.len;
+    const int least = paged_keys(w, p.causal, tfirst);
+    const int most = paged_keys(w, p.causal, tlast);
     const int blocks = (most + 31) >> 5, per = paged_share(blocks, p.per, p.nsplit);
     const int b0 = min(blocks, w.split * per), b1 = min(blocks, b0 + per);
     const bool direct = blocks <= per;  // one split has all keys: it writes the result itself

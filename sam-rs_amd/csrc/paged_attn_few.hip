@@ -66,8 +66,8 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
     const int lane = (int)opaque(threadIdx.x & 63), n = lane & 15, g = lane >> 4;
     const int tfirst = (int)divide_magic(rt * TR, p.gmagic, p.gshift);
     const int tlast = (int)divide_magic(min((rt + 1) * TR, rows) - 1, p.gmagic, p.gshift);
-    const int most = p.causal ? max(0, min(w.len, w.len - w.lq + tlast + 1)) : w.len;
-    const int least = p.causal ? max(0, min(w.len, w.len - w.lq + tfirst + 1)) : w.len;
+    const int most = paged_keys(w, p.causal, tlast);
+    const int least = paged_keys(w, p.causal, tfirst);
     // this split's blocks of 32 keys: ranges of the hint's longest sequence, longer ones where that was too short
     const int blocks = (most + 31) >> 5, per = paged_share(blocks, p.per, p.nsplit);
     const int b0 = min(blocks, w.split * per), b1 = min(blocks, b0 + per);
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
     for (int rb = 0; rb < RB; ++rb) {
       const int r = min(rt * TR + 16 * rb + n, rows - 1);
       const int t = (int)divide_magic(r, p.gmagic, p.gshift);
-      limit[rb] = p.causal ? max(0, min(w.len, w.len - w.lq + t + 1)) : w.len;
+      limit[rb] = paged_keys(w, p.causal, t);
       const T* qr = reinterpret_cast<const T*>(p.q) + (w.s0 + t) * p.sq[0] + (w.head * p.group + r - t * p.group) * p.sq[1];
 #pragma unroll
       for (int c = 0; c < NK; ++c) {

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
   for (int rt = w.tile; (long)rt * 128 < rows; rt += p.rtiles) {
     auto keys_of = [&](int r) {  // keys that row r sees
       const int t = (int)divide_magic(r, p.gmagic, p.gshift);
-      return p.causal ? max(0, min(w.len, w.len - w.lq + t + 1)) : w.len;
+      return paged_keys(w, p.causal, t);
     };
     const int most = keys_of(min((rt + 1) * 128, rows) - 1);
     const int least = keys_of(rt * 128);

@@ -1,4 +1,5 @@
-"""The paged memory at the edges of what its header defines: weights far below a row's largest."""
+"""The paged memory at the edges of what its header defines: weights far below a row's largest, sequences that
+outgrow their table or the new tokens."""
 import math
 
 import pytest
@@ -54,3 +55,28 @@ def test_thousands_of_keys_far_below_a_dominant_one(hip, dtype, d, rows, gap, le
         rel = 2 * P_UNIT[dtype] + (length + 16) * ref.F32_U + 2 * 4 * gap * ref.F32_U
         bound = ref.with_rounding(rel * want, want, dt)
         assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [1, 4, 40])
+def test_a_sequence_that_outgrows_its_table_or_its_tokens(hip, dtype, heads):
+    """kv_write and paged_attention give a token one position: lens past what the table names, and starts past the
+    tokens (whose last ones are not there), move no token that fits. lens 70 over a table of 64: tokens 0 .. 13 of 20
+    are stored at 50 .. 63, token t sees keys to 50 + t, those behind the table's end all 64."""
+    dt, d, page = DT[dtype], 64, 16
+    gen = torch.Generator(device="cuda").manual_seed(heads)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda").to(dt)
+    for chunk, end, length in ((20, 20, 70), (20, 26, 60), (20, 26, 68), (12, 12, 70), (20, 20, 2 ** 31 - 1), (20, 2 ** 31 - 1, 5),
+                               (20, 2 ** 31 - 1, -2 ** 31)):
+        kp, vp = rnd(4, 1, page, d), rnd(4, 1, page, d)
+        table = ints([[2, 0, 3, 1]])
+        q, k, v = rnd(chunk, heads, d), rnd(chunk, 1, d), rnd(chunk, 1, d)
+        hip.kv_write(k, v, kp, vp, table, ints([0, end]), ints([length]))
+        got = hip.paged_attention(q, kp, vp, table, ints([0, end]), ints([length])).cpu().double()
+        for t in range(chunk):
+            at = length - end + t  # its position
+            if 0 <= at < 64:
+                assert torch.equal(kp[int(table[0, at // page]), 0, at % page], k[t, 0])
+            want, bound = ref.attention(q[t:t + 1].cpu(), kp.cpu(), vp.cpu(), table.cpu(), [0, 1], [min(at + 1, 64)],
+                                        d ** -0.5, True, P_UNIT[dtype])
+            assert ((got[t:t + 1] - want).abs() <= ref.with_rounding(bound, want, dt)).all()
