@@ -67,7 +67,7 @@ int sam_hip_kv_read(void* k, void* v, const void* k_pages, const void* v_pages, 
  * and, with causal, j <= t's own position lens[b] - (starts[b+1] - t). q and out [tokens, heads, d] (strides (token,
  * head), multiples of 16 bytes; NULL = contiguous). A row that sees no key is 0; a key, or a value that is not finite,
  * reaches the rows that see it alone. Rows of no sequence stay as they are, or become 0 with zero_rest. out
- * must not overlap the other tensors.
+ * may be q with the same strides; it must not overlap q otherwise, nor the other tensors.
  * max_q and max_len are the longest chunk and the longest sequence as the caller expects them: they size the grid and
  * the key splits, and a call whose sequences exceed them is computed all the same, more slowly.
  * Workspace: sam_hip_paged_attention_workspace_size() bytes of device memory for the key splits' partial results (it

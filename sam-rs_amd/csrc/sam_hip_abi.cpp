@@ -797,6 +797,9 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
   if (int rc = token_strides("paged-attention", "out", strides_o, p.so, heads, d, dtype); rc != SAM_HIP_OK) return rc;
   if ((tokens > 1 && p.so[0] == 0) || (heads > 1 && p.so[1] == 0))
     return fail(SAM_HIP_EINVAL, "paged-attention: out's rows must lie apart (a stride of 0)");
+  // in place is sound: a row of q is read by the workgroups that its result comes from alone, and written after that
+  if (q == out && ((tokens > 1 && p.sq[0] != p.so[0]) || (heads > 1 && p.sq[1] != p.so[1])))
+    return fail(SAM_HIP_EINVAL, "paged-attention: in place, q and out must have the same strides");
   if (!aligned16(q) || !aligned16(out))
     return fail(SAM_HIP_EUNSUPPORTED, "paged-attention: q and out must be 16-byte aligned");
   const samhip::PagedPlan plan = samhip::paged_plan(dtype, cache_dtype, tokens, batch, heads, kv_heads, d, max_q, max_len,

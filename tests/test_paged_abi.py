@@ -119,6 +119,14 @@ def test_outputs_whose_rows_share_memory_are_refused(lib):
     assert rope(lib, b=2, so=strides(0, 128, 64)) == 1
 
 
+def test_attention_in_place_keeps_its_strides(lib):
+    assert attend(lib, so=strides(512, 64)) == 1 and b"in place" in lib.sam_hip_last_error()
+    assert attend(lib, sq=strides(64, 256), so=strides(256, 64)) == 1 and b"in place" in lib.sam_hip_last_error()
+    need = dict(ws=None, d=128, kv_heads=1, batch=1, max_q=1, max_len=1 << 16, width=1 << 12)  # fails at its workspace
+    assert attend(lib, tokens=1, heads=8, so=strides(1 << 20, 128), **need) == 1  # one token: its stride means nothing
+    assert b"workspace" in lib.sam_hip_last_error()
+
+
 def test_a_missing_or_short_workspace_is_refused(lib):
     size = lib.sam_hip_paged_attention_workspace_size
     need = size(1, 1, 1, 1, 8, 1, 128, 1, 1 << 16)

@@ -1,5 +1,5 @@
 """The paged memory at the edges of what its header defines: weights far below a row's largest, sequences that
-outgrow their table or the new tokens."""
+outgrow their table or the new tokens, results in place of their queries."""
 import math
 
 import pytest
@@ -80,3 +80,24 @@ def test_a_sequence_that_outgrows_its_table_or_its_tokens(hip, dtype, heads):
             want, bound = ref.attention(q[t:t + 1].cpu(), kp.cpu(), vp.cpu(), table.cpu(), [0, 1], [min(at + 1, 64)],
                                         d ** -0.5, True, P_UNIT[dtype])
             assert ((got[t:t + 1] - want).abs() <= ref.with_rounding(bound, want, dt)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("chunks, lens, d", [([1, 1], [3000, 40], 128), ([300, 70], [300, 2000], 64), ([20, 5], [4000, 9], 256)])
+def test_results_in_place_of_their_queries(hip, dtype, chunks, lens, d):
+    """out = q, contiguous and as a part of packed rows, with split keys and without, equals a result apart bit for bit; the
+    rest of the packed rows stays."""
+    dt, page, t = DT[dtype], 16, sum(chunks)
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda").to(dt)
+    width = -(-max(lens) // page)
+    kp, vp = rnd(2 * width, 2, page, d), rnd(2 * width, 2, page, d)
+    args = kp, vp, torch.arange(2 * width, device="cuda", dtype=torch.int32).view(2, -1), ints([0, chunks[0], t]), ints(lens)
+    packed = rnd(t, 3, 4, d)
+    q = packed[:, 1].contiguous()
+    for causal in (True, False):
+        want = hip.paged_attention(q, *args, causal=causal)
+        own, rows = q.clone(), packed.clone()
+        assert hip.paged_attention(own, *args, causal=causal, out=own) is own and torch.equal(own, want)
+        hip.paged_attention(rows[:, 1], *args, causal=causal, out=rows[:, 1])
+        assert torch.equal(rows[:, 1], want) and torch.equal(rows[:, ::2], packed[:, ::2])
