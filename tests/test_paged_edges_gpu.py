@@ -1,5 +1,6 @@
 """The paged memory at the edges of what its header defines: weights far below a row's largest, sequences that
-outgrow their table or the new tokens, results in place of their queries."""
+outgrow their table or the new tokens, results in place of their queries,
+e4m3 rows of every scale."""
 import math
 
 import pytest
@@ -101,3 +102,29 @@ def test_results_in_place_of_their_queries(hip, dtype, chunks, lens, d):
         assert hip.paged_attention(own, *args, causal=causal, out=own) is own and torch.equal(own, want)
         hip.paged_attention(rows[:, 1], *args, causal=causal, out=rows[:, 1])
         assert torch.equal(rows[:, 1], want) and torch.equal(rows[:, ::2], packed[:, ::2])
+
+
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_an_e4m3_row_is_read_as_kv_read_returns_it(hip, dtype, d, rows):
+    """With one visible key the attention is that key's value, in q's dtype as kv_read rounds it: for each scale that
+    kv_write makes (bytes 1 .. 253), codes of every size, results past the type's range and below its normal one."""
+    dt, b = DT[dtype], 253
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    codes = torch.randint(0, 256, (b, 1, 1, d), generator=gen, device="cuda", dtype=torch.uint8)
+    codes[(codes & 0x7F) == 0x7F] = 0x7E  # the largest value in place of NaN
+    v = codes.view(torch.float8_e4m3fn)
+    k = torch.zeros(b, 1, 1, d, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)
+    vs = torch.arange(1, b + 1, device="cuda", dtype=torch.int32).to(torch.uint8).view(b, 1, 1)
+    ks = torch.full((b, 1, 1), 127, device="cuda", dtype=torch.uint8)
+    table, lens = torch.arange(b, device="cuda", dtype=torch.int32).view(b, 1), ints([1] * b)
+    _, want = hip.kv_read(k, v, table, lens, 1, ks, vs, dtype=dt)
+    q = torch.randn(b * rows, 1, d, generator=gen, device="cuda").to(dt)
+    starts = torch.arange(b + 1, device="cuda", dtype=torch.int32) * rows
+    got = hip.paged_attention(q, k, v, table, starts, lens, ks, vs, causal=False, max_q=rows)
+    got, want = got.view(b, rows, d), want.view(b, 1, d).expand(b, rows, d)
+    bad = (got != want).any(-1).any(-1).nonzero().flatten().tolist()
+    assert not bad, f"scale bytes {[x + 1 for x in bad]}"
