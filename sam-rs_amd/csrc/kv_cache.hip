@@ -26,7 +26,6 @@ struct KvWriteParams {
   const void* k;
   const void* v;
   long sk[2], sv[2];
-  int tokens;
   int rows;  // tokens * heads, below 2^27
   unsigned hmagic, hshift;  // division by heads
 };
@@ -288,7 +287,7 @@ template <typename T, bool FP8> hipError_t read_launch(const KvReadParams& p, hi
 
 hipError_t kv_write(int dtype, int cache_dtype, const void* k, const void* v, const long* sk, const long* sv,
                     const PagedKv& c, int tokens, hipStream_t stream) {
-  KvWriteParams p{c, k, v, {sk[0], sk[1]}, {sv[0], sv[1]}, tokens, tokens * c.heads, 0, 0};
+  KvWriteParams p{c, k, v, {sk[0], sk[1]}, {sv[0], sv[1]}, tokens * c.heads, 0, 0};
   if (p.rows == 0) return hipSuccess;
   division_magic(c.heads, &p.hmagic, &p.hshift);
   if (cache_dtype == kE4M3)

@@ -38,7 +38,6 @@ template <> struct Raw<16> {
 };
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // Workgroups a CU: as many as registers allow with a block of K and one of V in flight. Three for e4m3 at head dim 128
 // (131 us for the bf16 call above with eight splits, 137 with two).
