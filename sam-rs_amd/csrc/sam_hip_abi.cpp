@@ -624,8 +624,9 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
   if (b < 0 || l < 0 || h <= 0 || d <= 0 || pairs < 0 || naxes <= 0)
     return fail(SAM_HIP_EINVAL, "rope-axes: sizes b=%d l=%d h=%d d=%d pairs=%d axes=%d", b, l, h, d, pairs, naxes);
   if (2L * pairs > d) return fail(SAM_HIP_EINVAL, "rope-axes: %d pairs do not fit in a head dim of %d", pairs, d);
-  if ((long)b * l >= (1L << 31) || h > 65535 || (long)h * d >= (1L << 31) || (long)b * l * ((long)h * d) > (1L << 38))
-    return fail(SAM_HIP_EUNSUPPORTED, "rope-axes: more than 2^31 tokens, 65535 heads or 2^38 elements");
+  // a launch takes whole tokens, in workgroups of 256 threads that it counts in 32 bits: one token's must fit
+  if ((long)b * l >= (1L << 31) || h > 65535 || (long)h * d > (1L << 31) - 256 || (long)b * l * ((long)h * d) > (1L << 38))
+    return fail(SAM_HIP_EUNSUPPORTED, "rope-axes: more than 2^31 tokens or elements of one, 65535 heads or 2^38 elements");
   const int elem = dtype == 0 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(x) % elem || reinterpret_cast<uintptr_t>(out) % elem ||
       reinterpret_cast<uintptr_t>(pos) % 4 || reinterpret_cast<uintptr_t>(freqs) % 8 ||

@@ -113,6 +113,12 @@ def test_launches_past_32_bits_of_threads_are_refused(lib):
     assert size(1, 1, 1 << 26, 1, 2, 2, 128, 1, 1 << 20) == 0 < size(1, 1, 1 << 20, 1, 2, 2, 128, 1, 1 << 20)
 
 
+def test_a_token_that_no_launch_holds_is_refused(lib):
+    """Threads of one token past what a launch counts: the host would have gone on without a token done."""
+    for d in ((1 << 31) - 1, (1 << 31) - 255):
+        assert rope(lib, b=1, l=1, h=1, d=d, pairs=0) == 3
+
+
 def test_outputs_whose_rows_share_memory_are_refused(lib):
     assert attend(lib, so=strides(0, 64)) == 1 and attend(lib, so=strides(256, 0)) == 1
     assert rope(lib, so=strides(512, 0, 64)) == 1 and rope(lib, so=strides(512, 128, 0)) == 1
