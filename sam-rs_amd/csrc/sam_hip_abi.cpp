@@ -714,7 +714,8 @@ int check_paged_sizes(const char* what, int tokens, int batch, int heads, int kv
                 batch, heads, kv_heads, d, max_q, max_len);
   if (heads % kv_heads != 0)
     return fail(SAM_HIP_EINVAL, "%s: %d query heads do not share %d key heads evenly", what, heads, kv_heads);
-  if ((long)tokens * heads >= 1L << 31 || (long)max_q * (heads / kv_heads) >= 1L << 30 || (long)batch * kv_heads >= 1L << 24)
+  // the kernels number the rows of a sequence in 32 bits, to the end of their last tile
+  if ((long)tokens * heads > (1L << 31) - 256 || (long)max_q * (heads / kv_heads) >= 1L << 30 || (long)batch * kv_heads >= 1L << 24)
     return fail(SAM_HIP_EUNSUPPORTED, "%s: too many rows (tokens=%d heads=%d batch=%d)", what, tokens, heads, batch);
   return SAM_HIP_OK;
 }

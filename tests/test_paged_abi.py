@@ -119,6 +119,14 @@ def test_a_token_that_no_launch_holds_is_refused(lib):
         assert rope(lib, b=1, l=1, h=1, d=d, pairs=0) == 3
 
 
+def test_rows_whose_last_tile_passes_32_bits_are_refused(lib):
+    size = lib.sam_hip_paged_attention_workspace_size
+    for tokens in ((1 << 31) - 1, (1 << 31) - 255):
+        assert attend(lib, tokens=tokens, heads=1, kv_heads=1, batch=1, max_q=1) == 3
+        assert size(1, 1, tokens, 1, 1, 1, 64, 1, 64) == -1
+    assert size(1, 1, (1 << 31) - 256, 1, 1, 1, 64, 1, 64) >= 0
+
+
 def test_outputs_whose_rows_share_memory_are_refused(lib):
     assert attend(lib, so=strides(0, 64)) == 1 and attend(lib, so=strides(256, 0)) == 1
     assert rope(lib, so=strides(512, 0, 64)) == 1 and rope(lib, so=strides(512, 128, 0)) == 1
