@@ -612,6 +612,31 @@ int sam_hip_qkv_rope(const void* y, const void* bias, const float* cos_t, const 
 
 // ------------------------------------------------------------------------------------ the paged memory
 
+namespace {
+
+// Whether rows of d elements at `dims` strides (of n[i] steps each) lie apart: each stride passes all that the smaller
+// ones span, as in every permutation and slice of a contiguous tensor.
+bool rows_apart(int dims, const long* n, const long* s, long d) {
+  unsigned __int128 span = d;
+  long below = -1;  // strides up to here are done
+  for (int done = 0; done < dims;) {
+    long next = -1;
+    for (int i = 0; i < dims; ++i)
+      if (s[i] > below && (next < 0 || s[i] < next)) next = s[i];
+    for (int i = 0; i < dims; ++i) {
+      if (s[i] != next) continue;
+      ++done;
+      if (n[i] <= 1) continue;
+      if ((unsigned __int128)next < span) return false;
+      span += (unsigned __int128)next * (n[i] - 1);
+    }
+    below = next;
+  }
+  return true;
+}
+
+}  // namespace
+
 extern "C" {
 
 int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const int* axes, void* out, int dtype, int b,
@@ -644,8 +669,9 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
     if (strides_pos) sp[i] = strides_pos[i];
     if (sx[i] < 0 || so[i] < 0 || sp[i] < 0) return fail(SAM_HIP_EUNSUPPORTED, "rope-axes: strides must not be negative");
   }
-  if ((b > 1 && so[0] == 0) || (l > 1 && so[1] == 0) || (h > 1 && so[2] == 0))
-    return fail(SAM_HIP_EINVAL, "rope-axes: out's rows must lie apart (a stride of 0)");
+  const long steps[3] = {b, l, h};
+  if (!rows_apart(3, steps, so, d))
+    return fail(SAM_HIP_EINVAL, "rope-axes: out's rows must lie apart (strides %ld, %ld, %ld)", so[0], so[1], so[2]);
   if (x == out && (sx[0] != so[0] || sx[1] != so[1] || sx[2] != so[2]))
     return fail(SAM_HIP_EINVAL, "rope-axes: in place, x and out must have the same strides");
   return check_launch(samhip::rope_axes(dtype, x, pos, freqs, axes, out, b, l, h, d, pairs, naxes, sx, sp, so,
@@ -797,8 +823,9 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
     return fail(SAM_HIP_EINVAL, "paged-attention: scale must be finite and not negative, got %g", (double)scale);
   if (int rc = token_strides("paged-attention", "q", strides_q, p.sq, heads, d, dtype); rc != SAM_HIP_OK) return rc;
   if (int rc = token_strides("paged-attention", "out", strides_o, p.so, heads, d, dtype); rc != SAM_HIP_OK) return rc;
-  if ((tokens > 1 && p.so[0] == 0) || (heads > 1 && p.so[1] == 0))
-    return fail(SAM_HIP_EINVAL, "paged-attention: out's rows must lie apart (a stride of 0)");
+  const long steps[2] = {tokens, heads};
+  if (!rows_apart(2, steps, p.so, d))
+    return fail(SAM_HIP_EINVAL, "paged-attention: out's rows must lie apart (strides %ld, %ld)", p.so[0], p.so[1]);
   // in place is sound: a row of q is read by the workgroups that its result comes from alone, and written after that
   if (q == out && ((tokens > 1 && p.sq[0] != p.so[0]) || (heads > 1 && p.sq[1] != p.so[1])))
     return fail(SAM_HIP_EINVAL, "paged-attention: in place, q and out must have the same strides");

@@ -133,6 +133,19 @@ def test_outputs_whose_rows_share_memory_are_refused(lib):
     assert rope(lib, b=2, so=strides(0, 128, 64)) == 1
 
 
+def test_outputs_whose_rows_overlap_are_refused(lib):
+    """Rows that share a part, by one stride or by two together; layouts whose rows lie apart get past that (to the
+    refusal of an in-place call with other strides)."""
+    for so in ((32, 64), (256, 56), (64, 64), (248, 64), (64, 192)):
+        assert attend(lib, so=strides(*so)) == 1 and b"apart" in lib.sam_hip_last_error()
+    for so in ((64, 256), (1 << 40, 64), (64, 1 << 60)):
+        assert attend(lib, so=strides(*so)) == 1 and b"in place" in lib.sam_hip_last_error()
+    for so in ((0, 64, 64), (0, 128, 32), (0, 120, 64), (512, 64, 64), (256, 128, 64)):
+        assert rope(lib, b=2 if so[0] else 1, so=strides(*so)) == 1 and b"apart" in lib.sam_hip_last_error()
+    for so in ((0, 64, 256), (0, 192, 64), (1 << 60, 64, 256), (8 * 64, 64, 4 * 64)):
+        assert rope(lib, out=FAKE, b=2 if so[0] else 1, so=strides(*so)) == 1 and b"in place" in lib.sam_hip_last_error()
+
+
 def test_attention_in_place_keeps_its_strides(lib):
     assert attend(lib, so=strides(512, 64)) == 1 and b"in place" in lib.sam_hip_last_error()
     assert attend(lib, sq=strides(64, 256), so=strides(256, 64)) == 1 and b"in place" in lib.sam_hip_last_error()
