@@ -645,6 +645,13 @@ def _sizes(what: str, *sizes) -> None:
             raise SamHipError(f"{what}: sizes must be below 2^31, got {sizes}")
 
 
+def _empty_call(what: str) -> None:
+    """A call that has nothing to compute obeys the switch as those that reach the library do."""
+    if not enabled():
+        raise SamHipDisabled(f"{what}: the HIP path is switched off (sam_hip_set_enabled(0) or SAM_HIP_DISABLE); take the "
+                             "reference path")
+
+
 def _is_current(dev: int) -> bool:
     return dev == (torch.cuda.current_device() if _raw_device is None else _raw_device())
 
@@ -710,6 +717,7 @@ def rope_axes(x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, axes: tor
             raise SamHipError(f"rope_axes: pos {tuple(at)} does not broadcast to {(b, l)} positions of its axes") from e
         sp = _long3(*pos.stride())
     if x.numel() == 0:
+        _empty_call("rope-axes")
         return out
     if not (freqs.is_contiguous() and axes.is_contiguous()):
         freqs, axes = freqs.contiguous(), axes.contiguous()
@@ -795,7 +803,7 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: t
         raise SamHipError(f"kv_write: k and v must be [T, {heads}, {d}], got {tuple(shape)} and {tuple(v.shape)}")
     tokens = shape[0]
     if tokens == 0 or b == 0 or width == 0:
-        return
+        return _empty_call("kv-write")
     if tokens >> 31:
         _sizes("kv_write", tokens)
     table, starts, lens = _plain(table), _plain(starts), _plain(lens)
@@ -825,8 +833,11 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, l
         _sizes("kv_read", max_len)
     k, v = k_pages.new_empty((2, b, max_len, heads, d), dtype=dtype).unbind()
     if width == 0:
+        _empty_call("kv-read")
         return k.zero_(), v.zero_()
-    if b and max_len and heads and d:
+    if not (b and max_len and heads and d):
+        _empty_call("kv-read")
+    else:
         table, lens = _plain(table), _plain(lens)
         _check(load().sam_hip_kv_read(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
                                       _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _DTYPES[dtype], code, b, max_len,
@@ -875,9 +886,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if out.stride(2) != 1 or _overlaps_itself(out):
             raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
         so = _long2(out.stride(0), out.stride(1))
-    if tokens == 0:
-        return out
-    if b == 0:
+    if tokens == 0 or b == 0:
+        _empty_call("paged-attention")
         return out.zero_() if rest else out
     if width == 0:  # no keys: as one page that is not there
         table, width = torch.full((b, 1), -1, dtype=torch.int32, device=q.device), 1

@@ -1,6 +1,6 @@
 """The paged memory at the edges of what its header defines: weights far below a row's largest, sequences that
 outgrow their table or the new tokens, results in place of their queries,
-e4m3 rows of every scale."""
+e4m3 rows of every scale, empty calls while the library is off."""
 import math
 
 import pytest
@@ -104,8 +104,6 @@ def test_results_in_place_of_their_queries(hip, dtype, chunks, lens, d):
         assert torch.equal(rows[:, 1], want) and torch.equal(rows[:, ::2], packed[:, ::2])
 
 
-
-
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("rows", [1, 40])
@@ -128,3 +126,28 @@ def test_an_e4m3_row_is_read_as_kv_read_returns_it(hip, dtype, d, rows):
     got, want = got.view(b, rows, d), want.view(b, 1, d).expand(b, rows, d)
     bad = (got != want).any(-1).any(-1).nonzero().flatten().tolist()
     assert not bad, f"scale bytes {[x + 1 for x in bad]}"
+
+
+def test_calls_without_work_obey_the_switch(hip):
+    """No tokens, no sequences, no pages in the table, no columns to read: while the library is off each call raises, and
+    otherwise returns its empty or zero result."""
+    h = lambda *s: torch.ones(s, device="cuda", dtype=torch.float16)
+    pages, x, table = h(3, 2, 16, 64), h(4, 2, 64), ints([[0, 1]])
+    s, n, none = ints([0, 4]), ints([4]), (ints([]).view(0, 2), ints([0]), ints([]))
+    freqs, axes = hip.rope_freqs((8, 8))
+    calls = [lambda: hip.rope_axes(x[:0], ints([]).view(0, 2), freqs, axes), lambda: hip.kv_write(x[:0], x[:0], pages, pages, table, s, n),
+             lambda: hip.kv_write(x, x, pages, pages, *none), lambda: hip.kv_write(x, x, pages, pages, table[:, :0], s, n),
+             lambda: hip.kv_read(pages, pages, table, n, 0)[0], lambda: hip.kv_read(pages, pages, table[:, :0], n, 4)[0],
+             lambda: hip.kv_read(pages, pages, none[0], none[2], 4)[0], lambda: hip.paged_attention(x[:0], pages, pages, table, s, n),
+             lambda: hip.paged_attention(x, pages, pages, *none), lambda: hip.paged_attention(x, pages, pages, table[:, :0], s, n)]
+    shapes = [(0, 2, 64), None, None, None, (1, 0, 2, 64), (1, 4, 2, 64), (0, 4, 2, 64), (0, 2, 64), (4, 2, 64), (4, 2, 64)]
+    hip.set_enabled(False)
+    try:
+        for call in calls:
+            with pytest.raises(hip.SamHipDisabled, match="switched off"):
+                call()
+    finally:
+        hip.set_enabled(True)
+    for call, shape in zip(calls, shapes):
+        got = call()
+        assert got is None if shape is None else got.shape == shape and not got.any()
