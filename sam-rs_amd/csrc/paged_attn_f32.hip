@@ -9,9 +9,12 @@
 // value row is A of four products with the output columns permuted, so K and V go from memory to the matrix units
 // without passing LDS, and P stays in the lane that made it.
 //
+// A weight is exp2((score - maximum) * scale): exact in the difference, so that scores of any size keep their order
+// (score * scale - maximum * scale, one instruction less, rounds the latter and overflows from 2^31 on; 387 us below at 128).
+//
 // What bounds it: the f32 matrix rate (64 flops a cycle and SIMD) where many rows share the keys, else the bytes of
 // K and V. 16 rows use each value loaded for 8 flops a byte, twice what L1 would need to keep up. 2048 rows over 4096 keys,
-// 8 heads: head dim 64 191 us (90 TFLOP/s), 128 387 (89; a large library product 153), 256 with 4 heads 515 (67); a step of 32
+// 8 heads: head dim 64 191 us (90 TFLOP/s), 128 396 (87; a large library product 153), 256 with 4 heads 520 (66); a step of 32
 // sequences of 4096 keys, 8 key heads of 128, 210 (5.1 TB/s).
 #include "lds_dma.hpp"
 #include "paged.hpp"
@@ -173,9 +176,9 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = max_nc(top, s[rb][i][e]);
-        const float mn = fmaxf(m[rb], max_over_rows16(top) * p.sc);
+        const float mn = fmaxf(m[rb], max_over_rows16(top));
         const float base = mn == -INFINITY ? 0.f : mn;
-        const float alpha = exp2_fast(m[rb] - base);
+        const float alpha = exp2_fast((m[rb] - base) * p.sc);
         m[rb] = mn;
         l[rb] *= alpha;
 #pragma unroll
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[rb][i][e] = exp2_fast(s[rb][i][e] * p.sc - base);
+            s[rb][i][e] = exp2_fast((s[rb][i][e] - base) * p.sc);
             l[rb] += s[rb][i][e];
           }
       }
@@ -263,7 +266,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
         for (int rb = 0; rb < RB; ++rb) {
           const float mo = sm_m[wave][16 * rb + n], mn = fmaxf(m[rb], mo);
           const float base = mn == -INFINITY ? 0.f : mn;
-          const float a = exp2_fast(m[rb] - base), c = exp2_fast(mo - base);
+          const float a = exp2_fast((m[rb] - base) * p.sc), c = exp2_fast((mo - base) * p.sc);
           l[rb] = l[rb] * a + sm_l[wave][16 * rb + n] * c;
           m[rb] = mn;
 #pragma unroll
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
         if (rt * TR + 16 * rb + n >= rows) continue;
         const long row = ((long)w.split * p.tokens + tok[rb]) * p.heads + head[rb];
         if (p.nsplit > 1 && g == 0)
-          *reinterpret_cast<float2*>(p.ml + 2 * row) = direct ? float2{0.f, -1.f} : float2{m[rb], l[rb]};
+          *reinterpret_cast<float2*>(p.ml + 2 * row) = direct ? float2{0.f, -1.f} : float2{m[rb] * p.sc, l[rb]};
         if (direct) {
           const float inv = l[rb] == 0.f ? 0.f : 1.f / l[rb];  // a row that sees no key is 0
           float* orow = reinterpret_cast<float*>(p.out) + tok[rb] * p.so[0] + head[rb] * p.so[1];

@@ -11,7 +11,8 @@
 // e4m3 codes become 16-bit values with their row's scale in one conversion, exactly (in f16, values below 2^-14 to
 // f16's subnormal step). Softmax statistics and sums are f32. f16 P is rounded to f16 and its sum taken over the rounded
 // values, all of it times 2^15, which O / l cancels: weights keep f16's 11 bits down to 2^-29 of the largest, so that
-// thousands of keys far below one that dominates are not lost (each is off by 2^-40 of it at most). bf16 P goes as
+// thousands of keys far below one that dominates are not lost (each is off by 2^-40 of it at most). The exponent is taken of
+// (score - maximum) * scale, so that scores of any size keep P in f16's range. bf16 P goes as
 // hi + lo, which leaves 2^-16 of it (one bf16 term would leave 2^-8, as much as the output's own rounding).
 //
 // The four waves of a workgroup join at its end, the key ranges of a sequence in paged_combine_kernel.
@@ -187,9 +188,9 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = max_nc(top, s[rb][i][e]);
-        const float m_new = fmaxf(m[rb], max_over_rows16(top) * p.sc - kLift);
+        const float m_new = fmaxf(m[rb], max_over_rows16(top));
         const float base = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = exp2_fast(m[rb] - base);
+        const float alpha = exp2_fast((m[rb] - base) * p.sc);
         m[rb] = m_new;
         l[rb] *= alpha;
 #pragma unroll
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
         float pv[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          pv[j] = exp2_fast(fmaf(s[rb][j >> 2][j & 3], p.sc, -base));
+          pv[j] = exp2_fast(fmaf(s[rb][j >> 2][j & 3] - base, p.sc, kLift));
         }
         if constexpr (kSplitP) {
 #pragma unroll
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
         for (int rb = 0; rb < RB; ++rb) {
           const float mo = sm_m[wave][16 * rb + n], mn = fmaxf(m[rb], mo);
           const float base = mn == -INFINITY ? 0.f : mn;
-          const float a = exp2_fast(m[rb] - base), c = exp2_fast(mo - base);
+          const float a = exp2_fast((m[rb] - base) * p.sc), c = exp2_fast((mo - base) * p.sc);
           l[rb] = l[rb] * a + sm_l[wave][16 * rb + n] * c;
           m[rb] = mn;
 #pragma unroll
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
             }
           }
         if (p.nsplit > 1 && g == 0)
-          *reinterpret_cast<float2*>(p.ml + 2 * part) = direct ? float2{0.f, -1.f} : float2{m[rb], l[rb]};
+          *reinterpret_cast<float2*>(p.ml + 2 * part) = direct ? float2{0.f, -1.f} : float2{m[rb] * p.sc, l[rb]};
       }
     }
     __syncthreads();

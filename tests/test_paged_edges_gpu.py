@@ -1,6 +1,6 @@
-"""The paged memory at the edges of what its header defines: weights far below a row's largest, sequences that
-outgrow their table or the new tokens, results in place of their queries,
-e4m3 rows of every scale, empty calls while the library is off."""
+"""The paged memory at the edges of what its header defines: weights far below a row's largest, scores of any size,
+sequences that outgrow their table or the new tokens, results in place of their queries, e4m3 rows of every scale, empty
+calls while the library is off."""
 import math
 
 import pytest
@@ -56,6 +56,36 @@ def test_thousands_of_keys_far_below_a_dominant_one(hip, dtype, d, rows, gap, le
         rel = 2 * P_UNIT[dtype] + (length + 16) * ref.F32_U + 2 * 4 * gap * ref.F32_U
         bound = ref.with_rounding(rel * want, want, dt)
         assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 20, 50])
+@pytest.mark.parametrize("power, scale", [(19, 1.0), (21, 0.37), (24, 0.37), (28, 1.0), (30, 1.0), (30, 0.37)])
+def test_scores_of_any_size(hip, dtype, d, rows, power, scale):
+    """Scores of 0 and +- 2^power, exact in f32: the largest ones share all the weight evenly (the others are 2^18 nats lower
+    at least), wherever they lie and whether the maximum is reached from below, at once or is a negative one. The bound
+    is P's rounding, the sums' at one f32 rounding a key and the output's."""
+    dt, page, length = DT[dtype], 16, 3000
+    gen = torch.Generator(device="cuda").manual_seed(d + rows)
+    v = torch.randn(length, 1, d, generator=gen, device="cuda").to(dt)
+    q = torch.zeros(rows, 1, d, device="cuda", dtype=dt)
+    q[:, 0, 0] = 2.0 ** (power // 2)
+    pages = -(-length // page)
+    kp, vp = (torch.zeros(pages, 1, page, d, device="cuda", dtype=dt) for _ in range(2))
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).view(1, -1)
+    at = torch.arange(length, device="cuda")
+    pair = (at == 5) | (at == 2950)
+    for step in (torch.where(pair, 1, -1), torch.where(pair, -1, 1), torch.where(at < 300, -1, 0), torch.where(at < 300, 0, 1),
+                 torch.where(pair, 0, -1), torch.full_like(at, -1)):
+        k = torch.zeros(length, 1, d, device="cuda", dtype=dt)
+        k[:, 0, 0] = step * 2.0 ** (power - power // 2)
+        hip.kv_write(k, v, kp, vp, table, ints([0, length]), ints([length]))
+        got = hip.paged_attention(q, kp, vp, table, ints([0, rows]), ints([length]), scale=scale, causal=False).cpu().double()
+        top = v[step == step.max()].double()
+        want, spread = (x.mean(0).expand(rows, 1, d).cpu() for x in (top, top.abs()))
+        bound = ref.with_rounding((2 * P_UNIT[dtype] + (length + 16) * ref.F32_U) * spread, want, dt)
+        assert ((got - want).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
