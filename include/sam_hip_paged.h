@@ -21,10 +21,11 @@ extern "C" {
  * for (x0, x1) = (x[2i], x[2i+1]) or, with halves, (x[i], x[i + pairs]); columns past 2 * pairs are copied. inverse
  * turns by the negative angle (the gradient's way back). pos [b, l, naxes] int32 with strides (batch, token, axis), 0 to
  * share positions; freqs [pairs] f64, radians per unit of position; axes [pairs] int32 in [0, naxes) (another value
- * takes position 0); with pairs == 0 all three may be NULL. The angle is formed in f64, sine, cosine and the turn in f32. Strides of x and out: (batch, token,
- * head) elements, NULL = contiguous; the head dimension is contiguous. out's rows lie apart; out may be x with the
- * same strides and must not overlap x otherwise. Pointers are aligned to their elements; 16-byte aligned rows with pairs % 4 == 0 (halves:
- * pairs % 8 == 0) run on the vector kernel.
+ * takes position 0); with pairs == 0 all three may be NULL. The angle is formed in f64, sine, cosine and the turn in
+ * f32. Strides of x and out: (batch, token, head) elements, NULL = contiguous; the head dimension is contiguous. out's
+ * rows lie apart; out may be x with the same strides and must not overlap x otherwise. Pointers are aligned to their
+ * elements; 16-byte aligned rows with pairs % 4 == 0 (halves: pairs % 8 == 0) run on the vector kernel. Fewer than 2^31
+ * tokens and 2^31 - 256 elements of one, up to 65535 heads and 2^38 elements.
  */
 int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const int* axes, void* out, int dtype, int b,
                       int l, int h, int d, int pairs, int naxes, const long* strides_x, const long* strides_pos,
@@ -65,9 +66,10 @@ int sam_hip_kv_read(void* k, void* v, const void* k_pages, const void* v_pages, 
  * Attention of each sequence's new tokens over its pages, the new tokens' own keys (written before) among them:
  *   out[t, hq, :] = softmax_j(scale * q[t, hq, :] . k_j) . v_j over the keys j < lens[b] of key head hq / (heads / kv_heads)
  * and, with causal, j <= t's own position lens[b] - (starts[b+1] - t). q and out [tokens, heads, d] (strides (token,
- * head), multiples of 16 bytes, out's rows apart; NULL = contiguous). A row that sees no key is 0; a key, or a value that is not finite,
- * reaches the rows that see it alone. Rows of no sequence stay as they are, or become 0 with zero_rest. out
- * may be q with the same strides; it must not overlap q otherwise, nor the other tensors.
+ * head), multiples of 16 bytes, out's rows apart; NULL = contiguous). A row that sees no key is 0; a key, or a value that
+ * is not finite, reaches the rows that see it alone (an infinite value may come out as NaN there). Rows of no sequence
+ * stay as they are, or become 0 with zero_rest. out may be q with the same strides; it must not overlap q otherwise, nor
+ * the other tensors.
  * max_q and max_len are the longest chunk and the longest sequence as the caller expects them: they size the grid and
  * the key splits, and a call whose sequences exceed them is computed all the same, more slowly.
  * Workspace: sam_hip_paged_attention_workspace_size() bytes of device memory for the key splits' partial results (it

@@ -23,7 +23,8 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
   const long group = heads / kv_heads, rows = (long)std::max(std::min(max_q, tokens), 1) * group;
   // The many-row kernel past 32 rows a key head, which the other takes in two passes over the keys: 8 sequences of 8192, 8
   // heads of 128 in f16, 33 rows each 56 against 110 us, 32 rows 55 against 62; at 64 42 against 52 and 41 against 35; 4 of 4
-  // heads of 256, 54 against 69 and 53 against 42; one of 65536 with 2 heads of 128 35 against 29 and 33 against 28.
+  // heads of 256, 54 against 69 and 53 against 42; one of 65536 with 2 heads of 128 35 against 29 and 33 against 28 (the rule
+  // counts rows alone, so this one call loses).
   plan.many = dtype != kF32 && rows > 32;
   // 32 rows a tile above 16 where registers allow it: the first of these calls at 17 rows 61 us against 90 with two tiles of
   // 16, the third (which they do not) 42

@@ -26,11 +26,12 @@
 // 390 us at head dim 64 where this takes 371, 8192 rows and keys of 16 heads in f16, and 310 against 303 at 128 with 8).
 //
 // What bounds it: products, softmax and LDS reads beside each other on too few waves (a loop of the products alone, fed
-// from LDS, reaches 1.11 PFLOP/s at head dim 128). The vector units' and the matrix units' busy cycles add up to the whole
-// time, also where more of them run beside each other: fewer instructions count, not a closer order. 8192 rows over 8192
-// keys, f16: head dim 64 367 us (16 heads, 0.75 PFLOP/s), 96 255 (8 heads, 0.81), 128 301 (8 heads, 0.91), 256 329 (4 heads,
-// 0.83); bf16 at 64 535 (0.51), at 128 377 (0.73), with 1.5 times the products; e4m3 at 128 321 (0.86), at 256 372 (0.74), where
-// 8 codes a load instead of 16 took 377 and 417. On a card a tenth slower kAhead 2 took 319, 279 and 370 us at 128, 96 and
+// from LDS, reaches 1.11 PFLOP/s at head dim 128). Vector and matrix units are busy 60% and 33% of the cycles at head dim 64,
+// 43% and 40% at 128, together nearly the whole time, also where more of them run beside each other: fewer instructions
+// count, not a closer order. At 256, with one wave a SIMD, they are 33% and 32%, and the rest is waiting. 8192 rows over
+// 8192 keys, f16: head dim 64 374 us (16 heads, 0.73 PFLOP/s), 96 259 (8 heads, 0.80), 128 309 (8 heads, 0.89), 256 337 (4
+// heads, 0.82); bf16 at 64 542 (0.51), at 128 383 (0.72), with 1.5 times the products; e4m3 at 128 321 (0.86), at 256 374 (0.74),
+// where 8 codes a load instead of 16 took 377 and 417. On a card a tenth slower kAhead 2 took 319, 279 and 370 us at 128, 96 and
 // 256, and 4 317, 271 and 345.
 #include <type_traits>
 
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
   typedef typename Vec<T>::x8 X8;
   constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
   constexpr float kLift = kSplitP ? 0.f : 15.f - kSlack;  // P is lifted by 2^kLift
-  // LDS fragments in flight ahead of their products: bf16 at head dim 64 has registers for two (8192 rows
+  // LDS fragments in flight ahead of their products: bf16 at head dim 64 has fewer registers for them (8192 rows
   // and keys, 16 heads: 561 us against 568 with four, from e4m3 577 against 608)
   constexpr int kAhead = DP <= 64 && kSplitP ? 2 : 4;
   typedef __attribute__((address_space(3))) X8 lds_x8;
