@@ -89,6 +89,60 @@ def test_scores_of_any_size(hip, dtype, d, rows, power, scale):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 50])
+def test_scores_of_any_size_from_e4m3_pages(hip, dtype, d, rows):
+    """As above from 8 bits (scores of 2^30 are powers of two there too), the values as they are read back."""
+    dt, page, length = DT[dtype], 16, 3000
+    gen = torch.Generator(device="cuda").manual_seed(d + rows)
+    v = torch.randn(length, 1, d, generator=gen, device="cuda").to(dt)
+    q = torch.zeros(rows, 1, d, device="cuda", dtype=dt)
+    q[:, 0, 0] = 2.0 ** 15
+    pages = -(-length // page)
+    kp, vp = (torch.zeros(pages, 1, page, d, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+    ks, vs = (torch.full((pages, 1, page), 127, device="cuda", dtype=torch.uint8) for _ in range(2))
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).view(1, -1)
+    at = torch.arange(length, device="cuda")
+    pair = (at == 5) | (at == 2950)
+    for step in (torch.where(pair, 1, -1), torch.where(pair, -1, 1), torch.where(at < 300, -1, 0)):
+        k = torch.zeros(length, 1, d, device="cuda", dtype=dt)
+        k[:, 0, 0] = step * 2.0 ** 15
+        hip.kv_write(k, v, kp, vp, table, ints([0, length]), ints([length]), ks, vs)
+        held = hip.kv_read(kp, vp, table, ints([length]), length, ks, vs, dtype=dt)[1][0]
+        got = hip.paged_attention(q, kp, vp, table, ints([0, rows]), ints([length]), ks, vs, scale=1.0, causal=False).cpu().double()
+        top = held[step == step.max()].double()
+        want, spread = (x.mean(0).expand(rows, 1, d).cpu() for x in (top, top.abs()))
+        bound = ref.with_rounding((2 * P_UNIT[dtype] + (length + 16) * ref.F32_U) * spread, want, dt)
+        assert ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("chunk", [1, 20, 150])
+def test_scores_of_any_size_keep_masks_and_values_apart(hip, dtype, d, chunk):
+    """Scores that grow by 2^22 a key: a causal row is its own key's value, and a NaN at one position reaches the rows from
+    there on, in its column alone."""
+    dt, page, length, col, bad = DT[dtype], 16, 190, 3, 187
+    gen = torch.Generator(device="cuda").manual_seed(d + chunk)
+    v = torch.randn(length, 1, d, generator=gen, device="cuda").to(dt)
+    v[bad, 0, col] = float("nan")
+    k = torch.zeros(length, 1, d, device="cuda", dtype=dt)
+    k[:, 0, 0] = torch.arange(length, device="cuda") * 2.0 ** 8
+    q = torch.zeros(chunk, 1, d, device="cuda", dtype=dt)
+    q[:, 0, 0] = 2.0 ** 14
+    kp, vp = (torch.full((12, 1, page, d), float("nan"), device="cuda", dtype=dt) for _ in range(2))
+    table = torch.arange(12, device="cuda", dtype=torch.int32).view(1, -1)
+    hip.kv_write(k, v, kp, vp, table, ints([0, length]), ints([length]))
+    got = hip.paged_attention(q, kp, vp, table, ints([0, chunk]), ints([length]), scale=1.0).cpu().double()
+    at = torch.arange(length - chunk, length)
+    want = v[length - chunk:].cpu().double()
+    assert torch.equal(torch.isnan(got[:, 0, col]), at >= bad)
+    got[at >= bad, 0, col], want[at >= bad, 0, col] = 0, 0
+    bound = ref.with_rounding((2 * P_UNIT[dtype] + (length + 16) * ref.F32_U) * want.abs(), want, dt)
+    assert ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("heads", [1, 4, 40])
 def test_a_sequence_that_outgrows_its_table_or_its_tokens(hip, dtype, heads):
     """kv_write and paged_attention give a token one position: lens past what the table names, and starts past the
