@@ -35,6 +35,7 @@ SOURCES = [
     "rope.hip", "qkv_rope.hip",
     "rope_axes.hip", "kv_cache.hip", "paged_attn.hip", "paged_attn_f32.hip", "paged_attn_few.hip", "paged_attn_many.hip",
     "paged_combine.hip",
+    "mx_pack.hip", "mx_matmul.hip",
     "sam_hip_abi.cpp",
 ]
 

@@ -1,0 +1,292 @@
+// Products of microscaled 4-bit matrices on gfx950: out[m, n] = act(sum_k A[m, k] B[n, k] + bias[n]), A and B in blocks of 32
+// e2m1 codes under a power of two along k (mx.hpp), sums in f32, out in f32, f16 or bf16, act nothing or the exact GELU.
+//
+// The matrix units multiply such blocks as they are: v_mfma_scale_f32_32x32x64 takes a lane's 16 bytes (a block of a row)
+// and its scale byte. Products of two codes and two scales are exact, so the f32 sums are the only roundings before the
+// output's. B is the first operand, so that a lane ends with four consecutive columns of one row of out.
+#include <algorithm>
+
+#include "gelu.hpp"
+#include "lds_dma.hpp"
+#include "mx.hpp"
+
+namespace samhip {
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ i32x8 codes8(u32x4 w) { return i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0}; }
+
+// D(32x32) += A(32x64) B(64x32) of 4-bit codes. Lane l supplies row l % 32 of A and of B^T, block l / 32, and the scales in
+// byte SEL of sa and sb; it receives D[8 * (i / 4) + 4 * (l / 32) + i % 4][l % 32] in element i.
+template <int SEL> __device__ __forceinline__ f32x16 mma_mx32(u32x4 a, unsigned sa, u32x4 b, unsigned sb, f32x16 c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes8(a), codes8(b), c, 4, 4, SEL, (int)sa, SEL, (int)sb);
+}
+// D(16x16) += A(16x128) B(128x16): row l % 16, block l / 16, D[4 * (l / 16) + i][l % 16].
+__device__ __forceinline__ f32x4 mma_mx16(u32x4 a, unsigned sa, u32x4 b, unsigned sb, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes8(a), codes8(b), c, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+// Stores columns n .. n + 3 of row m.
+template <typename T> __device__ __forceinline__ void put4(const MxProduct& p, int m, int n, f32x4 x, bool whole) {
+  if (m >= p.m || n >= p.n) return;
+  const T* bias = reinterpret_cast<const T*>(p.bias);
+  T* to = reinterpret_cast<T*>(p.out) + (long)m * p.n + n;
+  if (whole) {  // n % 4 == 0: whole vectors, aligned
+    if (bias) {
+      const typename Vec<T>::x4 b = *reinterpret_cast<const typename Vec<T>::x4*>(bias + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] += to_f32(b[i]);
+    }
+    typename Vec<T>::x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(f32_result(p.gelu ? gelu_erf(x[i]) : x[i]));
+    *reinterpret_cast<typename Vec<T>::x4*>(to) = y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i >= p.n) break;
+      const float v = x[i] + (bias ? to_f32(bias[n + i]) : 0.f);
+      to[i] = from_f32<T>(f32_result(p.gelu ? gelu_erf(v) : v));
+    }
+  }
+}
+
+// Many rows. A workgroup of four waves takes TM x TN of out, a wave a quarter of it, in steps of 128 along k: rows of 64 bytes
+// of both matrices go straight to LDS (buffer loads, of which those past a matrix's or row's end bring zeros), NB steps'
+// worth, and come to the matrix units one 16-byte block a lane. 16-byte chunk c of row r lies at c ^ (r / 4 % 4), so that the
+// 16 rows of which a read takes a chunk each fall on all 64 banks alike. Scales travel beside them: a dword with a row's
+// four where those are aligned to it (k % 128 == 0), else a byte a load.
+template <typename T, int TM, int TN, int NB, bool ALIGNED, bool GELU>
+__global__ __launch_bounds__(256) void mx_product_kernel(MxProduct p, int mt, int nt) {
+  constexpr int ROWS = TM + TN, CB = ROWS * 64, SB = ROWS * (ALIGNED ? 4 : 16), BUF = CB + SB;
+  constexpr int FM = TM / 64, FN = TN / 64, NC = ROWS / 64, NS = (ROWS + 255) / 256 * (ALIGNED ? 1 : 4), VM = NC + NS;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const unsigned lds0 = lds_addr(smem);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroup i runs on XCD i % 8: neighbours in out, which share rows, on the same one
+  const int tiles = mt * nt, share = (tiles + 7) / 8, lin = (int)(blockIdx.x % 8) * share + (int)(blockIdx.x / 8);
+  if (lin >= tiles) return;
+  const int m0 = lin / nt * TM, n0 = lin % nt * TN;
+  const int G = p.k / 32, steps = (p.k + 127) / 128;
+  const unsigned rb = (unsigned)p.k / 2;  // bytes of a row's codes
+  const int mr = min(TM, p.m - m0), nr = min(TN, p.n - n0);
+  // rows 0 .. TN - 1 of a step are B's, the others A's
+  const i32x4 rsb = buffer_rsrc(p.b + (long)n0 * rb, nr * rb), rsa = buffer_rsrc(p.a + (long)m0 * rb, mr * rb);
+  const i32x4 rssb = buffer_rsrc(p.sb + (long)n0 * G, nr * G), rssa = buffer_rsrc(p.sa + (long)m0 * G, mr * G);
+  const int chunk = (lane & 3) ^ (lane >> 4);  // of this lane's row
+  auto stage = [&](int t, int buf) {
+    const unsigned to = lds0 + buf * BUF;
+    const unsigned none = ALIGNED || 4 * t + chunk < G ? 0u : 0x80000000u;  // past the row's end: out of the buffer's range
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r0 = 16 * (wave + 4 * i);
+      const bool of_b = r0 < TN;
+      const unsigned off = (unsigned)((of_b ? r0 : r0 - TN) + lane / 4) * rb + 64 * t + 16 * chunk;
+      bdma16(of_b ? rsb : rsa, off | none, to + r0 * 64);
+    }
+#pragma unroll
+    for (int i = 0; i < NS / (ALIGNED ? 1 : 4); ++i) {
+      const int r0 = (64 * (wave + 4 * i)) % ROWS;  // waves past the last row bring the first ones again
+      const bool of_b = r0 < TN;
+      const unsigned off = (unsigned)((of_b ? r0 : r0 - TN) + lane) * (unsigned)G + 4 * t;
+      if constexpr (ALIGNED) {
+        bdma4(of_b ? rssb : rssa, off, to + CB + r0 * 4);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          bdma1(of_b ? rssb : rssa, (off + c) | (4 * t + c < G ? 0u : 0x80000000u), to + CB + (c * ROWS + r0) * 4);
+      }
+    }
+  };
+  const int wm = wave & 1, wn = wave >> 1, r = lane & 31, hh = lane >> 5;
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+  typedef __attribute__((address_space(3))) unsigned lds_u32;
+  const int brow = wn * (TN / 2) + r, arow = TN + wm * (TM / 2) + r;
+  const unsigned swz = 16 * (hh ^ (r >> 2 & 3));
+  f32x16 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x16{};
+#pragma unroll
+  for (int t = 0; t < NB - 1; ++t) stage(min(t, steps - 1), t);
+  for (int t = 0, buf = 0; t < steps; ++t) {
+    wait_vm<VM * (NB - 2)>();  // this step's loads, NB - 2 later ones in flight
+    __syncthreads();
+    // after the last step its loads again, into a buffer that nothing reads: the count above stays what it is
+    stage(min(t + NB - 1, steps - 1), buf == 0 ? NB - 1 : buf - 1);
+    const unsigned at = lds0 + buf * BUF;
+    unsigned sb[FN][2], sa[FM][2];
+    auto scales_of = [&](int row, unsigned* s) {
+      if constexpr (ALIGNED) {
+        s[0] = *(const lds_u32*)(size_t)(at + CB + 4 * row) >> (8 * hh);  // bytes 0 and 2: the blocks of the two halves
+      } else {
+        s[0] = *(const lds_u32*)(size_t)(at + CB + 4 * (hh * ROWS + row));
+        s[1] = *(const lds_u32*)(size_t)(at + CB + 4 * ((2 + hh) * ROWS + row));
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < FN; ++j) scales_of(brow + 32 * j, sb[j]);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) scales_of(arow + 32 * i, sa[i]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 b[FN], a[FM];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) b[j] = *(const lds_u32x4*)(size_t)(at + 64 * (brow + 32 * j) + (swz ^ 32 * h));
+#pragma unroll
+      for (int i = 0; i < FM; ++i) a[i] = *(const lds_u32x4*)(size_t)(at + 64 * (arow + 32 * i) + (swz ^ 32 * h));
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          if constexpr (ALIGNED)
+            acc[i][j] = h ? mma_mx32<2>(b[j], sb[j][0], a[i], sa[i][0], acc[i][j]) : mma_mx32<0>(b[j], sb[j][0], a[i], sa[i][0], acc[i][j]);
+          else
+            acc[i][j] = mma_mx32<0>(b[j], sb[j][h], a[i], sa[i][h], acc[i][j]);
+        }
+    }
+    buf = buf + 1 == NB ? 0 : buf + 1;
+  }
+  wait_vm<0>();  // nothing may land in the LDS that the results pass through
+  __syncthreads();
+  // A wave's results go through LDS, 32 rows at a time, so that a row's columns leave together: in f32, 16-byte chunk c of
+  // row r at c ^ (r % CH), then V columns a lane with their bias and activation.
+  constexpr int COLS = TN / 2, CH = COLS / 4, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR;
+  const unsigned own = lds0 + wave * (32 * COLS * 4);
+  const int n = n0 + wn * COLS + V * (lane % LPR);
+  const T* bias = reinterpret_cast<const T*>(p.bias);
+  float add[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) add[v] = bias && n + v < p.n ? to_f32(bias[n + v]) : 0.f;
+  const bool whole = p.n % V == 0;
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *(lds_f32x4*)(size_t)(own + r * (COLS * 4) + 16 * ((8 * j + 2 * e + hh) ^ (r % CH))) =
+            f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+#pragma unroll
+    for (int k = 0; k < 32 / RPP; ++k) {
+      const int row = RPP * k + lane / LPR, m = m0 + wm * (TM / 2) + 32 * i + row;
+      T y[V];
+#pragma unroll
+      for (int c = 0; c < V / 4; ++c) {
+        const f32x4 x = *(const lds_f32x4*)(size_t)(own + row * (COLS * 4) + 16 * ((V / 4 * (lane % LPR) + c) ^ (row % CH)));
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float z = x[v] + add[4 * c + v];
+          y[4 * c + v] = from_f32<T>(f32_result(GELU ? gelu_erf(z) : z));
+        }
+      }
+      T* to = reinterpret_cast<T*>(p.out) + (long)m * p.n + n;
+      if (m < p.m && n < p.n) {
+        if (whole) {
+          *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(y);
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (n + v < p.n) to[v] = y[v];
+        }
+      }
+    }
+  }
+}
+
+// Few rows: B's bytes bound it, so they go from memory straight to the matrix units. A workgroup takes 16 columns of out and
+// RB blocks of 16 rows; its waves take steps of 128 along k in turn and join at the end, in order.
+template <typename T, int RB>
+__global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
+  constexpr int U = 4;  // steps in flight
+  __shared__ __attribute__((aligned(16))) f32x4 part[16][RB][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int r = lane & 15, g = lane >> 4, n0 = 16 * blockIdx.x, m0 = 16 * RB * blockIdx.y;
+  const int G = p.k / 32, steps = (G + 3) / 4;
+  const long rb = p.k / 2;
+  const unsigned char* br = p.b + min(n0 + r, p.n - 1) * rb;
+  const unsigned char* bs = p.sb + min(n0 + r, p.n - 1) * (long)G;
+  const unsigned char *ar[RB], *as[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    ar[i] = p.a + min(m0 + 16 * i + r, p.m - 1) * rb;
+    as[i] = p.sa + min(m0 + 16 * i + r, p.m - 1) * (long)G;
+  }
+  f32x4 acc[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) acc[i] = f32x4{};
+  for (int t0 = wave; t0 < steps; t0 += U * waves) {
+    u32x4 b[U], a[U][RB];
+    unsigned char sb[U], sa[U][RB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = min(4 * (t0 + u * waves) + g, G - 1);
+      b[u] = *reinterpret_cast<const u32x4*>(br + 16 * c);
+      sb[u] = bs[c];
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        a[u][i] = *reinterpret_cast<const u32x4*>(ar[i] + 16 * c);
+        sa[u][i] = as[i][c];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = 4 * (t0 + u * waves) + g < G;  // blocks past the row's end: zeros under 2^-127
+      const u32x4 bu = in ? b[u] : u32x4{};
+#pragma unroll
+      for (int i = 0; i < RB; ++i) acc[i] = mma_mx16(bu, in ? sb[u] : 0u, a[u][i], in ? sa[u][i] : 0u, acc[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RB; ++i) part[wave][i][lane] = acc[i];
+  __syncthreads();
+  for (int i = wave; i < RB; i += waves) {
+    f32x4 x = part[0][i][lane];
+    for (int w = 1; w < waves; ++w) x += part[w][i][lane];
+    put4<T>(p, m0 + 16 * i + r, n0 + 4 * g, x, p.n % 4 == 0);
+  }
+}
+
+template <typename T, int TM, int TN, int NB, bool ALIGNED, bool GELU> hipError_t launch_product(const MxProduct& p, hipStream_t stream) {
+  constexpr int lds = NB * (TM + TN) * (64 + (ALIGNED ? 4 : 16));
+  static_assert(lds >= 4 * 32 * (TN / 2) * 4, "the results' way out");
+  auto kern = mx_product_kernel<T, TM, TN, NB, ALIGNED, GELU>;
+  static std::atomic<unsigned long long> done;
+  if (const hipError_t e = lds_opt_in(done, (const void*)kern, lds); e != hipSuccess) return e;
+  const int mt = (p.m + TM - 1) / TM, nt = (p.n + TN - 1) / TN;
+  const long grid = ((long)mt * nt + 7) / 8 * 8;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, p, mt, nt);
+  return hipGetLastError();
+}
+template <typename T, int TM, int TN, int NB> hipError_t by_alignment(const MxProduct& p, hipStream_t stream) {
+  if (p.k % 128 == 0 && reinterpret_cast<uintptr_t>(p.sa) % 4 == 0 && reinterpret_cast<uintptr_t>(p.sb) % 4 == 0)
+    return p.gelu ? launch_product<T, TM, TN, NB, true, true>(p, stream) : launch_product<T, TM, TN, NB, true, false>(p, stream);
+  return p.gelu ? launch_product<T, TM, TN, NB, false, true>(p, stream) : launch_product<T, TM, TN, NB, false, false>(p, stream);
+}
+
+template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream) {
+  if (p.m <= 32) {
+    const int waves = (int)std::min(16, std::max(1, (p.k + 511) / 512));
+    const dim3 grid((unsigned)((p.n + 15) / 16), 1);
+    if (p.m <= 16)
+      hipLaunchKernelGGL((mx_few_kernel<T, 1>), grid, dim3(64 * waves), 0, stream, p);
+    else
+      hipLaunchKernelGGL((mx_few_kernel<T, 2>), grid, dim3(64 * waves), 0, stream, p);
+    return hipGetLastError();
+  }
+  const long wide = (long)((p.m + 127) / 128) * ((p.n + 127) / 128);
+  return wide >= 192 ? by_alignment<T, 128, 128, 4>(p, stream) : by_alignment<T, 64, 64, 4>(p, stream);
+}
+
+}  // namespace
+
+hipError_t mx_matmul(int dtype, const MxProduct& p, hipStream_t stream) {
+  if (p.m == 0 || p.n == 0) return hipSuccess;
+  return dtype == kF32 ? product<float>(p, stream) : dtype == kF16 ? product<f16>(p, stream) : product<bf16>(p, stream);
+}
+
+}  // namespace samhip

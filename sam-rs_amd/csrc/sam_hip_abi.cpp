@@ -11,6 +11,7 @@
 
 #include "../../include/sam_hip.h"
 #include "flash_attn.hpp"
+#include "mx.hpp"
 #include "paged.hpp"
 
 namespace samhip {
@@ -856,6 +857,60 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
   p.ml = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.part_bytes);
   return check_launch(samhip::paged_attention(dtype, cache_dtype, p, plan, reinterpret_cast<hipStream_t>(stream)),
                       "paged-attention");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------ 4-bit numbers
+
+namespace {
+
+int check_mx_rows(const char* what, int dtype, long rows, int k) {
+  if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
+  if (rows < 0 || k <= 0 || k % samhip::kMxBlock != 0)
+    return fail(SAM_HIP_EINVAL, "%s: rows of a positive multiple of 32 values, got %ld of %d", what, rows, k);
+  if (rows >= (1L << 36) / k) return fail(SAM_HIP_EUNSUPPORTED, "%s: 2^36 values or more (%ld rows of %d)", what, rows, k);
+  return SAM_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sam_hip_mx_pack(const void* x, unsigned char* codes, unsigned char* scales, int dtype, long rows, int k, void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("mx-pack");
+  if (!x || !codes || !scales) return fail(SAM_HIP_EINVAL, "mx-pack: null pointer argument");
+  if (int rc = check_mx_rows("mx-pack", dtype, rows, k); rc != SAM_HIP_OK) return rc;
+  if (!aligned16(x) || !aligned16(codes)) return fail(SAM_HIP_EUNSUPPORTED, "mx-pack: x and codes must be 16-byte aligned");
+  return check_launch(samhip::mx_pack(dtype, x, codes, scales, rows * (k / 32), reinterpret_cast<hipStream_t>(stream)), "mx-pack");
+}
+
+int sam_hip_mx_unpack(const unsigned char* codes, const unsigned char* scales, void* x, int dtype, long rows, int k,
+                      void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("mx-unpack");
+  if (!x || !codes || !scales) return fail(SAM_HIP_EINVAL, "mx-unpack: null pointer argument");
+  if (int rc = check_mx_rows("mx-unpack", dtype, rows, k); rc != SAM_HIP_OK) return rc;
+  if (!aligned16(x) || !aligned16(codes)) return fail(SAM_HIP_EUNSUPPORTED, "mx-unpack: x and codes must be 16-byte aligned");
+  return check_launch(samhip::mx_unpack(dtype, codes, scales, x, rows * (k / 32), reinterpret_cast<hipStream_t>(stream)),
+                      "mx-unpack");
+}
+
+int sam_hip_mx_matmul(const unsigned char* a, const unsigned char* a_scale, const unsigned char* b,
+                      const unsigned char* b_scale, const void* bias, void* out, int dtype, int m, int n, int k, int gelu,
+                      void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("mx-matmul");
+  if (!a || !a_scale || !b || !b_scale || !out) return fail(SAM_HIP_EINVAL, "mx-matmul: null pointer argument");
+  if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
+  if (m < 0 || n < 0 || k <= 0 || k % samhip::kMxBlock != 0)
+    return fail(SAM_HIP_EINVAL, "mx-matmul: sizes m=%d n=%d k=%d (k a positive multiple of 32)", m, n, k);
+  // the launches count workgroups of up to 1024 threads for 16 columns, or of 256 for 128 x 128 results, in 32 bits of threads
+  if ((long)m * n >= 1L << 36 || m > (1 << 30) || n > (1 << 25) || k > 1 << 22 ||
+      ((long)m + 127) / 128 * (((long)n + 127) / 128) >= 1L << 23)
+    return fail(SAM_HIP_EUNSUPPORTED, "mx-matmul: too many results, or k beyond 2^22 (m=%d n=%d k=%d)", m, n, k);
+  if (!aligned16(a) || !aligned16(b) || !aligned16(bias) || !aligned16(out))
+    return fail(SAM_HIP_EUNSUPPORTED, "mx-matmul: a, b, bias and out must be 16-byte aligned");
+  const samhip::MxProduct p = {a, a_scale, b, b_scale, bias, out, m, n, k, gelu != 0};
+  return check_launch(samhip::mx_matmul(dtype, p, reinterpret_cast<hipStream_t>(stream)), "mx-matmul");
 }
 
 }  // extern "C"

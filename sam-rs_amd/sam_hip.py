@@ -17,6 +17,9 @@ Names, argument meaning and errors follow the reference:
     kv_write(k, v, k_pages, v_pages, table, ...)         new keys and values into a paged cache (16 or 8 bits)
     kv_read(k_pages, v_pages, table, lens, max_len)      what its sequences hold, dense
     paged_attention(q, k_pages, v_pages, table, ...)     attention of new tokens over the pages
+    mx_pack(x), mx_unpack(codes, scale)  rows as 4-bit numbers in scaled blocks of 32, and back
+    mx_matmul(a, a_scale, b, b_scale)    products of such matrices
+    mx_linear(x, w, w_scale, bias=None)  a linear layer with 4-bit weights on rows that it packs
     set_enabled(on), enabled()                           cpu_gemm.rs:11, 25-32 (the process-wide switch)
 
 rope_axes to paged_attention are the paged form of the video memory (sam3/video.rs:133-145, 356-406); the reference
@@ -114,6 +117,12 @@ def load():
         L.sam_hip_paged_attention_workspace_size.restype = ctypes.c_long
         L.sam_hip_paged_attention.argtypes = [_vp] * 9 + [_i] * 10 + [_lp] * 2 + [_f] + [_i] * 4 + [_vp, ctypes.c_long, _vp]
         L.sam_hip_paged_attention.restype = _i
+        L.sam_hip_mx_pack.argtypes = [_vp] * 3 + [_i, ctypes.c_long, _i, _vp]
+        L.sam_hip_mx_pack.restype = _i
+        L.sam_hip_mx_unpack.argtypes = [_vp] * 3 + [_i, ctypes.c_long, _i, _vp]
+        L.sam_hip_mx_unpack.restype = _i
+        L.sam_hip_mx_matmul.argtypes = [_vp] * 6 + [_i] * 5 + [_vp]
+        L.sam_hip_mx_matmul.restype = _i
         L.sam_hip_set_enabled.argtypes = [_i]
         L.sam_hip_set_enabled.restype = None
         L.sam_hip_enabled.argtypes = []
@@ -907,3 +916,112 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                                           tokens, b, hq, pages, heads, page, d, width, sq, so, scale, bool(causal), rest,
                                           max_q, max_len, _ptr(ws), ws_bytes, _stream()))
     return out
+
+
+# ------------------------------------------------------------------------------------------ 4-bit numbers
+
+_E2M1 = torch.float4_e2m1fn_x2  # two codes a byte, the even column's in the low half
+_BLOCK = 32
+
+
+def _mx_k(what, shape) -> int:
+    """The length of rows that blocks of 32 divide."""
+    if not shape or shape[-1] == 0 or shape[-1] % _BLOCK:
+        raise SamHipError(f"{what}: rows must hold a positive multiple of {_BLOCK} values, got {tuple(shape)}")
+    if shape[-1] >> 31:
+        _sizes(what, shape[-1])
+    return shape[-1]
+
+
+def _mx_operand(what, name, codes, scale):
+    """A packed matrix as (codes, scale, shape of the values), contiguous and aligned, after its checks."""
+    if codes.dtype != _E2M1 or codes.dim() == 0:
+        raise SamHipError(f"{what}: {name} must hold torch.float4_e2m1fn_x2, [.., K / 2], got {codes.dtype} {tuple(codes.shape)}")
+    shape = codes.shape[:-1] + (2 * codes.shape[-1],)
+    _mx_k(what, shape)
+    if scale.dtype != torch.uint8 or scale.shape != shape[:-1] + (shape[-1] // _BLOCK,):
+        raise SamHipError(f"{what}: {name}'s scales must be uint8 {tuple(shape[:-1]) + (shape[-1] // _BLOCK,)}, got {scale.dtype} "
+                          f"{tuple(scale.shape)}")
+    codes, scale = _plain(codes), _plain(scale)
+    return (codes if codes.data_ptr() % 16 == 0 else codes.clone()), scale, shape
+
+
+def mx_pack(x: torch.Tensor):
+    """The rows of x [.., K] (K a multiple of 32; f32, f16, bf16) as 4-bit numbers: (codes torch.float4_e2m1fn_x2 [.., K / 2],
+    scale uint8 [.., K / 32]). Each block of 32 values has a power of two 2^s, s the least integer within +-126 with
+    max|x| <= 6 * 2^s (0 for zeros), held as s + 127; a code is x / 2^s rounded to the nearest of 0 0.5 1 1.5 2 3 4 6 (ties to
+    even). A block with a value that is not finite has 255 and is NaN throughout."""
+    dev = _device_of("mx_pack", x)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return mx_pack(x)
+    dt = _dtype(x)
+    shape = x.shape
+    k = _mx_k("mx_pack", shape)
+    x = _plain(x)
+    if x.data_ptr() % 16:
+        x = x.clone()
+    codes = x.new_empty(shape[:-1] + (k // 2,), dtype=_E2M1)
+    scale = x.new_empty(shape[:-1] + (k // _BLOCK,), dtype=torch.uint8)
+    if x.numel() == 0:
+        _empty_call("mx-pack")
+        return codes, scale
+    _check(load().sam_hip_mx_pack(x.data_ptr(), codes.data_ptr(), scale.data_ptr(), dt, x.numel() // k, k, _stream()))
+    return codes, scale
+
+
+def mx_unpack(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values [.., K] that codes and scale (mx_pack) stand for, each rounded to dtype once."""
+    dev = _device_of("mx_unpack", codes, scale)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return mx_unpack(codes, scale, dtype)
+    if dtype not in _DTYPES:
+        raise SamHipError(f"unsupported dtype {dtype} for a sam-rs HIP kernel")
+    codes, scale, shape = _mx_operand("mx_unpack", "codes", codes, scale)
+    x = codes.new_empty(shape, dtype=dtype)
+    if x.numel() == 0:
+        _empty_call("mx-unpack")
+        return x
+    _check(load().sam_hip_mx_unpack(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), _DTYPES[dtype], x.numel() // shape[-1],
+                                    shape[-1], _stream()))
+    return x
+
+
+def mx_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, bias: torch.Tensor | None = None,
+              gelu: bool = False, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """act(A B^T + bias) over the values that packed A [.., K] and B [N, K] (mx_pack) stand for -> [.., N] of dtype, which is
+    bias's [N] too. The products of codes and scales are exact, the sums f32; act is the identity or the exact GELU."""
+    dev = _device_of("mx_matmul", a, a_scale, b, b_scale, bias)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return mx_matmul(a, a_scale, b, b_scale, bias, gelu, dtype)
+    if dtype not in _DTYPES:
+        raise SamHipError(f"unsupported dtype {dtype} for a sam-rs HIP kernel")
+    a, a_scale, shape = _mx_operand("mx_matmul", "A", a, a_scale)
+    b, b_scale, of = _mx_operand("mx_matmul", "B", b, b_scale)
+    if len(of) != 2 or of[1] != shape[-1]:
+        raise SamHipError(f"mx_matmul: B must be [N, {shape[-1]}], got {tuple(of)}")
+    n, k = of
+    if bias is not None:
+        if bias.dtype != dtype or bias.shape != (n,):
+            raise SamHipError(f"mx_matmul: bias must be {dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
+        bias, = _aligned16(_plain(bias))
+    out = a.new_empty(shape[:-1] + (n,), dtype=dtype)
+    if out.numel() == 0:
+        _empty_call("mx-matmul")
+        return out
+    m = out.numel() // n
+    if (m | n) >> 31:
+        _sizes("mx_matmul", m, n)
+    _check(load().sam_hip_mx_matmul(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), _ptr(bias),
+                                    out.data_ptr(), _DTYPES[dtype], m, n, k, bool(gelu), _stream()))
+    return out
+
+
+def mx_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+              gelu: bool = False) -> torch.Tensor:
+    """A linear layer with 4-bit weights w, w_scale (mx_pack of [N, K]) on x [.., K], which it packs likewise:
+    act(x w^T + bias) -> [.., N] in x's dtype, bias's too; act is the identity or, with gelu, the exact GELU."""
+    codes, scale = mx_pack(x)
+    return mx_matmul(codes, scale, w, w_scale, bias, gelu, x.dtype)
