@@ -12,7 +12,7 @@ extern "C" {
 /*
  * The paged memory: rotary positions over several axes, a cache of keys and values in pages, and the attention of new
  * tokens over it. The reference gathers its video memory into one tensor and rotates every key again on each frame
- * (sam3/video.rs:133-145, 356-406); here a frame's keys are rotated and stored once, in 16 or 8 bits, and sequences
+ * (sam3/video.rs:133-145, 356-406); here a frame's keys are rotated and stored once, in 16, 8 or 4 bits, and sequences
  * (tracked objects, say) of different lengths are read through their page tables. No entry point of the reference's
  * corresponds to these five.
  *
@@ -33,17 +33,19 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
 
 /*
  * The cache. k_pages and v_pages are pools [pages, kv_heads, page_size, d], contiguous and 16-byte aligned, of the call's
- * dtype or of e4m3 (cache_dtype SAM_HIP_E4M3) with scales k_scale, v_scale [pages, kv_heads, page_size] of one byte. Key
+ * dtype, or of e4m3 (cache_dtype SAM_HIP_E4M3) with scales k_scale, v_scale [pages, kv_heads, page_size] of one byte. Key
  * j of sequence b lies in page table[b][j / page_size], slot j % page_size; table [batch, table_width], lens [batch]
  * (tokens that a sequence holds) and starts [batch + 1] (where its new tokens begin among `tokens` of them, ascending)
  * are int32 in device memory. In 8 bits a row of d values has the scale 2^s, s the least integer (within +-126) with
  * max|x| <= 448 * 2^s over its finite values (0 for a row of zeros), held as s + 127; its codes are x / 2^s rounded to
- * the nearest e4m3, values that are not finite NaN.
+ * the nearest e4m3, values that are not finite NaN. In 4 bits (SAM_HIP_E2M1; d % 32 == 0) the pools are
+ * [pages, kv_heads, page_size, d / 2] bytes, the scales [pages, kv_heads, page_size, d / 32], a row as sam_hip_mx_pack holds it
+ * (sam_hip_mx.h): each block of 32 values with its own scale, NaN throughout if one of them is not finite.
  *
  * sam_hip_kv_write stores the new tokens' rows k, v [tokens, kv_heads, d] (strides (token, head), multiples of 16
  * bytes; NULL = contiguous): token t of sequence b goes to position lens[b] - (starts[b+1] - t), the sequence's last
  * ones. sam_hip_kv_read writes rows 0 .. max_len of every sequence to k, v [batch, max_len, kv_heads, d] of `dtype`, zeros
- * from lens[b] on (from an e4m3 cache in any dtype, each value rounded to it once).
+ * from lens[b] on (from an e4m3 or e2m1 cache in any dtype, each value rounded to it once).
  *
  * What the tables say is checked on the device. A sequence holds its keys below both lens[b] and table_width * page_size;
  * its new tokens are those of 0 .. tokens - 1 that starts names, at the positions that lens[b] and starts[b+1] as they are
@@ -53,6 +55,7 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
  * a pool and 2^27 in a write or a read.
  */
 #define SAM_HIP_E4M3 3
+#define SAM_HIP_E2M1 4
 int sam_hip_kv_write(const void* k, const void* v, void* k_pages, void* v_pages, unsigned char* k_scale,
                      unsigned char* v_scale, const int* table, const int* starts, const int* lens, int dtype,
                      int cache_dtype, int tokens, int batch, int pages, int kv_heads, int page_size, int d,
@@ -74,7 +77,7 @@ int sam_hip_kv_read(void* k, void* v, const void* k_pages, const void* v_pages, 
  * the key splits, and a call whose sequences exceed them is computed all the same, more slowly.
  * Workspace: sam_hip_paged_attention_workspace_size() bytes of device memory for the key splits' partial results (it
  * depends on the current device's CU count; 0 needs none, -1 is an error); calls that may overlap need their own, and
- * so does each captured graph that may run beside another. Softmax statistics and sums are f32. An e4m3 row is read as
+ * so does each captured graph that may run beside another. Softmax statistics and sums are f32. An e4m3 or e2m1 row is read as
  * sam_hip_kv_read would return it in q's dtype. Limits as above; heads % kv_heads == 0; scale >= 0.
  */
 long sam_hip_paged_attention_workspace_size(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads,

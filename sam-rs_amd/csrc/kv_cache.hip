@@ -4,6 +4,7 @@
 // largest value 448) holds each row of d values of a head with one scale 2^s:
 //   s = the least integer with max|x| <= 448 * 2^s (over the finite values; 0 for a row of zeros; within +-126)
 //   code = x / 2^s rounded to the nearest e4m3, ties to even;  value = code * 2^s.
+// An e2m1 cache (4 bits) holds each block of 32 of a row's values with a scale of its own, as mx.hpp describes.
 // A power of two makes the division and the product exact, so the rounding to e4m3 is the only one (at most 2^-4
 // of a value, or 2^-10 of 2^s below 2^-6 * 2^s), and it costs e4m3 nothing: its own exponent takes up the factor of
 // up to two by which the largest code may stay below 448. Values that are not finite become e4m3's NaN.
@@ -13,8 +14,7 @@
 // that the page lookup, a chain of dependent loads, is paid once. 65536 tokens of 8 heads of 128, bf16: written as e4m3
 // in 81 us, 5.0 TB/s (113 with 64-bit divisions, values widened one by one and non-finite ones looked for in each), read
 // back in 80, and moved as they are in 100 each way, 5.3 TB/s; a copy reaches 4.8 to 5.1. A few tokens are latency: 3.3 us.
-#include <type_traits>
-
+#include "mx.hpp"
 #include "paged.hpp"
 
 namespace samhip {
@@ -39,32 +39,6 @@ struct KvReadParams {
   unsigned hmagic, hshift, lmagic, lshift;  // divisions by heads and max_len
 };
 
-template <typename T> struct Eight {
-  u32x4 w[sizeof(T) / 2];
-};
-template <typename T> __device__ __forceinline__ Eight<T> load_eight(const T* p) {
-  Eight<T> r;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = reinterpret_cast<const u32x4*>(p)[i];
-  return r;
-}
-template <typename T> __device__ __forceinline__ void store_eight(T* p, const Eight<T>& r) {
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<u32x4*>(p)[i] = r.w[i];
-}
-
-// Largest of v over a row's LPR lanes, in each 16-bit half (T of 16 bits) or as one number. Every lane calls it.
-template <typename T> __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
-  if constexpr (sizeof(T) == 2) {
-    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
-  } else {
-    return max(a, b);
-  }
-}
-template <int CTRL> __device__ __forceinline__ unsigned moved(unsigned v) {
-  return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, true);
-}
 template <typename T, int LPR> __device__ __forceinline__ unsigned row_max(unsigned v) {
   v = larger<T>(v, moved<0xb1>(v));   // quad_perm 1 0 3 2
   v = larger<T>(v, moved<0x4e>(v));   // quad_perm 2 3 0 1
@@ -74,20 +48,10 @@ template <typename T, int LPR> __device__ __forceinline__ unsigned row_max(unsig
   return v;
 }
 
-// Largest magnitude of a lane's 8 values, as T's bits (16-bit T: in the low half).
-template <typename T> __device__ __forceinline__ unsigned magnitude(const Eight<T>& x) {
-  constexpr unsigned sign = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
-  unsigned top = 0;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = larger<T>(top, x.w[i][j] & sign);
-  return sizeof(T) == 2 ? max(top >> 16, top & 0xffffu) : top;
-}
-// The same over the values that are finite.
+// The largest magnitude of a lane's 8 values, as T's bits, over those that are finite.
 template <typename T> __device__ __forceinline__ unsigned finite_magnitude(const Eight<T>& x) {
   typedef typename std::conditional<sizeof(T) == 2, unsigned short, unsigned>::type U;
-  constexpr unsigned inf = __is_same(T, f16) ? 0x7c00u : __is_same(T, bf16) ? 0x7f80u : 0x7f800000u;
+  constexpr unsigned inf = kInfBits<T>;
   const U* e = reinterpret_cast<const U*>(&x);
   unsigned top = 0;
 #pragma unroll
@@ -100,11 +64,7 @@ template <typename T> __device__ __forceinline__ unsigned finite_magnitude(const
 
 // The least s with top <= 448 * 2^s = 1.75 * 2^(8 + s), top = 1.f * 2^e in T's bits.
 template <typename T> __device__ __forceinline__ int scale_of(unsigned top) {
-  unsigned b;
-  if constexpr (__is_same(T, f16))
-    b = __float_as_uint((float)__builtin_bit_cast(f16, (unsigned short)top));
-  else
-    b = sizeof(T) == 2 ? top << 16 : top;
+  const unsigned b = f32_bits<T>(top);
   return b ? max((int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0), -126) : 0;
 }
 
@@ -144,7 +104,7 @@ template <typename T> __device__ __forceinline__ u32x2 codes_of(const Eight<T>& 
 // finite in some row of the wave.
 template <typename T, int LPR>
 __device__ __forceinline__ void quantise(const Eight<T>& k, const Eight<T>& v, u32x2& kc, u32x2& vc, int& ks, int& vs) {
-  constexpr unsigned inf = __is_same(T, f16) ? 0x7c00u : __is_same(T, bf16) ? 0x7f80u : 0x7f800000u;
+  constexpr unsigned inf = kInfBits<T>;
   unsigned kt, vt;
   auto over_rows = [&](unsigned a, unsigned b) {
     if constexpr (sizeof(T) == 2) {
@@ -182,7 +142,7 @@ template <int LPR> __device__ __forceinline__ int sequence_of(const PagedKv& c, 
   return n;
 }
 
-template <typename T, bool FP8, int LPR>
+template <typename T, typename C, int LPR>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteParams p) {
   const int r = (int)((blockIdx.x * 256u + threadIdx.x) / LPR);
   const int col = (int)(threadIdx.x % LPR) * 8;
@@ -199,7 +159,18 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteParams p) {
     const long j = (long)p.c.lens[b] - p.c.starts[b + 1] + t;  // its position: the last tokens of the sequence
     if (j >= 0 && j < (long)p.c.width * p.c.page) row = paged_row(p.c, b, head, (int)j, p.c.width * p.c.page);
   }
-  if constexpr (FP8) {
+  if constexpr (__is_same(C, e2m1)) {
+    unsigned ks, vs;
+    const unsigned kc = mx_quantise(k, ks), vc = mx_quantise(v, vs);
+    if (row < 0 || !inside) return;
+    const long at = row * p.c.d + col;
+    reinterpret_cast<unsigned*>(p.c.k)[at / 8] = kc;
+    reinterpret_cast<unsigned*>(p.c.v)[at / 8] = vc;
+    if (col % kMxBlock == 0) {
+      p.c.ks[at / kMxBlock] = (unsigned char)ks;
+      p.c.vs[at / kMxBlock] = (unsigned char)vs;
+    }
+  } else if constexpr (__is_same(C, e4m3)) {
     u32x2 kc, vc;
     int ks, vs;
     quantise<T, LPR>(k, v, kc, vc, ks, vs);
@@ -234,7 +205,7 @@ template <typename T> __device__ __forceinline__ Eight<T> dequantise(u32x2 c, fl
   return r;
 }
 
-template <typename T, bool FP8, int LPR>
+template <typename T, typename C, int LPR>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvReadParams p) {
   const int r = (int)((blockIdx.x * 256u + threadIdx.x) / LPR);
   const int col = (int)(threadIdx.x % LPR) * 8;
@@ -244,7 +215,13 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadParams p) {
   const long row = paged_row(p.c, b, head, j, paged_len(p.c, b));
   Eight<T> k = {}, v = {};
   if (row >= 0) {
-    if constexpr (FP8) {
+    if constexpr (__is_same(C, e2m1)) {
+      const long at = row * p.c.d + col;
+      const unsigned kc = reinterpret_cast<const unsigned*>(p.c.k)[at / 8], vc = reinterpret_cast<const unsigned*>(p.c.v)[at / 8];
+      const unsigned char ks = p.c.ks[at / kMxBlock], vs = p.c.vs[at / kMxBlock];
+      k = mx_dequantise<T>(kc, mx_scale(ks));
+      v = mx_dequantise<T>(vc, mx_scale(vs));
+    } else if constexpr (__is_same(C, e4m3)) {
       const u32x2 kc = *reinterpret_cast<const u32x2*>(reinterpret_cast<const unsigned char*>(p.c.k) + row * p.c.d + col);
       const u32x2 vc = *reinterpret_cast<const u32x2*>(reinterpret_cast<const unsigned char*>(p.c.v) + row * p.c.d + col);
       const float ks = pow2_of(p.c.ks[row]), vs = pow2_of(p.c.vs[row]);
@@ -259,27 +236,27 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadParams p) {
   store_eight(reinterpret_cast<T*>(p.v) + (long)r * p.c.d + col, v);
 }
 
-template <typename T, bool FP8> hipError_t write_launch(const KvWriteParams& p, hipStream_t stream) {
+template <typename T, typename C> hipError_t write_launch(const KvWriteParams& p, hipStream_t stream) {
   const int lpr = p.c.d <= 64 ? 8 : p.c.d <= 128 ? 16 : 32;
   const dim3 grid((unsigned)(((long)p.rows * lpr + 255) / 256));
   if (lpr == 8)
-    hipLaunchKernelGGL((kv_write_kernel<T, FP8, 8>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((kv_write_kernel<T, C, 8>), grid, dim3(256), 0, stream, p);
   else if (lpr == 16)
-    hipLaunchKernelGGL((kv_write_kernel<T, FP8, 16>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((kv_write_kernel<T, C, 16>), grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((kv_write_kernel<T, FP8, 32>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((kv_write_kernel<T, C, 32>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
-template <typename T, bool FP8> hipError_t read_launch(const KvReadParams& p, hipStream_t stream) {
+template <typename T, typename C> hipError_t read_launch(const KvReadParams& p, hipStream_t stream) {
   const int lpr = p.c.d <= 64 ? 8 : p.c.d <= 128 ? 16 : 32;
   const dim3 grid((unsigned)(((long)p.rows * lpr + 255) / 256));
   if (lpr == 8)
-    hipLaunchKernelGGL((kv_read_kernel<T, FP8, 8>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((kv_read_kernel<T, C, 8>), grid, dim3(256), 0, stream, p);
   else if (lpr == 16)
-    hipLaunchKernelGGL((kv_read_kernel<T, FP8, 16>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((kv_read_kernel<T, C, 16>), grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((kv_read_kernel<T, FP8, 32>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((kv_read_kernel<T, C, 32>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -290,11 +267,14 @@ hipError_t kv_write(int dtype, int cache_dtype, const void* k, const void* v, co
   KvWriteParams p{c, k, v, {sk[0], sk[1]}, {sv[0], sv[1]}, tokens * c.heads, 0, 0};
   if (p.rows == 0) return hipSuccess;
   division_magic(c.heads, &p.hmagic, &p.hshift);
+  if (cache_dtype == kE2M1)
+    return dtype == kF32 ? write_launch<float, e2m1>(p, stream)
+                         : dtype == kF16 ? write_launch<f16, e2m1>(p, stream) : write_launch<bf16, e2m1>(p, stream);
   if (cache_dtype == kE4M3)
-    return dtype == kF32 ? write_launch<float, true>(p, stream)
-                         : dtype == kF16 ? write_launch<f16, true>(p, stream) : write_launch<bf16, true>(p, stream);
+    return dtype == kF32 ? write_launch<float, e4m3>(p, stream)
+                         : dtype == kF16 ? write_launch<f16, e4m3>(p, stream) : write_launch<bf16, e4m3>(p, stream);
   // moves of 2 or 4 bytes a value, whatever they mean
-  return dtype == kF32 ? write_launch<float, false>(p, stream) : write_launch<f16, false>(p, stream);
+  return dtype == kF32 ? write_launch<float, float>(p, stream) : write_launch<f16, f16>(p, stream);
 }
 
 hipError_t kv_read(int dtype, int cache_dtype, void* k, void* v, const PagedKv& c, int max_len, hipStream_t stream) {
@@ -302,10 +282,13 @@ hipError_t kv_read(int dtype, int cache_dtype, void* k, void* v, const PagedKv& 
   if (p.rows == 0) return hipSuccess;
   division_magic(c.heads, &p.hmagic, &p.hshift);
   division_magic(max_len, &p.lmagic, &p.lshift);
+  if (cache_dtype == kE2M1)
+    return dtype == kF32 ? read_launch<float, e2m1>(p, stream)
+                         : dtype == kF16 ? read_launch<f16, e2m1>(p, stream) : read_launch<bf16, e2m1>(p, stream);
   if (cache_dtype == kE4M3)
-    return dtype == kF32 ? read_launch<float, true>(p, stream)
-                         : dtype == kF16 ? read_launch<f16, true>(p, stream) : read_launch<bf16, true>(p, stream);
-  return dtype == kF32 ? read_launch<float, false>(p, stream) : read_launch<f16, false>(p, stream);
+    return dtype == kF32 ? read_launch<float, e4m3>(p, stream)
+                         : dtype == kF16 ? read_launch<f16, e4m3>(p, stream) : read_launch<bf16, e4m3>(p, stream);
+  return dtype == kF32 ? read_launch<float, float>(p, stream) : read_launch<f16, f16>(p, stream);
 }
 
 }  // namespace samhip

@@ -3,9 +3,10 @@
 //
 // A pool holds pages [pages, heads, page_size, d] of keys and another of values. Sequence b's key j lies in page
 // table[b][j / page_size], slot j % page_size. In 8 bits (e4m3) a row of d values has one scale, a power of two held
-// as its biased exponent: value = code * 2^(scale - 127).
+// as its biased exponent: value = code * 2^(scale - 127). In 4 bits (e2m1, mx.hpp) each block of 32 values of a row has one,
+// and d is a multiple of 32.
 #pragma once
-#include "common.hpp"
+#include "mx.hpp"
 
 namespace samhip {
 
@@ -13,11 +14,15 @@ constexpr int kE4M3 = 3;  // cache dtype code beside DType's
 struct e4m3 {
   unsigned char bits;
 };
+constexpr int kE2M1 = 4;
+struct e2m1 {
+  unsigned char bits;  // two codes
+};
 
 struct PagedKv {
   void* k;
   void* v;
-  unsigned char* ks;  // scales [pages, heads, page_size], e4m3 only
+  unsigned char* ks;  // scales [pages, heads, page_size] of e4m3, [pages, heads, page_size, d / 32] of e2m1
   unsigned char* vs;
   const int* table;   // [batch, width]
   const int* starts;  // [batch + 1] first token of each sequence among the new ones (null: kv_read)
@@ -64,6 +69,10 @@ __device__ __forceinline__ int paged_len(const PagedKv& c, int b) {
 __device__ __forceinline__ float pow2_of(unsigned char biased) {
   return __uint_as_float(biased ? (unsigned)biased << 23 : 0x00400000u);  // 2^-127 is subnormal
 }
+
+// Bytes of n elements of a held row, and where element n lies; n is even where two share a byte.
+template <typename C> constexpr int held_bytes(int n) { return __is_same(C, e2m1) ? n / 2 : n * (int)sizeof(C); }
+template <typename C, typename N> __device__ __forceinline__ const C* held_at(const C* p, N n) { return p + (__is_same(C, e2m1) ? n / 2 : n); }
 
 // Arguments of one paged-attention launch. Strides in elements: [0] token, [1] head.
 struct PagedParams {
@@ -134,7 +143,10 @@ __device__ __forceinline__ unsigned without2(unsigned w, unsigned bad) {
 // Four values of a cache row in T (each rounded to it), as f32: those that are not finite, and 0 for the others.
 template <typename T, typename C> __device__ __forceinline__ f32x4 only_not_finite4(const C* p, float s) {
   u32x2 x;
-  if constexpr (__is_same(C, e4m3)) {
+  if constexpr (__is_same(C, e2m1)) {
+    const unsigned w = *reinterpret_cast<const unsigned short*>(p);
+    x = u32x2{mx_decode2<T, 0>(w, s), mx_decode2<T, 1>(w, s)};
+  } else if constexpr (__is_same(C, e4m3)) {
     const unsigned w = *reinterpret_cast<const unsigned*>(p);
     x = u32x2{decode2<T, false>(w, s), decode2<T, true>(w, s)};
   } else {

@@ -49,7 +49,8 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
     // the card, of 512 KB of keys and values each at least. 32 sequences, 8 key heads of 128 in e4m3: 820 to 8192 keys 92, 94,
     // 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125, 134 and 148; 4 heads of 256 in e4m3,
     // 8192 each, 103, 112 and 132 with 2, 4 and 8. Calls that f32 products bound count rounds.
-    const long bytes = 2L * d * (cache_dtype == kE4M3 ? 1 : dtype == kF32 ? 4 : 2) * max_len;  // a sequence's, of one head
+    const long row = cache_dtype == kE2M1 ? d / 2 + d / kMxBlock : d * (cache_dtype == kE4M3 ? 1L : dtype == kF32 ? 4L : 2L);
+    const long bytes = 2 * row * max_len;  // a sequence's, of one head
     const long want = plan.rtiles > 1 && dtype == kF32 ? f32_splits(base, (d > 64 ? 1L : 2L) * cus)
                                                        : ((d > 128 ? 2L : 4L) * cus + base - 1) / base;
     const long many = std::min(want, bytes >> 19);

@@ -34,6 +34,9 @@ template <typename C> struct Raw4 {
 template <> struct Raw4<e4m3> {
   typedef int t;
 };
+template <> struct Raw4<e2m1> {
+  typedef unsigned short t;
+};
 __device__ __forceinline__ f32x4 widen(f32x4 x, float) { return x; }
 __device__ __forceinline__ f32x4 widen(int c, float s) {
   typedef float f2 __attribute__((ext_vector_type(2)));
@@ -41,10 +44,15 @@ __device__ __forceinline__ f32x4 widen(int c, float s) {
   return f32x4{a[0] * s, a[1] * s, b[0] * s, b[1] * s};
 }
 
+__device__ __forceinline__ f32x4 widen(unsigned short c, float s) {
+  const f32x2 a = mx_decode2_f32<0>(c, s), b = mx_decode2_f32<1>(c, s);
+  return f32x4{a[0], a[1], b[0], b[1]};
+}
+
 template <typename C, int DP, int RB>
 __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(PagedParams p) {
   constexpr int NC = DP / 16, ND = (DP + 63) / 64, TR = 16 * RB;
-  constexpr bool kScaled = __is_same(C, e4m3);
+  constexpr bool kMx = __is_same(C, e2m1), kScaled = __is_same(C, e4m3);
   typedef typename Raw4<C>::t Raw;
   __shared__ float sm_m[2][TR], sm_l[2][TR];
   extern __shared__ __attribute__((aligned(16))) float sm_o[];  // [2][RB][4 ND][256]
@@ -103,22 +111,36 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
     };
     Raw kx[2][NC], vx[8][ND];
     unsigned char ksx = 127, vsx = 127;
+    // e2m1: the scales of the key blocks that the lane multiplies, and of every other of its own key's value blocks (lanes
+    // 0 .. 31 the even ones)
+    constexpr int KB = (DP + kMxBlock - 1) / kMxBlock;
+    unsigned char kmx[2][KB], vmx[ND];
+    const int G = d / kMxBlock;
     auto load_k = [&](int row) {
       if constexpr (kScaled) ksx = p.c.ks[max(row, 0)];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const C* kr = kp + (long)max(from_n(i, row), 0) * d;
+        const long r = max(from_n(i, row), 0);
+        const C* kr = held_at(kp, r * d);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) kx[i][c] = *reinterpret_cast<const Raw*>(kr + min(16 * c + 4 * g, d - 4));
+        for (int c = 0; c < NC; ++c) kx[i][c] = *reinterpret_cast<const Raw*>(held_at(kr, min(16 * c + 4 * g, d - 4)));
+        if constexpr (kMx) {
+#pragma unroll
+          for (int b = 0; b < KB; ++b) kmx[i][b] = p.c.ks[r * G + min(b, G - 1)];
+        }
       }
     };
     auto load_v = [&](int row) {
       if constexpr (kScaled) vsx = p.c.vs[max(row, 0)];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const C* vr = vp + (long)max(from_key(j, row), 0) * d;
+        const C* vr = held_at(vp, (long)max(from_key(j, row), 0) * d);
 #pragma unroll
-        for (int q = 0; q < ND; ++q) vx[j][q] = *reinterpret_cast<const Raw*>(vr + min(64 * q + 4 * n, d - 4));
+        for (int q = 0; q < ND; ++q) vx[j][q] = *reinterpret_cast<const Raw*>(held_at(vr, min(64 * q + 4 * n, d - 4)));
+      }
+      if constexpr (kMx) {
+#pragma unroll
+        for (int q = 0; q < ND; ++q) vmx[q] = p.c.vs[(long)max(row, 0) * G + min(2 * q + (lane >> 5), G - 1)];
       }
     };
     // Table entries two blocks ahead, K one, V while its block's scores are made
@@ -150,6 +172,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
         if constexpr (kScaled) f = __int_as_float(from_n(i, __float_as_int(kso)));
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
+          if constexpr (kMx) f = mx_scale(kmx[i][c / 2]);
           f32x4 a = widen(kx[i][c], f);
           if (16 * c + 16 > d && 16 * c + 4 * g >= d) a = f32x4{};
 #pragma unroll
@@ -198,11 +221,19 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
 #pragma unroll
         for (int j = 0; j < 8; ++j) vs[j] = __int_as_float(from_key(j, __float_as_int(vso)));
       }
+      unsigned vm[8];
+      if constexpr (kMx) {
+        unsigned vmo = 0;
+#pragma unroll
+        for (int q = 0; q < ND; ++q) vmo |= (unsigned)vmx[q] << (8 * q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vm[j] = (unsigned)__builtin_amdgcn_ds_bpermute((int)at_g + 128 * (n >> 3) + 64 * (j >> 2) + 4 * (j & 3), (int)vmo);
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int q = 0; q < ND; ++q) {
-          f32x4 a = widen(vx[j][q], kScaled ? vs[j] : 1.f);
+          f32x4 a = widen(vx[j][q], kMx ? mx_scale(vm[j] >> (8 * q) & 255) : kScaled ? vs[j] : 1.f);
           if (part) {  // rows that are not there hold anything; values that are not finite go apart
             const bool ok = mine >> (16 * (j >> 2) + (j & 3)) & 1;
 #pragma unroll
@@ -230,7 +261,8 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
             for (int e = 0; e < 4; ++e) {
               const int col = 64 * q + 16 * g + 4 * e;
               if (col < d) {
-                const f32x4 x = widen(*reinterpret_cast<const Raw*>(vp + (long)kr * d + col), f);
+                const float fc = kMx ? mx_scale(p.c.vs[(long)kr * G + col / kMxBlock]) : f;
+                const f32x4 x = widen(*reinterpret_cast<const Raw*>(held_at(vp, (long)kr * d + col)), fc);
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -333,6 +365,7 @@ template <typename C> hipError_t by_size(const PagedParams& p, int rows, hipStre
 }  // namespace
 
 hipError_t paged_f32(int cache_dtype, const PagedParams& p, int rows, hipStream_t stream) {
+  if (cache_dtype == kE2M1) return by_size<e2m1>(p, rows, stream);
   return cache_dtype == kE4M3 ? by_size<e4m3>(p, rows, stream) : by_size<float>(p, rows, stream);
 }
 

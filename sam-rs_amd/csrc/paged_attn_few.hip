@@ -28,6 +28,9 @@ namespace samhip {
 namespace {
 
 template <int BYTES> struct Raw;
+template <> struct Raw<2> {
+  typedef unsigned short t;
+};
 template <> struct Raw<4> {
   typedef unsigned t;
 };
@@ -45,12 +48,16 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 template <typename T, typename C, int DP, int RB>
 __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C, e4m3) ? 2 : 3) void paged_few_kernel(PagedParams p) {
   typedef typename Vec<T>::x8 X8;
-  constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
+  constexpr bool kMx = __is_same(C, e2m1), kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
   constexpr float kLift = kSplitP ? 0.f : 15.f;  // P is lifted by 2^kLift
   constexpr int TR = 16 * RB, NK = DP / 32;
   constexpr int CW = DP >= 128 ? 8 : DP / 16, NV = DP / (16 * CW);  // columns of a value row that a lane takes at once
-  typedef typename Raw<8 * (int)sizeof(C)>::t KRaw;
-  typedef typename Raw<CW * (int)sizeof(C)>::t VRaw;
+  typedef typename Raw<held_bytes<C>(8)>::t KRaw;
+  typedef typename Raw<held_bytes<C>(CW)>::t VRaw;
+  // e2m1: a lane's words of a key row lie side by side, DP / 4 columns, so that they are one load or two and have one scale
+  // or two; q's columns follow
+  constexpr int KL = NK < 4 ? NK : 4, KSC = DP <= 128 ? 1 : 2;  // words of a load, scales of a lane
+  constexpr int VSC = DP / 64;                                  // scales of a value row that a lane fetches
   __shared__ float sm_m[2][TR], sm_l[2][TR];
   __shared__ __attribute__((aligned(16))) float sm_o[2][RB * DP / 16][256];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -84,7 +91,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
       const T* qr = reinterpret_cast<const T*>(p.q) + (w.s0 + t) * p.sq[0] + (w.head * p.group + r - t * p.group) * p.sq[1];
 #pragma unroll
       for (int c = 0; c < NK; ++c) {
-        const int col = 32 * c + 8 * g;
+        const int col = kMx ? DP / 4 * g + 8 * c : 32 * c + 8 * g;
         qf[rb][c] = col < d ? *reinterpret_cast<const X8*>(qr + col) : X8{};
       }
     }
@@ -109,7 +116,30 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
     KRaw kx[2][NK];
     VRaw vx[8][NV];
     unsigned char ksx = 127, vsx = 127;  // scales of the lane's own key
+    // e2m1: the scales of the lane's key blocks, and of half of its own key's value blocks (lanes 0 .. 31 the lower half of
+    // each 128 columns' four, or of two)
+    unsigned char kmx[2][KSC], vmx[VSC];
+    const int G = d / kMxBlock;
     auto load_k = [&](int row) {
+      if constexpr (kMx) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = max(from_n(i, row), 0);
+          const unsigned char* kr = reinterpret_cast<const unsigned char*>(kp) + (unsigned long)(unsigned)r * (unsigned)(d / 2);
+#pragma unroll
+          for (int c = 0; c < NK; c += KL) {
+            const int at = min(DP / 4 * g + 8 * c, d - 8 * KL) / 2;
+            if constexpr (KL == 2)
+              *reinterpret_cast<u32x2*>(&kx[i][c]) = *reinterpret_cast<const u32x2*>(kr + at);
+            else
+              *reinterpret_cast<u32x4*>(&kx[i][c]) = *reinterpret_cast<const u32x4*>(kr + at);
+          }
+#pragma unroll
+          for (int b = 0; b < KSC; ++b)
+            kmx[i][b] = p.c.ks[(unsigned long)(unsigned)r * (unsigned)G + (unsigned)min(DP / 4 * g / kMxBlock + b, G - 1)];
+        }
+        return;
+      }
       if constexpr (kCoded) ksx = p.c.ks[max(row, 0)];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -119,12 +149,17 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
       }
     };
     auto load_v = [&](int row) {
+      if constexpr (kMx) {
+        const unsigned char* vs = p.c.vs + (unsigned long)(unsigned)max(row, 0) * (unsigned)G;
+#pragma unroll
+        for (int b = 0; b < VSC; ++b) vmx[b] = vs[min(DP == 64 ? lane >> 5 : 4 * (b >> 1) + 2 * (lane >> 5) + (b & 1), G - 1)];
+      }
       if constexpr (kCoded) vsx = p.c.vs[max(row, 0)];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const C* vr = vp + (long)max(from_key(j, row), 0) * d;
+        const C* vr = held_at(vp, (long)max(from_key(j, row), 0) * d);
 #pragma unroll
-        for (int q = 0; q < NV; ++q) vx[j][q] = *reinterpret_cast<const VRaw*>(vr + min(CW * (16 * q + n), d - CW));
+        for (int q = 0; q < NV; ++q) vx[j][q] = *reinterpret_cast<const VRaw*>(held_at(vr, min(CW * (16 * q + n), d - CW)));
       }
     };
 
@@ -149,6 +184,11 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
       const unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
       f32x4 s[RB][2];
       const float kso = kCoded ? pow2_of(ksx) : 1.f, vso = kCoded ? pow2_of(vsx) : 1.f;
+      unsigned vmo = 0;
+      if constexpr (kMx) {
+#pragma unroll
+        for (int b = 0; b < VSC; ++b) vmo |= (unsigned)vmx[b] << (8 * b);
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float ks = 1.f;
@@ -156,12 +196,15 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
 #pragma unroll
         for (int c = 0; c < NK; ++c) {
           u32x4 a;
-          if constexpr (kCoded)
+          if constexpr (kMx) {
+            const float f = mx_scale(kmx[i][8 * c / kMxBlock % KSC]);
+            a = u32x4{mx_decode2<T, 0>(kx[i][c], f), mx_decode2<T, 1>(kx[i][c], f), mx_decode2<T, 2>(kx[i][c], f), mx_decode2<T, 3>(kx[i][c], f)};
+          } else if constexpr (kCoded)
             a = u32x4{decode2<T, false>(kx[i][c][0], ks), decode2<T, true>(kx[i][c][0], ks),
                       decode2<T, false>(kx[i][c][1], ks), decode2<T, true>(kx[i][c][1], ks)};
           else
             a = kx[i][c];
-          if (32 * c + 32 > d && 32 * c + 8 * g >= d) a = u32x4{};
+          if (kMx ? DP / 4 * g + 8 * c >= d : 32 * c + 32 > d && 32 * c + 8 * g >= d) a = u32x4{};
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb)
             s[rb][i] = mma16(__builtin_bit_cast(X8, a), qf[rb][c], c == 0 ? f32x4{} : s[rb][i]);
@@ -217,12 +260,25 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
 #pragma unroll
         for (int j = 0; j < 8; ++j) vs[j] = __int_as_float(from_key(j, __float_as_int(vso)));
       }
+      unsigned vm[8];
+      if constexpr (kMx) {  // the lane's blocks' half of the four
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vm[j] = (unsigned)__builtin_amdgcn_ds_bpermute((int)at_g + 128 * (n >> 3) + 64 * (j >> 2) + 4 * (j & 3), (int)vmo);
+      }
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
         unsigned v[8][CW / 2];  // key j's columns, two to a register
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if constexpr (kCoded) {
+          if constexpr (kMx) {
+            const float f = mx_scale(vm[j] >> (DP == 64 ? 0 : 16 * q + 8 * (n >> 2 & 1)) & 255);
+            v[j][0] = mx_decode2<T, 0>(vx[j][q], f);
+            v[j][1] = mx_decode2<T, 1>(vx[j][q], f);
+            if constexpr (CW == 8) {
+              v[j][2] = mx_decode2<T, 2>(vx[j][q], f);
+              v[j][3] = mx_decode2<T, 3>(vx[j][q], f);
+            }
+          } else if constexpr (kCoded) {
 #pragma unroll
             for (int h = 0; h < CW / 4; ++h) {
               unsigned word;
@@ -276,7 +332,8 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
               for (int c = 0; c < CW; c += 4) {
                 const int col = CW * (16 * q + 4 * g + e) + c;
                 if (col < d) {
-                  const f32x4 x = only_not_finite4<T>(vp + (long)kr * d + col, s1);
+                  const float f = kMx ? mx_scale(p.c.vs[(unsigned long)(unsigned)kr * (unsigned)G + (unsigned)(col / kMxBlock)]) : s1;
+                  const f32x4 x = only_not_finite4<T>(held_at(vp, (long)kr * d + col), f);
 #pragma unroll
                   for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -380,6 +437,7 @@ template <typename T, typename C> hipError_t by_size(const PagedParams& p, int r
 }  // namespace
 
 hipError_t paged_few(int dtype, int cache_dtype, const PagedParams& p, int rows, hipStream_t stream) {
+  if (cache_dtype == kE2M1) return dtype == kF16 ? by_size<f16, e2m1>(p, rows, stream) : by_size<bf16, e2m1>(p, rows, stream);
   if (dtype == kF16)
     return cache_dtype == kE4M3 ? by_size<f16, e4m3>(p, rows, stream) : by_size<f16, f16>(p, rows, stream);
   return cache_dtype == kE4M3 ? by_size<bf16, e4m3>(p, rows, stream) : by_size<bf16, bf16>(p, rows, stream);

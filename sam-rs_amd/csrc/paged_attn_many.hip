@@ -66,7 +66,7 @@ template <typename T, typename C, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_many_kernel(PagedParams p) {
   typedef ManyGeom<DP> G;
   typedef typename Vec<T>::x8 X8;
-  constexpr bool kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
+  constexpr bool kMx = __is_same(C, e2m1), kCoded = kMx || __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
   constexpr float kLift = kSplitP ? 0.f : 15.f - kSlack;  // P is lifted by 2^kLift
   // LDS fragments in flight ahead of their products: bf16 at head dim 64 has fewer registers for them (8192 rows
   // and keys, 16 heads: 561 us against 568 with four, from e4m3 577 against 608)
@@ -91,8 +91,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
   auto srow = [&](int u) { return 16 * wave + RPI * u + lane / CPR; };
   auto kcol = [&](int u) { return 8 * (spos ^ G::kswz(RPI * u + lane / CPR)); };
   auto vcol = [&](int u) { return 8 * (spos ^ G::vswz(RPI * u + lane / CPR)); };
-  // e4m3: a load brings two chunks of a row, 16 codes, to the lane of LPR that stores them
-  constexpr int CH = kCoded ? 2 : 1, PR = PT / CH, LPR = CPR / CH;
+  // e4m3: a load brings two chunks of a row, 16 codes, to the lane of LPR that stores them; e2m1 four, a block, or two where
+  // a tile has no more for a lane
+  constexpr int CH = kMx && DP > 64 ? 4 : kCoded ? 2 : 1, PR = PT / CH, LPR = CPR / CH;
   const int rlane = lane / LPR, rcol = 8 * CH * (lane % LPR);
   auto rrow = [&](int u) { return 16 * wave + CH * RPI * u + rlane; };
 
@@ -153,11 +154,25 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
       // them, V once K is stored, in registers that the products have had.
       u32x4 kreg[PR], vbuf[kCoded ? PR : 1];
       u32x4* vreg = kCoded ? vbuf : kreg;
-      unsigned char kscale = 127, vscale = 127;  // of the lane's own key
-      auto load = [&](const C* base, const unsigned char* scales, int own, auto col, u32x4* reg, unsigned char& scale) {
+      unsigned char kscale[kMx ? PR : 1], vscale[kMx ? PR : 1];  // of the lane's own key, or of the blocks that it loads
+      auto load = [&](const C* base, const unsigned char* scales, int own, auto col, u32x4* reg, unsigned char* scale) {
         auto at = [&](int u) { return base + (unsigned long)(unsigned)max(__shfl(own, rrow(u)), 0) * (unsigned)d; };
-        if constexpr (kCoded) {
-          scale = scales[max(own, 0)];
+        if constexpr (kMx) {
+  #pragma unroll
+          for (int u = 0; u < PR; ++u) {
+            const unsigned long r = (unsigned)max(__shfl(own, rrow(u)), 0);
+            const int from = min(rcol, d - 8 * CH);
+            const C* x = base + r * (unsigned)(d / 2) + from / 2;
+            scale[u] = scales[r * (unsigned)(d / kMxBlock) + (unsigned)(from / kMxBlock)];
+            if constexpr (CH == 4) {
+              reg[u] = *reinterpret_cast<const u32x4*>(x);
+            } else {
+              const u32x2 w = *reinterpret_cast<const u32x2*>(x);
+              reg[u] = u32x4{w[0], w[1], 0, 0};
+            }
+          }
+        } else if constexpr (kCoded) {
+          *scale = scales[max(own, 0)];
           if (d % 16 == 0) {
   #pragma unroll
             for (int u = 0; u < PR; ++u) reg[u] = *reinterpret_cast<const u32x4*>(at(u) + min(rcol, d - 16));
@@ -177,10 +192,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
       };
       auto load_k = [&](int own) { load(kp, p.c.ks, own, kcol, kreg, kscale); };
       auto load_v = [&](int own) { load(vp, p.c.vs, own, vcol, vreg, vscale); };
-      auto values = [&](const u32x4* reg, unsigned char scale, u32x4* x) {  // x[CH u + c]: chunk c of load u
-        if constexpr (kCoded) {
+      auto values = [&](const u32x4* reg, const unsigned char* scale, u32x4* x) {  // x[CH u + c]: chunk c of load u
+        if constexpr (kMx) {
+  #pragma unroll
+          for (int u = 0; u < PR; ++u) {
+            const float f = mx_scale(scale[u]);
+  #pragma unroll
+            for (int c = 0; c < CH; ++c)
+              x[CH * u + c] = u32x4{mx_decode2<T, 0>(reg[u][c], f), mx_decode2<T, 1>(reg[u][c], f), mx_decode2<T, 2>(reg[u][c], f),
+                                    mx_decode2<T, 3>(reg[u][c], f)};
+          }
+        } else if constexpr (kCoded) {
           float f[PR];
-          const float mine = pow2_of(scale);
+          const float mine = pow2_of(*scale);
   #pragma unroll
           for (int u = 0; u < PR; ++u) f[u] = __shfl(mine, rrow(u));  // all before their use: each takes LDS's latency
   #pragma unroll
@@ -418,7 +442,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
             for (int kk = 0; kk < 64; ++kk) {
               if (!(there >> kk & 1)) continue;
               const int row = __shfl(own, kk);
-              const float vs = kCoded ? pow2_of(p.c.vs[row]) : 1.f;
+              const float vs = kCoded && !kMx ? pow2_of(p.c.vs[row]) : 1.f;
               const bool sees = key0 + kk < limit;
   #pragma unroll
               for (int ob = 0; ob < MBO; ++ob)
@@ -426,7 +450,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
                 for (int a = 0; a < 4; ++a) {
                   const int col = 32 * ob + 8 * a + 4 * hh;
                   if (col < d) {
-                    const f32x4 x = only_not_finite4<T>(vp + (long)row * d + col, vs);
+                    const float f = kMx ? mx_scale(p.c.vs[(unsigned long)(unsigned)row * (unsigned)(d / kMxBlock) + (unsigned)(col / kMxBlock)]) : vs;
+                    const f32x4 x = only_not_finite4<T>(held_at(vp, (long)row * d + col), f);
   #pragma unroll
                     for (int e = 0; e < 4; ++e) o[ob][4 * a + e] += sees ? x[e] : 0.f;
                   }
@@ -508,6 +533,7 @@ template <typename T, typename C> hipError_t by_size(const PagedParams& p, hipSt
 }  // namespace
 
 hipError_t paged_many(int dtype, int cache_dtype, const PagedParams& p, hipStream_t stream) {
+  if (cache_dtype == kE2M1) return dtype == kF16 ? by_size<f16, e2m1>(p, stream) : by_size<bf16, e2m1>(p, stream);
   if (dtype == kF16)
     return cache_dtype == kE4M3 ? by_size<f16, e4m3>(p, stream) : by_size<f16, f16>(p, stream);
   return cache_dtype == kE4M3 ? by_size<bf16, e4m3>(p, stream) : by_size<bf16, bf16>(p, stream);

@@ -684,21 +684,28 @@ int sam_hip_rope_axes(const void* x, const int* pos, const double* freqs, const 
 
 namespace {
 
+bool cache_dtype_ok(int dtype, int cache_dtype) {
+  return cache_dtype == dtype || cache_dtype == samhip::kE4M3 || cache_dtype == samhip::kE2M1;
+}
+
 // The checks that every call on a paged cache shares, and its description for the kernels.
 int check_pool(const char* what, const void* k_pages, const void* v_pages, const unsigned char* k_scale,
                const unsigned char* v_scale, const int* table, const int* lens, int dtype, int cache_dtype, int batch,
                int pages, int kv_heads, int page_size, int d, int table_width, samhip::PagedKv* c) {
   if (!k_pages || !v_pages || !table || !lens) return fail(SAM_HIP_EINVAL, "%s: null pointer argument", what);
   if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
-  if (cache_dtype != dtype && cache_dtype != samhip::kE4M3)
-    return fail(SAM_HIP_EDTYPE, "%s: the cache holds dtype %d or e4m3 (%d), got %d", what, dtype, samhip::kE4M3, cache_dtype);
-  if (cache_dtype == samhip::kE4M3 && (!k_scale || !v_scale))
-    return fail(SAM_HIP_EINVAL, "%s: an e4m3 cache needs its scales", what);
+  if (!cache_dtype_ok(dtype, cache_dtype))
+    return fail(SAM_HIP_EDTYPE, "%s: the cache holds dtype %d, e4m3 (%d) or e2m1 (%d), got %d", what, dtype, samhip::kE4M3,
+                samhip::kE2M1, cache_dtype);
+  if (cache_dtype != dtype && (!k_scale || !v_scale))
+    return fail(SAM_HIP_EINVAL, "%s: an e4m3 or e2m1 cache needs its scales", what);
   if (batch <= 0 || pages <= 0 || kv_heads <= 0 || page_size <= 0 || d <= 0 || table_width <= 0)
     return fail(SAM_HIP_EINVAL, "%s: sizes must be positive (batch=%d pages=%d heads=%d page=%d d=%d width=%d)", what,
                 batch, pages, kv_heads, page_size, d, table_width);
   if (d % 8 != 0 || d > 256)
     return fail(SAM_HIP_EUNSUPPORTED, "%s: head dim must be a multiple of 8 and at most 256, got %d", what, d);
+  if (cache_dtype == samhip::kE2M1 && d % samhip::kMxBlock != 0)
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: an e2m1 cache's head dim must be a multiple of 32, got %d", what, d);
   if ((long)table_width * page_size >= 1L << 30)
     return fail(SAM_HIP_EUNSUPPORTED, "%s: a table of %d pages of %d tokens is beyond 2^30 tokens", what, table_width,
                 page_size);
@@ -795,7 +802,7 @@ int sam_hip_kv_read(void* k, void* v, const void* k_pages, const void* v_pages, 
 
 long sam_hip_paged_attention_workspace_size(int dtype, int cache_dtype, int tokens, int batch, int heads, int kv_heads,
                                             int d, int max_q, int max_len) {
-  if (!dtype_ok(dtype) || (cache_dtype != dtype && cache_dtype != samhip::kE4M3)) {
+  if (!dtype_ok(dtype) || !cache_dtype_ok(dtype, cache_dtype)) {
     fail(SAM_HIP_EDTYPE, "paged-attention: dtype %d over a cache of dtype %d", dtype, cache_dtype);
     return -1;
   }

@@ -14,7 +14,7 @@ Names, argument meaning and errors follow the reference:
     rope(x, cos, sin)                                    sam3/video.rs:106-113
     rope_attention(q, k, v, cos, sin, n_exclude)         sam3/video.rs:129-145 (after the projections)
     rope_axes(x, pos, freqs, axes), rope_freqs(...)      rotary positions over several axes
-    kv_write(k, v, k_pages, v_pages, table, ...)         new keys and values into a paged cache (16 or 8 bits)
+    kv_write(k, v, k_pages, v_pages, table, ...)         new keys and values into a paged cache (16, 8 or 4 bits)
     kv_read(k_pages, v_pages, table, lens, max_len)      what its sequences hold, dense
     paged_attention(q, k_pages, v_pages, table, ...)     attention of new tokens over the pages
     mx_pack(x), mx_unpack(codes, scale)  rows as 4-bit numbers in scaled blocks of 32, and back
@@ -625,7 +625,9 @@ def rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch
 
 # ------------------------------------------------------------------------------------------ the paged memory
 
-_E4M3 = 3  # SAM_HIP_E4M3
+_E4M3, _E2M1_CODE = 3, 4  # SAM_HIP_E4M3, SAM_HIP_E2M1
+_E2M1 = torch.float4_e2m1fn_x2  # two codes a byte, the even column's in the low half
+_BLOCK = 32  # values of a row that share a scale
 
 
 # The calls below are made once a layer and token, where the host's time counts: an index in place of a device object
@@ -752,8 +754,17 @@ def _pool(what, k_pages, v_pages, k_scale, v_scale, table, starts, lens, dtype):
         for s in (k_scale, v_scale):
             if s is None or s.dtype != torch.uint8 or s.shape != shape[:3] or not s.is_contiguous():
                 raise SamHipError(f"{what}: an e4m3 cache needs k_scale and v_scale, uint8 {tuple(shape[:3])} and contiguous")
+    elif held == _E2M1:
+        code = _E2M1_CODE
+        shape = shape[:3] + (2 * shape[3],)
+        if shape[3] % _BLOCK:
+            raise SamHipError(f"{what}: an e2m1 cache's head dim must be a multiple of {_BLOCK}, got {shape[3]}")
+        for s in (k_scale, v_scale):
+            if s is None or s.dtype != torch.uint8 or s.shape != shape[:3] + (shape[3] // _BLOCK,) or not s.is_contiguous():
+                raise SamHipError(f"{what}: an e2m1 cache needs k_scale and v_scale, uint8 "
+                                  f"{tuple(shape[:3]) + (shape[3] // _BLOCK,)} and contiguous")
     else:
-        raise SamHipError(f"{what}: the cache must hold {dtype} or torch.float8_e4m3fn, got {held}")
+        raise SamHipError(f"{what}: the cache must hold {dtype}, torch.float8_e4m3fn or torch.float4_e2m1fn_x2, got {held}")
     rows = table.shape
     if len(rows) != 2 or table.dtype != torch.int32:
         raise SamHipError(f"{what}: table must be int32 [batch, width], got {table.dtype} {tuple(rows)}")
@@ -799,7 +810,8 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: t
     in page table[b][position // page_size]. k_pages, v_pages [pages, heads, page_size, D] hold k's dtype, or
     torch.float8_e4m3fn with k_scale, v_scale uint8 [pages, heads, page_size]: a row's scale is the power of two
     2^(byte - 127) that brings its largest value nearest to 448 from below, its codes round to nearest even, and values
-    that are not finite become NaN. Tokens at a negative position, past the table, or whose table entry names no page are
+    that are not finite become NaN. Or they hold torch.float4_e2m1fn_x2 [pages, heads, page_size, D / 2] with k_scale, v_scale
+    uint8 [pages, heads, page_size, D / 32], D a multiple of 32, rows as mx_pack makes them. Tokens at a negative position, past the table, or whose table entry names no page are
     not stored; two positions in one page slot must not be written by one call."""
     dev = _device_of("kv_write", k, v, k_pages, v_pages, table, starts, lens, k_scale, v_scale)
     if not _is_current(dev):
@@ -826,7 +838,7 @@ def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, l
             k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
             dtype: torch.dtype | None = None):
     """What the sequences of a cache hold, dense: (k, v) [B, max_len, heads, D], zeros from lens[b] on and where a table
-    entry names no page. dtype defaults to the cache's; an e4m3 cache needs one (each value is rounded to it once)."""
+    entry names no page. dtype defaults to the cache's; an e4m3 or e2m1 cache needs one (each value is rounded to it once)."""
     dev = _device_of("kv_read", k_pages, v_pages, table, lens, k_scale, v_scale)
     if not _is_current(dev):
         with torch.cuda.device(dev):
@@ -919,9 +931,6 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 # ------------------------------------------------------------------------------------------ 4-bit numbers
-
-_E2M1 = torch.float4_e2m1fn_x2  # two codes a byte, the even column's in the low half
-_BLOCK = 32
 
 
 def _mx_k(what, shape) -> int:

@@ -91,3 +91,15 @@ def test_reference_quantiser_rounds_to_the_nearest():
             assert torch.equal((v.abs() / two - y.abs() / two).abs(), (y.abs()[:, None] / two - grid).abs().min(-1).values)
     tie = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0] * 4, dtype=torch.float64)
     assert ref.quantise(tie)[0][:8].tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0]
+
+
+def test_the_paged_memory_refuses_what_4_bits_cannot_hold(lib):
+    from test_paged_abi import attend, read, write
+
+    for call in (write, read, attend):
+        for change, code in (({"cache": 4, "d": 72}, 3), ({"cache": 4, "d": 80}, 3), ({"cache": 4, "ks": None}, 1), ({"cache": 4, "vs": None}, 1),
+                             ({"cache": 5}, 2), ({"cache": 4, "dtype": 3}, 2), ({"cache": 4, "k_pages": vp(0x1008)}, 3)):
+            assert call(lib, **change) == code
+            assert lib.sam_hip_last_error()
+    size = lib.sam_hip_paged_attention_workspace_size
+    assert size(1, 4, 1, 1, 8, 1, 128, 1, 1 << 16) > 0 and size(1, 5, 1, 1, 8, 1, 128, 1, 64) == -1
