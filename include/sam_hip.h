@@ -287,6 +287,7 @@ const char* sam_hip_last_error(void);
 int sam_hip_abi_version(void);
 
 #include "sam_hip_paged.h" /* the paged memory: multi-axis rotary positions, the cache, attention over it */
+#include "sam_hip_append.h" /* new tokens into it with their rotation, in one call */
 #include "sam_hip_mx.h"    /* microscaled 4-bit numbers: packing and products */
 
 #ifdef __cplusplus

@@ -1,0 +1,319 @@
+// New tokens into a paged cache with the position rotation on the way, on gfx950: queries and keys turn as in rope_axes.hip
+//   y0 = x0 cos a - x1 sin a, y1 = x1 cos a + x0 sin a, a = pos[axes[i]] * freqs[i]
+// and queries go out, keys and values into their pages as in kv_cache.hip, in one launch in place of three and without
+// the turned keys' way through memory.
+//
+// Keys are turned in f64 and rounded once, to their type or to their codes, so that a code is the definition's also next to
+// the border between two (an f32 turn, off by 2^-22, would flip one of a million). The angle is the f64 product; it is reduced
+// by quarter turns with pi / 2 in two parts (exact to 2^-52 up to 2^48 radians), sine and cosine are Taylor sums on an eighth
+// of a turn either way, whose first terms left out are below 2^-56. Queries, which go out in their own type, take the angle's
+// sine and cosine in f32.
+//
+// What bounds it: HBM bytes, each row in and out once. A row belongs to LPR lanes of 8 columns, as in kv_cache.hip; they form
+// their angles once for HP heads of a token. In the halves layout a lane loads its partners' columns too (their lines are on
+// their way for the partner lane), so that nothing passes between lanes and a row may be turned in place: its loads come
+// before its wave's stores. Key heads come first in the grid, whose chain of table reads is the longer one.
+#include "kv_rows.hpp"
+
+namespace samhip {
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+struct KvAppendParams {
+  PagedKv c;
+  const void* q;
+  const void* k;
+  const void* v;
+  const int* pos;  // null: a token's position in its sequence, on every axis
+  const double* freqs;
+  const int* axes;
+  void* out;
+  long sq[2], sk[2], sv[2], sp[2], so[2];
+  int tokens, heads, pairs, naxes;
+  int zero_rest;
+  int kgroups, qgroups;                       // groups of HP heads of a token
+  unsigned kmagic, kshift, qmagic, qshift;    // divisions by them
+  int kunits, qunits;                         // tokens * groups
+  unsigned kblocks;                           // workgroups for keys and values; the queries' follow
+};
+
+// cos and sin of a.
+__device__ __forceinline__ void turn_of(double a, double& c, double& s) {
+  const double k = rint(a * 0.63661977236758134308);  // quarter turns
+  double r = fma(-k, 1.57079632679489661923, a);      // pi / 2 as a double, whose product with k fma takes exactly,
+  r = fma(-k, 6.12323399573676588613e-17, r);         // and what it lacks
+  const double r2 = r * r;
+  double sn = 1.0 / 355687428096000.0, cs = -1.0 / 6402373705728000.0;  // 1 / 17!, -1 / 18!
+  sn = fma(sn, r2, -1.0 / 1307674368000.0);
+  cs = fma(cs, r2, 1.0 / 20922789888000.0);
+  sn = fma(sn, r2, 1.0 / 6227020800.0);
+  cs = fma(cs, r2, -1.0 / 87178291200.0);
+  sn = fma(sn, r2, -1.0 / 39916800.0);
+  cs = fma(cs, r2, 1.0 / 479001600.0);
+  sn = fma(sn, r2, 1.0 / 362880.0);
+  cs = fma(cs, r2, -1.0 / 3628800.0);
+  sn = fma(sn, r2, -1.0 / 5040.0);
+  cs = fma(cs, r2, 1.0 / 40320.0);
+  sn = fma(sn, r2, 1.0 / 120.0);
+  cs = fma(cs, r2, -1.0 / 720.0);
+  sn = fma(sn, r2, -1.0 / 6.0);
+  cs = fma(cs, r2, 1.0 / 24.0);
+  sn = fma(sn * r2, r, r);
+  cs = fma(cs, r2, -0.5);
+  cs = fma(cs, r2, 1.0);
+  const int quarter = (int)(long)k & 3;  // (c, s) -> (-s, c) each
+  const double u = quarter & 1 ? -sn : cs, w = quarter & 1 ? cs : sn;
+  c = quarter & 2 ? -u : u;
+  s = quarter & 2 ? -w : w;
+}
+
+// x in f32, rounded to odd: cut short, and its last bit set if anything was cut off. Rounding that to fewer bits (up to 22)
+// gives what rounding x to them would.
+__device__ __forceinline__ float to_odd(double x) {
+  const float f = (float)x;
+  unsigned u = __float_as_uint(f);
+  if ((double)f != x) u = (fabs((double)f) > fabs(x) ? u - 1 : u) | 1u;
+  return __uint_as_float(u);
+}
+
+// 8 values turned by their pairs' (c, s): with HALVES, x's partners are o's and `low` says which of the two x are; else pairs
+// are neighbours, and a pair's (c, s) is at its first element's half.
+template <typename F, bool HALVES> __device__ __forceinline__ F turned(int j, const F* x, const F* o, const F* c, const F* s, bool low) {
+  if constexpr (HALVES) {
+    return low ? fma(x[j], c[j], -(o[j] * s[j])) : fma(x[j], c[j], o[j] * s[j]);
+  } else {
+    const int i = j / 2;
+    return j % 2 == 0 ? fma(x[j], c[i], -(x[j + 1] * s[i])) : fma(x[j], c[i], x[j - 1] * s[i]);
+  }
+}
+
+template <typename T, typename C, int LPR, int HP, bool HALVES>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
+  constexpr int NP = HALVES ? 8 : 4;  // pairs of a lane
+  const bool keys = blockIdx.x < p.kblocks;
+  const int r = (int)(((blockIdx.x - (keys ? 0u : p.kblocks)) * 256u + threadIdx.x) / LPR);
+  const int col = (int)(threadIdx.x % LPR) * 8, d = p.c.d;
+  const int units = keys ? p.kunits : p.qunits, groups = keys ? p.kgroups : p.qgroups, heads = keys ? p.c.heads : p.heads;
+  const int own = min(r, units - 1);
+  const int t = (int)divide_magic((unsigned)own, keys ? p.kmagic : p.qmagic, keys ? p.kshift : p.qshift), hg = own - t * groups;
+  const bool inside = r < units && col < d;
+  // which of the lane's elements turn, and where their partners are
+  unsigned turn = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) turn |= col + j < 2 * p.pairs ? 1u << j : 0u;
+  const bool even = p.pairs % 8 == 0;  // halves: a lane's elements have one role
+  const bool low = col < p.pairs;
+
+  Eight<T> x[HP], o[HALVES ? HP : 1], v[HP];
+  auto load_rows = [&](const void* base, const long* st, Eight<T>* a, bool partners) {
+#pragma unroll
+    for (int i = 0; i < HP; ++i) {
+      const T* row = reinterpret_cast<const T*>(base) + t * st[0] + min(hg + i * groups, heads - 1) * st[1];
+      a[i] = load_eight(row + min(col, d - 8));
+      if constexpr (HALVES) {
+        if (!partners) continue;
+        if (p.pairs == 0) {
+          o[i] = Eight<T>{};
+        } else if (even) {
+          o[i] = load_eight(row + min(turn ? (low ? col + p.pairs : col - p.pairs) : col, d - 8));
+        } else {
+          T* e = reinterpret_cast<T*>(&o[i]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int at = col + j < p.pairs ? col + j + p.pairs : col + j < 2 * p.pairs ? col + j - p.pairs : col + j;
+            e[j] = row[min(at, d - 1)];
+          }
+        }
+      }
+    }
+  };
+  if (keys) {
+    load_rows(p.k, p.sk, x, true);
+    load_rows(p.v, p.sv, v, false);
+  } else {
+    load_rows(p.q, p.sq, x, true);
+  }
+
+  // the token's sequence and position
+  const int b = sequence_of<LPR>(p.c, t);
+  const bool known = b < p.c.batch && t >= p.c.starts[min(b, p.c.batch - 1)] && t < p.c.starts[min(b, p.c.batch - 1) + 1];
+  long at = 0;
+  if (known) at = (long)p.c.lens[b] - p.c.starts[b + 1] + t;
+
+  double c[NP], s[NP];
+  if (p.pairs > 0) {
+    i32x4 ps = {};  // up to four axes' positions, loaded before it is known which of them the pairs want
+    const int* pr = p.pos + (long)t * p.sp[0];
+    if (p.pos && p.naxes <= 4) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) ps[a] = pr[min(a, p.naxes - 1) * p.sp[1]];
+    }
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      int i = HALVES ? col + j : col / 2 + j;
+      if (HALVES && i >= p.pairs) i -= p.pairs;
+      i = min(i, p.pairs - 1);
+      const double f = p.freqs[i];
+      double where = (double)at;
+      if (p.pos) {
+        const int ax = p.axes[i];
+        int w = 0;
+        if ((unsigned)ax < (unsigned)p.naxes) {
+          if (p.naxes <= 4) {
+            const int lo = ax & 1 ? ps.y : ps.x, hi = ax & 1 ? ps.w : ps.z;
+            w = ax & 2 ? hi : lo;
+          } else {
+            w = pr[ax * p.sp[1]];
+          }
+        }
+        where = (double)w;
+      }
+      turn_of(where * f, c[j], s[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NP; ++j) c[j] = 1.0, s[j] = 0.0;
+  }
+
+  if (!keys) {
+    const bool rest = !known;
+    if (!inside || (rest && !p.zero_rest)) return;
+    float cf[NP], sf[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) cf[j] = (float)c[j], sf[j] = (float)s[j];
+#pragma unroll
+    for (int i = 0; i < HP; ++i) {
+      const int h = hg + i * groups;
+      if (h >= heads) break;
+      const T* e = reinterpret_cast<const T*>(&x[i]);
+      const T* po = reinterpret_cast<const T*>(&o[HALVES ? i : 0]);
+      float xf[8], of[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xf[j] = to_f32(e[j]), of[j] = HALVES ? to_f32(po[j]) : 0.f;
+      Eight<T> y;
+      T* ye = reinterpret_cast<T*>(&y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float z = turned<float, HALVES>(j, xf, of, cf, sf, col + j < p.pairs);
+        ye[j] = rest ? from_f32<T>(0.f) : turn >> j & 1 ? from_f32<T>(f32_result(z)) : e[j];
+      }
+      store_eight(reinterpret_cast<T*>(p.out) + t * p.so[0] + h * p.so[1] + col, y);
+    }
+    return;
+  }
+
+  const long end = (long)p.c.width * p.c.page;
+  const bool fits = r < units && known && at >= 0 && at < end;
+  PagedEntry entry = {-1, -1};
+  if (fits) entry = paged_entry(p.c, b, (int)at, (int)end);
+#pragma unroll
+  for (int i = 0; i < HP; ++i) {
+    const int h = hg + i * groups;
+    const long row = fits && h < heads ? paged_row(p.c, entry, h) : -1;  // 64 bits: row * d passes 32
+    const T* e = reinterpret_cast<const T*>(&x[i]);
+    const T* po = reinterpret_cast<const T*>(&o[HALVES ? i : 0]);
+    double xd[8], od[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) xd[j] = to_f32(e[j]), od[j] = HALVES ? to_f32(po[j]) : 0.f;
+    constexpr bool kHeld = !__is_same(C, e4m3) && !__is_same(C, e2m1);
+    Eight<float> y;
+    float* ye = reinterpret_cast<float*>(&y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double z = turned<double, HALVES>(j, xd, od, c, s, col + j < p.pairs);
+      ye[j] = turn >> j & 1 ? kHeld && sizeof(T) == 4 ? (float)z : to_odd(z) : to_f32(e[j]);
+    }
+    if (!inside) {  // columns past d take part in the row's maximum
+      y = Eight<float>{};
+      v[i] = Eight<T>{};
+    }
+    const long to = row * d + col;
+    if constexpr (__is_same(C, e2m1)) {
+      unsigned ks, vs;
+      const unsigned kc = mx_quantise(y, ks), vc = mx_quantise(v[i], vs);
+      if (row >= 0 && inside) {
+        reinterpret_cast<unsigned*>(p.c.k)[to / 8] = kc;
+        reinterpret_cast<unsigned*>(p.c.v)[to / 8] = vc;
+        if (col % kMxBlock == 0) {
+          p.c.ks[to / kMxBlock] = (unsigned char)ks;
+          p.c.vs[to / kMxBlock] = (unsigned char)vs;
+        }
+      }
+    } else if constexpr (__is_same(C, e4m3)) {
+      u32x2 kc, vc;
+      int ks, vs;
+      quantise_row<float, LPR>(y, kc, ks);
+      quantise_row<T, LPR>(v[i], vc, vs);
+      if (row >= 0 && inside) {
+        *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.c.k) + to) = kc;
+        *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.c.v) + to) = vc;
+        if (col == 0) {
+          p.c.ks[row] = (unsigned char)(ks + 127);
+          p.c.vs[row] = (unsigned char)(vs + 127);
+        }
+      }
+    } else if (row >= 0 && inside) {
+      Eight<T> held;
+      T* he = reinterpret_cast<T*>(&held);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) he[j] = from_f32<T>(ye[j]);
+      store_eight(reinterpret_cast<T*>(p.c.k) + to, held);
+      store_eight(reinterpret_cast<T*>(p.c.v) + to, v[i]);
+    }
+  }
+}
+
+template <typename T, typename C, int LPR, int HP> hipError_t launch(KvAppendParams p, bool halves, hipStream_t stream) {
+  p.kgroups = (p.c.heads + HP - 1) / HP;
+  p.qgroups = (p.heads + HP - 1) / HP;
+  division_magic(p.kgroups, &p.kmagic, &p.kshift);
+  if (p.qgroups) division_magic(p.qgroups, &p.qmagic, &p.qshift);
+  p.kunits = p.tokens * p.kgroups;
+  p.qunits = p.tokens * p.qgroups;
+  p.kblocks = (unsigned)(((long)p.kunits * LPR + 255) / 256);
+  const dim3 grid(p.kblocks + (unsigned)(((long)p.qunits * LPR + 255) / 256));
+  if (halves)
+    hipLaunchKernelGGL((kv_append_kernel<T, C, LPR, HP, true>), grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((kv_append_kernel<T, C, LPR, HP, false>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+template <typename T, typename C, int LPR> hipError_t by_heads(const KvAppendParams& p, bool halves, hipStream_t stream) {
+  const long rows = (long)p.tokens * (p.heads + p.c.heads);
+  constexpr int kHeads = sizeof(T) == 4 ? 2 : 4;
+  return rows * LPR >= 1 << 18 && p.c.heads >= kHeads ? launch<T, C, LPR, kHeads>(p, halves, stream) : launch<T, C, LPR, 1>(p, halves, stream);
+}
+template <typename T, typename C> hipError_t by_size(const KvAppendParams& p, bool halves, hipStream_t stream) {
+  return p.c.d <= 64 ? by_heads<T, C, 8>(p, halves, stream)
+                     : p.c.d <= 128 ? by_heads<T, C, 16>(p, halves, stream) : by_heads<T, C, 32>(p, halves, stream);
+}
+template <typename T> hipError_t by_held(int cache_dtype, const KvAppendParams& p, bool halves, hipStream_t stream) {
+  return cache_dtype == kE2M1 ? by_size<T, e2m1>(p, halves, stream)
+                              : cache_dtype == kE4M3 ? by_size<T, e4m3>(p, halves, stream) : by_size<T, T>(p, halves, stream);
+}
+
+}  // namespace
+
+hipError_t kv_append(int dtype, int cache_dtype, const KvAppendCall& a, const PagedKv& c, hipStream_t stream) {
+  KvAppendParams p = {};
+  p.c = c;
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.pos = a.pos;
+  p.freqs = a.freqs;
+  p.axes = a.axes;
+  p.out = a.out;
+  for (int i = 0; i < 2; ++i) p.sq[i] = a.sq[i], p.sk[i] = a.sk[i], p.sv[i] = a.sv[i], p.sp[i] = a.sp[i], p.so[i] = a.so[i];
+  p.tokens = a.tokens;
+  p.heads = a.q ? a.heads : 0;
+  p.pairs = a.pairs;
+  p.naxes = a.naxes;
+  p.zero_rest = a.zero_rest;
+  return dtype == kF32 ? by_held<float>(cache_dtype, p, a.halves, stream)
+                       : dtype == kF16 ? by_held<f16>(cache_dtype, p, a.halves, stream) : by_held<bf16>(cache_dtype, p, a.halves, stream);
+}
+
+}  // namespace samhip

@@ -109,6 +109,22 @@ hipError_t kv_write(int dtype, int cache_dtype, const void* k, const void* v, co
                     const PagedKv& c, int tokens, hipStream_t stream);
 hipError_t kv_read(int dtype, int cache_dtype, void* k, void* v, const PagedKv& c, int max_len, hipStream_t stream);
 
+// One call that turns new tokens' queries and keys and stores their keys and values. Strides in elements: (token, head), of
+// pos (token, axis).
+struct KvAppendCall {
+  const void* q;  // null: keys and values alone
+  const void* k;
+  const void* v;
+  const int* pos;
+  const double* freqs;
+  const int* axes;
+  void* out;
+  long sq[2], sk[2], sv[2], sp[2], so[2];
+  int tokens, heads, pairs, naxes;
+  bool halves, zero_rest;
+};
+hipError_t kv_append(int dtype, int cache_dtype, const KvAppendCall& a, const PagedKv& c, hipStream_t stream);
+
 hipError_t rope_axes(int dtype, const void* x, const int* pos, const double* freqs, const int* axes, void* out, int b,
                      int l, int h, int d, int pairs, int naxes, const long* sx, const long* sp, const long* so,
                      int halves, int inverse, hipStream_t stream);

@@ -868,6 +868,65 @@ int sam_hip_paged_attention(const void* q, const void* k_pages, const void* v_pa
 
 }  // extern "C"
 
+extern "C" {
+
+int sam_hip_kv_append(const void* q, const void* k, const void* v, const int* pos, const double* freqs, const int* axes,
+                      void* out, void* k_pages, void* v_pages, unsigned char* k_scale, unsigned char* v_scale,
+                      const int* table, const int* starts, const int* lens, int dtype, int cache_dtype, int tokens,
+                      int batch, int heads, int pages, int kv_heads, int page_size, int d, int table_width, int pairs,
+                      int naxes, const long* strides_q, const long* strides_k, const long* strides_v,
+                      const long* strides_pos, const long* strides_out, int halves, int zero_rest, void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("kv-append");
+  if (!k || !v || !starts || !q != !out || (pairs != 0 && (!freqs || (pos && !axes))))
+    return fail(SAM_HIP_EINVAL, "kv-append: null pointer argument");
+  samhip::PagedKv c;
+  if (int rc = check_pool("kv-append", k_pages, v_pages, k_scale, v_scale, table, lens, dtype, cache_dtype, batch, pages,
+                          kv_heads, page_size, d, table_width, &c);
+      rc != SAM_HIP_OK)
+    return rc;
+  c.starts = starts;
+  if (tokens < 0 || (q && heads <= 0) || pairs < 0 || (pos && naxes <= 0))
+    return fail(SAM_HIP_EINVAL, "kv-append: sizes tokens=%d heads=%d pairs=%d axes=%d", tokens, heads, pairs, naxes);
+  if (2L * pairs > d) return fail(SAM_HIP_EINVAL, "kv-append: %d pairs do not fit in a head dim of %d", pairs, d);
+  samhip::KvAppendCall a = {};
+  a.heads = q ? heads : 0;
+  // up to 32 threads a row, which a launch counts in 32 bits
+  if (a.heads > 65535 || (long)tokens * (a.heads + (long)kv_heads) >= 1L << 27)
+    return fail(SAM_HIP_EUNSUPPORTED, "kv-append: too many rows (tokens=%d heads=%d kv_heads=%d)", tokens, heads, kv_heads);
+  if (int rc = token_strides("kv-append", "q", strides_q, a.sq, a.heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if (int rc = token_strides("kv-append", "k", strides_k, a.sk, kv_heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if (int rc = token_strides("kv-append", "v", strides_v, a.sv, kv_heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  if (int rc = token_strides("kv-append", "out", strides_out, a.so, a.heads, d, dtype); rc != SAM_HIP_OK) return rc;
+  const long steps[2] = {tokens, a.heads};
+  if (q && !rows_apart(2, steps, a.so, d))
+    return fail(SAM_HIP_EINVAL, "kv-append: out's rows must lie apart (strides %ld, %ld)", a.so[0], a.so[1]);
+  if (q && q == out && ((tokens > 1 && a.sq[0] != a.so[0]) || (heads > 1 && a.sq[1] != a.so[1])))
+    return fail(SAM_HIP_EINVAL, "kv-append: in place, q and out must have the same strides");
+  a.sp[0] = strides_pos ? strides_pos[0] : naxes;
+  a.sp[1] = strides_pos ? strides_pos[1] : 1;
+  if (a.sp[0] < 0 || a.sp[1] < 0) return fail(SAM_HIP_EUNSUPPORTED, "kv-append: strides must not be negative");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail(SAM_HIP_EUNSUPPORTED, "kv-append: q, k, v and out must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(pos) % 4 || reinterpret_cast<uintptr_t>(freqs) % 8 || reinterpret_cast<uintptr_t>(axes) % 4)
+    return fail(SAM_HIP_EUNSUPPORTED, "kv-append: pos, freqs and axes must be aligned to their elements");
+  if (tokens == 0) return ok();
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.pos = pos;
+  a.freqs = freqs;
+  a.axes = axes;
+  a.out = out;
+  a.tokens = tokens;
+  a.pairs = pairs;
+  a.naxes = naxes;
+  a.halves = halves != 0;
+  a.zero_rest = zero_rest != 0;
+  return check_launch(samhip::kv_append(dtype, cache_dtype, a, c, reinterpret_cast<hipStream_t>(stream)), "kv-append");
+}
+
+}  // extern "C"
+
 // ------------------------------------------------------------------------------------ 4-bit numbers
 
 namespace {

@@ -15,6 +15,7 @@ Names, argument meaning and errors follow the reference:
     rope_attention(q, k, v, cos, sin, n_exclude)         sam3/video.rs:129-145 (after the projections)
     rope_axes(x, pos, freqs, axes), rope_freqs(...)      rotary positions over several axes
     kv_write(k, v, k_pages, v_pages, table, ...)         new keys and values into a paged cache (16, 8 or 4 bits)
+    kv_append(q, k, v, freqs, axes, k_pages, ...)        rope_axes of q and k and kv_write in one launch
     kv_read(k_pages, v_pages, table, lens, max_len)      what its sequences hold, dense
     paged_attention(q, k_pages, v_pages, table, ...)     attention of new tokens over the pages
     mx_pack(x), mx_unpack(codes, scale)  rows as 4-bit numbers in scaled blocks of 32, and back
@@ -117,6 +118,8 @@ def load():
         L.sam_hip_paged_attention_workspace_size.restype = ctypes.c_long
         L.sam_hip_paged_attention.argtypes = [_vp] * 9 + [_i] * 10 + [_lp] * 2 + [_f] + [_i] * 4 + [_vp, ctypes.c_long, _vp]
         L.sam_hip_paged_attention.restype = _i
+        L.sam_hip_kv_append.argtypes = [_vp] * 14 + [_i] * 12 + [_lp] * 5 + [_i, _i, _vp]
+        L.sam_hip_kv_append.restype = _i
         L.sam_hip_mx_pack.argtypes = [_vp] * 3 + [_i, ctypes.c_long, _i, _vp]
         L.sam_hip_mx_pack.restype = _i
         L.sam_hip_mx_unpack.argtypes = [_vp] * 3 + [_i, ctypes.c_long, _i, _vp]
@@ -832,6 +835,79 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: t
     _check(load().sam_hip_kv_write(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
                                    _ptr(v_scale), table.data_ptr(), starts.data_ptr(), lens.data_ptr(), dt, code,
                                    tokens, b, pages, heads, page, d, width, sk, sv, _stream()))
+
+
+def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, freqs: torch.Tensor, axes: torch.Tensor,
+              k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor,
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, pos: torch.Tensor | None = None,
+              pairs: str = "adjacent", out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """What rope_axes of q and of k and kv_write do with new tokens, in one launch: returns q [T, Hq, D] turned, and stores k
+    [T, heads, D] turned and v in their pages (kv_write has the cache's arguments). Pair i turns by pos[t, axes[i]] * freqs[i],
+    pos int32 [T, A] or anything that broadcasts to it; without pos by the token's position in its sequence, lens[b] -
+    (starts[b+1] - t), on every axis. pairs, freqs and axes are rope_axes's. A turned key is rounded once, to its type or to
+    its codes. Rows of q of no sequence are 0, or as they were in an `out` that is given, which may be q itself and must not
+    overlap it otherwise, nor the other tensors. q may be None: keys and values alone."""
+    dev = _device_of("kv_append", k, v, k_pages, v_pages, table, starts, lens, k_scale, v_scale, q, out, pos, freqs, axes)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return kv_append(q, k, v, freqs, axes, k_pages, v_pages, table, starts, lens, k_scale, v_scale, pos, pairs, out)
+    dt = _dtype(k, v)
+    code, pages, heads, page, d, b, width = _pool("kv_append", k_pages, v_pages, k_scale, v_scale, table, starts, lens, k.dtype)
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape or shape[1] != heads or shape[2] != d:
+        raise SamHipError(f"kv_append: k and v must be [T, {heads}, {d}], got {tuple(shape)} and {tuple(v.shape)}")
+    tokens = shape[0]
+    if pairs not in ("adjacent", "halves"):
+        raise SamHipError(f'kv_append: pairs must be "adjacent" or "halves", got {pairs!r}')
+    n = freqs.shape
+    if freqs.dtype != torch.float64 or axes.dtype != torch.int32:
+        raise SamHipError(f"kv_append: freqs must be f64 and axes int32, got {freqs.dtype}, {axes.dtype}")
+    if len(n) != 1 or axes.shape != n or 2 * n[0] > d:
+        raise SamHipError(f"kv_append: freqs {tuple(n)} and axes {tuple(axes.shape)} must be [P], 2 P <= {d}")
+    naxes, sp = 1, None
+    if pos is not None:
+        if pos.dtype != torch.int32 or pos.dim() == 0 or pos.shape[-1] == 0:
+            raise SamHipError(f"kv_append: pos must be int32 [T, axes], got {pos.dtype} {tuple(pos.shape)}")
+        naxes = pos.shape[-1]
+        if pos.shape != (tokens, naxes) or not pos.is_contiguous():
+            try:
+                pos = pos.expand(tokens, naxes)
+            except RuntimeError as e:
+                raise SamHipError(f"kv_append: pos {tuple(pos.shape)} does not broadcast to {tokens} positions of its axes") from e
+            sp = _long2(*pos.stride())
+    hq, sq, so, rest = 0, None, None, out is None
+    if q is None:
+        if out is not None:
+            raise SamHipError("kv_append: out without q")
+    else:
+        at = q.shape
+        if q.dtype != k.dtype or len(at) != 3 or at[0] != tokens or at[1] == 0 or at[2] != d:
+            raise SamHipError(f"kv_append: q must be {k.dtype} [{tokens}, heads, {d}], got {q.dtype} {tuple(at)}")
+        hq = at[1]
+        if rest:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != at or out.dtype != q.dtype:
+            raise SamHipError(f"kv_append: out must match q (shape {tuple(at)}, {q.dtype}), got {tuple(out.shape)}, {out.dtype}")
+        elif not out.is_contiguous():
+            if out.stride(2) != 1 or _overlaps_itself(out):
+                raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
+            so = _long2(out.stride(0), out.stride(1))
+    if tokens == 0 or b == 0 or heads == 0 or d == 0:
+        _empty_call("kv-append")
+        return out.zero_() if rest and out is not None else out
+    if (tokens | hq | naxes) >> 31:
+        _sizes("kv_append", tokens, hq, naxes)
+    if width == 0:  # no pages: as one that is not there
+        table, width = torch.full((b, 1), -1, dtype=torch.int32, device=k.device), 1
+    table, starts, lens, freqs, axes = _plain(table), _plain(starts), _plain(lens), _plain(freqs), _plain(axes)
+    (k, sk), (v, sv) = _token_rows(k), _token_rows(v)
+    if q is not None:
+        q, sq = _token_rows(q)
+    _check(load().sam_hip_kv_append(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(pos), freqs.data_ptr(), axes.data_ptr(), _ptr(out),
+                                    k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(),
+                                    starts.data_ptr(), lens.data_ptr(), dt, code, tokens, b, hq, pages, heads, page, d, width,
+                                    n[0], naxes, sq, sk, sv, sp, so, pairs == "halves", rest, _stream()))
+    return out
 
 
 def kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int,
