@@ -94,10 +94,8 @@ template <typename T> __device__ __forceinline__ unsigned mx_quantise(const Eigh
   return fine ? w : 0u;
 }
 
-// A block's scale; 255 gives what the conversions below take as NaN.
-__device__ __forceinline__ float mx_scale(unsigned byte) {
-  return __uint_as_float(byte ? byte << 23 : 0x00400000u);  // 2^-127 is subnormal
-}
+// A block's scale for the conversions below, which read its exponent alone: 0 is 2^-127, 255 NaN.
+__device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float(byte << 23); }
 // Two values of a word of eight codes (byte SEL) in T, rounded to it once.
 template <typename T, int SEL> __device__ __forceinline__ unsigned mx_decode2(unsigned w, float s) {
   if constexpr (__is_same(T, f16))

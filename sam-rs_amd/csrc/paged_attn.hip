@@ -49,16 +49,22 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
     // the card, of 512 KB of keys and values each at least. 32 sequences, 8 key heads of 128 in e4m3: 820 to 8192 keys 92, 94,
     // 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125, 134 and 148; 4 heads of 256 in e4m3,
     // 8192 each, 103, 112 and 132 with 2, 4 and 8. Calls that f32 products bound count rounds.
-    const long row = cache_dtype == kE2M1 ? d / 2 + d / kMxBlock : d * (cache_dtype == kE4M3 ? 1L : dtype == kF32 ? 4L : 2L);
-    const long bytes = 2 * row * max_len;  // a sequence's, of one head
+    const bool mx = cache_dtype == kE2M1;
+    const long bytes = 2L * d * (cache_dtype == kE4M3 ? 1 : dtype == kF32 ? 4 : 2) * max_len;  // a sequence's, of one head
     const long want = plan.rtiles > 1 && dtype == kF32 ? f32_splits(base, (d > 64 ? 1L : 2L) * cus)
-                                                       : ((d > 128 ? 2L : 4L) * cus + base - 1) / base;
-    const long many = std::min(want, bytes >> 19);
+                                                       : ((d > 128 ? mx ? 1L : 2L : 4L) * cus + base - 1) / base;
+    // From e2m1 pages instructions bound it, so keys count, 2048 of a split at least, and past head dim 128 one workgroup a CU.
+    // Bf16, 32 sequences of 820 to 8192 keys, 8 heads: at 128 67, 57, 59, 55, 56 and 57 us with 1, 2, 3, 4, 6 and 8 splits, at 64
+    // 47, 42, 39, 38, 40 and 40, at 256 (4 heads) 109, 64, 81, 70, 79 and 86; 64 of up to 2000, at 128 30, 35, 36 and 40 with 1 to 4.
+    const long many = std::min(want, mx ? max_len / 2048L : bytes >> 19);
     // One a CU, of 128 KB each at least: a CU alone reads 60 GB/s. In f16, 2048 keys of 4 heads of 128 take 22.6, 16.4, 12.2 and
     // 10.3 us with 1, 2, 4 and 8 splits, 4096 of 4 heads of 64 25.4, 17.2, 11.9 and 9.6, 1024 of 8 heads of 128 14.0, 11.7 and
     // 9.7 with 1, 2 and 4. Below 448 KB the second launch costs what it gains (577 keys of 8 heads of 64 8.0 and 8.1 with 1
     // and 4, without the host's 3 us).
-    const long few = bytes > 448 << 10 ? std::min(cus / base, (bytes + (1 << 17) - 1) >> 17) : 1;
+    // From e2m1 pages past 1536 keys, 512 each: in f16, 2048 of 4 heads of 128 19.3, 15.6 and 14.3 us with 1, 2 and 3, 4096 of 4
+    // heads of 64 23.3, 17.2, 14.6 and 14.5 with 1, 2, 4 and 8, 1024 of 8 heads of 128 13.1 and 14.4 with 1 and 2.
+    const long few = mx ? (max_len > 1536 ? std::min(cus / base, (max_len + 511L) / 512) : 1)
+                        : bytes > 448 << 10 ? std::min(cus / base, (bytes + (1 << 17) - 1) >> 17) : 1;
     plan.nsplit = (int)std::min(std::max(std::max(many, few), 1L), 256L);
   }
   // no more threads for the launch that joins the splits than 32 bits count: d / 4 a row to 8 splits, 512 for 32 columns past

@@ -20,6 +20,8 @@
 // Measured, 32 sequences of 8192 keys, 8 key heads of 128, one token of 4 query heads a key head: f16 pages 187 us (5.7
 // TB/s), e4m3 pages 107 with f16 queries and 123 with bf16 (5.0 and 4.4; not for their instructions: a fifth fewer took as
 // long). 64-key blocks of e4m3 were no faster.
+#include <type_traits>
+
 #include "lds_dma.hpp"
 #include "paged.hpp"
 
@@ -43,10 +45,16 @@ template <> struct Raw<16> {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+constexpr int few_workgroups(bool wide, bool mx, bool split, int dp, int rb) {
+  return dp * rb > 128 ? 1 : dp == 128 && (wide || (mx && split)) ? 2 : 3;
+}
+
+// QUADS (e2m1 of a full head dim, pages of whole quads): the four neighbouring keys of a lane follow one another in their
+// page, so that a quad has one address, its rows lie at constant offsets and their scales are one load.
 // Workgroups a CU: as many as registers allow with a block of K and one of V in flight. Three for e4m3 at head dim 128
 // (131 us for the bf16 call above with eight splits, 137 with two).
-template <typename T, typename C, int DP, int RB>
-__global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C, e4m3) ? 2 : 3) void paged_few_kernel(PagedParams p) {
+template <typename T, typename C, int DP, int RB, bool QUADS>
+__global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, __is_same(C, e2m1), __is_same(T, bf16), DP, RB)) void paged_few_kernel(PagedParams p) {
   typedef typename Vec<T>::x8 X8;
   constexpr bool kMx = __is_same(C, e2m1), kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
   constexpr float kLift = kSplitP ? 0.f : 15.f;  // P is lifted by 2^kLift
@@ -58,6 +66,8 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
   // or two; q's columns follow
   constexpr int KL = NK < 4 ? NK : 4, KSC = DP <= 128 ? 1 : 2;  // words of a load, scales of a lane
   constexpr int VSC = DP / 64;                                  // scales of a value row that a lane fetches
+  constexpr int KB = QUADS && DP * RB == 64 ? 2 : 1, KEYS = 32 * KB;  // blocks and keys of an iteration
+  typedef typename std::conditional<KB == 2, unsigned long, unsigned>::type Bits;  // one of each key
   __shared__ float sm_m[2][TR], sm_l[2][TR];
   __shared__ __attribute__((aligned(16))) float sm_o[2][RB * DP / 16][256];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -112,18 +122,26 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
     auto from_key = [&](int j, int v) {  // the lane whose own key is element j of group g
       return __builtin_amdgcn_ds_bpermute((int)at_g + 64 * (j >> 2) + 4 * (j & 3), v);
     };
-    auto entry_of = [&](int blk) { return paged_entry(p.c, w.b, 32 * min(blk, b1 - 1) + (lane & 31), most); };
-    KRaw kx[2][NK];
-    VRaw vx[8][NV];
+    auto entry_of = [&](int blk) {
+      return paged_entry(p.c, w.b, 32 * min(KB == 2 ? blk + (lane >> 5) : blk, b1 - 1) + (lane & 31), most);
+    };
+    auto row_of = [&](const PagedEntry& e, int blk) {
+      const int r = paged_row(p.c, e, w.head);
+      return KB == 2 && blk + (lane >> 5) >= b1 ? -1 : r;  // the range may end between two blocks
+    };
+    KRaw kx[2 * KB][NK];
+    VRaw vx[8 * KB][NV];
     unsigned char ksx = 127, vsx = 127;  // scales of the lane's own key
     // e2m1: the scales of the lane's key blocks, and of half of its own key's value blocks (lanes 0 .. 31 the lower half of
     // each 128 columns' four, or of two)
-    unsigned char kmx[2][KSC], vmx[VSC];
+    unsigned char kmx[2 * KB][KSC], vmx[VSC];
+    // QUADS: of the lane's four neighbouring value rows, all of them: a row's DP / 32 bytes one after the other
+    u32x2 vq[2 * KB][QUADS ? VSC : 1];
     const int G = d / kMxBlock;
     auto load_k = [&](int row) {
       if constexpr (kMx) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2 * KB; ++i) {
           const int r = max(from_n(i, row), 0);
           const unsigned char* kr = reinterpret_cast<const unsigned char*>(kp) + (unsigned long)(unsigned)r * (unsigned)(d / 2);
 #pragma unroll
@@ -149,6 +167,21 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
       }
     };
     auto load_v = [&](int row) {
+      if constexpr (QUADS) {
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) {
+          const unsigned long r = (unsigned)max(from_key(4 * i, row), 0);  // its three neighbours follow it in its page
+          const C* vr = vp + r * (DP / 2);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int q = 0; q < NV; ++q) vx[4 * i + j][q] = *reinterpret_cast<const VRaw*>(vr + j * (DP / 2) + CW / 2 * (16 * q + n));
+          const u32x2* vs = reinterpret_cast<const u32x2*>(p.c.vs + r * (DP / kMxBlock));
+#pragma unroll
+          for (int b = 0; b < VSC; ++b) vq[i][b] = vs[b];
+        }
+        return;
+      }
       if constexpr (kMx) {
         const unsigned char* vs = p.c.vs + (unsigned long)(unsigned)max(row, 0) * (unsigned)G;
 #pragma unroll
@@ -168,29 +201,29 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
     // a condition would have the next scores wait for V too, as the compiler counts what is in flight on the shorter path.
     int row = -1;
     PagedEntry coming = {-1, -1};
-    if (b0 + wave < b1) {
-      const PagedEntry first = entry_of(b0 + wave);
-      coming = entry_of(b0 + wave + 4);
-      row = paged_row(p.c, first, w.head);
+    if (b0 + KB * wave < b1) {
+      const PagedEntry first = entry_of(b0 + KB * wave);
+      coming = entry_of(b0 + KB * (wave + 4));
+      row = row_of(first, b0 + KB * wave);
       load_k(row);
       load_v(row);
     }
     // Q is here: told to the compiler, whose own wait for it would stand in the loop, behind the next block's loads
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    for (int blk = b0 + wave; blk < b1; blk += 4) {
+    for (int blk = b0 + KB * wave; blk < b1; blk += 4 * KB) {
       const int key0 = 32 * blk;
-      const int next = paged_row(p.c, coming, w.head);
-      coming = entry_of(blk + 8);
-      const unsigned there = (unsigned)__builtin_amdgcn_ballot_w64(row >= 0);
-      f32x4 s[RB][2];
+      const int next = row_of(coming, blk + 4 * KB);
+      coming = entry_of(blk + 8 * KB);
+      const Bits there = (Bits)__builtin_amdgcn_ballot_w64(row >= 0);
+      f32x4 s[RB][2 * KB];
       const float kso = kCoded ? pow2_of(ksx) : 1.f, vso = kCoded ? pow2_of(vsx) : 1.f;
       unsigned vmo = 0;
-      if constexpr (kMx) {
+      if constexpr (kMx && !QUADS) {
 #pragma unroll
         for (int b = 0; b < VSC; ++b) vmo |= (unsigned)vmx[b] << (8 * b);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2 * KB; ++i) {
         float ks = 1.f;
         if constexpr (kCoded) ks = __int_as_float(from_n(i, __float_as_int(kso)));
 #pragma unroll
@@ -212,15 +245,15 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
       }
       // s[rb][i][e]: key key0 + 16 i + 4 g + e, row 16 rb + n
       load_k(next);  // in flight while this block's V is weighed
-      const bool part = key0 + 32 > least || there != 0xffffffffu;
-      const unsigned mine = there >> (4 * g);  // bit 16 i + e: the lane's key 16 i + 4 g + e
-      X8 b[RB], blo[RB];
+      const bool part = key0 + KEYS > least || there != (Bits)~(Bits)0;
+      const Bits mine = there >> (4 * g);  // bit 16 i + e: the lane's key 16 i + 4 g + e
+      X8 b[KB][RB], blo[KB][RB];
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         float top = -INFINITY;
         if (part) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int kk = 16 * i + e;
@@ -228,7 +261,7 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = max_nc(top, s[rb][i][e]);
         const float m_new = fmaxf(m[rb], max_over_rows16(top));
@@ -236,22 +269,27 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
         const float alpha = exp2_fast((m[rb] - base) * p.sc);
         m[rb] = m_new;
         l[rb] *= alpha;
+        if (!kMx || wave_any(alpha != 1.f)) {
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) o[rb][i] *= alpha;
-        float pv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          pv[j] = exp2_fast(fmaf(s[rb][j >> 2][j & 3] - base, p.sc, kLift));
+          for (int i = 0; i < DP / 16; ++i) o[rb][i] *= alpha;
         }
-        if constexpr (kSplitP) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) l[rb] += pv[j];
-          split_hi_lo(pv, b[rb], blo[rb]);
-        } else {
-          b[rb] = pack8(pv, (X8*)nullptr);
+        for (int u = 0; u < KB; ++u) {
+          float pv[8];
 #pragma unroll
-          for (int j = 0; j < 8; j += 2)
-            l[rb] = __builtin_amdgcn_fdot2(f16x2{b[rb][j], b[rb][j + 1]}, f16x2{(f16)1.f, (f16)1.f}, l[rb], false);
+          for (int j = 0; j < 8; ++j) {
+            pv[j] = exp2_fast(fmaf(s[rb][2 * u + (j >> 2)][j & 3] - base, p.sc, kLift));
+          }
+          if constexpr (kSplitP) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) l[rb] += pv[j];
+            split_hi_lo(pv, b[u][rb], blo[u][rb]);
+          } else {
+            b[u][rb] = pack8(pv, (X8*)nullptr);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+              l[rb] = __builtin_amdgcn_fdot2(f16x2{b[u][rb][j], b[u][rb][j + 1]}, f16x2{(f16)1.f, (f16)1.f}, l[rb], false);
+          }
         }
       }
       unsigned odd = 0;
@@ -261,66 +299,117 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
         for (int j = 0; j < 8; ++j) vs[j] = __int_as_float(from_key(j, __float_as_int(vso)));
       }
       unsigned vm[8];
-      if constexpr (kMx) {  // the lane's blocks' half of the four
+      if constexpr (kMx && !QUADS) {  // the lane's blocks' half of the four
 #pragma unroll
         for (int j = 0; j < 8; ++j) vm[j] = (unsigned)__builtin_amdgcn_ds_bpermute((int)at_g + 128 * (n >> 3) + 64 * (j >> 2) + 4 * (j & 3), (int)vmo);
       }
+      if constexpr (kMx) {
+        // columns 4 H .. 4 H + 3 of a lane's words: with all eight at a time, bf16 at head dim 128 spills at three
+        // workgroups a CU
+        auto columns = [&](auto half, int u, int q, const float* f) {
+          constexpr int H = decltype(half)::value;
+          unsigned v[8][2];
 #pragma unroll
-      for (int q = 0; q < NV; ++q) {
-        unsigned v[8][CW / 2];  // key j's columns, two to a register
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if constexpr (kMx) {
-            const float f = mx_scale(vm[j] >> (DP == 64 ? 0 : 16 * q + 8 * (n >> 2 & 1)) & 255);
-            v[j][0] = mx_decode2<T, 0>(vx[j][q], f);
-            v[j][1] = mx_decode2<T, 1>(vx[j][q], f);
-            if constexpr (CW == 8) {
-              v[j][2] = mx_decode2<T, 2>(vx[j][q], f);
-              v[j][3] = mx_decode2<T, 3>(vx[j][q], f);
-            }
-          } else if constexpr (kCoded) {
-#pragma unroll
-            for (int h = 0; h < CW / 4; ++h) {
-              unsigned word;
-              if constexpr (CW == 8)
-                word = vx[j][q][h];
-              else
-                word = vx[j][q];
-              v[j][2 * h] = decode2<T, false>(word, vs[j]);
-              v[j][2 * h + 1] = decode2<T, true>(word, vs[j]);
-            }
-          } else {
-#pragma unroll
-            for (int h = 0; h < CW / 2; ++h) v[j][h] = vx[j][q][h];
+          for (int j = 0; j < 8; ++j) {
+            v[j][0] = mx_decode2<T, 2 * H>(vx[8 * u + j][q], f[j]);
+            v[j][1] = mx_decode2<T, 2 * H + 1>(vx[8 * u + j][q], f[j]);
           }
           if (part) {  // rows that are not there hold anything; values that are not finite go apart
-            const bool ok = mine >> (16 * (j >> 2) + (j & 3)) & 1;
+            __builtin_amdgcn_sched_barrier(0);  // one branch, where the compiler would make one of each key's part
 #pragma unroll
-            for (int h = 0; h < CW / 2; ++h) {
-              const unsigned bad = not_finite2<T>(v[j][h]);
-              v[j][h] = ok ? without2(v[j][h], bad) : 0u;
-              odd |= ok ? bad : 0u;
+            for (int j = 0; j < 8; ++j) {
+              const bool ok = mine >> (32 * u + 16 * (j >> 2) + (j & 3)) & 1;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const unsigned bad = not_finite2<T>(v[j][h]);
+                v[j][h] = ok ? without2(v[j][h], bad) : 0u;
+                odd |= ok ? bad : 0u;
+              }
             }
           }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            u32x4 a;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // keys 2 j and 2 j + 1 of column c
+              a[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              f32x4& acc = o[rb][q * CW + 4 * H + c];
+              acc = mma16(__builtin_bit_cast(X8, a), b[u][rb], acc);
+              if constexpr (kSplitP) acc = mma16(__builtin_bit_cast(X8, a), blo[u][rb], acc);
+            }
+          }
+        };
+#pragma unroll
+        for (int uq = 0; uq < KB * NV; ++uq) {
+          const int u = uq / NV, q = uq % NV;
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (QUADS) {
+              const int at = (j & 3) * (DP / 64) + 2 * q;  // in pairs of the four rows' scales
+              f[j] = mx_scale(__builtin_amdgcn_ubfe(vq[2 * u + (j >> 2)][at / 4][at / 2 % 2], DP == 64 ? 16 * (at & 1) + 8 * (n >> 3) : 8 * (n >> 2), 8));
+            } else {
+              f[j] = mx_scale(vm[j] >> (DP == 64 ? 0 : 16 * q + 8 * (n >> 2 & 1)) & 255);
+            }
+          }
+          columns(std::integral_constant<int, 0>{}, u, q, f);
+          if constexpr (CW == 8) {
+            __builtin_amdgcn_sched_barrier(0);
+            columns(std::integral_constant<int, 1>{}, u, q, f);
+          }
         }
+      } else {
 #pragma unroll
-        for (int c = 0; c < CW; ++c) {
-          u32x4 a;
+        for (int q = 0; q < NV; ++q) {
+          unsigned v[8][CW / 2];  // key j's columns, two to a register
 #pragma unroll
-          for (int j = 0; j < 4; ++j)  // keys 2 j and 2 j + 1 of column c
-            a[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (kCoded) {
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            f32x4& acc = o[rb][q * CW + c];
-            acc = mma16(__builtin_bit_cast(X8, a), b[rb], acc);
-            if constexpr (kSplitP) acc = mma16(__builtin_bit_cast(X8, a), blo[rb], acc);
+              for (int h = 0; h < CW / 4; ++h) {
+                unsigned word;
+                if constexpr (CW == 8)
+                  word = vx[j][q][h];
+                else
+                  word = vx[j][q];
+                v[j][2 * h] = decode2<T, false>(word, vs[j]);
+                v[j][2 * h + 1] = decode2<T, true>(word, vs[j]);
+              }
+            } else {
+#pragma unroll
+              for (int h = 0; h < CW / 2; ++h) v[j][h] = vx[j][q][h];
+            }
+            if (part) {  // rows that are not there hold anything; values that are not finite go apart
+              const bool ok = mine >> (16 * (j >> 2) + (j & 3)) & 1;
+#pragma unroll
+              for (int h = 0; h < CW / 2; ++h) {
+                const unsigned bad = not_finite2<T>(v[j][h]);
+                v[j][h] = ok ? without2(v[j][h], bad) : 0u;
+                odd |= ok ? bad : 0u;
+              }
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < CW; ++c) {
+            u32x4 a;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // keys 2 j and 2 j + 1 of column c
+              a[j] = __builtin_amdgcn_perm(v[2 * j + 1][c >> 1], v[2 * j][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              f32x4& acc = o[rb][q * CW + c];
+              acc = mma16(__builtin_bit_cast(X8, a), b[0][rb], acc);
+              if constexpr (kSplitP) acc = mma16(__builtin_bit_cast(X8, a), blo[0][rb], acc);
+            }
           }
         }
       }
       if (wave_any(odd != 0)) {
         // A value that is not finite must not reach the rows that do not see its key (0 * inf = NaN): it was taken out
         // above, and the rows that see it add it here
-        for (int kk = 0; kk < 32; ++kk) {
+        for (int kk = 0; kk < KEYS; ++kk) {
           if (!(there >> kk & 1)) continue;
           const int kr = __shfl(row, kk);
           const float s1 = kCoded ? pow2_of(p.c.vs[kr]) : 1.f;
@@ -423,7 +512,11 @@ __global__ __launch_bounds__(256, DP * RB > 128 ? 1 : DP == 128 && !__is_same(C,
 
 template <typename T, typename C, int DP, int RB> hipError_t launch_few(const PagedParams& p, hipStream_t stream) {
   const long blocks = (long)p.rtiles * p.nsplit * p.c.heads * p.c.batch;
-  hipLaunchKernelGGL((paged_few_kernel<T, C, DP, RB>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+  auto run = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, p); };
+  if (__is_same(C, e2m1) && p.c.d == DP && p.c.page % 4 == 0 && reinterpret_cast<uintptr_t>(p.c.vs) % 8 == 0)
+    run(paged_few_kernel<T, C, DP, RB, __is_same(C, e2m1)>);
+  else
+    run(paged_few_kernel<T, C, DP, RB, false>);
   return hipGetLastError();
 }
 template <typename T, typename C> hipError_t by_size(const PagedParams& p, int rows, hipStream_t stream) {
