@@ -193,16 +193,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
       auto load_k = [&](int own) { load(kp, p.c.ks, own, kcol, kreg, kscale); };
       auto load_v = [&](int own) { load(vp, p.c.vs, own, vcol, vreg, vscale); };
       auto values = [&](const u32x4* reg, const unsigned char* scale, u32x4* x) {  // x[CH u + c]: chunk c of load u
-        if constexpr (kMx) {
-  #pragma unroll
-          for (int u = 0; u < PR; ++u) {
-            const float f = mx_scale(scale[u]);
-  #pragma unroll
-            for (int c = 0; c < CH; ++c)
-              x[CH * u + c] = u32x4{mx_decode2<T, 0>(reg[u][c], f), mx_decode2<T, 1>(reg[u][c], f), mx_decode2<T, 2>(reg[u][c], f),
-                                    mx_decode2<T, 3>(reg[u][c], f)};
-          }
-        } else if constexpr (kCoded) {
+        if constexpr (kCoded) {
           float f[PR];
           const float mine = pow2_of(*scale);
   #pragma unroll
@@ -226,7 +217,27 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
                                    : to + 16 * wave * ROW + 16 * lane + 1024 * u;
         if (chunk_col(u, c, col) < d) *(lds_u32x4*)(size_t)at = x;
       };
+      // e2m1: a load's chunks are all inside the row or none is. Their places are hidden from the optimiser, which would keep
+      // every one of them in a register across tiles (at head dim 256 in scratch memory: 8192 rows and keys 410 us).
+      auto mx_chunk = [&](unsigned w, float f) {
+        return u32x4{mx_decode2<T, 0>(w, f), mx_decode2<T, 1>(w, f), mx_decode2<T, 2>(w, f), mx_decode2<T, 3>(w, f)};
+      };
+      auto mx_place = [&](unsigned to, int lane_swz) { return opaque(to + (16 * wave + rlane) * ROW + 16 * ((rcol / 8) ^ lane_swz)); };
+      auto mx_store = [&](unsigned place, int u, int c, int u_swz, u32x4 x) {
+        *(lds_u32x4*)(size_t)((place ^ 16 * (c ^ u_swz)) + CH * RPI * ROW * u) = x;
+      };
       auto store_k = [&](int buf) {
+        if constexpr (kMx) {
+          if (rcol >= d) return;
+          const unsigned place = mx_place(lds0 + buf * BUF, G::kswz(rlane));
+  #pragma unroll
+          for (int u = 0; u < PR; ++u) {
+            const float f = mx_scale(kscale[u]);
+  #pragma unroll
+            for (int c = 0; c < CH; ++c) mx_store(place, u, c, G::kswz(CH * RPI * u), mx_chunk(kreg[u][c], f));
+          }
+          return;
+        }
         u32x4 x[PT];
         values(kreg, kscale, x);
   #pragma unroll
@@ -235,6 +246,37 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
           for (int c = 0; c < CH; ++c) store(lds0 + buf * BUF, u, c, kcol, G::kswz(rlane), G::kswz(CH * RPI * u), x[CH * u + c]);
       };
       auto store_v = [&](int t, unsigned long there, int buf) {
+        if constexpr (kMx) {
+          if (rcol >= d) return;
+          const unsigned place = mx_place(lds0 + (2 + buf) * BUF, G::vswz(rlane));
+          auto put = [&](auto look) {
+            unsigned any = 0;
+  #pragma unroll
+            for (int u = 0; u < PR; ++u) {
+              const float f = mx_scale(vscale[u]);
+              const bool ok = there >> rrow(u) & 1;
+  #pragma unroll
+              for (int c = 0; c < CH; ++c) {
+                u32x4 x = mx_chunk(vreg[u][c], f);
+                if constexpr (decltype(look)::value) {
+  #pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const unsigned bad = not_finite2<T>(x[i]);
+                    x[i] = ok ? without2(x[i], bad) : 0u;
+                    any |= ok ? bad : 0u;
+                  }
+                }
+                mx_store(place, u, c, G::vswz(CH * RPI * u), x);
+              }
+            }
+            if (decltype(look)::value && any) odd[buf] = t;
+          };
+          if (whole(t, there))
+            put(std::false_type{});
+          else
+            put(std::true_type{});
+          return;
+        }
         u32x4 x[PT];
         values(vreg, vscale, x);
         if (!whole(t, there)) {
