@@ -222,19 +222,32 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
       auto mx_chunk = [&](unsigned w, float f) {
         return u32x4{mx_decode2<T, 0>(w, f), mx_decode2<T, 1>(w, f), mx_decode2<T, 2>(w, f), mx_decode2<T, 3>(w, f)};
       };
-      auto mx_place = [&](unsigned to, int lane_swz) { return opaque(to + (16 * wave + rlane) * ROW + 16 * ((rcol / 8) ^ lane_swz)); };
+      // A lane stores its chunks in an order of its own, c ^ turn, so that the 16 lanes of a step fall on all 64 banks: those of
+      // its rows (V's swizzle leaves chunks of one place in a block on the same banks), and at head dim 256 those of a row's
+      // two halves (8192 rows and keys 397 us with V's stores four times as long, 357 so). At 64, where they take twice as long,
+      // it costs what it gains (363 us without, 370 with).
+      const int half = lane % LPR >> 2;
+      const int kturn = DP > 128 ? 2 * half : 0, vturn = DP > 128 ? half | (rlane & 1) << 1 : DP > 64 ? rlane & 3 : 0;
+      auto turned = [&](u32x4 w, int turn) {
+        const u32x4 x = turn & 1 ? u32x4{w[1], w[0], w[3], w[2]} : w;
+        return turn & 2 ? u32x4{x[2], x[3], x[0], x[1]} : x;
+      };
+      auto mx_place = [&](unsigned to, int lane_swz, int turn) {
+        return opaque(to + (16 * wave + rlane) * ROW + 16 * ((rcol / 8) ^ lane_swz ^ turn));
+      };
       auto mx_store = [&](unsigned place, int u, int c, int u_swz, u32x4 x) {
         *(lds_u32x4*)(size_t)((place ^ 16 * (c ^ u_swz)) + CH * RPI * ROW * u) = x;
       };
       auto store_k = [&](int buf) {
         if constexpr (kMx) {
           if (rcol >= d) return;
-          const unsigned place = mx_place(lds0 + buf * BUF, G::kswz(rlane));
+          const unsigned place = mx_place(lds0 + buf * BUF, G::kswz(rlane), kturn);
   #pragma unroll
           for (int u = 0; u < PR; ++u) {
             const float f = mx_scale(kscale[u]);
+            const u32x4 w = turned(kreg[u], kturn);
   #pragma unroll
-            for (int c = 0; c < CH; ++c) mx_store(place, u, c, G::kswz(CH * RPI * u), mx_chunk(kreg[u][c], f));
+            for (int c = 0; c < CH; ++c) mx_store(place, u, c, G::kswz(CH * RPI * u), mx_chunk(w[c], f));
           }
           return;
         }
@@ -248,16 +261,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : DP > 64 ? 2 : 3) void paged_man
       auto store_v = [&](int t, unsigned long there, int buf) {
         if constexpr (kMx) {
           if (rcol >= d) return;
-          const unsigned place = mx_place(lds0 + (2 + buf) * BUF, G::vswz(rlane));
+          const unsigned place = mx_place(lds0 + (2 + buf) * BUF, G::vswz(rlane), vturn);
           auto put = [&](auto look) {
             unsigned any = 0;
   #pragma unroll
             for (int u = 0; u < PR; ++u) {
               const float f = mx_scale(vscale[u]);
               const bool ok = there >> rrow(u) & 1;
+              const u32x4 w = turned(vreg[u], vturn);
   #pragma unroll
               for (int c = 0; c < CH; ++c) {
-                u32x4 x = mx_chunk(vreg[u][c], f);
+                u32x4 x = mx_chunk(w[c], f);
                 if constexpr (decltype(look)::value) {
   #pragma unroll
                   for (int i = 0; i < 4; ++i) {
