@@ -14,7 +14,7 @@ extern "C" {
  * its block's scale 2^s, s the least integer within +-126 with max|x| <= 6 * 2^s (0 for a block of zeros), held as the
  * byte s + 127. codes [rows, k / 2]: two a byte, the even column's in the low half; scales [rows, k / 32]. A code is x / 2^s
  * rounded to the nearest e2m1, ties to even; a block with a value that is not finite has the scale byte 255 and is NaN
- * throughout. No entry point of the reference's corresponds to these three: its linears (candle_nn::Linear, as in
+ * throughout. No entry point of the reference's corresponds to these: its linears (candle_nn::Linear, as in
  * sam1/encoder.rs:64) hold 16- or 32-bit weights.
  *
  * sam_hip_mx_pack writes the codes and scales of x [rows, k] in dtype; sam_hip_mx_unpack gives back the values that they
@@ -33,6 +33,16 @@ int sam_hip_mx_unpack(const unsigned char* codes, const unsigned char* scales, v
 int sam_hip_mx_matmul(const unsigned char* a, const unsigned char* a_scale, const unsigned char* b,
                       const unsigned char* b_scale, const void* bias, void* out, int dtype, int m, int n, int k, int gelu,
                       void* stream);
+
+/*
+ * A linear layer with 4-bit weights: sam_hip_mx_pack of x [m, k] into the workspace, then sam_hip_mx_matmul of it and of w,
+ * w_scale (as sam_hip_mx_pack makes them from [n, k]) to out [m, n]. Workspace: sam_hip_mx_linear_workspace_size() bytes of
+ * device memory, 16-byte aligned (-1 is an error); calls that may overlap need their own, and so does each captured graph
+ * that may run beside another.
+ */
+long sam_hip_mx_linear_workspace_size(int m, int k);
+int sam_hip_mx_linear(const void* x, const unsigned char* w, const unsigned char* w_scale, const void* bias, void* out,
+                      int dtype, int m, int n, int k, int gelu, void* workspace, long workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,4 +28,25 @@ __device__ __forceinline__ float gelu_erf(float x) {
   return 0.5f * x * (x >= 0.f ? 2.f - e : e);
 }
 
+// The same for results of 16 bits, with seven instructions less: erfc(z) exp(z^2) as a polynomial of degree 6 in
+// t = 1 / (1 + 0.44 z) without constant term, fitted here for the least relative error over 0 <= z <= 14 (6.6e-6; 1.1e-5 with
+// f32's roundings, down to x = -12), a fortieth of half a step of f16. Halves of the coefficients.
+__device__ __forceinline__ float gelu_erf16(float x) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.31112698372208092f, 1.f));
+  float p = -0.0721961836f;
+  p = fmaf(t, p, 0.172969651f);
+  p = fmaf(t, p, 0.0228032338f);
+  p = fmaf(t, p, 0.130619835f);
+  p = fmaf(t, p, 0.121544765f);
+  p = fmaf(t, p, 0.124259499f);
+  const float e = p * t * __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
+  return x * (x >= 0.f ? 1.f - e : e);
+}
+template <typename T> __device__ __forceinline__ float gelu_for(float x) {
+  if constexpr (sizeof(T) == 2)
+    return gelu_erf16(x);
+  else
+    return gelu_erf(x);
+}
+
 }  // namespace samhip

@@ -41,120 +41,122 @@ template <typename T> __device__ __forceinline__ void put4(const MxProduct& p, i
     }
     typename Vec<T>::x4 y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(f32_result(p.gelu ? gelu_erf(x[i]) : x[i]));
+    for (int i = 0; i < 4; ++i) y[i] = from_f32<T>(f32_result(p.gelu ? gelu_for<T>(x[i]) : x[i]));
     *reinterpret_cast<typename Vec<T>::x4*>(to) = y;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (n + i >= p.n) break;
       const float v = x[i] + (bias ? to_f32(bias[n + i]) : 0.f);
-      to[i] = from_f32<T>(f32_result(p.gelu ? gelu_erf(v) : v));
+      to[i] = from_f32<T>(f32_result(p.gelu ? gelu_for<T>(v) : v));
     }
   }
 }
 
-// Many rows. A workgroup of four waves takes TM x TN of out, a wave a quarter of it, in steps of 128 along k: rows of 64 bytes
-// of both matrices go straight to LDS (buffer loads, of which those past a matrix's or row's end bring zeros), NB steps'
-// worth, and come to the matrix units one 16-byte block a lane. 16-byte chunk c of row r lies at c ^ (r / 4 % 4), so that the
-// 16 rows of which a read takes a chunk each fall on all 64 banks alike. Scales travel beside them: a dword with a row's
-// four where those are aligned to it (k % 128 == 0), else a byte a load.
-template <typename T, int TM, int TN, int NB, bool ALIGNED, bool GELU>
-__global__ __launch_bounds__(256) void mx_product_kernel(MxProduct p, int mt, int nt) {
-  constexpr int ROWS = TM + TN, CB = ROWS * 64, SB = ROWS * (ALIGNED ? 4 : 16), BUF = CB + SB;
-  constexpr int FM = TM / 64, FN = TN / 64, NC = ROWS / 64, NS = (ROWS + 255) / 256 * (ALIGNED ? 1 : 4), VM = NC + NS;
+// Many rows. A workgroup of WM x WN waves takes TM x TN of out in steps of 256 along k: rows of 128 bytes, whole cache lines,
+// of both matrices go straight to LDS (buffer loads, of which those past a matrix's or row's end bring zeros), the next
+// step's while this one is worked on, and come to the matrix units one 16-byte block a lane. 16-byte chunk c of row r lies at
+// c ^ (r / 2 % 8), so that the 16 rows of which a read takes a chunk each fall on all 64 banks alike. A row's scales come 16
+// bytes at a time, as the loads are bound by the cache lines that they touch: those of two steps where rows of scales are
+// whole dwords (k % 128 == 0), else of one step from the dword on in which they begin.
+template <typename T, int TM, int TN, int WM, int WN, bool ALIGNED, bool GELU>
+__global__ __launch_bounds__(64 * WM * WN) void mx_product_kernel(MxProduct p, int mt, int nt) {
+  constexpr int NW = WM * WN, ROWS = TM + TN, CB = ROWS * 128, SB = ROWS * 16;
+  constexpr int FM = TM / WM / 32, FN = TN / WN / 32, NC = ROWS / 8 / NW, NG = (ROWS / 64 + NW - 1) / NW;
+  static_assert(ROWS % (16 * NW) == 0, "shares of a step");
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const unsigned lds0 = lds_addr(smem);
+  const unsigned lds0 = lds_addr(smem), lds1 = lds0 + 2 * CB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroup i runs on XCD i % 8: neighbours in out, which share rows, on the same one
+  // Workgroup i runs on XCD i % 8, whose share of the tiles lies together in bands of GROUP rows of tiles, so that what runs
+  // there at once is a block of tiles that share rows of both matrices in its L2
+  constexpr int GROUP = 8;
   const int tiles = mt * nt, share = (tiles + 7) / 8, lin = (int)(blockIdx.x % 8) * share + (int)(blockIdx.x / 8);
   if (lin >= tiles) return;
-  const int m0 = lin / nt * TM, n0 = lin % nt * TN;
-  const int G = p.k / 32, steps = (p.k + 127) / 128;
+  const int band = lin / (GROUP * nt), rows = min(GROUP, mt - band * GROUP), in = lin - band * GROUP * nt;
+  const int m0 = (band * GROUP + in % rows) * TM, n0 = in / rows * TN;
+  const int G = p.k / 32, steps = (p.k + 255) / 256;
   const unsigned rb = (unsigned)p.k / 2;  // bytes of a row's codes
   const int mr = min(TM, p.m - m0), nr = min(TN, p.n - n0);
   // rows 0 .. TN - 1 of a step are B's, the others A's
   const i32x4 rsb = buffer_rsrc(p.b + (long)n0 * rb, nr * rb), rsa = buffer_rsrc(p.a + (long)m0 * rb, mr * rb);
-  const i32x4 rssb = buffer_rsrc(p.sb + (long)n0 * G, nr * G), rssa = buffer_rsrc(p.sa + (long)m0 * G, mr * G);
-  const int chunk = (lane & 3) ^ (lane >> 4);  // of this lane's row
-  auto stage = [&](int t, int buf) {
-    const unsigned to = lds0 + buf * BUF;
-    const unsigned none = ALIGNED || 4 * t + chunk < G ? 0u : 0x80000000u;  // past the row's end: out of the buffer's range
+  // scales in whole dwords: from the one in which the tile's begin to the one in which they end
+  const unsigned long sbp = (unsigned long)(p.sb + (long)n0 * G), sap = (unsigned long)(p.sa + (long)m0 * G);
+  const unsigned sbo = (unsigned)sbp & 3, sao = (unsigned)sap & 3;
+  const i32x4 rssb = buffer_rsrc((const void*)(sbp - sbo), (nr * G + sbo + 3) & ~3u);
+  const i32x4 rssa = buffer_rsrc((const void*)(sap - sao), (mr * G + sao + 3) & ~3u);
+  auto stage = [&](int t) {
+    const unsigned to = lds0 + (t & 1) * CB;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int r0 = 16 * (wave + 4 * i);
+      const int r0 = 8 * (wave + NW * i);
       const bool of_b = r0 < TN;
-      const unsigned off = (unsigned)((of_b ? r0 : r0 - TN) + lane / 4) * rb + 64 * t + 16 * chunk;
-      bdma16(of_b ? rsb : rsa, off | none, to + r0 * 64);
+      const int chunk = (lane & 7) ^ (lane >> 4) ^ (r0 >> 1 & 4);  // of this lane's row, r0 + lane / 8
+      const unsigned off = (unsigned)((of_b ? r0 : r0 - TN) + lane / 8) * rb + 128 * t + 16 * chunk;
+      bdma16(of_b ? rsb : rsa, 8 * t + chunk < G ? off : 0x80000000u, to + r0 * 128);  // past the row's end: out of range
     }
+    if (ALIGNED && t % 2) return;
 #pragma unroll
-    for (int i = 0; i < NS / (ALIGNED ? 1 : 4); ++i) {
-      const int r0 = (64 * (wave + 4 * i)) % ROWS;  // waves past the last row bring the first ones again
+    for (int i = 0; i < NG; ++i) {
+      const int r0 = (64 * (wave + NW * i)) % ROWS;  // waves past the last row bring the first ones again
       const bool of_b = r0 < TN;
-      const unsigned off = (unsigned)((of_b ? r0 : r0 - TN) + lane) * (unsigned)G + 4 * t;
-      if constexpr (ALIGNED) {
-        bdma4(of_b ? rssb : rssa, off, to + CB + r0 * 4);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          bdma1(of_b ? rssb : rssa, (off + c) | (4 * t + c < G ? 0u : 0x80000000u), to + CB + (c * ROWS + r0) * 4);
-      }
+      const unsigned off = (unsigned)((of_b ? r0 : r0 - TN) + lane) * (unsigned)G + 8 * t + (of_b ? sbo : sao);
+      bdma16(of_b ? rssb : rssa, ALIGNED ? off : off & ~3u, lds1 + ((ALIGNED ? t >> 1 : t) & 1) * SB + r0 * 16);
     }
   };
-  const int wm = wave & 1, wn = wave >> 1, r = lane & 31, hh = lane >> 5;
+  const int wm = wave % WM, wn = wave / WM, r = lane & 31, hh = lane >> 5;
+  typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
   typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-  typedef __attribute__((address_space(3))) unsigned lds_u32;
-  const int brow = wn * (TN / 2) + r, arow = TN + wm * (TM / 2) + r;
-  const unsigned swz = 16 * (hh ^ (r >> 2 & 3));
+  const int brow = wn * (TN / WN) + r, arow = TN + wm * (TM / WM) + r;
+  const unsigned swz = 16 * (hh ^ (r >> 1 & 7));
   f32x16 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x16{};
-#pragma unroll
-  for (int t = 0; t < NB - 1; ++t) stage(min(t, steps - 1), t);
-  for (int t = 0, buf = 0; t < steps; ++t) {
-    wait_vm<VM * (NB - 2)>();  // this step's loads, NB - 2 later ones in flight
+  stage(0);
+  for (int t = 0; t < steps; ++t) {
+    wait_vm<0>();
     __syncthreads();
-    // after the last step its loads again, into a buffer that nothing reads: the count above stays what it is
-    stage(min(t + NB - 1, steps - 1), buf == 0 ? NB - 1 : buf - 1);
-    const unsigned at = lds0 + buf * BUF;
-    unsigned sb[FN][2], sa[FM][2];
-    auto scales_of = [&](int row, unsigned* s) {
+    if (t + 1 < steps) stage(t + 1);
+    const unsigned at = lds0 + (t & 1) * CB, sat = lds1 + ((ALIGNED ? t >> 1 : t) & 1) * SB;
+    // a row's eight scales, those past its end as 2^-127: what came there is another row's, which may be NaN. Then moved so
+    // that bytes 0 and 2 of a dword are the lane's.
+    const int left = G - 8 * t;
+    const unsigned keep[2] = {left >= 4 ? ~0u : (1u << 8 * left) - 1, left >= 8 ? ~0u : left <= 4 ? 0u : (1u << (8 * left - 32)) - 1};
+    auto scales_of = [&](int row, unsigned shift) {
+      u32x2 s;
       if constexpr (ALIGNED) {
-        s[0] = *(const lds_u32*)(size_t)(at + CB + 4 * row) >> (8 * hh);  // bytes 0 and 2: the blocks of the two halves
+        s = *(const lds_u32x2*)(size_t)(sat + 16 * row + 8 * (t & 1));
       } else {
-        s[0] = *(const lds_u32*)(size_t)(at + CB + 4 * (hh * ROWS + row));
-        s[1] = *(const lds_u32*)(size_t)(at + CB + 4 * ((2 + hh) * ROWS + row));
+        const u32x4 w = *(const lds_u32x4*)(size_t)(sat + 16 * row);
+        s = u32x2{__builtin_amdgcn_alignbyte(w[1], w[0], shift), __builtin_amdgcn_alignbyte(w[2], w[1], shift)};
       }
+      return u32x2{(s[0] & keep[0]) >> (8 * hh), (s[1] & keep[1]) >> (8 * hh)};
     };
+    u32x2 sb[FN], sa[FM];
 #pragma unroll
-    for (int j = 0; j < FN; ++j) scales_of(brow + 32 * j, sb[j]);
+    for (int j = 0; j < FN; ++j) sb[j] = scales_of(brow + 32 * j, ((unsigned)(brow + 32 * j) * (unsigned)G + sbo) & 3);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) scales_of(arow + 32 * i, sa[i]);
+    for (int i = 0; i < FM; ++i) sa[i] = scales_of(arow + 32 * i, ((unsigned)(arow - TN + 32 * i) * (unsigned)G + sao) & 3);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int q = 0; q < 4; ++q) {  // 64 along k
       u32x4 b[FN], a[FM];
 #pragma unroll
-      for (int j = 0; j < FN; ++j) b[j] = *(const lds_u32x4*)(size_t)(at + 64 * (brow + 32 * j) + (swz ^ 32 * h));
+      for (int j = 0; j < FN; ++j) b[j] = *(const lds_u32x4*)(size_t)(at + 128 * (brow + 32 * j) + (swz ^ 32 * q));
 #pragma unroll
-      for (int i = 0; i < FM; ++i) a[i] = *(const lds_u32x4*)(size_t)(at + 64 * (arow + 32 * i) + (swz ^ 32 * h));
+      for (int i = 0; i < FM; ++i) a[i] = *(const lds_u32x4*)(size_t)(at + 128 * (arow + 32 * i) + (swz ^ 32 * q));
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          if constexpr (ALIGNED)
-            acc[i][j] = h ? mma_mx32<2>(b[j], sb[j][0], a[i], sa[i][0], acc[i][j]) : mma_mx32<0>(b[j], sb[j][0], a[i], sa[i][0], acc[i][j]);
-          else
-            acc[i][j] = mma_mx32<0>(b[j], sb[j][h], a[i], sa[i][h], acc[i][j]);
-        }
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = q % 2 ? mma_mx32<2>(b[j], sb[j][q / 2], a[i], sa[i][q / 2], acc[i][j])
+                            : mma_mx32<0>(b[j], sb[j][q / 2], a[i], sa[i][q / 2], acc[i][j]);
     }
-    buf = buf + 1 == NB ? 0 : buf + 1;
   }
-  wait_vm<0>();  // nothing may land in the LDS that the results pass through
   __syncthreads();
   // A wave's results go through LDS, 32 rows at a time, so that a row's columns leave together: in f32, 16-byte chunk c of
   // row r at c ^ (r % CH), then V columns a lane with their bias and activation.
-  constexpr int COLS = TN / 2, CH = COLS / 4, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR;
+  constexpr int COLS = TN / WN, CH = COLS / 4, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR;
   const unsigned own = lds0 + wave * (32 * COLS * 4);
   const int n = n0 + wn * COLS + V * (lane % LPR);
   const T* bias = reinterpret_cast<const T*>(p.bias);
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(256) void mx_product_kernel(MxProduct p, int mt, in
             f32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
 #pragma unroll
     for (int k = 0; k < 32 / RPP; ++k) {
-      const int row = RPP * k + lane / LPR, m = m0 + wm * (TM / 2) + 32 * i + row;
+      const int row = RPP * k + lane / LPR, m = m0 + wm * (TM / WM) + 32 * i + row;
       T y[V];
 #pragma unroll
       for (int c = 0; c < V / 4; ++c) {
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(256) void mx_product_kernel(MxProduct p, int mt, in
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const float z = x[v] + add[4 * c + v];
-          y[4 * c + v] = from_f32<T>(f32_result(GELU ? gelu_erf(z) : z));
+          y[4 * c + v] = from_f32<T>(f32_result(GELU ? gelu_for<T>(z) : z));
         }
       }
       T* to = reinterpret_cast<T*>(p.out) + (long)m * p.n + n;
@@ -251,21 +253,22 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
   }
 }
 
-template <typename T, int TM, int TN, int NB, bool ALIGNED, bool GELU> hipError_t launch_product(const MxProduct& p, hipStream_t stream) {
-  constexpr int lds = NB * (TM + TN) * (64 + (ALIGNED ? 4 : 16));
-  static_assert(lds >= 4 * 32 * (TN / 2) * 4, "the results' way out");
-  auto kern = mx_product_kernel<T, TM, TN, NB, ALIGNED, GELU>;
+template <typename T, int TM, int TN, int WM, int WN, bool ALIGNED, bool GELU>
+hipError_t launch_product(const MxProduct& p, hipStream_t stream) {
+  constexpr int lds = 2 * (TM + TN) * (128 + 16);
+  static_assert(lds >= WM * WN * 32 * (TN / WN) * 4, "the results' way out");
+  auto kern = mx_product_kernel<T, TM, TN, WM, WN, ALIGNED, GELU>;
   static std::atomic<unsigned long long> done;
   if (const hipError_t e = lds_opt_in(done, (const void*)kern, lds); e != hipSuccess) return e;
   const int mt = (p.m + TM - 1) / TM, nt = (p.n + TN - 1) / TN;
   const long grid = ((long)mt * nt + 7) / 8 * 8;
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, p, mt, nt);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * WM * WN), lds, stream, p, mt, nt);
   return hipGetLastError();
 }
-template <typename T, int TM, int TN, int NB> hipError_t by_alignment(const MxProduct& p, hipStream_t stream) {
+template <typename T, int TM, int TN, int WM, int WN> hipError_t by_alignment(const MxProduct& p, hipStream_t stream) {
   if (p.k % 128 == 0 && reinterpret_cast<uintptr_t>(p.sa) % 4 == 0 && reinterpret_cast<uintptr_t>(p.sb) % 4 == 0)
-    return p.gelu ? launch_product<T, TM, TN, NB, true, true>(p, stream) : launch_product<T, TM, TN, NB, true, false>(p, stream);
-  return p.gelu ? launch_product<T, TM, TN, NB, false, true>(p, stream) : launch_product<T, TM, TN, NB, false, false>(p, stream);
+    return p.gelu ? launch_product<T, TM, TN, WM, WN, true, true>(p, stream) : launch_product<T, TM, TN, WM, WN, true, false>(p, stream);
+  return p.gelu ? launch_product<T, TM, TN, WM, WN, false, true>(p, stream) : launch_product<T, TM, TN, WM, WN, false, false>(p, stream);
 }
 
 template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream) {
@@ -278,8 +281,18 @@ template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream)
       hipLaunchKernelGGL((mx_few_kernel<T, 2>), grid, dim3(64 * waves), 0, stream, p);
     return hipGetLastError();
   }
-  const long wide = (long)((p.m + 127) / 128) * ((p.n + 127) / 128);
-  return wide >= 192 ? by_alignment<T, 128, 128, 4>(p, stream) : by_alignment<T, 64, 64, 4>(p, stream);
+  // The tiles that take least: so many a CU, each its steps and its beginning and end, in ns (what a CU's tiles cost together,
+  // as one's waits are another's work). Kernel times in f16 by tiles of 64, 128 and 256: 300 x 1280 of k = 5120 10.7 and 16.7 us,
+  // 4096 x 1280 of 1280 13.4 and 11.4, 4096 x 1280 of 5120 34, 27 and 38, 4096 x 3840 of 1280 30, 22 and 19, 4096 x 5120 of 1280
+  // 28 and 32 (128, 256), 16001 x 1024 of 4096 49 and 40, 16384 x 4096 of 4096 184 and 156.
+  const long cus = device_cu_count(), steps = (p.k + 255) / 256;
+  auto cost = [&](long tile, long step, long ends) {
+    const long tiles = (p.m + tile - 1) / tile * ((p.n + tile - 1) / tile);
+    return (tiles + cus - 1) / cus * (steps * step + ends);
+  };
+  const long large = cost(256, 2100, 5000), middle = cost(128, 670, 2300), small = cost(64, 360, 500);
+  if (large < middle && large < small) return by_alignment<T, 256, 256, 2, 4>(p, stream);
+  return middle < small ? by_alignment<T, 128, 128, 2, 2>(p, stream) : by_alignment<T, 64, 64, 2, 2>(p, stream);
 }
 
 }  // namespace

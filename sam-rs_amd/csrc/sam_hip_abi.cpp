@@ -931,6 +931,17 @@ int sam_hip_kv_append(const void* q, const void* k, const void* v, const int* po
 
 namespace {
 
+int check_mx_product(const char* what, int dtype, int m, int n, int k) {
+  if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
+  if (m < 0 || n < 0 || k <= 0 || k % samhip::kMxBlock != 0)
+    return fail(SAM_HIP_EINVAL, "%s: sizes m=%d n=%d k=%d (k a positive multiple of 32)", what, m, n, k);
+  // the launches count workgroups of up to 1024 threads for 16 columns, or of 256 for 128 x 128 results, in 32 bits of threads
+  if ((long)m * n >= 1L << 36 || m > (1 << 30) || n > (1 << 25) || k > 1 << 22 ||
+      ((long)m + 127) / 128 * (((long)n + 127) / 128) >= 1L << 23)
+    return fail(SAM_HIP_EUNSUPPORTED, "%s: too many results, or k beyond 2^22 (m=%d n=%d k=%d)", what, m, n, k);
+  return SAM_HIP_OK;
+}
+
 int check_mx_rows(const char* what, int dtype, long rows, int k) {
   if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
   if (rows < 0 || k <= 0 || k % samhip::kMxBlock != 0)
@@ -966,17 +977,36 @@ int sam_hip_mx_matmul(const unsigned char* a, const unsigned char* a_scale, cons
                       void* stream) {
   SAM_HIP_REQUIRE_ENABLED("mx-matmul");
   if (!a || !a_scale || !b || !b_scale || !out) return fail(SAM_HIP_EINVAL, "mx-matmul: null pointer argument");
-  if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
-  if (m < 0 || n < 0 || k <= 0 || k % samhip::kMxBlock != 0)
-    return fail(SAM_HIP_EINVAL, "mx-matmul: sizes m=%d n=%d k=%d (k a positive multiple of 32)", m, n, k);
-  // the launches count workgroups of up to 1024 threads for 16 columns, or of 256 for 128 x 128 results, in 32 bits of threads
-  if ((long)m * n >= 1L << 36 || m > (1 << 30) || n > (1 << 25) || k > 1 << 22 ||
-      ((long)m + 127) / 128 * (((long)n + 127) / 128) >= 1L << 23)
-    return fail(SAM_HIP_EUNSUPPORTED, "mx-matmul: too many results, or k beyond 2^22 (m=%d n=%d k=%d)", m, n, k);
+  if (int rc = check_mx_product("mx-matmul", dtype, m, n, k); rc != SAM_HIP_OK) return rc;
   if (!aligned16(a) || !aligned16(b) || !aligned16(bias) || !aligned16(out))
     return fail(SAM_HIP_EUNSUPPORTED, "mx-matmul: a, b, bias and out must be 16-byte aligned");
   const samhip::MxProduct p = {a, a_scale, b, b_scale, bias, out, m, n, k, gelu != 0};
   return check_launch(samhip::mx_matmul(dtype, p, reinterpret_cast<hipStream_t>(stream)), "mx-matmul");
+}
+
+long sam_hip_mx_linear_workspace_size(int m, int k) {
+  if (check_mx_rows("mx-linear", samhip::kF16, m, k) != SAM_HIP_OK) return -1;
+  return (long)m * (k / 2) + (long)m * (k / 32);
+}
+
+int sam_hip_mx_linear(const void* x, const unsigned char* w, const unsigned char* w_scale, const void* bias, void* out,
+                      int dtype, int m, int n, int k, int gelu, void* workspace, long workspace_bytes, void* stream) {
+  SAM_HIP_REQUIRE_ENABLED("mx-linear");
+  if (!x || !w || !w_scale || !out) return fail(SAM_HIP_EINVAL, "mx-linear: null pointer argument");
+  if (int rc = check_mx_product("mx-linear", dtype, m, n, k); rc != SAM_HIP_OK) return rc;
+  if (int rc = check_mx_rows("mx-linear", dtype, m, k); rc != SAM_HIP_OK) return rc;
+  if (!aligned16(x) || !aligned16(w) || !aligned16(bias) || !aligned16(out) || !aligned16(workspace))
+    return fail(SAM_HIP_EUNSUPPORTED, "mx-linear: x, w, bias, out and the workspace must be 16-byte aligned");
+  if (m == 0 || n == 0) return ok();
+  const long codes = (long)m * (k / 2), need = codes + (long)m * (k / 32);
+  if (!workspace || workspace_bytes < need)
+    return fail(SAM_HIP_EINVAL, "mx-linear: workspace of %ld bytes needed, got %ld", need, workspace ? workspace_bytes : 0L);
+  unsigned char* a = reinterpret_cast<unsigned char*>(workspace);
+  const samhip::MxProduct p = {a, a + codes, w, w_scale, bias, out, m, n, k, gelu != 0};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipError_t e = samhip::mx_pack(dtype, x, a, a + codes, (long)m * (k / 32), s);
+  if (e == hipSuccess) e = samhip::mx_matmul(dtype, p, s);
+  return check_launch(e, "mx-linear");
 }
 
 }  // extern "C"

@@ -126,6 +126,10 @@ def load():
         L.sam_hip_mx_unpack.restype = _i
         L.sam_hip_mx_matmul.argtypes = [_vp] * 6 + [_i] * 5 + [_vp]
         L.sam_hip_mx_matmul.restype = _i
+        L.sam_hip_mx_linear_workspace_size.argtypes = [_i, _i]
+        L.sam_hip_mx_linear_workspace_size.restype = ctypes.c_long
+        L.sam_hip_mx_linear.argtypes = [_vp] * 5 + [_i] * 5 + [_vp, ctypes.c_long, _vp]
+        L.sam_hip_mx_linear.restype = _i
         L.sam_hip_set_enabled.argtypes = [_i]
         L.sam_hip_set_enabled.restype = None
         L.sam_hip_enabled.argtypes = []
@@ -1108,5 +1112,33 @@ def mx_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: tor
               gelu: bool = False) -> torch.Tensor:
     """A linear layer with 4-bit weights w, w_scale (mx_pack of [N, K]) on x [.., K], which it packs likewise:
     act(x w^T + bias) -> [.., N] in x's dtype, bias's too; act is the identity or, with gelu, the exact GELU."""
-    codes, scale = mx_pack(x)
-    return mx_matmul(codes, scale, w, w_scale, bias, gelu, x.dtype)
+    dev = _device_of("mx_linear", x, w, w_scale, bias)
+    if not _is_current(dev):
+        with torch.cuda.device(dev):
+            return mx_linear(x, w, w_scale, bias, gelu)
+    dt = _dtype(x)
+    shape = x.shape
+    k = _mx_k("mx_linear", shape)
+    w, w_scale, of = _mx_operand("mx_linear", "w", w, w_scale)
+    if len(of) != 2 or of[1] != k:
+        raise SamHipError(f"mx_linear: w must be [N, {k}], got {tuple(of)}")
+    n = of[0]
+    if bias is not None:
+        if bias.dtype != x.dtype or bias.shape != (n,):
+            raise SamHipError(f"mx_linear: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
+        bias, = _aligned16(_plain(bias))
+    x = _plain(x)
+    if x.data_ptr() % 16:
+        x = x.clone()
+    out = x.new_empty(shape[:-1] + (n,))
+    if out.numel() == 0:
+        _empty_call("mx-linear")
+        return out
+    m = out.numel() // n
+    if (m | n) >> 31:
+        _sizes("mx_linear", m, n)
+    ws_bytes = m * (k // 2) + m * (k // _BLOCK)
+    ws = x.new_empty(-(-ws_bytes // x.element_size()))
+    _check(load().sam_hip_mx_linear(x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), _ptr(bias), out.data_ptr(), dt, m, n, k,
+                                    bool(gelu), ws.data_ptr(), ws_bytes, _stream()))
+    return out

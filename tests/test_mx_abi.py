@@ -33,6 +33,24 @@ def matmul(lib, a=FAKE, sa=FAKE, b=FAKE, sb=FAKE, bias=None, out=FAKE, dtype=1, 
     return lib.sam_hip_mx_matmul(a, sa, b, sb, bias, out, dtype, m, n, k, gelu, None)
 
 
+def linear(lib, x=FAKE, w=FAKE, sw=FAKE, bias=None, out=FAKE, dtype=1, m=4, n=4, k=64, ws=FAKE, ws_bytes=1 << 20):
+    return lib.sam_hip_mx_linear(x, w, sw, bias, out, dtype, m, n, k, 0, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("change, code", [
+    ({"x": None}, 1), ({"w": None}, 1), ({"sw": None}, 1), ({"out": None}, 1), ({"dtype": 3}, 2), ({"m": -1}, 1), ({"n": -1}, 1),
+    ({"k": 40}, 1), ({"k": (1 << 22) + 32}, 3), ({"m": 1 << 15, "k": 1 << 22, "n": 1}, 3), ({"x": vp(0x1008)}, 3), ({"w": vp(0x1008)}, 3),
+    ({"ws": None}, 1), ({"ws": vp(0x1008)}, 3), ({"ws_bytes": 4 * 34 - 1}, 1), ({"bias": vp(0x1008)}, 3), ({"out": vp(0x1008)}, 3)])
+def test_linear_refuses(lib, change, code):
+    assert linear(lib, **change) == code
+    assert lib.sam_hip_last_error()
+
+
+def test_linear_workspace(lib):
+    size = lib.sam_hip_mx_linear_workspace_size
+    assert size(4, 64) == 4 * 34 and size(0, 64) == 0 and size(3, 48) == size(-1, 64) == -1 and linear(lib, m=0) == 0
+
+
 @pytest.mark.parametrize("call", [pack, unpack])
 @pytest.mark.parametrize("change, code", [
     ({"x": None}, 1), ({"codes": None}, 1), ({"scales": None}, 1), ({"dtype": 3}, 2), ({"dtype": -1}, 2), ({"rows": -1}, 1),
@@ -55,14 +73,14 @@ def test_matmul_refuses(lib, change, code):
 def test_the_header_declares_what_the_library_exports(lib):
     text = open(os.path.join(os.path.dirname(__file__), "..", "include", "sam_hip_mx.h")).read()
     names = set(re.findall(r"\b(sam_hip_\w+)\s*\(", re.sub(r"/\*.*?\*/", "", text, flags=re.S)))
-    assert names == {"sam_hip_mx_pack", "sam_hip_mx_unpack", "sam_hip_mx_matmul"}
+    assert names == {"sam_hip_mx_pack", "sam_hip_mx_unpack", "sam_hip_mx_matmul", "sam_hip_mx_linear", "sam_hip_mx_linear_workspace_size"}
     assert all(hasattr(lib, n) for n in names)
 
 
 def test_the_switch_covers_them(lib):
     lib.sam_hip_set_enabled(0)
     try:
-        assert pack(lib, x=None) == unpack(lib, x=None) == matmul(lib, a=None) == 5
+        assert pack(lib, x=None) == unpack(lib, x=None) == matmul(lib, a=None) == linear(lib, x=None) == 5
     finally:
         lib.sam_hip_set_enabled(1)
 
