@@ -6,8 +6,8 @@
 // Keys are turned in f64 and rounded once, to their type or to their codes, so that a code is the definition's also next to
 // the border between two (an f32 turn, off by 2^-22, would flip one of a million). The angle is the f64 product; it is reduced
 // by quarter turns with pi / 2 in two parts (exact to 2^-52 up to 2^48 radians), sine and cosine are Taylor sums on an eighth
-// of a turn either way, whose first terms left out are below 2^-56. Queries, which go out in their own type, take the angle's
-// sine and cosine in f32.
+// of a turn either way, whose first terms left out are below 2^-56. Queries, which go out in their own type, take sine
+// and cosine in f32, from the angle so reduced.
 //
 // What bounds it: HBM bytes, each row in and out once. A row belongs to LPR lanes of 8 columns, as in kv_cache.hip; they form
 // their angles once for HP heads of a token. In the halves layout a lane loads its partners' columns too (their lines are on
@@ -39,11 +39,24 @@ struct KvAppendParams {
   unsigned kblocks;                           // workgroups for keys and values; the queries' follow
 };
 
+// a less the nearest k quarter turns.
+__device__ __forceinline__ double reduced(double a, double& k) {
+  k = rint(a * 0.63661977236758134308);
+  // pi / 2 as a double, whose product with k fma takes exactly, and what it lacks
+  return fma(-k, 6.12323399573676588613e-17, fma(-k, 1.57079632679489661923, a));
+}
+// (c, s) after k quarter turns: (c, s) -> (-s, c) each.
+template <typename F> __device__ __forceinline__ void quarters(double k, F& c, F& s) {
+  const int quarter = (int)(long)k & 3;
+  const F u = quarter & 1 ? -s : c, w = quarter & 1 ? c : s;
+  c = quarter & 2 ? -u : u;
+  s = quarter & 2 ? -w : w;
+}
+
 // cos and sin of a.
 __device__ __forceinline__ void turn_of(double a, double& c, double& s) {
-  const double k = rint(a * 0.63661977236758134308);  // quarter turns
-  double r = fma(-k, 1.57079632679489661923, a);      // pi / 2 as a double, whose product with k fma takes exactly,
-  r = fma(-k, 6.12323399573676588613e-17, r);         // and what it lacks
+  double k;
+  const double r = reduced(a, k);
   const double r2 = r * r;
   double sn = 1.0 / 355687428096000.0, cs = -1.0 / 6402373705728000.0;  // 1 / 17!, -1 / 18!
   sn = fma(sn, r2, -1.0 / 1307674368000.0);
@@ -63,10 +76,16 @@ __device__ __forceinline__ void turn_of(double a, double& c, double& s) {
   sn = fma(sn * r2, r, r);
   cs = fma(cs, r2, -0.5);
   cs = fma(cs, r2, 1.0);
-  const int quarter = (int)(long)k & 3;  // (c, s) -> (-s, c) each
-  const double u = quarter & 1 ? -sn : cs, w = quarter & 1 ? cs : sn;
-  c = quarter & 2 ? -u : u;
-  s = quarter & 2 ? -w : w;
+  c = cs;
+  s = sn;
+  quarters(k, c, s);
+}
+__device__ __forceinline__ void turn_of(double a, float& c, float& s) {
+  double k;
+  const float y = (float)reduced(a, k), y2 = y * y;
+  s = y + y * y2 * (-1.f / 6 + y2 * (1.f / 120 + y2 * (-1.f / 5040 + y2 * (1.f / 362880))));
+  c = 1.f + y2 * (-0.5f + y2 * (1.f / 24 + y2 * (-1.f / 720 + y2 * (1.f / 40320 - y2 * (1.f / 3628800)))));
+  quarters(k, c, s);
 }
 
 // x in f32, rounded to odd: cut short, and its last bit set if anything was cut off. Rounding that to fewer bits (up to 22)
@@ -106,6 +125,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
   const bool even = p.pairs % 8 == 0;  // halves: a lane's elements have one role
   const bool low = col < p.pairs;
 
+  // Everything that depends on nothing goes out at once, the ends and lengths of the first 64 sequences first, one to a lane:
+  // the way from them to the pages is the longest
+  const int lane = threadIdx.x & 63;
+  const int seq = min(lane, p.c.batch - 1), ends = p.c.starts[seq + 1], held = p.c.lens[seq], first = p.c.starts[0];
   Eight<T> x[HP], o[HALVES ? HP : 1], v[HP];
   auto load_rows = [&](const void* base, const long* st, Eight<T>* a, bool partners) {
 #pragma unroll
@@ -129,60 +152,68 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
       }
     }
   };
-  if (keys) {
-    load_rows(p.k, p.sk, x, true);
-    load_rows(p.v, p.sv, v, false);
-  } else {
-    load_rows(p.q, p.sq, x, true);
-  }
-
-  // the token's sequence and position
-  const int b = sequence_of<LPR>(p.c, t);
-  const bool known = b < p.c.batch && t >= p.c.starts[min(b, p.c.batch - 1)] && t < p.c.starts[min(b, p.c.batch - 1) + 1];
-  long at = 0;
-  if (known) at = (long)p.c.lens[b] - p.c.starts[b + 1] + t;
-
-  double c[NP], s[NP];
+  load_rows(keys ? p.k : p.q, keys ? p.sk : p.sq, x, true);
+  if (keys) load_rows(p.v, p.sv, v, false);
+  double freq[NP];
+  int axis[NP];
+  i32x4 ps = {};  // up to four axes' positions, loaded before it is known which of them the pairs want
+  const int* pr = p.pos + (long)t * p.sp[0];
   if (p.pairs > 0) {
-    i32x4 ps = {};  // up to four axes' positions, loaded before it is known which of them the pairs want
-    const int* pr = p.pos + (long)t * p.sp[0];
-    if (p.pos && p.naxes <= 4) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a) ps[a] = pr[min(a, p.naxes - 1) * p.sp[1]];
-    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       int i = HALVES ? col + j : col / 2 + j;
       if (HALVES && i >= p.pairs) i -= p.pairs;
       i = min(i, p.pairs - 1);
-      const double f = p.freqs[i];
-      double where = (double)at;
-      if (p.pos) {
-        const int ax = p.axes[i];
-        int w = 0;
-        if ((unsigned)ax < (unsigned)p.naxes) {
-          if (p.naxes <= 4) {
-            const int lo = ax & 1 ? ps.y : ps.x, hi = ax & 1 ? ps.w : ps.z;
-            w = ax & 2 ? hi : lo;
-          } else {
-            w = pr[ax * p.sp[1]];
-          }
-        }
-        where = (double)w;
-      }
-      turn_of(where * f, c[j], s[j]);
+      freq[j] = p.freqs[i];
+      axis[j] = p.pos ? p.axes[i] : 0;
     }
-  } else {
+    if (p.pos && p.naxes <= 4) {
 #pragma unroll
-    for (int j = 0; j < NP; ++j) c[j] = 1.0, s[j] = 0.0;
+      for (int a = 0; a < 4; ++a) ps[a] = pr[min(a, p.naxes - 1) * p.sp[1]];
+    }
   }
+
+  // the token's sequence and position
+  const int b = sequence_of<LPR>(p.c, t, lane < p.c.batch ? ends : 0x7fffffff);
+  int from, to, len;
+  if (p.c.batch <= 64) {
+    from = b > 0 ? __shfl(ends, min(b, p.c.batch) - 1) : first;
+    to = __shfl(ends, min(b, p.c.batch - 1));
+    len = __shfl(held, min(b, p.c.batch - 1));
+  } else {
+    const int at = min(b, p.c.batch - 1);
+    from = p.c.starts[at], to = p.c.starts[at + 1], len = p.c.lens[at];
+  }
+  const bool known = b < p.c.batch && t >= from && t < to;
+  const long at = known ? (long)len - to + t : 0;
+  const long end = (long)p.c.width * p.c.page;
+  const bool fits = keys && r < units && known && at >= 0 && at < end;
+  PagedEntry entry = {-1, -1};
+  if (fits) entry = paged_entry(p.c, b, (int)at, (int)end);
+
+  auto angle = [&](int j) {
+    if (!p.pos) return (double)at * freq[j];
+    int w = 0;
+    if ((unsigned)axis[j] < (unsigned)p.naxes) {
+      if (p.naxes <= 4) {
+        const int lo = axis[j] & 1 ? ps.y : ps.x, hi = axis[j] & 1 ? ps.w : ps.z;
+        w = axis[j] & 2 ? hi : lo;
+      } else {
+        w = pr[axis[j] * p.sp[1]];
+      }
+    }
+    return (double)w * freq[j];
+  };
 
   if (!keys) {
     const bool rest = !known;
     if (!inside || (rest && !p.zero_rest)) return;
-    float cf[NP], sf[NP];
+    float c[NP], s[NP];
 #pragma unroll
-    for (int j = 0; j < NP; ++j) cf[j] = (float)c[j], sf[j] = (float)s[j];
+    for (int j = 0; j < NP; ++j) {
+      c[j] = 1.f, s[j] = 0.f;
+      if (p.pairs > 0) turn_of(angle(j), c[j], s[j]);
+    }
 #pragma unroll
     for (int i = 0; i < HP; ++i) {
       const int h = hg + i * groups;
@@ -196,7 +227,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
       T* ye = reinterpret_cast<T*>(&y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float z = turned<float, HALVES>(j, xf, of, cf, sf, col + j < p.pairs);
+        const float z = turned<float, HALVES>(j, xf, of, c, s, col + j < p.pairs);
         ye[j] = rest ? from_f32<T>(0.f) : turn >> j & 1 ? from_f32<T>(f32_result(z)) : e[j];
       }
       store_eight(reinterpret_cast<T*>(p.out) + t * p.so[0] + h * p.so[1] + col, y);
@@ -204,10 +235,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
     return;
   }
 
-  const long end = (long)p.c.width * p.c.page;
-  const bool fits = r < units && known && at >= 0 && at < end;
-  PagedEntry entry = {-1, -1};
-  if (fits) entry = paged_entry(p.c, b, (int)at, (int)end);
+  double c[NP], s[NP];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    c[j] = 1.0, s[j] = 0.0;
+    if (p.pairs > 0) turn_of(angle(j), c[j], s[j]);
+  }
 #pragma unroll
   for (int i = 0; i < HP; ++i) {
     const int h = hg + i * groups;
@@ -229,16 +262,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
       y = Eight<float>{};
       v[i] = Eight<T>{};
     }
-    const long to = row * d + col;
+    const long place = row * d + col;
     if constexpr (__is_same(C, e2m1)) {
       unsigned ks, vs;
       const unsigned kc = mx_quantise(y, ks), vc = mx_quantise(v[i], vs);
       if (row >= 0 && inside) {
-        reinterpret_cast<unsigned*>(p.c.k)[to / 8] = kc;
-        reinterpret_cast<unsigned*>(p.c.v)[to / 8] = vc;
+        reinterpret_cast<unsigned*>(p.c.k)[place / 8] = kc;
+        reinterpret_cast<unsigned*>(p.c.v)[place / 8] = vc;
         if (col % kMxBlock == 0) {
-          p.c.ks[to / kMxBlock] = (unsigned char)ks;
-          p.c.vs[to / kMxBlock] = (unsigned char)vs;
+          p.c.ks[place / kMxBlock] = (unsigned char)ks;
+          p.c.vs[place / kMxBlock] = (unsigned char)vs;
         }
       }
     } else if constexpr (__is_same(C, e4m3)) {
@@ -247,8 +280,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
       quantise_row<float, LPR>(y, kc, ks);
       quantise_row<T, LPR>(v[i], vc, vs);
       if (row >= 0 && inside) {
-        *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.c.k) + to) = kc;
-        *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.c.v) + to) = vc;
+        *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.c.k) + place) = kc;
+        *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.c.v) + place) = vc;
         if (col == 0) {
           p.c.ks[row] = (unsigned char)(ks + 127);
           p.c.vs[row] = (unsigned char)(vs + 127);
@@ -259,8 +292,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
       T* he = reinterpret_cast<T*>(&held);
 #pragma unroll
       for (int j = 0; j < 8; ++j) he[j] = from_f32<T>(ye[j]);
-      store_eight(reinterpret_cast<T*>(p.c.k) + to, held);
-      store_eight(reinterpret_cast<T*>(p.c.v) + to, v[i]);
+      store_eight(reinterpret_cast<T*>(p.c.k) + place, held);
+      store_eight(reinterpret_cast<T*>(p.c.v) + place, v[i]);
     }
   }
 }

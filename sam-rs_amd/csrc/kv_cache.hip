@@ -74,7 +74,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteParams p) {
     k = load_eight(reinterpret_cast<const T*>(p.k) + t * p.sk[0] + head * p.sk[1] + col);
     v = load_eight(reinterpret_cast<const T*>(p.v) + t * p.sv[0] + head * p.sv[1] + col);
   }
-  const int b = sequence_of<LPR>(p.c, t);
+  const int lane = threadIdx.x & 63;
+  const int b = sequence_of<LPR>(p.c, t, lane < p.c.batch ? p.c.starts[lane + 1] : 0x7fffffff);
   long row = -1;  // 64 bits: row * d passes 32
   if (r < p.rows && b < p.c.batch && t >= p.c.starts[b] && t < p.c.starts[b + 1]) {
     const long j = (long)p.c.lens[b] - p.c.starts[b + 1] + t;  // its position: the last tokens of the sequence

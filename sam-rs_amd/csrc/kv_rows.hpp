@@ -79,21 +79,22 @@ template <typename T, int LPR> __device__ __forceinline__ void quantise_row(cons
   codes = codes_of(x, s, odd);
 }
 
-// The sequence of token t: how many sequences end at or before it. Every lane of the wave calls it; the starts come
-// 64 at a time, one to a lane, and each of the wave's tokens counts over them.
-template <int LPR> __device__ __forceinline__ int sequence_of(const PagedKv& c, int t) {
+// The sequence of token t: how many sequences end at or before it. Every lane of the wave calls it; the ends come 64 at a
+// time, one to a lane (0x7fffffff past the last; the first 64 from the caller), and each of the wave's tokens counts over them.
+template <int LPR> __device__ __forceinline__ int sequence_of(const PagedKv& c, int t, int end) {
   const int lane = threadIdx.x & 63;
   int n = 0;
-  for (int b0 = 0; b0 < c.batch; b0 += 64) {
-    const int end = b0 + lane < c.batch ? c.starts[b0 + lane + 1] : 0x7fffffff;
+  for (int b0 = 0;;) {
 #pragma unroll
     for (int r = 0; r < 64 / LPR; ++r) {
       const int tr = __builtin_amdgcn_readlane(t, r * LPR);
       const int ended = __popcll(__builtin_amdgcn_ballot_w64(end <= tr));
       n += lane / LPR == r ? ended : 0;
     }
+    b0 += 64;
+    if (b0 >= c.batch) return n;
+    end = b0 + lane < c.batch ? c.starts[b0 + lane + 1] : 0x7fffffff;
   }
-  return n;
 }
 
 }  // namespace samhip
