@@ -984,9 +984,10 @@ int sam_hip_mx_matmul(const unsigned char* a, const unsigned char* a_scale, cons
   return check_launch(samhip::mx_matmul(dtype, p, reinterpret_cast<hipStream_t>(stream)), "mx-matmul");
 }
 
-long sam_hip_mx_linear_workspace_size(int m, int k) {
+long sam_hip_mx_linear_workspace_size(int m, int n, int k) {
+  if (check_mx_product("mx-linear", samhip::kF16, m, n, k) != SAM_HIP_OK) return -1;
   if (check_mx_rows("mx-linear", samhip::kF16, m, k) != SAM_HIP_OK) return -1;
-  return (long)m * (k / 2) + (long)m * (k / 32);
+  return m == 0 || n == 0 || samhip::mx_packs_on_the_way(m, n, k) ? 0 : (long)m * (k / 2) + (long)m * (k / 32);
 }
 
 int sam_hip_mx_linear(const void* x, const unsigned char* w, const unsigned char* w_scale, const void* bias, void* out,
@@ -998,12 +999,16 @@ int sam_hip_mx_linear(const void* x, const unsigned char* w, const unsigned char
   if (!aligned16(x) || !aligned16(w) || !aligned16(bias) || !aligned16(out) || !aligned16(workspace))
     return fail(SAM_HIP_EUNSUPPORTED, "mx-linear: x, w, bias, out and the workspace must be 16-byte aligned");
   if (m == 0 || n == 0) return ok();
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (samhip::mx_packs_on_the_way(m, n, k)) {
+    const samhip::MxProduct p = {x, nullptr, w, w_scale, bias, out, m, n, k, gelu != 0};
+    return check_launch(samhip::mx_matmul(dtype, p, s), "mx-linear");
+  }
   const long codes = (long)m * (k / 2), need = codes + (long)m * (k / 32);
   if (!workspace || workspace_bytes < need)
     return fail(SAM_HIP_EINVAL, "mx-linear: workspace of %ld bytes needed, got %ld", need, workspace ? workspace_bytes : 0L);
   unsigned char* a = reinterpret_cast<unsigned char*>(workspace);
   const samhip::MxProduct p = {a, a + codes, w, w_scale, bias, out, m, n, k, gelu != 0};
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipError_t e = samhip::mx_pack(dtype, x, a, a + codes, (long)m * (k / 32), s);
   if (e == hipSuccess) e = samhip::mx_matmul(dtype, p, s);
   return check_launch(e, "mx-linear");

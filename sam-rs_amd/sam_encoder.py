@@ -11,7 +11,10 @@ GELU) and the neck. Per block, the reference's kernel calls map to:
   sam_hip.bias_residual;
 - bias_gelu (kernels.rs:1052) -> sam_hip.bias_gelu.
 
-The linears run as torch's F.linear (hipBLASLt) and LayerNorm as torch's layer_norm. Their weights
+pack_linears() holds the blocks' four linears in 4 bits (blocks of 32 e2m1 values under a power of two); they then run on
+sam_hip.mx_linear, which packs their inputs likewise, and the MLP's first one takes its bias and GELU along.
+
+The linears otherwise run as torch's F.linear (hipBLASLt) and LayerNorm as torch's layer_norm. Their weights
 are held as [out, in], the layout in which hipBLASLt runs these shapes fastest on gfx950 (10-25%
 faster than [in, out] for the four ViT-H linears); a loader of the reference's weights, whose Linear
 holds weight^T as [in, out] (encoder.rs:64), transposes each once. The two
@@ -24,7 +27,7 @@ same. window_partition / window_unpartition below are the reference's steps, kep
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import torch
 import torch.nn.functional as F
@@ -51,7 +54,14 @@ VIT_H = EncoderConfig(1280, 32, 16, (7, 15, 23, 31))
 
 
 @dataclass
-class BlockWeights:
+class MxWeight:
+    """A linear's weight [out, in] in 4 bits (sam_hip.mx_pack)."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+
+
+@dataclass
+class BlockWeights:  # qkv_w, proj_w, lin1_w and lin2_w may be MxWeights
     norm1_w: torch.Tensor
     norm1_b: torch.Tensor
     qkv_w: torch.Tensor  # [3C, C], [out, in]
@@ -112,6 +122,19 @@ def random_weights(cfg: EncoderConfig, dtype=torch.float16, device="cuda", seed:
     return w
 
 
+def pack_linears(w: EncoderWeights) -> EncoderWeights:
+    """The same weights with the blocks' linears in 4 bits: an eighth (f32) or a quarter (f16, bf16) of their memory."""
+    def packed(p: BlockWeights) -> BlockWeights:
+        return replace(p, **{n: MxWeight(*sam_hip.mx_pack(getattr(p, n))) for n in ("qkv_w", "proj_w", "lin1_w", "lin2_w")})
+
+    return replace(w, blocks=[packed(p) for p in w.blocks])
+
+
+def linear(x: torch.Tensor, w) -> torch.Tensor:
+    """x w^T without a bias, w [out, in] as it is or in 4 bits."""
+    return sam_hip.mx_linear(x, w.codes, w.scale) if isinstance(w, MxWeight) else F.linear(x, w)
+
+
 def window_partition(x: torch.Tensor, ws: int):
     """encoder.rs:129-137: [B, H, W, C] zero-padded to multiples of ws -> [B * nH * nW, ws, ws, C]."""
     b, h, w, c = x.shape
@@ -144,11 +167,11 @@ def attention(x: torch.Tensor, p: BlockWeights, heads: int) -> torch.Tensor:
     if ws != wsw:
         raise ValueError("square windows only")
     hd = c // heads
-    y = F.linear(x.reshape(b * h * w, c), p.qkv_w)
+    y = linear(x.reshape(b * h * w, c), p.qkv_w)
     q, kt, v = sam_hip.qkv_split_grid(y, p.qkv_b, b, h, w, ws, heads, hd)
     ctx = sam_hip.attention_relpos(q, kt, v, p.rel, ws, ws, hd ** -0.5)
     out = sam_hip.window_merge(ctx, b, h, w, ws, heads).reshape(b * h * w, c)
-    return F.linear(out, p.proj_w).view(b, h, w, c)
+    return linear(out, p.proj_w).view(b, h, w, c)
 
 
 def block(x: torch.Tensor, xn: torch.Tensor, p: BlockWeights, heads: int, nxt: BlockWeights = None):
@@ -158,8 +181,11 @@ def block(x: torch.Tensor, xn: torch.Tensor, p: BlockWeights, heads: int, nxt: B
     y = attention(xn, p, heads)
     x, xn2 = sam_hip.bias_residual_ln(x, y, p.proj_b, p.norm2_w, p.norm2_b, 1e-6)
     t = b * h * w
-    m = sam_hip.bias_gelu(F.linear(xn2.reshape(t, c), p.lin1_w), p.lin1_b)
-    y = F.linear(m, p.lin2_w).view(b, h, w, c)
+    if isinstance(p.lin1_w, MxWeight):
+        m = sam_hip.mx_linear(xn2.reshape(t, c), p.lin1_w.codes, p.lin1_w.scale, p.lin1_b, gelu=True)
+    else:
+        m = sam_hip.bias_gelu(F.linear(xn2.reshape(t, c), p.lin1_w), p.lin1_b)
+    y = linear(m, p.lin2_w).view(b, h, w, c)
     if nxt is None:
         return sam_hip.bias_residual(x, y, p.lin2_b), None
     return sam_hip.bias_residual_ln(x, y, p.lin2_b, nxt.norm1_w, nxt.norm1_b, 1e-6)

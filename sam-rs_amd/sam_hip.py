@@ -126,7 +126,7 @@ def load():
         L.sam_hip_mx_unpack.restype = _i
         L.sam_hip_mx_matmul.argtypes = [_vp] * 6 + [_i] * 5 + [_vp]
         L.sam_hip_mx_matmul.restype = _i
-        L.sam_hip_mx_linear_workspace_size.argtypes = [_i, _i]
+        L.sam_hip_mx_linear_workspace_size.argtypes = [_i] * 3
         L.sam_hip_mx_linear_workspace_size.restype = ctypes.c_long
         L.sam_hip_mx_linear.argtypes = [_vp] * 5 + [_i] * 5 + [_vp, ctypes.c_long, _vp]
         L.sam_hip_mx_linear.restype = _i
@@ -1108,6 +1108,15 @@ def mx_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _mx_workspace(m: int, n: int, k: int) -> int:
+    """Bytes that sam_hip_mx_linear needs for a layer of these sizes (an error's are not kept)."""
+    size = load().sam_hip_mx_linear_workspace_size(m, n, k)
+    if size < 0:
+        raise SamHipError(load().sam_hip_last_error().decode())
+    return size
+
+
 def mx_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
               gelu: bool = False) -> torch.Tensor:
     """A linear layer with 4-bit weights w, w_scale (mx_pack of [N, K]) on x [.., K], which it packs likewise:
@@ -1137,8 +1146,8 @@ def mx_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: tor
     m = out.numel() // n
     if (m | n) >> 31:
         _sizes("mx_linear", m, n)
-    ws_bytes = m * (k // 2) + m * (k // _BLOCK)
-    ws = x.new_empty(-(-ws_bytes // x.element_size()))
+    ws_bytes = _mx_workspace(m, n, k)
+    ws = x.new_empty(-(-ws_bytes // x.element_size())) if ws_bytes else None
     _check(load().sam_hip_mx_linear(x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), _ptr(bias), out.data_ptr(), dt, m, n, k,
-                                    bool(gelu), ws.data_ptr(), ws_bytes, _stream()))
+                                    bool(gelu), _ptr(ws), ws_bytes, _stream()))
     return out

@@ -40,7 +40,7 @@ def linear(lib, x=FAKE, w=FAKE, sw=FAKE, bias=None, out=FAKE, dtype=1, m=4, n=4,
 @pytest.mark.parametrize("change, code", [
     ({"x": None}, 1), ({"w": None}, 1), ({"sw": None}, 1), ({"out": None}, 1), ({"dtype": 3}, 2), ({"m": -1}, 1), ({"n": -1}, 1),
     ({"k": 40}, 1), ({"k": (1 << 22) + 32}, 3), ({"m": 1 << 15, "k": 1 << 22, "n": 1}, 3), ({"x": vp(0x1008)}, 3), ({"w": vp(0x1008)}, 3),
-    ({"ws": None}, 1), ({"ws": vp(0x1008)}, 3), ({"ws_bytes": 4 * 34 - 1}, 1), ({"bias": vp(0x1008)}, 3), ({"out": vp(0x1008)}, 3)])
+    ({"ws": None, "m": 17}, 1), ({"ws": vp(0x1008)}, 3), ({"m": 17, "ws_bytes": 17 * 34 - 1}, 1), ({"bias": vp(0x1008)}, 3), ({"out": vp(0x1008)}, 3)])
 def test_linear_refuses(lib, change, code):
     assert linear(lib, **change) == code
     assert lib.sam_hip_last_error()
@@ -48,7 +48,8 @@ def test_linear_refuses(lib, change, code):
 
 def test_linear_workspace(lib):
     size = lib.sam_hip_mx_linear_workspace_size
-    assert size(4, 64) == 4 * 34 and size(0, 64) == 0 and size(3, 48) == size(-1, 64) == -1 and linear(lib, m=0) == 0
+    assert size(17, 9, 64) == 17 * 34 and size(16, 9, 1 << 20) == 16 * (34 << 14) and size(16, 4096, 8192) == size(0, 9, 64) == size(99, 0, 64) == 0
+    assert size(3, 9, 48) == size(-1, 9, 64) == size(1 << 15, 1, 1 << 22) == -1 and linear(lib, m=0) == 0
 
 
 @pytest.mark.parametrize("call", [pack, unpack])

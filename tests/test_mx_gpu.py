@@ -139,6 +139,22 @@ def test_views_leading_dimensions_and_alignment(hip):
     assert hip.mx_matmul(xc[:0], xs[:0], wc, ws).shape == (0, 100) and hip.mx_matmul(xc, xs, wc[:0], ws[:0]).shape == (100, 0)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m", [1, 16, 17])
+def test_the_workspace_size_and_extreme_rows(hip, dtype, m):
+    """A layer on rows that it packs on the way, and with a workspace, against packing them first: blocks of zeros, of the
+    largest and smallest values, of values that are not finite."""
+    f = torch.finfo(DT[dtype])
+    x, w = randn(m, 320, dtype=DT[dtype], seed=m), randn(50, 320, dtype=DT[dtype], seed=1)
+    x[0, :32], x[0, 32:64], x[0, 64:96], x[m // 2, 96:128], x[m - 1, 128:160] = 0, f.tiny, -0.0, f.smallest_normal * f.eps, 2.0 ** 10
+    wc, ws = hip.mx_pack(w)
+    assert hip.load().sam_hip_mx_linear_workspace_size(m, 50, 320) == (0 if m <= 16 else m * 170)
+    assert torch.equal(hip.mx_linear(x, wc, ws), hip.mx_matmul(*hip.mx_pack(x), wc, ws, dtype=DT[dtype]))
+    x[m - 1, 300], x[0, 10] = float("inf"), float("nan")
+    got = hip.mx_linear(x, wc, ws)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[m - 1]).all() and (m < 3 or torch.isfinite(got[1:m - 1]).all())
+
+
 def test_rows_behind_the_result_are_left_alone(hip):
     """A result of odd sizes inside a larger allocation: nothing around it changes (through the C entry)."""
     for m, n in ((5, 33), (70, 67), (1601, 2001)):
