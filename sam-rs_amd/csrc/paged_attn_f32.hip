@@ -48,6 +48,11 @@ __device__ __forceinline__ f32x4 widen(unsigned short c, float s) {
   const f32x2 a = mx_decode2_f32<0>(c, s), b = mx_decode2_f32<1>(c, s);
   return f32x4{a[0], a[1], b[0], b[1]};
 }
+// The low or the high four codes of a word.
+__device__ __forceinline__ f32x4 widen_half(unsigned w, bool high, float s) {
+  const f32x2 a = high ? mx_decode2_f32<2>(w, s) : mx_decode2_f32<0>(w, s), b = high ? mx_decode2_f32<3>(w, s) : mx_decode2_f32<1>(w, s);
+  return f32x4{a[0], a[1], b[0], b[1]};
+}
 
 template <typename C, int DP, int RB>
 __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(PagedParams p) {
@@ -79,7 +84,7 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
       const float* qr = reinterpret_cast<const float*>(p.q) + tok[rb] * p.sq[0] + head[rb] * p.sq[1];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int col = 16 * c + 4 * g;
+        const int col = kMx ? DP / 4 * g + 4 * c : 16 * c + 4 * g;
         qf[rb][c] = col < d ? *reinterpret_cast<const f32x4*>(qr + col) : f32x4{};
       }
     }
@@ -109,12 +114,13 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
     auto from_key = [&](int j, int v) {  // the lane whose own key is 16 (j / 4) + 4 g + j % 4
       return __builtin_amdgcn_ds_bpermute((int)at_g + 64 * (j >> 2) + 4 * (j & 3), v);
     };
-    Raw kx[2][NC], vx[8][ND];
+    Raw kx[2][kMx ? 1 : NC], vx[8][ND];
     unsigned char ksx = 127, vsx = 127;
-    // e2m1: the scales of the key blocks that the lane multiplies, and of every other of its own key's value blocks (lanes
-    // 0 .. 31 the even ones)
-    constexpr int KB = (DP + kMxBlock - 1) / kMxBlock;
-    unsigned char kmx[2][KB], vmx[ND];
+    // e2m1: a lane's words of a key row lie side by side, DP / 4 columns, of one or two blocks (a word each at 96), which q's
+    // columns follow; the scales of every other of its own key's value blocks (lanes 0 .. 31 the even ones)
+    constexpr int KW = DP / 32, KSC = DP == 96 ? 3 : DP <= 128 ? 1 : 2;
+    unsigned kw[2][KW];
+    unsigned char kmx[2][KSC], vmx[ND];
     const int G = d / kMxBlock;
     auto load_k = [&](int row) {
       if constexpr (kScaled) ksx = p.c.ks[max(row, 0)];
@@ -122,11 +128,23 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
       for (int i = 0; i < 2; ++i) {
         const long r = max(from_n(i, row), 0);
         const C* kr = held_at(kp, r * d);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) kx[i][c] = *reinterpret_cast<const Raw*>(held_at(kr, min(16 * c + 4 * g, d - 4)));
         if constexpr (kMx) {
+          constexpr int KL = KW % 4 == 0 ? 4 : KW == 2 ? 2 : 1;  // words of a load
 #pragma unroll
-          for (int b = 0; b < KB; ++b) kmx[i][b] = p.c.ks[r * G + min(b, G - 1)];
+          for (int w = 0; w < KW; w += KL) {
+            const C* at = held_at(kr, min(DP / 4 * g + 8 * w, d - 8 * KL));
+            if constexpr (KL == 4)
+              *reinterpret_cast<u32x4*>(&kw[i][w]) = *reinterpret_cast<const u32x4*>(at);
+            else if constexpr (KL == 2)
+              *reinterpret_cast<u32x2*>(&kw[i][w]) = *reinterpret_cast<const u32x2*>(at);
+            else
+              kw[i][w] = *reinterpret_cast<const unsigned*>(at);
+          }
+#pragma unroll
+          for (int b = 0; b < KSC; ++b) kmx[i][b] = p.c.ks[r * G + min((DP / 4 * g + (DP == 96 ? 8 : 32) * b) / kMxBlock, G - 1)];
+        } else {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) kx[i][c] = *reinterpret_cast<const Raw*>(held_at(kr, min(16 * c + 4 * g, d - 4)));
         }
       }
     };
@@ -172,9 +190,12 @@ __global__ __launch_bounds__(256, DP * RB <= 64 ? 2 : 1) void paged_f32_kernel(P
         if constexpr (kScaled) f = __int_as_float(from_n(i, __float_as_int(kso)));
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          if constexpr (kMx) f = mx_scale(kmx[i][c / 2]);
-          f32x4 a = widen(kx[i][c], f);
-          if (16 * c + 16 > d && 16 * c + 4 * g >= d) a = f32x4{};
+          f32x4 a;
+          if constexpr (kMx)
+            a = widen_half(kw[i][c / 2], c % 2, mx_scale(kmx[i][DP == 96 ? c / 2 : c / 8 % KSC]));
+          else
+            a = widen(kx[i][c], f);
+          if (kMx ? DP / 4 * g + 4 * c >= d : 16 * c + 16 > d && 16 * c + 4 * g >= d) a = f32x4{};
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll

@@ -46,7 +46,7 @@ template <> struct Raw<16> {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int few_workgroups(bool wide, bool mx, bool split, int dp, int rb) {
-  return dp * rb > 128 ? 1 : dp == 128 && (wide || (mx && split)) ? 2 : 3;
+  return dp * rb > 128 ? 1 : dp == 128 && wide ? 2 : 3;
 }
 
 // QUADS (e2m1 of a full head dim, pages of whole quads): the four neighbouring keys of a lane follow one another in their
@@ -70,6 +70,10 @@ __global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, __is_same(C, e2m
   typedef typename std::conditional<KB == 2, unsigned long, unsigned>::type Bits;  // one of each key
   __shared__ float sm_m[2][TR], sm_l[2][TR];
   __shared__ __attribute__((aligned(16))) float sm_o[2][RB * DP / 16][256];
+  // bf16 over e2m1 at head dim 128 reads its queries from LDS for each block: in registers they leave room for two workgroups a
+  // CU, not three (32 sequences of 820 to 8192 keys 55 and 51 us; f16, with three either way, 46 and 47)
+  constexpr bool kQInLds = kMx && kSplitP && DP == 128 && RB == 1;
+  __shared__ __attribute__((aligned(16))) u32x4 sm_q[kQInLds ? NK : 1][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int d = p.c.d;
   if (p.zero_rest) paged_zero_rest<T>(p);
@@ -92,7 +96,7 @@ __global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, __is_same(C, e2m
     if (direct && w.split > 0) continue;
 
     int limit[RB];
-    X8 qf[RB][NK];
+    X8 qf[RB][kQInLds ? 1 : NK];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const int r = min(rt * TR + 16 * rb + n, rows - 1);
@@ -102,7 +106,12 @@ __global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, __is_same(C, e2m
 #pragma unroll
       for (int c = 0; c < NK; ++c) {
         const int col = kMx ? DP / 4 * g + 8 * c : 32 * c + 8 * g;
-        qf[rb][c] = col < d ? *reinterpret_cast<const X8*>(qr + col) : X8{};
+        const X8 x = col < d ? *reinterpret_cast<const X8*>(qr + col) : X8{};
+        if constexpr (kQInLds) {
+          if (wave == 0) sm_q[c][lane] = __builtin_bit_cast(u32x4, x);
+        } else {
+          qf[rb][c] = x;
+        }
       }
     }
 
@@ -210,12 +219,20 @@ __global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, __is_same(C, e2m
     }
     // Q is here: told to the compiler, whose own wait for it would stand in the loop, behind the next block's loads
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    if constexpr (kQInLds) __syncthreads();
     for (int blk = b0 + KB * wave; blk < b1; blk += 4 * KB) {
       const int key0 = 32 * blk;
       const int next = row_of(coming, blk + 4 * KB);
       coming = entry_of(blk + 8 * KB);
       const Bits there = (Bits)__builtin_amdgcn_ballot_w64(row >= 0);
       f32x4 s[RB][2 * KB];
+      X8 ql[kQInLds ? NK : 1];
+      if constexpr (kQInLds) {
+        typedef __attribute__((address_space(3))) X8 lds_x8;
+        const unsigned at = opaque(lds_addr(sm_q) + 16 * lane);  // hidden: not to be read once for all blocks
+#pragma unroll
+        for (int c = 0; c < NK; ++c) ql[c] = *(const lds_x8*)(size_t)(at + 1024 * c);
+      }
       const float kso = kCoded ? pow2_of(ksx) : 1.f, vso = kCoded ? pow2_of(vsx) : 1.f;
       unsigned vmo = 0;
       if constexpr (kMx && !QUADS) {
@@ -240,7 +257,7 @@ __global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, __is_same(C, e2m
           if (kMx ? DP / 4 * g + 8 * c >= d : 32 * c + 32 > d && 32 * c + 8 * g >= d) a = u32x4{};
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb)
-            s[rb][i] = mma16(__builtin_bit_cast(X8, a), qf[rb][c], c == 0 ? f32x4{} : s[rb][i]);
+            s[rb][i] = mma16(__builtin_bit_cast(X8, a), kQInLds ? ql[kQInLds ? c : 0] : qf[rb][kQInLds ? 0 : c], c == 0 ? f32x4{} : s[rb][i]);
         }
       }
       // s[rb][i][e]: key key0 + 16 i + 4 g + e, row 16 rb + n
