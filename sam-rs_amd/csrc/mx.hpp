@@ -94,24 +94,6 @@ template <typename T> __device__ __forceinline__ unsigned mx_quantise(const Eigh
   return fine ? w : 0u;
 }
 
-// The same for a whole block in one lane.
-template <typename T> __device__ __forceinline__ u32x4 mx_quantise(const Eight<T>* x, unsigned& scale) {
-  unsigned top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, magnitude(x[i]));
-  const bool fine = top < kInfBits<T>;
-  const unsigned s = (unsigned)(mx_scale_of(f32_bits<T>(fine ? top : 0u)) + 127);
-  const float f = __uint_as_float(s << 23);
-  u32x4 w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const T* e = reinterpret_cast<const T*>(&x[i]);
-    w[i] = fine ? mx_encode2<T, 3>(e + 6, f, mx_encode2<T, 2>(e + 4, f, mx_encode2<T, 1>(e + 2, f, mx_encode2<T, 0>(e, f, 0u)))) : 0u;
-  }
-  scale = fine ? s : 255u;
-  return w;
-}
-
 // A block's scale for the conversions below, which read its exponent alone: 0 is 2^-127, 255 NaN.
 __device__ __forceinline__ float mx_scale(unsigned byte) { return __uint_as_float(byte << 23); }
 // Two values of a word of eight codes (byte SEL) in T, rounded to it once.

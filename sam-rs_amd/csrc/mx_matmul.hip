@@ -201,24 +201,46 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_product_kernel(MxProduct p, i
 }
 
 // Few rows: B's bytes bound it, so they go from memory straight to the matrix units. A workgroup takes 16 columns of out and
-// RB blocks of 16 rows; its waves take steps of 128 along k in turn and join at the end, in order. RAW: A comes as it is, a
-// block a lane, and is packed in registers.
+// RB blocks of 16 rows; its waves take steps of 128 along k in turn and join at the end, in order. RAW: A comes as it is, and
+// each workgroup packs it into LDS first.
 template <typename T, int RB, bool RAW>
 __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
-  constexpr int U = RAW && sizeof(T) == 4 ? 2 : 4;  // steps in flight
+  constexpr int U = 4;  // steps in flight
   __shared__ __attribute__((aligned(16))) f32x4 part[16][RB][64];
+  extern __shared__ __attribute__((aligned(16))) unsigned char packed[];  // [m][k / 2] codes, then [m][k / 32] scales
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, g = lane >> 4, n0 = 16 * blockIdx.x;
   const int G = p.k / 32, steps = (G + 3) / 4;
   const long rb = p.k / 2;
   const unsigned char* br = p.b + min(n0 + r, p.n - 1) * rb;
   const unsigned char* bs = p.sb + min(n0 + r, p.n - 1) * (long)G;
+  const unsigned char* a0 = RAW ? packed : reinterpret_cast<const unsigned char*>(p.a);
+  const unsigned char* sa0 = RAW ? packed + p.m * (p.k / 2) : p.sa;
   const unsigned char *ar[RB], *as[RB];
-  const T* raw = reinterpret_cast<const T*>(p.a) + min(r, p.m - 1) * (long)p.k;
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
-    ar[i] = reinterpret_cast<const unsigned char*>(p.a) + min(16 * i + r, p.m - 1) * rb;
-    as[i] = p.sa + min(16 * i + r, p.m - 1) * (long)G;
+    ar[i] = a0 + min(16 * i + r, p.m - 1) * rb;
+    as[i] = sa0 + min(16 * i + r, p.m - 1) * (long)G;
+  }
+  if constexpr (RAW) {
+    const int vectors = p.m * (p.k / 8), rounds = (vectors + blockDim.x - 1) / blockDim.x;  // of 8 values, a quad a block
+    for (int v0 = 0; v0 < rounds; v0 += U) {
+      Eight<T> x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        x[u] = load_eight(reinterpret_cast<const T*>(p.a) + 8l * min((int)threadIdx.x + (v0 + u) * (int)blockDim.x, vectors - 1));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = threadIdx.x + (v0 + u) * blockDim.x;
+        unsigned s;
+        const unsigned w = mx_quantise(x[u], s);
+        if (at < vectors) {
+          reinterpret_cast<unsigned*>(packed)[at] = w;
+          if (at % 4 == 0) packed[p.m * (p.k / 2) + at / 4] = (unsigned char)s;
+        }
+      }
+    }
+    __syncthreads();
   }
   f32x4 acc[RB];
 #pragma unroll
@@ -226,21 +248,15 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
   for (int t0 = wave; t0 < steps; t0 += U * waves) {
     u32x4 b[U], a[U][RB];
     unsigned char sb[U], sa[U][RB];
-    Eight<T> x[RAW ? U : 1][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = min(4 * (t0 + u * waves) + g, G - 1);
       b[u] = *reinterpret_cast<const u32x4*>(br + 16 * c);
       sb[u] = bs[c];
-      if constexpr (RAW) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = load_eight(raw + 32 * c + 8 * i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < RB; ++i) {
-          a[u][i] = *reinterpret_cast<const u32x4*>(ar[i] + 16 * c);
-          sa[u][i] = as[i][c];
-        }
+      for (int i = 0; i < RB; ++i) {
+        a[u][i] = *reinterpret_cast<const u32x4*>(ar[i] + 16 * c);
+        sa[u][i] = as[i][c];
       }
     }
 #pragma unroll
@@ -248,15 +264,7 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
       const bool in = 4 * (t0 + u * waves) + g < G;  // blocks past the row's end: zeros under 2^-127
       const u32x4 bu = in ? b[u] : u32x4{};
 #pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        unsigned s;
-        u32x4 w;
-        if constexpr (RAW)
-          w = mx_quantise(x[u], s);
-        else
-          w = a[u][i], s = sa[u][i];
-        acc[i] = mma_mx16(bu, in ? sb[u] : 0u, w, in ? s : 0u, acc[i]);
-      }
+      for (int i = 0; i < RB; ++i) acc[i] = mma_mx16(bu, in ? sb[u] : 0u, a[u][i], in ? sa[u][i] : 0u, acc[i]);
     }
   }
 #pragma unroll
@@ -287,13 +295,18 @@ template <typename T, int TM, int TN, int WM, int WN> hipError_t by_alignment(co
   return p.gelu ? launch_product<T, TM, TN, WM, WN, false, true>(p, stream) : launch_product<T, TM, TN, WM, WN, false, false>(p, stream);
 }
 
+constexpr int kMostPacked = 16 * (8192 / 2 + 8192 / 32);  // bytes of LDS
+
 template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream) {
   if (p.m <= 32) {
     const int waves = (int)std::min(16, std::max(1, (p.k + 511) / 512));
     const dim3 grid((unsigned)((p.n + 15) / 16));
-    if (!p.sa)
-      hipLaunchKernelGGL((mx_few_kernel<T, 1, true>), grid, dim3(64 * waves), 0, stream, p);
-    else if (p.m <= 16)
+    if (!p.sa) {
+      const int lds = p.m * (p.k / 2 + p.k / 32);
+      static std::atomic<unsigned long long> done;
+      if (const hipError_t e = lds_opt_in(done, (const void*)mx_few_kernel<T, 1, true>, kMostPacked); e != hipSuccess) return e;
+      hipLaunchKernelGGL((mx_few_kernel<T, 1, true>), grid, dim3(64 * waves), lds, stream, p);
+    } else if (p.m <= 16)
       hipLaunchKernelGGL((mx_few_kernel<T, 1, false>), grid, dim3(64 * waves), 0, stream, p);
     else
       hipLaunchKernelGGL((mx_few_kernel<T, 2, false>), grid, dim3(64 * waves), 0, stream, p);
@@ -316,11 +329,9 @@ template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream)
 }  // namespace
 
 // Whether a linear layer's few rows are packed by each workgroup of 16 columns again, in place of a launch of their own: up to
-// 16 rows while a CU's workgroups pack 8192 values of a row in all. Through the front end with and
-// without that launch: 7 rows of 5120 to 1280 columns in f32 12.1 and 9.9 us; 16 rows of 8192 to 8192 in bf16 21 and 26.
-bool mx_packs_on_the_way(int m, int n, int k) {
-  return m <= 16 && ((long)n + 4095) / 4096 * k <= 1L << 13;
-}
+// 16 rows while a CU's workgroups pack 8192 values of a row in all. Kernel times: 7 rows of 5120 to 1280 columns in f32 7.4 us,
+// 2.3 and 6.2 in two launches; 16 rows of 8192 to 4096 columns in f16 13.4, and 2.5 and 10.2.
+bool mx_packs_on_the_way(int m, int n, int k) { return m <= 16 && ((long)n + 4095) / 4096 * k <= 8192; }
 
 hipError_t mx_matmul(int dtype, const MxProduct& p, hipStream_t stream) {
   if (p.m == 0 || p.n == 0) return hipSuccess;
