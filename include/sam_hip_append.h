@@ -24,7 +24,7 @@ extern "C" {
  * q and out may both be NULL (heads is ignored then); with pairs == 0 pos, freqs and axes may be. Strides: (token, head) of q,
  * k, v and out in multiples of 16 bytes, (token, axis) of pos; NULL = contiguous; out's rows lie apart. out may be q with the
  * same strides; it must not overlap q otherwise, nor the other tensors. Limits: those of the paged memory, up to 65535 query
- * heads, tokens * (heads + kv_heads) < 2^27.
+ * heads, tokens * (heads + kv_heads) <= 2^27 - 32.
  */
 int sam_hip_kv_append(const void* q, const void* k, const void* v, const int* pos, const double* freqs, const int* axes,
                       void* out, void* k_pages, void* v_pages, unsigned char* k_scale, unsigned char* v_scale,

@@ -28,7 +28,8 @@ int sam_hip_mx_unpack(const unsigned char* codes, const unsigned char* scales, v
  * out[i, j] = act(sum_l A[i, l] B[j, l] + bias[j]) over the values that a, a_scale [m, k] and b, b_scale [n, k] stand for:
  * a linear layer whose weights are B. Sums are f32, bias [n] (or NULL) and out [m, n] are of dtype, rounded once; act is the
  * identity or, with gelu, the exact GELU 0.5 x (1 + erf(x / sqrt 2)). out must not overlap the operands. m * n < 2^36,
- * m <= 2^30, n <= 2^25, k <= 2^22, fewer than 2^23 tiles of 128 x 128; a, b and out 16-byte aligned, bias aligned to 16 bytes too; k % 128 == 0 runs fastest.
+ * m <= 2^30, n <= 2^25, k <= 2^22, fewer than 2^23 tiles of 128 x 128; a, b, bias and out 16-byte aligned. Rows whose
+ * scales are no whole dwords (k % 128 != 0), and scales off a multiple of 4 bytes run slower.
  */
 int sam_hip_mx_matmul(const unsigned char* a, const unsigned char* a_scale, const unsigned char* b,
                       const unsigned char* b_scale, const void* bias, void* out, int dtype, int m, int n, int k, int gelu,
@@ -37,8 +38,8 @@ int sam_hip_mx_matmul(const unsigned char* a, const unsigned char* a_scale, cons
 /*
  * A linear layer with 4-bit weights: sam_hip_mx_pack of x [m, k] into the workspace, then sam_hip_mx_matmul of it and of w,
  * w_scale (as sam_hip_mx_pack makes them from [n, k]) to out [m, n]. Workspace: sam_hip_mx_linear_workspace_size() bytes of
- * device memory, 16-byte aligned (0 needs none, -1 is an error; a few rows are packed on their way to the product); calls that may overlap need their own, and so does each captured graph
- * that may run beside another.
+ * device memory, 16-byte aligned (0 needs none, as a few rows are packed on their way to the product; -1 is an error); calls
+ * that may overlap need their own, and so does each captured graph that may run beside another.
  */
 long sam_hip_mx_linear_workspace_size(int m, int n, int k);
 int sam_hip_mx_linear(const void* x, const unsigned char* w, const unsigned char* w_scale, const void* bias, void* out,

@@ -49,13 +49,6 @@ __device__ __forceinline__ void bdma16s(i32x4 rsrc, unsigned off, unsigned soff,
                : "memory", "m0");
 }
 
-// The same for a dword a lane (off a multiple of 4), at lds + 4 l, and for a byte a lane, which lands as a dword there.
-__device__ __forceinline__ void bdma4(i32x4 rsrc, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory", "m0");
-}
-__device__ __forceinline__ void bdma1(i32x4 rsrc, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_ubyte %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds) : "memory", "m0");
-}
 
 // LDS byte address of a pointer into dynamic shared memory.
 __device__ __forceinline__ unsigned lds_addr(const void* p) {

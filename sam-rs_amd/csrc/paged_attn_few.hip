@@ -45,16 +45,14 @@ template <> struct Raw<16> {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int few_workgroups(bool wide, bool mx, bool split, int dp, int rb) {
-  return dp * rb > 128 ? 1 : dp == 128 && wide ? 2 : 3;
-}
+// Workgroups a CU: as many as registers allow with a block of K and one of V in flight. Three for e4m3 at head dim 128
+// (131 us for the bf16 call above with eight splits, 137 with two).
+constexpr int few_workgroups(bool wide, int dp, int rb) { return dp * rb > 128 ? 1 : dp == 128 && wide ? 2 : 3; }
 
 // QUADS (e2m1 of a full head dim, pages of whole quads): the four neighbouring keys of a lane follow one another in their
 // page, so that a quad has one address, its rows lie at constant offsets and their scales are one load.
-// Workgroups a CU: as many as registers allow with a block of K and one of V in flight. Three for e4m3 at head dim 128
-// (131 us for the bf16 call above with eight splits, 137 with two).
 template <typename T, typename C, int DP, int RB, bool QUADS>
-__global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, __is_same(C, e2m1), __is_same(T, bf16), DP, RB)) void paged_few_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, few_workgroups(sizeof(C) > 1, DP, RB)) void paged_few_kernel(PagedParams p) {
   typedef typename Vec<T>::x8 X8;
   constexpr bool kMx = __is_same(C, e2m1), kCoded = __is_same(C, e4m3), kSplitP = __is_same(T, bf16);
   constexpr float kLift = kSplitP ? 0.f : 15.f;  // P is lifted by 2^kLift

@@ -890,8 +890,8 @@ int sam_hip_kv_append(const void* q, const void* k, const void* v, const int* po
   if (2L * pairs > d) return fail(SAM_HIP_EINVAL, "kv-append: %d pairs do not fit in a head dim of %d", pairs, d);
   samhip::KvAppendCall a = {};
   a.heads = q ? heads : 0;
-  // up to 32 threads a row, which a launch counts in 32 bits
-  if (a.heads > 65535 || (long)tokens * (a.heads + (long)kv_heads) >= 1L << 27)
+  // up to 32 threads a row and two parts of whole workgroups, which a launch counts in 32 bits
+  if (a.heads > 65535 || (long)tokens * (a.heads + (long)kv_heads) > (1L << 27) - 32)
     return fail(SAM_HIP_EUNSUPPORTED, "kv-append: too many rows (tokens=%d heads=%d kv_heads=%d)", tokens, heads, kv_heads);
   if (int rc = token_strides("kv-append", "q", strides_q, a.sq, a.heads, d, dtype); rc != SAM_HIP_OK) return rc;
   if (int rc = token_strides("kv-append", "k", strides_k, a.sk, kv_heads, d, dtype); rc != SAM_HIP_OK) return rc;

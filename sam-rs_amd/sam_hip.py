@@ -818,8 +818,9 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: t
     torch.float8_e4m3fn with k_scale, v_scale uint8 [pages, heads, page_size]: a row's scale is the power of two
     2^(byte - 127) that brings its largest value nearest to 448 from below, its codes round to nearest even, and values
     that are not finite become NaN. Or they hold torch.float4_e2m1fn_x2 [pages, heads, page_size, D / 2] with k_scale, v_scale
-    uint8 [pages, heads, page_size, D / 32], D a multiple of 32, rows as mx_pack makes them. Tokens at a negative position, past the table, or whose table entry names no page are
-    not stored; two positions in one page slot must not be written by one call."""
+    uint8 [pages, heads, page_size, D / 32], D a multiple of 32, rows as mx_pack makes them. Tokens at a negative position, past
+    the table, or whose table entry names no page are not stored; two positions in one page slot must not be written by one
+    call."""
     dev = _device_of("kv_write", k, v, k_pages, v_pages, table, starts, lens, k_scale, v_scale)
     if not _is_current(dev):
         with torch.cuda.device(dev):
@@ -896,6 +897,8 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, freqs: t
             if out.stride(2) != 1 or _overlaps_itself(out):
                 raise SamHipError("sam-rs kernels need contiguous inputs")  # kernels.rs:1100
             so = _long2(out.stride(0), out.stride(1))
+    if heads == 0 and hq:
+        raise SamHipError("kv_append: q without key heads")
     if tokens == 0 or b == 0 or heads == 0 or d == 0:
         _empty_call("kv-append")
         return out.zero_() if rest and out is not None else out

@@ -36,7 +36,7 @@ def test_bad_pools_are_refused(lib, change, code):
 @pytest.mark.parametrize("change, code", [
     ({"k": None}, 1), ({"v": None}, 1), ({"starts": None}, 1), ({"q": None}, 1), ({"out": None}, 1), ({"freqs": None}, 1), ({"axes": None}, 1),
     ({"tokens": -1}, 1), ({"heads": 0}, 1), ({"pairs": -1}, 1), ({"pairs": 33}, 1), ({"naxes": 0}, 1), ({"tokens": 1 << 26}, 3),
-    ({"heads": 65536}, 3), ({"sq": strides(252, 64)}, 3), ({"sk": strides(100, 64)}, 3), ({"sv": strides(-128, 64)}, 3),
+    ({"tokens": (1 << 26) - 8, "heads": 1, "kv_heads": 1}, 3), ({"heads": 65536}, 3), ({"sq": strides(252, 64)}, 3), ({"sk": strides(100, 64)}, 3), ({"sv": strides(-128, 64)}, 3),
     ({"so": strides(256, -64)}, 3), ({"so": strides(64, 64)}, 1), ({"sp": strides(-2, 1)}, 3), ({"q": vp(0x1008)}, 3), ({"k": vp(0x1002)}, 3),
     ({"out": vp(0x2008)}, 3), ({"pos": vp(0x1002)}, 3), ({"freqs": vp(0x1004)}, 3), ({"axes": vp(0x1001)}, 3),
     ({"out": FAKE, "sq": strides(512, 64)}, 1)])

@@ -311,6 +311,8 @@ def test_refusals(hip):
                    {"out": q.transpose(1, 2).contiguous().transpose(1, 2)}):
         with pytest.raises(hip.SamHipError):
             hip.kv_append(**{**ok, **change})
+    with pytest.raises(hip.SamHipError, match="key heads"):
+        hip.kv_append(**{**ok, "k": k[:, :0], "v": k[:, :0], "k_pages": kp[:, :0], "v_pages": vp[:, :0]})
     hip.set_enabled(False)
     try:
         for change in ({}, {"q": q[:0], "k": k[:0], "v": k[:0]}):
