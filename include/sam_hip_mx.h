@@ -18,7 +18,8 @@ extern "C" {
  * sam1/encoder.rs:64) hold 16- or 32-bit weights.
  *
  * sam_hip_mx_pack writes the codes and scales of x [rows, k] in dtype; sam_hip_mx_unpack gives back the values that they
- * stand for, rounded to dtype once (a scale byte of 0 is 2^-127). Fewer than 2^36 values; x and codes 16-byte aligned.
+ * stand for, rounded to dtype once (a scale byte of 0 is 2^-127). At most 2^35 - 2048 values; x and
+ * codes 16-byte aligned.
  */
 int sam_hip_mx_pack(const void* x, unsigned char* codes, unsigned char* scales, int dtype, long rows, int k, void* stream);
 int sam_hip_mx_unpack(const unsigned char* codes, const unsigned char* scales, void* x, int dtype, long rows, int k,

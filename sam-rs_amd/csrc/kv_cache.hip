@@ -13,7 +13,8 @@
 // values each (16-byte loads of 16-bit values, 8-byte stores of codes); keys and values go in the same thread, so
 // that the page lookup, a chain of dependent loads, is paid once. 65536 tokens of 8 heads of 128, bf16: written as e4m3
 // in 81 us, 5.0 TB/s (113 with 64-bit divisions, values widened one by one and non-finite ones looked for in each), read
-// back in 80, and moved as they are in 100 each way, 5.3 TB/s; a copy reaches 4.8 to 5.1. A few tokens are latency: 3.3 us.
+// back in 80, and moved as they are in 100 each way, 5.3 TB/s; a copy reaches 4.8 to 5.1. As e2m1 they take 75 and 81 us (4.5
+// and 4.2 TB/s: an eighth less to move, and the conversions beside it). A few tokens are latency: 3.3 us.
 #include "kv_rows.hpp"
 
 namespace samhip {

@@ -3,31 +3,26 @@
 // What bounds both: HBM bytes, a value in and its 4 bits out. A lane takes 8 values (16-byte loads of 16-bit ones), so that
 // the four lanes of a quad have a block and find its largest magnitude in two exchanges inside the quad; the scale is a
 // shift of that one's exponent, and one conversion instruction a pair of values divides and rounds.
+//
+// Measured, 16384 rows of 8192 in bf16: packed in 57 us (5.9 TB/s), unpacked in 58 (5.8); a copy of 1 GiB reaches 5.2. 196
+// rows of 1280 in f32 are a launch, 2.3 us.
 #include "mx.hpp"
 
 namespace samhip {
 
 namespace {
 
-// A thread takes U vectors of 8 values, a workgroup's threads a run of 256 neighbours each time.
-template <typename T, int U>
+template <typename T>
 __global__ __launch_bounds__(256) void mx_pack_kernel(const T* x, unsigned* codes, unsigned char* scales, long vectors) {
-  const long first = (long)blockIdx.x * (256 * U) + threadIdx.x;
-  Eight<T> v[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) v[u] = load_eight(x + 8 * min(first + 256 * u, vectors - 1));
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    unsigned s;
-    const unsigned w = mx_quantise(v[u], s);
-    const long at = first + 256 * u;
-    if (at < vectors) {
-      codes[at] = w;
-      if ((threadIdx.x & 3) == 0) scales[at >> 2] = (unsigned char)s;
-    }
-  }
+  const long at = (long)blockIdx.x * 256 + threadIdx.x;
+  unsigned s;
+  const unsigned w = mx_quantise(load_eight(x + 8 * min(at, vectors - 1)), s);
+  if (at >= vectors) return;
+  codes[at] = w;
+  if ((threadIdx.x & 3) == 0) scales[at >> 2] = (unsigned char)s;
 }
 
+// A thread takes U vectors of 8 values, a workgroup's threads a run of 256 neighbours each time.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void mx_unpack_kernel(const unsigned* codes, const unsigned char* scales, T* x, long vectors) {
   const long first = (long)blockIdx.x * (256 * U) + threadIdx.x;
@@ -45,22 +40,23 @@ __global__ __launch_bounds__(256) void mx_unpack_kernel(const unsigned* codes, c
 }
 
 template <typename T> hipError_t pack(const void* x, unsigned char* codes, unsigned char* scales, long vectors, hipStream_t stream) {
-  const T* from = reinterpret_cast<const T*>(x);
-  unsigned* to = reinterpret_cast<unsigned*>(codes);
-  if (vectors >= 1l << 18)
-    hipLaunchKernelGGL((mx_pack_kernel<T, 4>), dim3((unsigned)((vectors + 1023) / 1024)), dim3(256), 0, stream, from, to, scales, vectors);
-  else
-    hipLaunchKernelGGL((mx_pack_kernel<T, 1>), dim3((unsigned)((vectors + 255) / 256)), dim3(256), 0, stream, from, to, scales, vectors);
+  hipLaunchKernelGGL(mx_pack_kernel<T>, dim3((unsigned)((vectors + 255) / 256)), dim3(256), 0, stream, reinterpret_cast<const T*>(x),
+                     reinterpret_cast<unsigned*>(codes), scales, vectors);
   return hipGetLastError();
 }
-template <typename T> hipError_t unpack(const unsigned char* codes, const unsigned char* scales, void* x, long vectors, hipStream_t stream) {
-  const unsigned* from = reinterpret_cast<const unsigned*>(codes);
-  T* to = reinterpret_cast<T*>(x);
-  if (vectors >= 1l << 18)
-    hipLaunchKernelGGL((mx_unpack_kernel<T, 4>), dim3((unsigned)((vectors + 1023) / 1024)), dim3(256), 0, stream, from, scales, to, vectors);
-  else
-    hipLaunchKernelGGL((mx_unpack_kernel<T, 1>), dim3((unsigned)((vectors + 255) / 256)), dim3(256), 0, stream, from, scales, to, vectors);
+template <typename T, int U>
+hipError_t launch_unpack(const unsigned char* codes, const unsigned char* scales, void* x, long vectors, hipStream_t stream) {
+  hipLaunchKernelGGL((mx_unpack_kernel<T, U>), dim3((unsigned)((vectors + 256 * U - 1) / (256 * U))), dim3(256), 0, stream,
+                     reinterpret_cast<const unsigned*>(codes), scales, reinterpret_cast<T*>(x), vectors);
   return hipGetLastError();
+}
+// Four vectors a thread for 16-bit values of 256 MB on, which no cache holds: 2^27 values 58 us (62 with one), 2^26 25.8 (25.5),
+// 2^23 5.2 (4.9). f32 takes one (2^27 values 112 us, 137 with four), and so does packing (2^27 57 and 59, f32 105 and 112).
+template <typename T>
+hipError_t unpack(const unsigned char* codes, const unsigned char* scales, void* x, long vectors, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if (vectors >= 1l << 24) return launch_unpack<T, 4>(codes, scales, x, vectors, stream);
+  return launch_unpack<T, 1>(codes, scales, x, vectors, stream);
 }
 
 }  // namespace

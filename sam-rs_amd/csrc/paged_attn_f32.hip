@@ -15,7 +15,8 @@
 // What bounds it: the f32 matrix rate (64 flops a cycle and SIMD) where many rows share the keys, else the bytes of
 // K and V. 16 rows use each value loaded for 8 flops a byte, twice what L1 would need to keep up. 2048 rows over 4096 keys,
 // 8 heads: head dim 64 191 us (90 TFLOP/s), 128 396 (87; a large library product 153), 256 with 4 heads 520 (66); a step of 32
-// sequences of 4096 keys, 8 key heads of 128, 210 (5.1 TB/s).
+// sequences of 4096 keys, 8 key heads of 128, 210 (5.1 TB/s); of 8192 keys from e2m1 pages 201 (e4m3 216), which the products
+// bound.
 #include "lds_dma.hpp"
 #include "paged.hpp"
 

@@ -1,5 +1,5 @@
 // Paged attention on gfx950 for few rows a key head (a decoding step, a short chunk), f16 / bf16 queries over pages of
-// their own type or of e4m3.
+// their own type, of e4m3 or of e2m1.
 //
 // What bounds it: the bytes of K and V, each used for 4 flops a row. So nothing stands between memory and the matrix
 // units: a wave takes blocks of 32 keys of its workgroup's range, loads their K and V rows straight into registers, the
@@ -9,7 +9,7 @@
 //   into A operands (the output's columns come out permuted, which the store undoes); P stays where S^T left it, since
 //   the reduction index is permuted alike: element j of lane group g is key 16 (j / 4) + 4 g + j % 4.
 // e4m3 codes become 16-bit values with their row's scale in one conversion, exactly (in f16, values below 2^-14 to
-// f16's subnormal step). Softmax statistics and sums are f32. f16 P is rounded to f16 and its sum taken over the rounded
+// f16's subnormal step), and so do e2m1's with their block's. Softmax statistics and sums are f32. f16 P is rounded to f16 and its sum taken over the rounded
 // values, all of it times 2^15, which O / l cancels: weights keep f16's 11 bits down to 2^-29 of the largest, so that
 // thousands of keys far below one that dominates are not lost (each is off by 2^-40 of it at most). The exponent is taken of
 // (score - maximum) * scale, so that scores of any size keep P in f16's range. bf16 P goes as
@@ -19,7 +19,9 @@
 //
 // Measured, 32 sequences of 8192 keys, 8 key heads of 128, one token of 4 query heads a key head: f16 pages 187 us (5.7
 // TB/s), e4m3 pages 107 with f16 queries and 123 with bf16 (5.0 and 4.4; not for their instructions: a fifth fewer took as
-// long). 64-key blocks of e4m3 were no faster.
+// long). 64-key blocks of e4m3 were no faster. e2m1 pages 55 us with f16 queries and 66 with bf16 (5.2 and 4.3 TB/s): half of
+// the bytes of e4m3, so that instructions (conversions, transposition, the exponentials, bf16's two products) bound it as
+// much as memory does; a wave of head dim 64 takes two blocks at a time, whose latencies overlap.
 #include <type_traits>
 
 #include "lds_dma.hpp"

@@ -1,10 +1,10 @@
 // Paged attention on gfx950 for many rows a key head (a prompt's chunk, a frame's queries), f16 / bf16 queries over pages
-// of their own type or of e4m3.
+// of their own type, of e4m3 or of e2m1.
 //
 // Work: a workgroup of four waves takes 128 rows (new token x query head of one key head) and one range of keys; a wave
 // owns 32 rows. Tiles of 64 keys go from their pages into LDS, the next one on its way while this one is worked on, two
-// buffers each, one barrier a tile: 16-bit tiles that every row sees whole straight, others and e4m3 through registers
-// (codes become 16-bit values with their row's scale on the way, once per workgroup). A lane looks one key of the tile up;
+// buffers each, one barrier a tile: 16-bit tiles that every row sees whole straight, others, e4m3 and e2m1 through registers
+// (codes become 16-bit values with their row's or block's scale on the way, once per workgroup). A lane looks one key of the tile up;
 // the loads take their rows from that lane.
 //   S^T = K Q^T on v_mfma_f32_32x32x16 with Q in registers: a lane holds one row's scores of 32 keys, so that softmax
 //   needs one exchange between lane halves. O^T += V^T P^T takes the scores' registers as its B operand under a fixed
@@ -31,7 +31,8 @@
 // count, not a closer order. At 256, with one wave a SIMD, they are 33% and 32%, and the rest is waiting. 8192 rows over
 // 8192 keys, f16: head dim 64 374 us (16 heads, 0.73 PFLOP/s), 96 259 (8 heads, 0.80), 128 309 (8 heads, 0.89), 256 337 (4
 // heads, 0.82); bf16 at 64 542 (0.51), at 128 383 (0.72), with 1.5 times the products; e4m3 at 128 321 (0.86), at 256 374 (0.74),
-// where 8 codes a load instead of 16 took 377 and 417. On a card a tenth slower kAhead 2 took 319, 279 and 370 us at 128, 96 and
+// where 8 codes a load instead of 16 took 377 and 417; e2m1 in f16 363, 253, 301 (0.91) and 357 (0.77) at 64 to 256, in bf16 at
+// 128 382. On a card a tenth slower kAhead 2 took 319, 279 and 370 us at 128, 96 and
 // 256, and 4 317, 271 and 345.
 #include <type_traits>
 

@@ -946,7 +946,8 @@ int check_mx_rows(const char* what, int dtype, long rows, int k) {
   if (!dtype_ok(dtype)) return fail(SAM_HIP_EDTYPE, "unsupported dtype %d for a sam-rs HIP kernel", dtype);
   if (rows < 0 || k <= 0 || k % samhip::kMxBlock != 0)
     return fail(SAM_HIP_EINVAL, "%s: rows of a positive multiple of 32 values, got %ld of %d", what, rows, k);
-  if (rows >= (1L << 36) / k) return fail(SAM_HIP_EUNSUPPORTED, "%s: 2^36 values or more (%ld rows of %d)", what, rows, k);
+  // a thread for 8 values, in workgroups of 256, which a launch counts in 32 bits
+  if (rows > ((1L << 35) - 2048) / k) return fail(SAM_HIP_EUNSUPPORTED, "%s: more than 2^35 - 2048 values (%ld rows of %d)", what, rows, k);
   return SAM_HIP_OK;
 }
 

@@ -55,7 +55,8 @@ def test_linear_workspace(lib):
 @pytest.mark.parametrize("call", [pack, unpack])
 @pytest.mark.parametrize("change, code", [
     ({"x": None}, 1), ({"codes": None}, 1), ({"scales": None}, 1), ({"dtype": 3}, 2), ({"dtype": -1}, 2), ({"rows": -1}, 1),
-    ({"k": 0}, 1), ({"k": 48}, 1), ({"k": -32}, 1), ({"rows": 1 << 31}, 3), ({"x": vp(0x1008)}, 3), ({"codes": vp(0x1004)}, 3)])
+    ({"k": 0}, 1), ({"k": 48}, 1), ({"k": -32}, 1), ({"rows": 1 << 31}, 3), ({"rows": 1 << 30, "k": 32}, 3), ({"x": vp(0x1008)}, 3),
+    ({"codes": vp(0x1004)}, 3)])
 def test_pack_and_unpack_refuse(lib, call, change, code):
     assert call(lib, **change) == code
     assert lib.sam_hip_last_error()
