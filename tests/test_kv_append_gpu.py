@@ -237,6 +237,25 @@ def test_far_positions_keep_their_angles(hip):
 
 
 @pytest.mark.parametrize("held", ["own", "e4m3", "e2m1"])
+def test_pages_past_4_gib(hip, held):
+    """The last pages of pools of more than 2^32 bytes hold what the first ones do, and their neighbours stay."""
+    pages, heads, page, d, n = 72000, 8, 128, 128, 200
+    dt = {"own": torch.float16, "e4m3": torch.float8_e4m3fn, "e2m1": E2M1}[held]
+    raw = [torch.zeros(pages, heads, page, d * 2 if held == "own" else d if held == "e4m3" else d // 2, device="cuda", dtype=torch.uint8) for _ in range(2)]
+    kp, vp = (x.view(dt) for x in raw)
+    scales = [None, None] if held == "own" else [torch.zeros(pages, heads, page, *((d // 32,) if held == "e2m1" else ()), device="cuda", dtype=torch.uint8) for _ in range(2)]
+    assert raw[0].numel() > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(n, h, d, generator=g, device="cuda").half() for h in (16, heads, heads))
+    freqs, axes = hip.rope_freqs((64,))
+    i = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    got = [hip.kv_append(q, k, v, freqs, axes, kp, vp, table.view(1, 2), i(0, n), i(n), *scales) for table in (i(pages - 1, pages - 2), i(0, 1))]
+    assert torch.equal(*got)
+    for x in raw + [s for s in scales if s is not None]:
+        assert torch.equal(x[-1], x[0]) and torch.equal(x[-2], x[1]) and x[0].any() and not x[2].any() and not x[-3].any()
+
+
+@pytest.mark.parametrize("held", ["own", "e4m3", "e2m1"])
 def test_a_decoding_loop_in_a_graph(hip, held):
     """kv_append and paged_attention as a decoder calls them, captured once and replayed as its lengths grow, against the
     eager calls; and a step's results against the whole sequence's in one call."""
