@@ -9,7 +9,7 @@
 // units busy in half of the cycles, at 1.8 to 1.9 GHz; with zeros for codes 219), where the instructions alone, fed from
 // registers, reach 8.6 PFLOP/s at 2.4 GHz. With a short k the results' way out: 4096 x 5120 of k = 1280 in f16 28 us, with
 // bias and GELU 34, of which 42 MB of results need 8 and the activation 6. With few rows B's bytes: 7 rows, 1280 columns of
-// k = 5120 in f32 7.4 us, a launch and the way along a row.
+// k = 5120 in f32 6.0 us, a launch, the packing and the way along a row; 16 rows of 8192 to 8192 columns 12.7 (2.8 TB/s of B).
 #include <algorithm>
 
 #include "gelu.hpp"
@@ -207,19 +207,23 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_product_kernel(MxProduct p, i
 }
 
 // Few rows: B's bytes bound it, so they go from memory straight to the matrix units. A workgroup takes 16 columns of out and
-// RB blocks of 16 rows; its waves take steps of 128 along k in turn and join at the end, in order. RAW: A comes as it is, and
-// each workgroup packs it into LDS first.
+// RB blocks of 16 rows; its waves take rounds of 512 along k in turn and join at the end, in order. Of a round a lane takes four
+// neighbouring blocks of its row, one a step (which blocks meet in a step does not matter while A and B agree): whole lines of a
+// row, and four scales in one load (16 rows of k = 5120 to 1280 columns 5.2 us, 6.7 with neighbouring blocks in neighbouring
+// lanes; 16384 to 1024 11.3 and 16.5; 8192 to 8192 12.7 and 17.0; 8 or 4 columns a workgroup, for more of them, change nothing).
+// RAW: A comes as it is, and each workgroup packs it into LDS first.
 template <typename T, int RB, bool RAW>
 __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
-  constexpr int U = 4;  // steps in flight
+  constexpr int U = 4;  // steps in flight, and bytes of a load of scales
   __shared__ __attribute__((aligned(16))) f32x4 part[16][RB][64];
   extern __shared__ __attribute__((aligned(16))) unsigned char packed[];  // [m][k / 2] codes, then [m][k / 32] scales
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, g = lane >> 4, n0 = 16 * blockIdx.x;
-  const int G = p.k / 32, steps = (G + 3) / 4;
+  const int G = p.k / 32;
   const long rb = p.k / 2;
-  const unsigned char* br = p.b + min(n0 + r, p.n - 1) * rb;
-  const unsigned char* bs = p.sb + min(n0 + r, p.n - 1) * (long)G;
+  const int column = min(n0 + r, p.n - 1);
+  const unsigned char* br = p.b + column * rb;
+  const unsigned char* bs = p.sb + column * (long)G;
   const unsigned char* a0 = RAW ? packed : reinterpret_cast<const unsigned char*>(p.a);
   const unsigned char* sa0 = RAW ? packed + p.m * (p.k / 2) : p.sa;
   const unsigned char *ar[RB], *as[RB];
@@ -251,26 +255,37 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
   f32x4 acc[RB];
 #pragma unroll
   for (int i = 0; i < RB; ++i) acc[i] = f32x4{};
-  for (int t0 = wave; t0 < steps; t0 += U * waves) {
+  // a lane's U blocks of a round follow one another, so that their scales are one load where no row ends inside it
+  auto scales_of = [&](const unsigned char* p, int c) {
+    unsigned s = 0;
+    if (G % U == 0) {
+      __builtin_memcpy(&s, p + min(c, G - U), U);  // scales may begin at any byte
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) s |= (unsigned)p[min(c + u, G - 1)] << (8 * u);
+    }
+    return s;
+  };
+  for (int c0 = 4 * U * wave; c0 < G; c0 += 4 * U * waves) {
+    const int c = c0 + U * g;
     u32x4 b[U], a[U][RB];
-    unsigned char sb[U], sa[U][RB];
+    unsigned sb, sa[RB];
+    sb = scales_of(bs, c);
+#pragma unroll
+    for (int i = 0; i < RB; ++i) sa[i] = scales_of(as[i], c);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int c = min(4 * (t0 + u * waves) + g, G - 1);
-      b[u] = *reinterpret_cast<const u32x4*>(br + 16 * c);
-      sb[u] = bs[c];
+      const int at = 16 * min(c + u, G - 1);
+      b[u] = *reinterpret_cast<const u32x4*>(br + at);
 #pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        a[u][i] = *reinterpret_cast<const u32x4*>(ar[i] + 16 * c);
-        sa[u][i] = as[i][c];
-      }
+      for (int i = 0; i < RB; ++i) a[u][i] = *reinterpret_cast<const u32x4*>(ar[i] + at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool in = 4 * (t0 + u * waves) + g < G;  // blocks past the row's end: zeros under 2^-127
+      const bool in = c + u < G;  // blocks past the row's end: zeros under 2^-127
       const u32x4 bu = in ? b[u] : u32x4{};
 #pragma unroll
-      for (int i = 0; i < RB; ++i) acc[i] = mma_mx16(bu, in ? sb[u] : 0u, a[u][i], in ? sa[u][i] : 0u, acc[i]);
+      for (int i = 0; i < RB; ++i) acc[i] = mma_mx16(bu, in ? sb >> (8 * u) & 255 : 0u, a[u][i], in ? sa[i] >> (8 * u) & 255 : 0u, acc[i]);
     }
   }
 #pragma unroll
@@ -305,8 +320,8 @@ constexpr int kMostPacked = 16 * (8192 / 2 + 8192 / 32);  // bytes of LDS
 
 template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream) {
   if (p.m <= 32) {
-    // as many waves as have each its four steps in flight once: 16 rows of k = 5120 to 1280 columns 6.7 us with 10, 7.1, 7.7, 9.5 and
-    // 9.6 with 2, 4, 8 and 16; of 1280 to 5120 4.0 with 3, 4.5 and 7.0 with 2 and 8
+    // a wave for each round: 16 rows of k = 5120 to 1280 columns 5.2 us with 10, 6.7, 5.5, 5.4, 5.3 and 5.4 with 1, 2, 4, 8 and 16; of
+    // 1280 to 5120 3.8 with 3, 4.1, 3.9, 3.9, 4.1 and 4.2
     const int waves = (int)std::min(16, std::max(1, (p.k + 511) / 512));
     const dim3 grid((unsigned)((p.n + 15) / 16));
     if (!p.sa) {
@@ -337,8 +352,9 @@ template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream)
 }  // namespace
 
 // Whether a linear layer's few rows are packed by each workgroup of 16 columns again, in place of a launch of their own: up to
-// 16 rows while a CU's workgroups pack 8192 values of a row in all. Kernel times: 7 rows of 5120 to 1280 columns in f32 7.4 us,
-// 2.3 and 6.2 in two launches; 16 rows of 8192 to 4096 columns in f16 13.4, and 2.5 and 10.2.
+// 16 rows while a CU's workgroups pack 8192 values of a row in all. On the card 7 rows of 5120 to 1280 columns in f32 take 6.0 us
+// so and 6.5 in two launches, 16 of 1280 to 5120 in f16 6.2 and 5.8, 16 of 4096 to 4096 7.6 and 6.9, of 8192 to 4096 11.5 and 9.2;
+// a launch takes the host 3 more.
 bool mx_packs_on_the_way(int m, int n, int k) { return m <= 16 && ((long)n + 4095) / 4096 * k <= 8192; }
 
 hipError_t mx_matmul(int dtype, const MxProduct& p, hipStream_t stream) {
