@@ -206,24 +206,28 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_product_kernel(MxProduct p, i
   }
 }
 
-// Few rows: B's bytes bound it, so they go from memory straight to the matrix units. A workgroup takes 16 columns of out and
-// RB blocks of 16 rows; its waves take rounds of 512 along k in turn and join at the end, in order. Of a round a lane takes four
+// Few rows: B's bytes bound it, so they go from memory straight to the matrix units. A workgroup takes CB blocks of 16 columns
+// of out and RB of 16 rows; its waves take rounds of 512 along k in turn and join at the end, in order. Of a round a lane takes four
 // neighbouring blocks of its row, one a step (which blocks meet in a step does not matter while A and B agree): whole lines of a
 // row, and four scales in one load (16 rows of k = 5120 to 1280 columns 5.2 us, 6.7 with neighbouring blocks in neighbouring
 // lanes; 16384 to 1024 11.3 and 16.5; 8192 to 8192 12.7 and 17.0; 8 or 4 columns a workgroup, for more of them, change nothing).
 // RAW: A comes as it is, and each workgroup packs it into LDS first.
-template <typename T, int RB, bool RAW>
+template <typename T, int RB, int CB, bool RAW>
 __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
   constexpr int U = 4;  // steps in flight, and bytes of a load of scales
-  __shared__ __attribute__((aligned(16))) f32x4 part[16][RB][64];
+  __shared__ __attribute__((aligned(16))) f32x4 part[16][CB * RB][64];
   extern __shared__ __attribute__((aligned(16))) unsigned char packed[];  // [m][k / 2] codes, then [m][k / 32] scales
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int r = lane & 15, g = lane >> 4, n0 = 16 * blockIdx.x;
+  const int r = lane & 15, g = lane >> 4, n0 = 16 * CB * blockIdx.x;
   const int G = p.k / 32;
   const long rb = p.k / 2;
-  const int column = min(n0 + r, p.n - 1);
-  const unsigned char* br = p.b + column * rb;
-  const unsigned char* bs = p.sb + column * (long)G;
+  const unsigned char *br[CB], *bs[CB];
+#pragma unroll
+  for (int j = 0; j < CB; ++j) {
+    const int column = min(n0 + 16 * j + r, p.n - 1);
+    br[j] = p.b + column * rb;
+    bs[j] = p.sb + column * (long)G;
+  }
   const unsigned char* a0 = RAW ? packed : reinterpret_cast<const unsigned char*>(p.a);
   const unsigned char* sa0 = RAW ? packed + p.m * (p.k / 2) : p.sa;
   const unsigned char *ar[RB], *as[RB];
@@ -252,9 +256,11 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
     }
     __syncthreads();
   }
-  f32x4 acc[RB];
+  f32x4 acc[CB][RB];
 #pragma unroll
-  for (int i = 0; i < RB; ++i) acc[i] = f32x4{};
+  for (int j = 0; j < CB; ++j)
+#pragma unroll
+    for (int i = 0; i < RB; ++i) acc[j][i] = f32x4{};
   // a lane's U blocks of a round follow one another, so that their scales are one load where no row ends inside it
   auto scales_of = [&](const unsigned char* p, int c) {
     unsigned s = 0;
@@ -268,33 +274,41 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxProduct p) {
   };
   for (int c0 = 4 * U * wave; c0 < G; c0 += 4 * U * waves) {
     const int c = c0 + U * g;
-    u32x4 b[U], a[U][RB];
-    unsigned sb, sa[RB];
-    sb = scales_of(bs, c);
+    u32x4 b[U][CB], a[U][RB];
+    unsigned sb[CB], sa[RB];
+#pragma unroll
+    for (int j = 0; j < CB; ++j) sb[j] = scales_of(bs[j], c);
 #pragma unroll
     for (int i = 0; i < RB; ++i) sa[i] = scales_of(as[i], c);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = 16 * min(c + u, G - 1);
-      b[u] = *reinterpret_cast<const u32x4*>(br + at);
+#pragma unroll
+      for (int j = 0; j < CB; ++j) b[u][j] = *reinterpret_cast<const u32x4*>(br[j] + at);
 #pragma unroll
       for (int i = 0; i < RB; ++i) a[u][i] = *reinterpret_cast<const u32x4*>(ar[i] + at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = c + u < G;  // blocks past the row's end: zeros under 2^-127
-      const u32x4 bu = in ? b[u] : u32x4{};
 #pragma unroll
-      for (int i = 0; i < RB; ++i) acc[i] = mma_mx16(bu, in ? sb >> (8 * u) & 255 : 0u, a[u][i], in ? sa[i] >> (8 * u) & 255 : 0u, acc[i]);
+      for (int j = 0; j < CB; ++j) {
+        const u32x4 bu = in ? b[u][j] : u32x4{};
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+          acc[j][i] = mma_mx16(bu, in ? sb[j] >> (8 * u) & 255 : 0u, a[u][i], in ? sa[i] >> (8 * u) & 255 : 0u, acc[j][i]);
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < RB; ++i) part[wave][i][lane] = acc[i];
+  for (int j = 0; j < CB; ++j)
+#pragma unroll
+    for (int i = 0; i < RB; ++i) part[wave][j * RB + i][lane] = acc[j][i];
   __syncthreads();
-  for (int i = wave; i < RB; i += waves) {
+  for (int i = wave; i < CB * RB; i += waves) {
     f32x4 x = part[0][i][lane];
     for (int w = 1; w < waves; ++w) x += part[w][i][lane];
-    put4<T>(p, 16 * i + r, n0 + 4 * g, x, p.n % 4 == 0);
+    put4<T>(p, 16 * (i % RB) + r, n0 + 16 * (i / RB) + 4 * g, x, p.n % 4 == 0);
   }
 }
 
@@ -318,28 +332,37 @@ template <typename T, int TM, int TN, int WM, int WN> hipError_t by_alignment(co
 
 constexpr int kMostPacked = 16 * (8192 / 2 + 8192 / 32);  // bytes of LDS
 
+template <typename T, int CB> hipError_t few(const MxProduct& p, hipStream_t stream) {
+  // a wave for each round: 16 rows of k = 5120 to 1280 columns 5.2 us with 10, 6.7, 5.5, 5.4, 5.3 and 5.4 with 1, 2, 4, 8 and 16; of
+  // 1280 to 5120 3.8 with 3, 4.1, 3.9, 3.9, 4.1 and 4.2
+  const int waves = (int)std::min(16, std::max(1, (p.k + 511) / 512));
+  const dim3 grid((unsigned)((p.n + 16 * CB - 1) / (16 * CB)));
+  if (!p.sa) {
+    const int lds = p.m * (p.k / 2 + p.k / 32);
+    static std::atomic<unsigned long long> done;
+    if (const hipError_t e = lds_opt_in(done, (const void*)mx_few_kernel<T, 1, CB, true>, kMostPacked); e != hipSuccess) return e;
+    hipLaunchKernelGGL((mx_few_kernel<T, 1, CB, true>), grid, dim3(64 * waves), lds, stream, p);
+  } else if (p.m <= 16)
+    hipLaunchKernelGGL((mx_few_kernel<T, 1, CB, false>), grid, dim3(64 * waves), 0, stream, p);
+  else
+    hipLaunchKernelGGL((mx_few_kernel<T, 2, CB, false>), grid, dim3(64 * waves), 0, stream, p);
+  return hipGetLastError();
+}
+
 template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream) {
+  const long cus = device_cu_count(), steps = (p.k + 255) / 256;
   if (p.m <= 32) {
-    // a wave for each round: 16 rows of k = 5120 to 1280 columns 5.2 us with 10, 6.7, 5.5, 5.4, 5.3 and 5.4 with 1, 2, 4, 8 and 16; of
-    // 1280 to 5120 3.8 with 3, 4.1, 3.9, 3.9, 4.1 and 4.2
-    const int waves = (int)std::min(16, std::max(1, (p.k + 511) / 512));
-    const dim3 grid((unsigned)((p.n + 15) / 16));
-    if (!p.sa) {
-      const int lds = p.m * (p.k / 2 + p.k / 32);
-      static std::atomic<unsigned long long> done;
-      if (const hipError_t e = lds_opt_in(done, (const void*)mx_few_kernel<T, 1, true>, kMostPacked); e != hipSuccess) return e;
-      hipLaunchKernelGGL((mx_few_kernel<T, 1, true>), grid, dim3(64 * waves), lds, stream, p);
-    } else if (p.m <= 16)
-      hipLaunchKernelGGL((mx_few_kernel<T, 1, false>), grid, dim3(64 * waves), 0, stream, p);
-    else
-      hipLaunchKernelGGL((mx_few_kernel<T, 2, false>), grid, dim3(64 * waves), 0, stream, p);
-    return hipGetLastError();
+    // Two blocks of columns a workgroup, which share what it loads of A, past 8 rows and where no CU gets more columns so: 16 rows
+    // of 1280 to 5120 columns 3.6 and 3.9 us with two and one, 1 row 3.3 and 3.3; of 8192 to 8192 17 rows 12.2 and 14.5, 32 17.8 and
+    // 25.5, 8 10.1 and 10.2; of 4096 to 32768 12 rows 18.0 and 19.9, 4 17.3 and 15.9; of 4096 to 11000 (4 and 3 blocks a CU) 16 rows
+    // 10.6 and 9.3; of 5120 to 1280 6.6 and 5.2.
+    auto most = [&](long cb) { return cb * (((p.n + 16 * cb - 1) / (16 * cb) + cus - 1) / cus); };
+    return p.m > 8 && most(2) <= most(1) ? few<T, 2>(p, stream) : few<T, 1>(p, stream);
   }
   // The tiles that take least: so many a CU, each its steps and its beginning and end, in ns (what a CU's tiles cost together,
   // as one's waits are another's work). Kernel times in f16 by tiles of 64, 128 and 256: 300 x 1280 of k = 5120 10.7 and 16.7 us,
   // 4096 x 1280 of 1280 13.4 and 11.4, 4096 x 1280 of 5120 34, 27 and 38, 4096 x 3840 of 1280 30, 22 and 19, 4096 x 5120 of 1280
   // 28 and 32 (128, 256), 16001 x 1024 of 4096 49 and 40, 16384 x 4096 of 4096 184 and 156.
-  const long cus = device_cu_count(), steps = (p.k + 255) / 256;
   auto cost = [&](long tile, long step, long ends) {
     const long tiles = (p.m + tile - 1) / tile * ((p.n + tile - 1) / tile);
     return (tiles + cus - 1) / cus * (steps * step + ends);

@@ -100,6 +100,22 @@ def test_products(hip, dtype, size):
         assert torch.equal(hip.mx_linear(a, bc, bsc, bias if with_bias else None, gelu=act), got)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [(8, 4100, 64), (9, 4100, 32), (9, 5120, 1280), (12, 5003, 96), (16, 6144, 544), (17, 8189, 160), (32, 4600, 1120), (16, 8192, 4096)])
+def test_few_rows_of_wide_layers(hip, dtype, size):
+    """Two blocks of columns a workgroup, ragged ones too, with scales that begin at any byte."""
+    m, n, k = size
+    dt = DT[dtype]
+    a, b, bias = operands(m, n, k, dt, m + n + k)
+    (ac, asc), (bc, bsc) = hip.mx_pack(a), hip.mx_pack(b)
+    want, bound = ref.product(ref.values(ac, asc), ref.values(bc, bsc), bias.cpu(), True, dt)
+    off = [torch.full((s.numel() + 3,), 255, device="cuda", dtype=torch.uint8)[i:i + s.numel()].view(s.shape).copy_(s) for i, s in ((1, asc), (3, bsc))]
+    for sa, sb in ((asc, bsc), off):
+        got = hip.mx_matmul(ac, sa, bc, sb, bias, gelu=True, dtype=dt)
+        assert ((got.cpu().double() - want).abs() <= bound).all(), float(((got.cpu().double() - want).abs() / bound).max())
+        assert torch.equal(hip.mx_linear(a, bc, sb, bias, gelu=True), got)
+
+
 @pytest.mark.parametrize("m", [1, 20, 100, 1601])
 def test_nan_blocks_stay_in_their_rows_and_columns(hip, m):
     n, k = 2001 if m > 1000 else 90, 160
