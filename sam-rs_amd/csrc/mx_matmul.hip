@@ -376,8 +376,7 @@ template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream)
 
 // Whether a linear layer's few rows are packed by each workgroup of 16 columns again, in place of a launch of their own: up to
 // 16 rows while a CU's workgroups pack 8192 values of a row in all. On the card 7 rows of 5120 to 1280 columns in f32 take 6.0 us
-// so and 6.5 in two launches, 16 of 1280 to 5120 in f16 6.2 and 5.8, 16 of 4096 to 4096 7.6 and 6.9, of 8192 to 4096 11.5 and 9.2;
-// a launch takes the host 3 more.
+// so and 6.5 in two launches, 16 of 4096 to 4096 in f16 7.6 and 6.9, of 8192 to 4096 11.5 and 9.2; a launch takes the host 3 more.
 bool mx_packs_on_the_way(int m, int n, int k) { return m <= 16 && ((long)n + 4095) / 4096 * k <= 8192; }
 
 hipError_t mx_matmul(int dtype, const MxProduct& p, hipStream_t stream) {
