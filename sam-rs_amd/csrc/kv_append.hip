@@ -181,7 +181,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
   const int b = sequence_of<LPR>(p.c, t, lane < p.c.batch ? ends : 0x7fffffff);
   int from, to, len;
   if (p.c.batch <= 64) {
-    from = b > 0 ? __shfl(ends, min(b, p.c.batch) - 1) : first;
+    const int before = __shfl(ends, max(min(b, p.c.batch) - 1, 0));  // by every lane: a lane left out would give 0
+    from = b > 0 ? before : first;
     to = __shfl(ends, min(b, p.c.batch - 1));
     len = __shfl(held, min(b, p.c.batch - 1));
   } else {
