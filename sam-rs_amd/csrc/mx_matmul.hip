@@ -18,6 +18,20 @@
 
 namespace samhip {
 
+// The rows and columns of the tiles that take least: so many a CU, each its steps and its beginning and end, in ns (what a CU's
+// tiles cost together, as one's waits are another's work). Kernel times in f16 by tiles of 64, 128 and 256: 300 x 1280 of k = 5120
+// 10.7 and 16.7 us, 4096 x 1280 of 1280 13.4 and 11.4, 4096 x 1280 of 5120 34, 27 and 38, 4096 x 3840 of 1280 30, 22 and 19, 4096 x
+// 5120 of 1280 28 and 32 (128, 256), 16001 x 1024 of 4096 49 and 40, 16384 x 4096 of 4096 184 and 156. No tiles of 64, of 256 threads
+// each, where a launch would count past 32 bits of them.
+int mx_product_tile(int cus, int m, int n, int k) {
+  const long steps = (k + 255) / 256;
+  auto tiles = [&](long tile) { return (m + tile - 1) / tile * ((n + tile - 1) / tile); };
+  auto cost = [&](long tile, long step, long ends) { return (tiles(tile) + cus - 1) / cus * (steps * step + ends); };
+  const long large = cost(256, 2100, 5000), middle = cost(128, 670, 2300), small = cost(64, 360, 500);
+  if (large < middle && large < small) return 256;
+  return middle < small || tiles(64) > (1l << 24) - 8 ? 128 : 64;
+}
+
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -350,7 +364,7 @@ template <typename T, int CB> hipError_t few(const MxProduct& p, hipStream_t str
 }
 
 template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream) {
-  const long cus = device_cu_count(), steps = (p.k + 255) / 256;
+  const long cus = device_cu_count();
   if (p.m <= 32) {
     // Two blocks of columns a workgroup, which share what it loads of A, past 8 rows and where no CU gets more columns so: 16 rows
     // of 1280 to 5120 columns 3.6 and 3.9 us with two and one, 1 row 3.3 and 3.3; of 8192 to 8192 17 rows 12.2 and 14.5, 32 17.8 and
@@ -359,17 +373,9 @@ template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream)
     auto most = [&](long cb) { return cb * (((p.n + 16 * cb - 1) / (16 * cb) + cus - 1) / cus); };
     return p.m > 8 && most(2) <= most(1) ? few<T, 2>(p, stream) : few<T, 1>(p, stream);
   }
-  // The tiles that take least: so many a CU, each its steps and its beginning and end, in ns (what a CU's tiles cost together,
-  // as one's waits are another's work). Kernel times in f16 by tiles of 64, 128 and 256: 300 x 1280 of k = 5120 10.7 and 16.7 us,
-  // 4096 x 1280 of 1280 13.4 and 11.4, 4096 x 1280 of 5120 34, 27 and 38, 4096 x 3840 of 1280 30, 22 and 19, 4096 x 5120 of 1280
-  // 28 and 32 (128, 256), 16001 x 1024 of 4096 49 and 40, 16384 x 4096 of 4096 184 and 156.
-  auto cost = [&](long tile, long step, long ends) {
-    const long tiles = (p.m + tile - 1) / tile * ((p.n + tile - 1) / tile);
-    return (tiles + cus - 1) / cus * (steps * step + ends);
-  };
-  const long large = cost(256, 2100, 5000), middle = cost(128, 670, 2300), small = cost(64, 360, 500);
-  if (large < middle && large < small) return by_alignment<T, 256, 256, 2, 4>(p, stream);
-  return middle < small ? by_alignment<T, 128, 128, 2, 2>(p, stream) : by_alignment<T, 64, 64, 2, 2>(p, stream);
+  const int tile = mx_product_tile((int)cus, p.m, p.n, p.k);
+  if (tile == 256) return by_alignment<T, 256, 256, 2, 4>(p, stream);
+  return tile == 128 ? by_alignment<T, 128, 128, 2, 2>(p, stream) : by_alignment<T, 64, 64, 2, 2>(p, stream);
 }
 
 }  // namespace

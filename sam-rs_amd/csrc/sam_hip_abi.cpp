@@ -936,6 +936,7 @@ int check_mx_product(const char* what, int dtype, int m, int n, int k) {
   if (m < 0 || n < 0 || k <= 0 || k % samhip::kMxBlock != 0)
     return fail(SAM_HIP_EINVAL, "%s: sizes m=%d n=%d k=%d (k a positive multiple of 32)", what, m, n, k);
   // the launches count workgroups of up to 1024 threads for 16 columns, or of 256 for 128 x 128 results, in 32 bits of threads
+  // (smaller tiles are taken where those fit too)
   if ((long)m * n >= 1L << 36 || m > (1 << 30) || n > (1 << 25) || k > 1 << 22 ||
       ((long)m + 127) / 128 * (((long)n + 127) / 128) >= 1L << 23)
     return fail(SAM_HIP_EUNSUPPORTED, "%s: too many results, or k beyond 2^22 (m=%d n=%d k=%d)", what, m, n, k);
