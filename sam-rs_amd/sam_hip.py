@@ -25,6 +25,8 @@ Names, argument meaning and errors follow the reference:
 
 rope_axes to paged_attention are the paged form of the video memory (sam3/video.rs:133-145, 356-406); the reference
 has no entry points of that kind.
+4-bit codes are torch.float4_e2m1fn_x2; on a torch without that type the mx_ calls and pools of 4 bits are refused, all else
+works. Their scales are uint8; a torch.float8_e8m0fnu tensor has the same bytes, as s.view(torch.uint8).
 
 There is no CPU fallback: on a machine without the built library or a GPU every call raises. While the
 switch is off every call raises SamHipDisabled without touching the device; the caller then takes its
@@ -633,7 +635,7 @@ def rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch
 # ------------------------------------------------------------------------------------------ the paged memory
 
 _E4M3, _E2M1_CODE = 3, 4  # SAM_HIP_E4M3, SAM_HIP_E2M1
-_E2M1 = torch.float4_e2m1fn_x2  # two codes a byte, the even column's in the low half
+_E2M1 = getattr(torch, "float4_e2m1fn_x2", None)  # two codes a byte, the even column's in the low half; older torches lack it
 _BLOCK = 32  # values of a row that share a scale
 
 
@@ -1025,8 +1027,16 @@ def _mx_k(what, shape) -> int:
     return shape[-1]
 
 
+def _mx_type(what) -> torch.dtype:
+    """The dtype of codes."""
+    if _E2M1 is None:
+        raise SamHipError(f"{what}: this torch ({torch.__version__}) has no float4_e2m1fn_x2, which holds 4-bit numbers")
+    return _E2M1
+
+
 def _mx_operand(what, name, codes, scale):
     """A packed matrix as (codes, scale, shape of the values), contiguous and aligned, after its checks."""
+    _mx_type(what)
     if codes.dtype != _E2M1 or codes.dim() == 0:
         raise SamHipError(f"{what}: {name} must hold torch.float4_e2m1fn_x2, [.., K / 2], got {codes.dtype} {tuple(codes.shape)}")
     shape = codes.shape[:-1] + (2 * codes.shape[-1],)
@@ -1053,7 +1063,7 @@ def mx_pack(x: torch.Tensor):
     x = _plain(x)
     if x.data_ptr() % 16:
         x = x.clone()
-    codes = x.new_empty(shape[:-1] + (k // 2,), dtype=_E2M1)
+    codes = x.new_empty(shape[:-1] + (k // 2,), dtype=_mx_type("mx_pack"))
     scale = x.new_empty(shape[:-1] + (k // _BLOCK,), dtype=torch.uint8)
     if x.numel() == 0:
         _empty_call("mx-pack")
