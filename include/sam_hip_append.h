@@ -18,9 +18,9 @@ extern "C" {
  * reference's corresponds to it: its memory attention projects, rotates and concatenates (sam3/video.rs:129-145, 356-406).
  *
  * A turned key is rounded once, to dtype or to its e4m3 or e2m1 codes (the turn is formed in f64; angles are exact to 2^-50 up
- * to 2^48 radians); a turned query is formed in f32 and rounded to dtype. The cache, its tables and what is checked on the
- * device are those of sam_hip_kv_write. Rows of q that belong to no sequence stay as they are in out, or become 0 with
- * zero_rest; a token of a sequence that has no place in its pages still has its query turned.
+ * to 2^48 radians; beyond f32's largest number it is infinite); a turned query is formed in f32 and rounded to dtype. The cache,
+ * its tables and what is checked on the device are those of sam_hip_kv_write. Rows of q that belong to no sequence stay as they
+ * are in out, or become 0 with zero_rest; a token of a sequence that has no place in its pages still has its query turned.
  * q and out may both be NULL (heads is ignored then); with pairs == 0 pos, freqs and axes may be. Strides: (token, head) of q,
  * k, v and out in multiples of 16 bytes, (token, axis) of pos; NULL = contiguous; out's rows lie apart. out may be q with the
  * same strides; it must not overlap q otherwise, nor the other tensors. Limits: those of the paged memory, up to 65535 query

@@ -93,11 +93,11 @@ __device__ __forceinline__ void turn_of(double a, float& c, float& s) {
 }
 
 // x in f32, rounded to odd: cut short, and its last bit set if anything was cut off. Rounding that to fewer bits (up to 22)
-// gives what rounding x to them would.
+// gives what rounding x to them would. x beyond f32's largest number is infinite, as it is to kv_write.
 __device__ __forceinline__ float to_odd(double x) {
   const float f = (float)x;
   unsigned u = __float_as_uint(f);
-  if ((double)f != x) u = (fabs((double)f) > fabs(x) ? u - 1 : u) | 1u;
+  if ((double)f != x && fabsf(f) < INFINITY) u = (fabs((double)f) > fabs(x) ? u - 1 : u) | 1u;
   return __uint_as_float(u);
 }
 
