@@ -49,7 +49,11 @@ PagedPlan paged_plan(int dtype, int cache_dtype, int tokens, int batch, int head
     // the card, of 512 KB of keys and values each at least. 32 sequences, 8 key heads of 128 in e4m3: 820 to 8192 keys 92, 94,
     // 80, 84, 83 and 96 us with 2, 3, 4, 6, 8 and 12 splits, 8192 each 118, 118, 121, 125, 134 and 148; 4 heads of 256 in e4m3,
     // 8192 each, 103, 112 and 132 with 2, 4 and 8. Calls that f32 products bound count rounds.
-    const bool mx = cache_dtype == kE2M1;
+    // F32 over e2m1 pages is split as over f32 ones, whose products take as long: 41 chunks of 125 rows over 4320 keys, one head, at
+    // 96 191, 142 and 163 us with 2, 3 (f32's rule) and 4, 500 rows over 1500 keys of one head of 128 74 and 22 with 1 and 12 (f32's), a
+    // token over 1024 keys of 8 heads of 128 33 and 12 with 1 and 8 (f32's), 32 steps of 8192, 8 heads of 128, 201, 202 and 206 with 2, 4
+    // (f32's) and 8; the first of each but the last is what the rule of 16 bits below would take.
+    const bool mx = cache_dtype == kE2M1 && dtype != kF32;
     const long bytes = 2L * d * (cache_dtype == kE4M3 ? 1 : dtype == kF32 ? 4 : 2) * max_len;  // a sequence's, of one head
     const long want = plan.rtiles > 1 && dtype == kF32 ? f32_splits(base, (d > 64 ? 1L : 2L) * cus)
                                                        : ((d > 128 ? mx ? 1L : 2L : 4L) * cus + base - 1) / base;
