@@ -17,9 +17,25 @@
 // Measured: 65536 tokens of 8 query and 8 key heads of 128 in bf16, all pairs turned, into pages of bf16, e4m3 and e2m1 147,
 // 130 and 117 us (5.5, 5.2 and 5.2 TB/s; kv_write of the same keys alone takes 96, 83 and 75, rope_axes of the queries 44 and of
 // the keys as much again). 32 tokens of 32 and 8 heads are latency: 5.8 us, most of it the chain from the table to a store.
+#include <algorithm>
+
 #include "kv_rows.hpp"
 
 namespace samhip {
+
+static int lanes_of_row(int d) { return d <= 64 ? 8 : d <= 128 ? 16 : 32; }
+
+// How many heads of a token a thread takes, which share its angles: several where there are threads enough for all CUs without,
+// and as many query or key heads (the other part's threads then do less than they could, and there are fewer of them). 16 query
+// heads of 128 in bf16 over 1, 2, 3 and 4 key heads, 16384 tokens: 62, 63, 66 and 71 us with one, 36, 34, 35 and 36 with four; 1024
+// tokens over 1 key head 7.7 and 7.6, 512, which take one, 6.0 and 7.0; 4 over 2, 16384 tokens, 27 and 20; 2 over 2, which take one,
+// 22 and 20, 1 over 1 head of 256 22 and 30. In f32, whose rows take twice the registers, two: 16 over 1, 2, 3 and 4 74, 81, 89
+// and 98 with one, 64, 69, 78 and 82 with two; 512 tokens over 1, which take one, 6.1 and 5.8.
+int kv_append_heads(int element, int tokens, int heads, int kv_heads, int d) {
+  const long rows = (long)tokens * (heads + kv_heads);
+  const int most = element == 4 ? 2 : 4;
+  return rows * lanes_of_row(d) >= 1 << 18 && std::max(heads, kv_heads) >= most ? most : 1;
+}
 
 namespace {
 
@@ -126,7 +142,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
   unsigned turn = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) turn |= col + j < 2 * p.pairs ? 1u << j : 0u;
-  const bool even = p.pairs % 8 == 0;  // halves: a lane's elements have one role
+  // halves: a lane's elements have one role, and its partners are one load. With other counts of pairs they are loaded one by one:
+  // 16384 tokens of 16 and 4 heads of 128, bf16 with 64, 48 and 32 pairs 36 us, with 45, 29 and 13 47, 51 and 55, f32 83 and 103 to
+  // 109, 32 tokens 5.3 and 5.7
+  const bool even = p.pairs % 8 == 0;
   const bool low = col < p.pairs;
 
   // Everything that depends on nothing goes out at once, the ends and lengths of the first 64 sequences first, one to a lane:
@@ -318,17 +337,14 @@ template <typename T, typename C, int LPR, int HP> hipError_t launch(KvAppendPar
     hipLaunchKernelGGL((kv_append_kernel<T, C, LPR, HP, false>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
-// Several heads of a token to a thread, which share their angles, where there are threads enough for all CUs without: 4 key and 16
-// query heads of 128 in bf16, 512 tokens 6.4 us with one head and 7.1 with four, 1024 8.1 and 7.7, 2048 13.3 and 9.4, 16384 71
-// and 35; in f32, whose rows take twice the registers, two: 512 6.7 and 6.6, 1024 9.2 and 8.3, 16384 92 and 80.
 template <typename T, typename C, int LPR> hipError_t by_heads(const KvAppendParams& p, bool halves, hipStream_t stream) {
-  const long rows = (long)p.tokens * (p.heads + p.c.heads);
   constexpr int kHeads = sizeof(T) == 4 ? 2 : 4;
-  return rows * LPR >= 1 << 18 && p.c.heads >= kHeads ? launch<T, C, LPR, kHeads>(p, halves, stream) : launch<T, C, LPR, 1>(p, halves, stream);
+  return kv_append_heads(sizeof(T), p.tokens, p.heads, p.c.heads, p.c.d) > 1 ? launch<T, C, LPR, kHeads>(p, halves, stream)
+                                                                             : launch<T, C, LPR, 1>(p, halves, stream);
 }
 template <typename T, typename C> hipError_t by_size(const KvAppendParams& p, bool halves, hipStream_t stream) {
-  return p.c.d <= 64 ? by_heads<T, C, 8>(p, halves, stream)
-                     : p.c.d <= 128 ? by_heads<T, C, 16>(p, halves, stream) : by_heads<T, C, 32>(p, halves, stream);
+  const int lpr = lanes_of_row(p.c.d);
+  return lpr == 8 ? by_heads<T, C, 8>(p, halves, stream) : lpr == 16 ? by_heads<T, C, 16>(p, halves, stream) : by_heads<T, C, 32>(p, halves, stream);
 }
 template <typename T> hipError_t by_held(int cache_dtype, const KvAppendParams& p, bool halves, hipStream_t stream) {
   return cache_dtype == kE2M1 ? by_size<T, e2m1>(p, halves, stream)
