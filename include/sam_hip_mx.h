@@ -39,8 +39,9 @@ int sam_hip_mx_matmul(const unsigned char* a, const unsigned char* a_scale, cons
 /*
  * A linear layer with 4-bit weights: sam_hip_mx_pack of x [m, k] into the workspace, then sam_hip_mx_matmul of it and of w,
  * w_scale (as sam_hip_mx_pack makes them from [n, k]) to out [m, n]. Workspace: sam_hip_mx_linear_workspace_size() bytes of
- * device memory, 16-byte aligned (0 needs none, as a few rows are packed on their way to the product; -1 is an error); calls
- * that may overlap need their own, and so does each captured graph that may run beside another.
+ * device memory, 16-byte aligned (0 needs none, as a few rows are packed on their way to the product; -1 is an error; it depends
+ * on the current device's CU count); calls that may overlap need their own, and so does each captured graph that may run beside
+ * another.
  */
 long sam_hip_mx_linear_workspace_size(int m, int n, int k);
 int sam_hip_mx_linear(const void* x, const unsigned char* w, const unsigned char* w_scale, const void* bias, void* out,

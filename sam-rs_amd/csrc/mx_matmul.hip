@@ -32,6 +32,25 @@ int mx_product_tile(int cus, int m, int n, int k) {
   return middle < small || tiles(64) > (1l << 24) - 8 ? 128 : 64;
 }
 
+// Workgroups of the few-row kernel that a CU gets at `blocks` blocks of 16 columns each.
+static long few_share(int cus, int n, int blocks) { return ((n + 16l * blocks - 1) / (16l * blocks) + cus - 1) / cus; }
+// Two blocks of columns a workgroup, which share what it loads of A, past 8 rows and where no CU gets more columns so: 16 rows of
+// 1280 to 5120 columns 3.6 and 3.9 us with two and one, 1 row 3.3 and 3.3; of 8192 to 8192 17 rows 12.2 and 14.5, 32 17.8 and 25.5, 8
+// 10.1 and 10.2; of 4096 to 32768 12 rows 18.0 and 19.9, 4 17.3 and 15.9; of 4096 to 11000 (4 and 3 blocks a CU) 16 rows 10.6 and
+// 9.3; of 5120 to 1280 6.6 and 5.2.
+static int few_blocks(int cus, int m, int n) { return m > 8 && 2 * few_share(cus, n, 2) <= few_share(cus, n, 1) ? 2 : 1; }
+
+// Whether a linear layer's few rows are packed by each workgroup of the few-row kernel again, in place of a launch of their own: up
+// to 16 rows while a CU's workgroups pack 8192 values of a row in all, which is also what LDS holds of one. In f16 on the card, so
+// and in two launches: 4096 to 4096 columns 1 row 4.5 and 5.8 us, 8 5.7 and 6.4, 16 7.5 and 6.8; 8192 to 4096 8.7 and 8.7 with 8, 11.7
+// and 9.8 with 16; 8192 to 8192, where a CU packs once past 8 rows, 12.4 and 12.6 with 9, 14.7 and 14.8 with 16; 4096 to 16384 14.3
+// and 12.8 with 16; 5120 to 6144, which takes two up to 8 rows, 7.3 and 8.3 with 4, 9.2 and 8.8 with 8. A launch takes the host 3
+// more: called one after the other, 16 rows of 5120 to 8192 take 10.0 and 13.3, of 4096 to 16384 13.9 and 13.3.
+bool mx_packs_on_the_way(int m, int n, int k) {
+  const int cus = device_cu_count();
+  return m <= 16 && few_share(cus, n, few_blocks(cus, m, n)) * k <= 8192;
+}
+
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -364,26 +383,14 @@ template <typename T, int CB> hipError_t few(const MxProduct& p, hipStream_t str
 }
 
 template <typename T> hipError_t product(const MxProduct& p, hipStream_t stream) {
-  const long cus = device_cu_count();
-  if (p.m <= 32) {
-    // Two blocks of columns a workgroup, which share what it loads of A, past 8 rows and where no CU gets more columns so: 16 rows
-    // of 1280 to 5120 columns 3.6 and 3.9 us with two and one, 1 row 3.3 and 3.3; of 8192 to 8192 17 rows 12.2 and 14.5, 32 17.8 and
-    // 25.5, 8 10.1 and 10.2; of 4096 to 32768 12 rows 18.0 and 19.9, 4 17.3 and 15.9; of 4096 to 11000 (4 and 3 blocks a CU) 16 rows
-    // 10.6 and 9.3; of 5120 to 1280 6.6 and 5.2.
-    auto most = [&](long cb) { return cb * (((p.n + 16 * cb - 1) / (16 * cb) + cus - 1) / cus); };
-    return p.m > 8 && most(2) <= most(1) ? few<T, 2>(p, stream) : few<T, 1>(p, stream);
-  }
-  const int tile = mx_product_tile((int)cus, p.m, p.n, p.k);
+  const int cus = device_cu_count();
+  if (p.m <= 32) return few_blocks(cus, p.m, p.n) == 2 ? few<T, 2>(p, stream) : few<T, 1>(p, stream);
+  const int tile = mx_product_tile(cus, p.m, p.n, p.k);
   if (tile == 256) return by_alignment<T, 256, 256, 2, 4>(p, stream);
   return tile == 128 ? by_alignment<T, 128, 128, 2, 2>(p, stream) : by_alignment<T, 64, 64, 2, 2>(p, stream);
 }
 
 }  // namespace
-
-// Whether a linear layer's few rows are packed by each workgroup of 16 columns again, in place of a launch of their own: up to
-// 16 rows while a CU's workgroups pack 8192 values of a row in all. On the card 7 rows of 5120 to 1280 columns in f32 take 6.0 us
-// so and 6.5 in two launches, 16 of 4096 to 4096 in f16 7.6 and 6.9, of 8192 to 4096 11.5 and 9.2; a launch takes the host 3 more.
-bool mx_packs_on_the_way(int m, int n, int k) { return m <= 16 && ((long)n + 4095) / 4096 * k <= 8192; }
 
 hipError_t mx_matmul(int dtype, const MxProduct& p, hipStream_t stream) {
   if (p.m == 0 || p.n == 0) return hipSuccess;

@@ -1122,8 +1122,8 @@ def mx_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
 
 
 @functools.lru_cache(maxsize=1024)
-def _mx_workspace(m: int, n: int, k: int) -> int:
-    """Bytes that sam_hip_mx_linear needs for a layer of these sizes (an error's are not kept)."""
+def _mx_workspace(dev: int, m: int, n: int, k: int) -> int:
+    """Bytes that sam_hip_mx_linear needs for a layer of these sizes on a device (an error's are not kept)."""
     size = load().sam_hip_mx_linear_workspace_size(m, n, k)
     if size < 0:
         raise SamHipError(load().sam_hip_last_error().decode())
@@ -1159,7 +1159,7 @@ def mx_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: tor
     m = out.numel() // n
     if (m | n) >> 31:
         _sizes("mx_linear", m, n)
-    ws_bytes = _mx_workspace(m, n, k)
+    ws_bytes = _mx_workspace(dev, m, n, k)
     ws = x.new_empty(-(-ws_bytes // x.element_size())) if ws_bytes else None
     _check(load().sam_hip_mx_linear(x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), _ptr(bias), out.data_ptr(), dt, m, n, k,
                                     bool(gelu), _ptr(ws), ws_bytes, _stream()))
