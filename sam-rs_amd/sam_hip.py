@@ -1036,9 +1036,8 @@ def _mx_type(what) -> torch.dtype:
 
 def _mx_operand(what, name, codes, scale):
     """A packed matrix as (codes, scale, shape of the values), contiguous and aligned, after its checks."""
-    _mx_type(what)
     if codes.dtype != _E2M1 or codes.dim() == 0:
-        raise SamHipError(f"{what}: {name} must hold torch.float4_e2m1fn_x2, [.., K / 2], got {codes.dtype} {tuple(codes.shape)}")
+        raise SamHipError(f"{what}: {name} must hold {_mx_type(what)}, [.., K / 2], got {codes.dtype} {tuple(codes.shape)}")
     shape = codes.shape[:-1] + (2 * codes.shape[-1],)
     _mx_k(what, shape)
     if scale.dtype != torch.uint8 or scale.shape != shape[:-1] + (shape[-1] // _BLOCK,):
