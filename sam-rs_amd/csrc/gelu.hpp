@@ -30,7 +30,9 @@ __device__ __forceinline__ float gelu_erf(float x) {
 
 // The same for results of 16 bits, with seven instructions less: erfc(z) exp(z^2) as a polynomial of degree 6 in
 // t = 1 / (1 + 0.44 z) without constant term, fitted here for the least relative error over 0 <= z <= 14 (6.6e-6; 1.1e-5 with
-// f32's roundings, down to x = -12), a fortieth of half a step of f16. Halves of the coefficients.
+// f32's roundings, down to x = -12), a fortieth of half a step of f16: of N(0, 1) arguments one f16 result in 240 is the neighbour of the
+// exact one's rounding for it. A 4-bit product of 4096 x 5120 and k = 1280 takes 39.1 us with gelu_erf and 36.4 with this in f16, 16384
+// rows of it 119 and 109. Halves of the coefficients.
 __device__ __forceinline__ float gelu_erf16(float x) {
   const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.31112698372208092f, 1.f));
   float p = -0.0721961836f;

@@ -49,7 +49,6 @@ __device__ __forceinline__ void bdma16s(i32x4 rsrc, unsigned off, unsigned soff,
                : "memory", "m0");
 }
 
-
 // LDS byte address of a pointer into dynamic shared memory.
 __device__ __forceinline__ unsigned lds_addr(const void* p) {
   return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)(p);

@@ -5,11 +5,12 @@
 // and its scale byte. Products of two codes and two scales are exact, so the f32 sums are the only roundings before the
 // output's. B is the first operand, so that a lane ends with four consecutive columns of one row of out.
 //
-// What bounds it: with many rows and a long k, the matrix units' power: 8192 x 8192 of k = 8192 takes 273 us (4.0 PFLOP/s, the
-// units busy in half of the cycles, at 1.8 to 1.9 GHz; with zeros for codes 219), where the instructions alone, fed from
-// registers, reach 8.6 PFLOP/s at 2.4 GHz. With a short k the results' way out: 4096 x 5120 of k = 1280 in f16 28 us, with
-// bias and GELU 34, of which 42 MB of results need 8 and the activation 6. With few rows B's bytes: 7 rows, 1280 columns of
-// k = 5120 in f32 6.0 us, a launch, the packing and the way along a row; 16 rows of 8192 to 8192 columns 12.7 (2.8 TB/s of B).
+// What bounds it: with many rows and a long k, steps whose waves load, read LDS and multiply one after the other, and power: 8192 x
+// 8192 of k = 8192 takes 273 us (4.0 PFLOP/s), the units busy in half of the cycles, at 1.8 to 1.9 GHz. The instructions alone, fed
+// from registers, would take 127 at 2.4 GHz; with zeros for codes, which take less power, it is 219, so that a third of the gap is
+// power. With a short k the results' way out: 4096 x 5120 of k = 1280 in f16 28 us, with
+// bias and GELU 35, of which 42 MB of results need 8 and the activation 7. With few rows B's bytes: 7 rows, 1280 columns of
+// k = 5120 in f32 6.6 us, a launch, the packing and the way along a row; 16 rows of 8192 to 8192 columns 12.7 (2.8 TB/s of B).
 #include <algorithm>
 
 #include "gelu.hpp"

@@ -9,8 +9,9 @@
 //   into A operands (the output's columns come out permuted, which the store undoes); P stays where S^T left it, since
 //   the reduction index is permuted alike: element j of lane group g is key 16 (j / 4) + 4 g + j % 4.
 // e4m3 codes become 16-bit values with their row's scale in one conversion, exactly (in f16, values below 2^-14 to
-// f16's subnormal step), and so do e2m1's with their block's. Softmax statistics and sums are f32. f16 P is rounded to f16 and its sum taken over the rounded
-// values, all of it times 2^15, which O / l cancels: weights keep f16's 11 bits down to 2^-29 of the largest, so that
+// f16's subnormal step), and so do e2m1's with their block's. Softmax statistics and sums are f32. f16 P is rounded to f16 and
+// its sum taken over the rounded values: results of N(0, 1) keys and values are off by 2.5e-4 to 2.8e-4 of their size, of which their
+// own rounding is 2.1e-4, and a second term would double the products of V, as bf16's does. All of it is taken times 2^15, which O / l cancels: weights keep f16's 11 bits down to 2^-29 of the largest, so that
 // thousands of keys far below one that dominates are not lost (each is off by 2^-40 of it at most). The exponent is taken of
 // (score - maximum) * scale, so that scores of any size keep P in f16's range. bf16 P goes as
 // hi + lo, which leaves 2^-16 of it (one bf16 term would leave 2^-8, as much as the output's own rounding).
