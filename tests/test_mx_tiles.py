@@ -25,7 +25,7 @@ def accepted(m, n, k):
 def test_every_accepted_size_fits_a_launch(lib):
     tile_of = ctypes.CDLL(sam_hip.LIB_PATH)._ZN6samhip15mx_product_tileEiiii  # samhip::mx_product_tile(int cus, int m, int n, int k)
     tile_of.argtypes, tile_of.restype = [ctypes.c_int] * 4, ctypes.c_int
-    sizes = [33, 64, 65, 128, 160, 300, 1000, *(1 << b for b in range(11, 31)), *(3 << b for b in range(10, 29)), 420_000_000, (1 << 30) - 128,
+    sizes = [33, 64, 65, 128, 160, 300, 1000, *(1 << b for b in range(11, 31)), *(3 << b for b in range(11, 29)), 420_000_000, (1 << 30) - 128,
              (1 << 30) - 511, (1 << 30) - 700, (1 << 29) - 1, 5 << 27]
     seen = set()
     for cus in (1, 80, 256, 304):
